@@ -72,6 +72,7 @@ enum {
     SCR_CAUSAL_KV = 4,  // aligned copies of caches that are not
     SCR_GEMM_PART = 5,  // split-K products [split][M][N]
     SCR_HANDOVER = 6,   // htr_debug_handover's words
+    SCR_KV_ATTN = 7,    // the tree and window attention's partial sums (one size)
 };
 // the device's scratch buffer `slot` with at least `bytes` bytes (a larger one replaces it: the tickets' and best
 // keys' slots zero-filled, the others as htr_dev_alloc fills)

@@ -1,0 +1,462 @@
+// A layer's KV cache in f16 or q8_0 rows: rows normed, turned and stored at positions of their own, rows copied between
+// caches of either type (quantised, read back), and rows gathered in place.
+//
+// q8_0 rows are blocks of 32 values of a head's 128: int8 quants q and one f16 scale d, which stand for f16(q·d), the value
+// the read-back gives and the attention works with. For a block of finite values x, saturated to ±65468.5 (127 times the
+// largest scale whose 127-fold f16 holds: f16's own largest, 65504, moves by less than a twelfth of its step of 515.5),
+//   d = the smallest f16 number with 127·d ≥ max |x|,   q = x / d rounded to the nearest integer, ties to even,
+// so |q| ≤ 127 without a clamp and |x − q·d| ≤ d / 2, down to the smallest blocks (a d rounded to nearest would lose up to
+// half of a block whose scale is among f16's last subnormals). Both are exact: the quotient's rounding is checked against
+// the exact remainder x − q·d, which f32 holds. A block with a NaN or an infinity gets a NaN scale.
+//
+// Bound: memory. Each value passes once, in 16-byte loads and 8- or 16-byte stores.
+#include <algorithm>
+
+#include "kv_ops.h"
+#include "wave.h"
+
+namespace {
+
+constexpr int D = 128, KV_BLOCK = 32;
+constexpr float Q8_MAX = 127.0f * 515.5f;  // 515.5: the largest scale whose 127-fold f16 holds
+constexpr uint32_t F32_INF = 0x7F800000u;
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
+
+// the f16 scale (as bits) of a block whose largest |x| has the f32 bits `top`
+__device__ __forceinline__ uint32_t block_scale(uint32_t top) {
+    if (top >= F32_INF) return 0x7E00u;  // a NaN or an infinity
+    const float a = fminf(__uint_as_float(top), Q8_MAX);
+    const _Float16 h = (_Float16)(a * (1.0f / 127.0f));
+    uint16_t b;
+    __builtin_memcpy(&b, &h, 2);
+    return 127.0f * (float)h < a ? b + 1u : b;  // 127·h is exact: 18 bits
+}
+__device__ __forceinline__ float half_bits(uint32_t b) {
+    const uint16_t u = (uint16_t)b;
+    _Float16 h;
+    __builtin_memcpy(&h, &u, 2);
+    return (float)h;
+}
+
+// x / d rounded to the nearest integer, ties to even, for |x| ≤ 127·d (inv ≈ 1 / d, 0 where d is 0): the quotient in f32
+// is within 2^-16, so r is the nearest or, beside a border, its neighbour; x − r·d is exact
+__device__ __forceinline__ int quant(float x, float d, float inv) {
+    float r = rintf(x * inv);
+    const float e = fmaf(-r, d, x), hd = 0.5f * d;
+    if (fabsf(e) >= hd && d > 0.0f) {
+        const bool odd = ((int)r & 1) != 0;
+        if (e > hd || (e == hd && odd)) r += 1.0f;
+        else if (e < -hd || (e == -hd && odd)) r -= 1.0f;
+    }
+    return (int)r;
+}
+// 8 of a block's values, its scale's bits → 8 quants
+__device__ __forceinline__ uint2_t quant8(const float (&x)[8], uint32_t db) {
+    if (db > 0x7C00u) return uint2_t{0u, 0u};
+    const float d = half_bits(db), inv = d > 0.0f ? 1.0f / d : 0.0f;
+    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        w[e >> 2] |= ((uint32_t)quant(fminf(fmaxf(x[e], -Q8_MAX), Q8_MAX), d, inv) & 0xffu) << (8 * (e & 3));
+    return uint2_t{w[0], w[1]};
+}
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// the largest over the 4 lanes of a block (lanes 4b … 4b + 3 hold 8 values each)
+__device__ __forceinline__ uint32_t block_max(uint32_t v, int lane) {
+    v = max(v, lane_swap_u32<2>(v, lane));
+    return max(v, lane_swap_u32<1>(v, lane));
+}
+
+// int8 quants → f16(q·d): a byte q ^ 0x80 under the high byte 0x64 is the f16 number 1024 + 128 + q, so one packed
+// subtraction gives q exactly, and one packed product rounds q·d once
+__device__ __forceinline__ half2_t dequant2(uint32_t w, uint32_t sel, half2_t d) {
+    const uint32_t p = __builtin_amdgcn_perm(0x64646464u, w, sel);
+    half2_t h;
+    __builtin_memcpy(&h, &p, 4);
+    return (h - half2_t{(_Float16)1152.0f, (_Float16)1152.0f}) * d;
+}
+__device__ __forceinline__ half8 dequant8(uint2_t q, half2_t d) {
+    const uint32_t a = q[0] ^ 0x80808080u, b = q[1] ^ 0x80808080u;
+    half2_t r[4] = {dequant2(a, 0x07010700u, d), dequant2(a, 0x07030702u, d), dequant2(b, 0x07010700u, d),
+                    dequant2(b, 0x07030702u, d)};
+    half8 o;
+    __builtin_memcpy(&o, r, 16);
+    return o;
+}
+__device__ __forceinline__ half2_t scale_pair(uint16_t bits) {
+    _Float16 h;
+    __builtin_memcpy(&h, &bits, 2);
+    return half2_t{h, h};
+}
+
+// ---- rows normed, turned and stored ------------------------------------------------------------------------------------
+
+// the value of the lane across lane bit M (as lane_swap), of the lane 8 further in a row of 16 (M = 0: DPP row_ror)
+template <int M> __device__ __forceinline__ double swap_f64(double v, int lane) {
+    uint32_t u[2];
+    __builtin_memcpy(u, &v, 8);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        if constexpr (M == 0) u[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)u[i], (int)u[i], 0x128, 0xF, 0xF, false);
+        else u[i] = lane_swap_u32<M>(u[i], lane);
+    }
+    __builtin_memcpy(&v, u, 8);
+    return v;
+}
+// Σ over the 16 lanes of a row of lanes
+__device__ __forceinline__ double row_sum(double v, int lane) {
+    v += swap_f64<8>(v, lane);
+    v += swap_f64<4>(v, lane);
+    v += swap_f64<2>(v, lane);
+    return v + swap_f64<1>(v, lane);
+}
+
+struct PostRowsArgs {
+    const float *q, *k, *v;
+    size_t q_stride, kv_stride;
+    const float *qn, *kn, *rope;
+    float *q_out;
+    HtrKvPlanes kv;
+    double eps;
+    int n, n_head, pos0, row0;
+};
+struct TreeDepth {
+    uint8_t at[HTR_TREE_MAX];
+};
+
+// One head of one row to 16 lanes of 8 dims. The norm and the turn are in f64: what they give is rounded to f32, then to
+// the cache's type, and lies next to a border of that type often enough (4e-4 of f16 values for f32 sums, an f16 ulp off
+// each, and as many q8_0 quants a step off) that f32 sums would give each order of summation a cache of its own. It costs
+// nothing here: 70 f64 operations a lane for 100 bytes of traffic.
+template <bool Q8, bool TREE> __global__ __launch_bounds__(256) void k_post_rows(PostRowsArgs a, TreeDepth depth) {
+    const int lane = threadIdx.x & 63, j = lane & 15, heads = a.n_head + 2 * a.kv.n_kv;
+    const size_t id = blockIdx.x * (size_t)16 + (threadIdx.x >> 4), count = (size_t)a.n * heads;
+    const size_t at = id < count ? id : count - 1;
+    const int t = (int)(at / heads), h = (int)(at % heads), kvh = h - a.n_head;
+    const bool is_q = kvh < 0, is_v = kvh >= a.kv.n_kv;
+    const float *src = is_q   ? a.q + t * a.q_stride + (size_t)h * D
+                       : is_v ? a.v + t * a.kv_stride + (size_t)(kvh - a.kv.n_kv) * D
+                              : a.k + t * a.kv_stride + (size_t)kvh * D;
+    float x[8], y[8];
+    const float4 x0 = *reinterpret_cast<const float4 *>(src + 8 * j), x1 = *reinterpret_cast<const float4 *>(src + 8 * j + 4);
+    x[0] = x0.x, x[1] = x0.y, x[2] = x0.z, x[3] = x0.w, x[4] = x1.x, x[5] = x1.y, x[6] = x1.z, x[7] = x1.w;
+    const float *w = is_q ? a.qn : a.kn, *cs = a.rope + (size_t)(a.pos0 + (TREE ? depth.at[t] : t)) * D + 16 * (j & 7);
+    float wf[8], c[16];
+#pragma unroll
+    for (int i = 0; i < 2; i++) *reinterpret_cast<float4 *>(wf + 4 * i) = *reinterpret_cast<const float4 *>(w + 8 * j + 4 * i);
+#pragma unroll
+    for (int i = 0; i < 4; i++) *reinterpret_cast<float4 *>(c + 4 * i) = *reinterpret_cast<const float4 *>(cs + 4 * i);
+    double ss = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) ss = fma((double)x[e], (double)x[e], ss);
+    const double inv = 1.0 / sqrt(row_sum(ss, lane) / (double)D + a.eps);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const double own = (double)x[e] * inv * (double)wf[e], far = swap_f64<0>(own, lane);
+        const double turned = j < 8 ? own * (double)c[2 * e] - far * (double)c[2 * e + 1]
+                                    : far * (double)c[2 * e + 1] + own * (double)c[2 * e];
+        y[e] = is_v ? x[e] : (float)turned;
+    }
+    if (is_q) {
+        if (id >= count) return;
+        float *o = a.q_out + ((size_t)t * a.n_head + h) * D + 8 * j;
+        *reinterpret_cast<float4 *>(o) = make_float4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<float4 *>(o + 4) = make_float4(y[4], y[5], y[6], y[7]);
+        return;
+    }
+    const int head = is_v ? kvh - a.kv.n_kv : kvh;
+    const size_t row = (size_t)head * a.kv.n_ctx + a.row0 + t;
+    if constexpr (Q8) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = max(top, abs_bits(y[e]));
+        const uint32_t db = block_scale(block_max(top, lane));
+        if (id >= count) return;
+        *reinterpret_cast<uint2_t *>((char *)(is_v ? a.kv.v : a.kv.k) + row * D + 8 * j) = quant8(y, db);
+        if ((j & 3) == 0) (is_v ? a.kv.vd : a.kv.kd)[row * (D / KV_BLOCK) + (j >> 2)] = (uint16_t)db;
+    } else {
+        if (id >= count) return;
+        half8 o;
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = (_Float16)y[e];
+        *reinterpret_cast<half8 *>((_Float16 *)(is_v ? a.kv.v : a.kv.k) + row * D + 8 * j) = o;
+    }
+}
+
+// ---- rows between caches -------------------------------------------------------------------------------------------------
+
+struct CopyArgs {
+    HtrKvPlanes src, dst;
+    int src_row, dst_row, n;
+};
+constexpr int COPY_ROWS = 64;  // rows a workgroup
+
+// blockIdx.y: K and V of each KV head. Quantise: 16 lanes of 8 values to a row
+__global__ __launch_bounds__(256) void k_kv_quantise(CopyArgs a) {
+    const int lane = threadIdx.x & 63, j = lane & 15, head = blockIdx.y >> 1, is_v = blockIdx.y & 1;
+    const _Float16 *src = (const _Float16 *)(is_v ? a.src.v : a.src.k) + ((size_t)head * a.src.n_ctx + a.src_row) * D;
+    const size_t to = (size_t)head * a.dst.n_ctx + a.dst_row;
+    const int r0 = blockIdx.x * COPY_ROWS + (threadIdx.x >> 4);
+    half8 in[COPY_ROWS / 16];
+#pragma unroll
+    for (int i = 0; i < COPY_ROWS / 16; i++)
+        in[i] = *reinterpret_cast<const half8 *>(src + (size_t)min(r0 + 16 * i, a.n - 1) * D + 8 * j);
+#pragma unroll
+    for (int i = 0; i < COPY_ROWS / 16; i++) {
+        float x[8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            x[e] = (float)in[i][e];
+            top = max(top, abs_bits(x[e]));
+        }
+        const uint32_t db = block_scale(block_max(top, lane));
+        const uint2_t q = quant8(x, db);
+        if (r0 + 16 * i < a.n) {
+            const size_t row = to + r0 + 16 * i;
+            *reinterpret_cast<uint2_t *>((char *)(is_v ? a.dst.v : a.dst.k) + row * D + 8 * j) = q;
+            if ((j & 3) == 0) (is_v ? a.dst.vd : a.dst.kd)[row * (D / KV_BLOCK) + (j >> 2)] = (uint16_t)db;
+        }
+    }
+}
+
+// read back: 8 lanes of 16 values to a row
+__global__ __launch_bounds__(256) void k_kv_read_back(CopyArgs a) {
+    const int j = threadIdx.x & 7, head = blockIdx.y >> 1, is_v = blockIdx.y & 1;
+    const size_t from = (size_t)head * a.src.n_ctx + a.src_row, to = (size_t)head * a.dst.n_ctx + a.dst_row;
+    const int r0 = blockIdx.x * COPY_ROWS + (threadIdx.x >> 3);
+    uint4_t q[COPY_ROWS / 32];
+    uint16_t d[COPY_ROWS / 32];
+#pragma unroll
+    for (int i = 0; i < COPY_ROWS / 32; i++) {
+        const size_t row = from + min(r0 + 32 * i, a.n - 1);
+        q[i] = *reinterpret_cast<const uint4_t *>((const char *)(is_v ? a.src.v : a.src.k) + row * D + 16 * j);
+        d[i] = (is_v ? a.src.vd : a.src.kd)[row * (D / KV_BLOCK) + (j >> 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < COPY_ROWS / 32; i++) {
+        if (r0 + 32 * i >= a.n) continue;
+        _Float16 *o = (_Float16 *)(is_v ? a.dst.v : a.dst.k) + (to + r0 + 32 * i) * D + 16 * j;
+        const half2_t s = scale_pair(d[i]);
+        *reinterpret_cast<half8 *>(o) = dequant8(uint2_t{q[i][0], q[i][1]}, s);
+        *reinterpret_cast<half8 *>(o + 8) = dequant8(uint2_t{q[i][2], q[i][3]}, s);
+    }
+}
+
+// the same type on both sides: a row's bytes (16 or 8 units of 16), its 8 bytes of scales
+template <bool Q8> __global__ __launch_bounds__(256) void k_kv_copy(CopyArgs a) {
+    constexpr int U = Q8 ? 8 : 16;
+    const int head = blockIdx.y >> 1, is_v = blockIdx.y & 1;
+    const size_t from = (size_t)head * a.src.n_ctx + a.src_row, to = (size_t)head * a.dst.n_ctx + a.dst_row;
+    const uint4_t *src = (const uint4_t *)(is_v ? a.src.v : a.src.k) + from * U;
+    uint4_t *dst = (uint4_t *)(is_v ? a.dst.v : a.dst.k) + to * U;
+    const int r0 = blockIdx.x * COPY_ROWS, rows = min(COPY_ROWS, a.n - r0);
+    for (int i = threadIdx.x; i < rows * U; i += 256) dst[(size_t)r0 * U + i] = src[(size_t)r0 * U + i];
+    if (Q8 && (int)threadIdx.x < rows) {
+        const uint2_t *sd = (const uint2_t *)(is_v ? a.src.vd : a.src.kd) + from;
+        ((uint2_t *)(is_v ? a.dst.vd : a.dst.kd) + to)[r0 + threadIdx.x] = sd[r0 + threadIdx.x];
+    }
+}
+
+// ---- rows gathered in place ----------------------------------------------------------------------------------------------
+
+struct KeepArgs {
+    HtrKvPlanes kv;
+    int row0, n;
+    int idx[HTR_TREE_MAX];
+};
+// one plane of one head to a workgroup: every row is held in registers before the first is written
+template <bool Q8> __global__ __launch_bounds__(256) void k_kv_keep(KeepArgs a) {
+    constexpr int U = Q8 ? 8 : 16, PER = HTR_TREE_MAX * U / 256;
+    const int head = blockIdx.x >> 1, is_v = blockIdx.x & 1, tid = threadIdx.x;
+    const size_t row0 = (size_t)head * a.kv.n_ctx + a.row0;
+    uint4_t *rows = (uint4_t *)(is_v ? a.kv.v : a.kv.k) + row0 * U;
+    uint2_t *scales = Q8 ? (uint2_t *)(is_v ? a.kv.vd : a.kv.kd) + row0 : nullptr;
+    uint4_t held[PER];
+    uint2_t d = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int r = min((tid + 256 * i) / U, a.n - 1);
+        held[i] = rows[(size_t)a.idx[r] * U + tid % U];
+    }
+    if (Q8 && tid < a.n) d = scales[a.idx[tid]];
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int r = (tid + 256 * i) / U;
+        if (r < a.n) rows[(size_t)r * U + tid % U] = held[i];
+    }
+    if (Q8 && tid < a.n) scales[tid] = d;
+}
+
+bool overlap(const void *a, size_t na, const void *b, size_t nb) {
+    return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
+}  // namespace
+
+// ---- ABI -----------------------------------------------------------------------------------------------------------------
+
+HtrOnDevice::HtrOnDevice(htr_device *dev) {
+    if (hipGetDevice(&before) != hipSuccess) before = dev->ordinal;
+    if (before != dev->ordinal) (void)hipSetDevice(dev->ordinal);
+    else before = -1;
+}
+HtrOnDevice::~HtrOnDevice() {
+    if (before >= 0) (void)hipSetDevice(before);
+}
+
+int htr_kv_check(const char *what, const htr_kv *kv, HtrKvPlanes *out) {
+    if (!kv) return htr_fail("%s: null cache", what);
+    if (kv->type != HTR_GGML_F16 && kv->type != HTR_GGML_Q8_0)
+        return htr_fail("%s: a cache of type %d (HTR_GGML_F16 %d or HTR_GGML_Q8_0 %d)", what, kv->type, HTR_GGML_F16,
+                        HTR_GGML_Q8_0);
+    if (kv->n_kv < 1 || kv->n_kv > 4096 || kv->n_ctx < 1)
+        return htr_fail("%s: a cache of %d KV heads, %d rows (1 … 4096 heads, at least a row)", what, kv->n_kv, kv->n_ctx);
+    if (!kv->d_k || !kv->d_v) return htr_fail("%s: null cache rows", what);
+    if (((uintptr_t)kv->d_k | (uintptr_t)kv->d_v) & 15) return htr_fail("%s: the cache rows must be 16-byte aligned", what);
+    const bool q8 = kv->type == HTR_GGML_Q8_0;
+    if (q8 && (!kv->d_kd || !kv->d_vd)) return htr_fail("%s: a q8_0 cache without scales", what);
+    if (q8 && (((uintptr_t)kv->d_kd | (uintptr_t)kv->d_vd) & 7))
+        return htr_fail("%s: the cache scales must be 8-byte aligned", what);
+    *out = HtrKvPlanes{kv->d_k, kv->d_v, q8 ? kv->d_kd : nullptr, q8 ? kv->d_vd : nullptr, kv->n_kv, kv->n_ctx, q8};
+    return 0;
+}
+
+extern "C" int htr_tree_masks(const int32_t *h_parent, int n, uint64_t *h_mask, int32_t *h_depth) {
+    if (!h_parent || !h_mask || !h_depth) return htr_fail("htr_tree_masks: null argument");
+    if (n < 1 || n > HTR_TREE_MAX) return htr_fail("htr_tree_masks: %d nodes (1 … %d)", n, HTR_TREE_MAX);
+    for (int i = 0; i < n; i++) {
+        const int p = h_parent[i];
+        if (p < -1 || p >= i) return htr_fail("htr_tree_masks: node %d has parent %d (an earlier node, or -1)", i, p);
+        h_mask[i] = (p >= 0 ? h_mask[p] : 0) | 1ull << i;
+        h_depth[i] = p >= 0 ? h_depth[p] + 1 : 0;
+    }
+    return 0;
+}
+
+extern "C" int htr_qkv_post_rows(htr_device *dev, const float *d_q, size_t q_stride, const float *d_k, const float *d_v,
+                                 size_t kv_stride, int n, const float *d_q_norm, const float *d_k_norm,
+                                 const float *d_rope, int n_pos, int pos0, const int32_t *h_depth, int n_head, float eps,
+                                 const htr_kv *kv, int row0, float *d_q_out) {
+    const char *me = "htr_qkv_post_rows";
+    PostRowsArgs a{};
+    HTR_TRY(htr_kv_check(me, kv, &a.kv));
+    if (!d_q || !d_k || !d_v || !d_q_norm || !d_k_norm || !d_rope || !d_q_out) return htr_fail("%s: null argument", me);
+    if (n_head < 1 || n_head % kv->n_kv) return htr_fail("%s: %d q heads on %d KV heads", me, n_head, kv->n_kv);
+    const size_t qd = (size_t)n_head * D, kvd = (size_t)kv->n_kv * D;
+    if (q_stride < qd || kv_stride < kvd || ((q_stride | kv_stride) & 3))
+        return htr_fail("%s: rows %zu and %zu floats apart (multiples of 4, at least %zu and %zu)", me, q_stride, kv_stride,
+                        qd, kvd);
+    if (((uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_q_norm | (uintptr_t)d_k_norm | (uintptr_t)d_rope |
+         (uintptr_t)d_q_out) & 15)
+        return htr_fail("%s: pointers must be 16-byte aligned", me);
+    if (n < 1 || row0 < 0 || row0 > kv->n_ctx - n)
+        return htr_fail("%s: %d rows from row %d of a %d-row cache", me, n, row0, kv->n_ctx);
+    if (h_depth && n > HTR_TREE_MAX) return htr_fail("%s: %d drafted rows (at most %d)", me, n, HTR_TREE_MAX);
+    TreeDepth depth{};
+    int deepest = n - 1;
+    if (h_depth) {
+        deepest = 0;
+        for (int t = 0; t < n; t++) {
+            if (h_depth[t] < 0 || h_depth[t] >= HTR_TREE_MAX)
+                return htr_fail("%s: row %d at depth %d (0 … %d)", me, t, h_depth[t], HTR_TREE_MAX - 1);
+            depth.at[t] = (uint8_t)h_depth[t];
+            deepest = std::max(deepest, h_depth[t]);
+        }
+    }
+    if (pos0 < 0 || n_pos < 1 || deepest >= n_pos || pos0 > n_pos - 1 - deepest)
+        return htr_fail("%s: positions %d … %lld of a %d-position rope table", me, pos0, (long long)pos0 + deepest, n_pos);
+    // in place (q_out on q's own rows) is the only overlap that the kernel allows
+    const size_t q_bytes = 4 * (q_stride * (n - 1) + qd), out_bytes = 4 * qd * n;
+    const size_t kv_bytes = 4 * (kv_stride * (n - 1) + kvd);
+    if ((overlap(d_q, q_bytes, d_q_out, out_bytes) && !(d_q == d_q_out && (n == 1 || q_stride == qd))) ||
+        overlap(d_k, kv_bytes, d_q_out, out_bytes) || overlap(d_v, kv_bytes, d_q_out, out_bytes))
+        return htr_fail("%s: the q output overlaps the input rows", me);
+    const size_t grid = ((size_t)n * (n_head + 2 * kv->n_kv) + 15) / 16;
+    if (grid > (size_t)INT32_MAX) return htr_fail("%s: %d rows of %d heads", me, n, n_head);
+    HTR_TRY(htr_check_alive(dev));
+    const HtrOnDevice on(dev);
+    a.q = d_q, a.k = d_k, a.v = d_v, a.q_stride = q_stride, a.kv_stride = kv_stride;
+    a.qn = d_q_norm, a.kn = d_k_norm, a.rope = d_rope, a.q_out = d_q_out;
+    a.eps = (double)eps, a.n = n, a.n_head = n_head, a.pos0 = pos0, a.row0 = row0;
+    const dim3 g((unsigned)grid), b(256);
+#define HTR_POST(Q8, TREE) hipLaunchKernelGGL((k_post_rows<Q8, TREE>), g, b, 0, dev->stream, a, depth)
+    if (a.kv.q8 && h_depth) HTR_POST(true, true);
+    else if (a.kv.q8) HTR_POST(true, false);
+    else if (h_depth) HTR_POST(false, true);
+    else HTR_POST(false, false);
+#undef HTR_POST
+    return htr_launched(dev, a.kv.q8 ? "k_post_rows<q8_0>" : "k_post_rows<f16>");
+}
+
+extern "C" int htr_kv_copy(htr_device *dev, const htr_kv *src, int src_row, const htr_kv *dst, int dst_row, int n) {
+    const char *me = "htr_kv_copy";
+    CopyArgs a{};
+    HTR_TRY(htr_kv_check(me, src, &a.src));
+    HTR_TRY(htr_kv_check(me, dst, &a.dst));
+    if (src->n_kv != dst->n_kv) return htr_fail("%s: %d KV heads into %d", me, src->n_kv, dst->n_kv);
+    if (n < 0 || src_row < 0 || src_row > src->n_ctx - n || dst_row < 0 || dst_row > dst->n_ctx - n)
+        return htr_fail("%s: %d rows from row %d of %d to row %d of %d", me, n, src_row, src->n_ctx, dst_row, dst->n_ctx);
+    // the caches' planes: apart, or the same ones with rows apart
+    auto bytes = [](const htr_kv *c) { return (size_t)c->n_kv * c->n_ctx * D * (c->type == HTR_GGML_Q8_0 ? 1 : 2); };
+    auto scale_bytes = [](const htr_kv *c) { return (size_t)c->n_kv * c->n_ctx * 8; };
+    struct Plane {
+        const void *p;
+        size_t n;
+    };
+    const Plane s[4] = {{a.src.k, bytes(src)}, {a.src.v, bytes(src)}, {a.src.kd, a.src.q8 ? scale_bytes(src) : 0},
+                        {a.src.vd, a.src.q8 ? scale_bytes(src) : 0}};
+    const Plane d[4] = {{a.dst.k, bytes(dst)}, {a.dst.v, bytes(dst)}, {a.dst.kd, a.dst.q8 ? scale_bytes(dst) : 0},
+                        {a.dst.vd, a.dst.q8 ? scale_bytes(dst) : 0}};
+    const bool apart = src_row + n <= dst_row || dst_row + n <= src_row;
+    for (int i = 0; i < 4; i++)
+        for (int j = 0; j < 4; j++) {
+            if (!s[i].n || !d[j].n || !overlap(s[i].p, s[i].n, d[j].p, d[j].n)) continue;
+            if (!(i == j && src->type == dst->type && s[i].p == d[j].p && src->n_ctx == dst->n_ctx && apart))
+                return htr_fail("%s: rows %d … of the source overlap rows %d … of the destination", me, src_row, dst_row);
+        }
+    HTR_TRY(htr_check_alive(dev));
+    if (n == 0) return 0;
+    const HtrOnDevice on(dev);
+    a.src_row = src_row, a.dst_row = dst_row, a.n = n;
+    const dim3 g((unsigned)((n + COPY_ROWS - 1) / COPY_ROWS), (unsigned)(2 * src->n_kv)), b(256);
+    if (!a.src.q8 && a.dst.q8) {
+        hipLaunchKernelGGL(k_kv_quantise, g, b, 0, dev->stream, a);
+        return htr_launched(dev, "k_kv_quantise");
+    }
+    if (a.src.q8 && !a.dst.q8) {
+        hipLaunchKernelGGL(k_kv_read_back, g, b, 0, dev->stream, a);
+        return htr_launched(dev, "k_kv_read_back");
+    }
+    if (a.src.q8) hipLaunchKernelGGL(k_kv_copy<true>, g, b, 0, dev->stream, a);
+    else hipLaunchKernelGGL(k_kv_copy<false>, g, b, 0, dev->stream, a);
+    return htr_launched(dev, a.src.q8 ? "k_kv_copy<q8_0>" : "k_kv_copy<f16>");
+}
+
+extern "C" int htr_kv_keep(htr_device *dev, const htr_kv *kv, int row0, const int32_t *h_idx, int n) {
+    const char *me = "htr_kv_keep";
+    KeepArgs a{};
+    HTR_TRY(htr_kv_check(me, kv, &a.kv));
+    if (n < 0 || n > HTR_TREE_MAX) return htr_fail("%s: %d rows (at most %d)", me, n, HTR_TREE_MAX);
+    if (n && !h_idx) return htr_fail("%s: null rows", me);
+    if (row0 < 0 || row0 > kv->n_ctx - n) return htr_fail("%s: %d rows from row %d of %d", me, n, row0, kv->n_ctx);
+    for (int i = 0; i < n; i++) {
+        if (h_idx[i] < 0 || h_idx[i] >= kv->n_ctx - row0)
+            return htr_fail("%s: row %d + %d of %d", me, row0, h_idx[i], kv->n_ctx);
+        a.idx[i] = h_idx[i];
+    }
+    HTR_TRY(htr_check_alive(dev));
+    if (n == 0) return 0;
+    const HtrOnDevice on(dev);
+    a.row0 = row0, a.n = n;
+    const dim3 g((unsigned)(2 * kv->n_kv)), b(256);
+    if (a.kv.q8) hipLaunchKernelGGL(k_kv_keep<true>, g, b, 0, dev->stream, a);
+    else hipLaunchKernelGGL(k_kv_keep<false>, g, b, 0, dev->stream, a);
+    return htr_launched(dev, a.kv.q8 ? "k_kv_keep<q8_0>" : "k_kv_keep<f16>");
+}

@@ -1,0 +1,21 @@
+// What the operators on a layer's KV cache share (kv_cache.hip, kv_attention.hip).
+#pragma once
+
+#include "htr_internal.h"
+
+// a checked cache's planes, as the kernels take them
+struct HtrKvPlanes {
+    void *k, *v;          // f16 or int8 [n_kv][n_ctx][128]
+    uint16_t *kd, *vd;    // q8_0: f16 scales [n_kv][n_ctx][4]
+    int n_kv, n_ctx;
+    bool q8;
+};
+// 0 with *out filled, or -1 with the message of what is wrong with the cache
+int htr_kv_check(const char *what, const htr_kv *kv, HtrKvPlanes *out);
+
+// the device made current for a call's launches, and the caller's own again afterwards
+struct HtrOnDevice {
+    explicit HtrOnDevice(htr_device *dev);
+    ~HtrOnDevice();
+    int before = -1;
+};

@@ -39,6 +39,7 @@ SYMBOLS = [
     "htr_session_kv_cache", "htr_debug_last_kernel", "htr_capture_begin", "htr_capture_end", "htr_graph_launch",
     "htr_graph_free", "htr_decode_attention_static", "htr_session_profile_step", "htr_session_set_fused_step",
     "htr_session_fused_step", "htr_session_profile_fused_step", "htr_debug_handover", "htr_session_set_wait_limit",
+    "htr_tree_masks", "htr_qkv_post_rows", "htr_kv_copy", "htr_kv_keep", "htr_tree_attention", "htr_window_attention",
 ]
 STEP_EMBED, STEP_QKV, STEP_ATTENTION, STEP_O, STEP_FFN, STEP_DOWN, STEP_HEAD, STEP_ALL = 1, 2, 4, 8, 16, 32, 64, 127
 
@@ -74,6 +75,11 @@ READ_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_uint64, C.c_void_p, C.c_size_t)
 class KvViewC(C.Structure):
     _fields_ = [("d_k", C.c_void_p), ("d_v", C.c_void_p), ("n_layer", C.c_int), ("n_kv", C.c_int),
                 ("n_ctx", C.c_int), ("d_head", C.c_int), ("layer_stride", C.c_size_t)]
+
+
+class KvC(C.Structure):
+    _fields_ = [("type", C.c_int), ("n_kv", C.c_int), ("n_ctx", C.c_int), ("d_k", C.c_void_p), ("d_v", C.c_void_p),
+                ("d_kd", C.c_void_p), ("d_vd", C.c_void_p)]
 
 
 class PresetC(C.Structure):
@@ -191,6 +197,12 @@ def lib() -> C.CDLL:
             "htr_choice_create": (i32, [vp, C.POINTER(PresetC), vp, sz, sz, sz, pp]),
             "htr_choice_free": (i32, [vp]),
             "htr_decode_gpu": (i32, [vp, vp, sz, TOKEN_CB, vp]),
+            "htr_tree_masks": (i32, [vp, i32, vp, vp]),
+            "htr_qkv_post_rows": (i32, [vp, vp, sz, vp, vp, sz, i32, vp, vp, vp, i32, i32, vp, i32, f32, vp, i32, vp]),
+            "htr_kv_copy": (i32, [vp, vp, i32, vp, i32, i32]),
+            "htr_kv_keep": (i32, [vp, vp, i32, vp, i32]),
+            "htr_tree_attention": (i32, [vp, vp, sz, i32, vp, i32, vp, i32, f32, vp]),
+            "htr_window_attention": (i32, [vp, vp, sz, i32, i32, i32, i32, vp, i32, f32, vp]),
             "htr_synth_q8_0": (i32, [C.c_uint64, sz, sz, vp]),
             "htr_synth_normal": (i32, [C.c_uint64, sz, f32, f32, vp]),
             "htr_choose_host": (i32, [vp, sz, C.POINTER(PresetC), vp, sz, vp, vp, sz, C.POINTER(C.c_uint64),
@@ -454,6 +466,106 @@ def decode_attention(dev: Device, q: Buffer, kc: Buffer, vc: Buffer, n_head: int
 def causal_attention(dev: Device, q: Buffer, kc: Buffer, vc: Buffer, n_q: int, pos0: int, n_head: int, n_kv: int,
                      n_ctx: int, scale: float, out: Buffer) -> None:
     _check(lib().htr_causal_attention(dev.h, q.ptr, kc.ptr, vc.ptr, n_q, pos0, n_head, n_kv, n_ctx, scale, out.ptr))
+
+
+class KvCache:
+    """One layer's KV cache (htr_kv): f16 rows, or q8_0 blocks as int8 quants and f16 scales. ``KvCache(dev, n_kv, n_ctx)``
+    allocates one (freed by ``free``); ``KvCache.of`` takes buffers that the caller holds."""
+
+    def __init__(self, dev: Device, n_kv: int, n_ctx: int, q8_0: bool = False):
+        rows = n_kv * n_ctx
+        self.held = []
+        try:
+            for nbytes in (rows * 128 * (1 if q8_0 else 2),) * 2 + (rows * 8,) * (2 if q8_0 else 0):
+                self.held.append(Buffer(dev, nbytes, MEM_KV_CACHE))
+        except HtrError:
+            self.free()
+            raise
+        self._set(n_kv, n_ctx, *self.held)
+
+    @classmethod
+    def of(cls, n_kv: int, n_ctx: int, k, v, kd=None, vd=None) -> "KvCache":
+        """a cache on buffers (anything with ``ptr``): f16 rows k, v, or int8 quants with the f16 scales kd, vd"""
+        self = cls.__new__(cls)
+        self.held = []
+        self._set(n_kv, n_ctx, k, v, kd, vd)
+        return self
+
+    def _set(self, n_kv: int, n_ctx: int, k, v, kd=None, vd=None) -> None:
+        if (kd is None) != (vd is None):
+            raise ValueError("scales of both K and V, or of neither")
+        self.n_kv, self.n_ctx, self.q8_0 = n_kv, n_ctx, kd is not None
+        self.k, self.v, self.kd, self.vd = k, v, kd, vd
+        self.c = KvC(GGML_Q8_0 if self.q8_0 else GGML_F16, n_kv, n_ctx, k.ptr, v.ptr, _p(kd), _p(vd))
+        self.ref = C.addressof(self.c)
+
+    def free(self) -> None:
+        for b in self.held:
+            b.free()
+        self.held = []
+
+
+class Tree:
+    """A drafted tree: node i continues node ``parents[i]`` < i, or the last committed token (-1). ``masks`` (one u64 a
+    node: the nodes on its path) and ``depths`` (0 for a root)."""
+
+    def __init__(self, parents):
+        p = np.ascontiguousarray(parents, dtype=np.int32)
+        self.n = p.size
+        self.masks, self.depths = np.zeros(max(self.n, 1), np.uint64), np.zeros(max(self.n, 1), np.int32)
+        _check(lib().htr_tree_masks(_ptr(p), self.n, _ptr(self.masks), _ptr(self.depths)))
+        self.masks_ptr, self.depths_ptr = _ptr(self.masks), _ptr(self.depths)
+
+    @classmethod
+    def of_masks(cls, masks, depths=None) -> "Tree":
+        """any masks: bit j of masks[i] shows node i row j of the draft"""
+        self = cls.__new__(cls)
+        self.masks = np.ascontiguousarray(masks, dtype=np.uint64)
+        self.n = self.masks.size
+        self.depths = np.zeros(self.n, np.int32) if depths is None else np.ascontiguousarray(depths, dtype=np.int32)
+        if self.depths.size != self.n:
+            raise ValueError(f"{self.depths.size} depths for {self.n} masks")
+        self.masks_ptr, self.depths_ptr = _ptr(self.masks), _ptr(self.depths)
+        return self
+
+
+def qkv_post_rows(dev: Device, q, k, v, n: int, q_norm, k_norm, rope, n_pos: int, pos0: int, n_head: int, eps: float,
+                  kv: KvCache, row0: int, q_out, q_stride: int | None = None, kv_stride: int | None = None,
+                  tree: Tree | None = None) -> None:
+    """rows of raw q / k / v normed and turned at positions pos0 + t (a tree: pos0 + depth), q to q_out, k and v to the
+    cache's rows row0 + t. Strides in floats (None: rows without a gap)"""
+    if tree is not None and tree.n != n:
+        raise ValueError(f"{n} rows of a tree of {tree.n} nodes")
+    _check(lib().htr_qkv_post_rows(dev.h, q.ptr, n_head * 128 if q_stride is None else q_stride, k.ptr, v.ptr,
+                                   kv.n_kv * 128 if kv_stride is None else kv_stride, n, q_norm.ptr, k_norm.ptr, rope.ptr,
+                                   n_pos, pos0, None if tree is None else tree.depths_ptr, n_head, eps, kv.ref, row0,
+                                   q_out.ptr))
+
+
+def kv_copy(dev: Device, src: KvCache, src_row: int, dst: KvCache, dst_row: int, n: int) -> None:
+    """n rows between caches: f16 to q8_0 quantises, q8_0 to f16 reads back, like types copy"""
+    _check(lib().htr_kv_copy(dev.h, src.ref, src_row, dst.ref, dst_row, n))
+
+
+def kv_keep(dev: Device, kv: KvCache, row0: int, rows) -> None:
+    """rows row0 + rows[i] to row0 + i, all read before any is written"""
+    n = len(rows)
+    _check(lib().htr_kv_keep(dev.h, kv.ref, row0, (C.c_int32 * max(n, 1))(*rows), n))
+
+
+def tree_attention(dev: Device, q, tree: Tree | int, n_past: int, kv: KvCache, n_head: int, scale: float, out,
+                   q_stride: int | None = None) -> None:
+    """attention of a drafted tree's queries (or of a chain of that many) over n_past committed rows and the draft's"""
+    n, masks = (tree, None) if isinstance(tree, int) else (tree.n, tree.masks_ptr)
+    _check(lib().htr_tree_attention(dev.h, q.ptr, n_head * 128 if q_stride is None else q_stride, n, masks, n_past, kv.ref,
+                                    n_head, scale, out.ptr))
+
+
+def window_attention(dev: Device, q, n_q: int, pos0: int, window: int, n_sink: int, kv: KvCache, n_head: int, scale: float,
+                     out, q_stride: int | None = None) -> None:
+    """attention of the queries at pos0 … over the last `window` rows up to each one's own and the first n_sink"""
+    _check(lib().htr_window_attention(dev.h, q.ptr, n_head * 128 if q_stride is None else q_stride, n_q, pos0, window,
+                                      n_sink, kv.ref, n_head, scale, out.ptr))
 
 
 def choose(dev: Device, logits: Buffer, n_vocab: int, hist: Buffer, length: int, window: int, rp: float, tok: Buffer,

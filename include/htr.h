@@ -177,6 +177,55 @@ int htr_decode_attention_static(htr_device *dev, const float *d_q, const uint16_
  * [n_q][n_head·128] f32 = softmax(q·scale·Kᵀ over the keys ≤ each query's position)·V. GQA group 2. */
 int htr_causal_attention(htr_device *dev, const float *d_q, const uint16_t *d_k, const uint16_t *d_v, int n_q,
                          int pos0, int n_head, int n_kv, int n_ctx, float scale, float *d_out);
+/* ---- operators on a layer's KV cache in f16 or q8_0 rows (no reference counterpart: the reference's cache is f16, one
+ *      row a step, every key visible): drafted tokens, caches in half the memory, reads that keep a window ------------- */
+/* One layer's cache, head-major: HTR_GGML_F16 — f16 [n_kv][n_ctx][128] each —, or HTR_GGML_Q8_0 — int8 quants of that
+ * shape and f16 scales [n_kv][n_ctx][4], a block of 32 dims standing for f16(q·d). Rows 16-byte, scales 8-byte aligned;
+ * d_kd / d_vd are not read for f16. A session's layer i as one: htr_session_kv_cache's d_k + i·layer_stride, its n_ctx. */
+typedef struct {
+    int type, n_kv, n_ctx;
+    void *d_k, *d_v;
+    uint16_t *d_kd, *d_vd;
+} htr_kv;
+/* the most nodes of a drafted tree */
+enum { HTR_TREE_MAX = 64 };
+/* host only: the masks and depths of a tree of n nodes (1 … 64) whose node i continues node h_parent[i] < i, or the last
+ * committed token (−1): h_mask[i] has the bits of the nodes on the path to i, i among them; a root's depth is 0 */
+int htr_tree_masks(const int32_t *h_parent, int n, uint64_t *h_mask, int32_t *h_depth);
+/* htr_qkv_post for n rows at once, into either type of cache: the raw q [n] rows q_stride floats apart (n_head heads of
+ * 128), k and v rows kv_stride floats apart (n_kv heads), each q and k head RMS-normed with its weights and turned by
+ * RoPE at position pos0 + h_depth[t] (row t of a draft: n ≤ 64, depths 0 … 63; h_depth NULL: pos0 + t) from the table
+ * d_rope [n_pos][64] × (cos, sin); q to d_q_out [n][n_head·128], k and v to the cache's rows row0 + t. The norm and the
+ * turn are computed in f64 and rounded to f32, then to f16 or q8_0 (a block's scale the smallest f16 number d with
+ * 127·d ≥ max |x|, its quants x / d to the nearest integer, ties to even; finite values saturate at ±65468.5 = 127·515.5, a block with a
+ * NaN or an infinity is NaN). Strides multiples of 4, pointers 16-byte aligned; d_q_out may be d_q where its rows are
+ * n_head·128 apart, and overlaps the inputs in no other way (refused). */
+int htr_qkv_post_rows(htr_device *dev, const float *d_q, size_t q_stride, const float *d_k, const float *d_v,
+                      size_t kv_stride, int n, const float *d_q_norm, const float *d_k_norm, const float *d_rope,
+                      int n_pos, int pos0, const int32_t *h_depth, int n_head, float eps, const htr_kv *kv, int row0,
+                      float *d_q_out);
+/* rows src_row … + n − 1 of one cache to rows dst_row … of another of as many KV heads: f16 to q8_0 quantises as above,
+ * q8_0 to f16 reads back f16(q·d), like types copy. The caches' memory is apart, or it is one cache and the rows are
+ * (else refused). */
+int htr_kv_copy(htr_device *dev, const htr_kv *src, int src_row, const htr_kv *dst, int dst_row, int n);
+/* rows row0 + h_idx[i] to rows row0 + i, i < n ≤ 64, all read before any is written (any order, a row more than once): a
+ * draft's accepted path moved together, or beams reordered. The rows from row0 + n on stay as they are. */
+int htr_kv_keep(htr_device *dev, const htr_kv *kv, int row0, const int32_t *h_idx, int n);
+/* attention of a drafted tree over a cache: queries d_q [n], rows q_stride floats apart (n ≤ 64 nodes, n_head heads of
+ * 128, n_head a multiple of n_kv), query t over rows 0 … n_past − 1 and the rows n_past + j whose bit j h_mask[t] has (the
+ * host array of htr_tree_masks, or any other: read before the call returns; NULL: a chain, j ≤ t) →
+ * d_out [n][n_head·128] = softmax(scale·q·Kᵀ)·V, zeros for a query that sees no row. n = 1 is a decode step's attention.
+ * A row that a query does not see does not touch its output, whatever it holds. All sums in f32, q and the weights held
+ * to 22 bits; over a q8_0 cache the same bits as over its read-back. Up to 17 MB of scratch, the same for every size:
+ * made at the first call that splits a query's keys, which cannot be one that is being captured. Output apart from the
+ * queries (else refused); strides multiples of 4, pointers 16-byte aligned. */
+int htr_tree_attention(htr_device *dev, const float *d_q, size_t q_stride, int n, const uint64_t *h_mask, int n_past,
+                       const htr_kv *kv, int n_head, float scale, float *d_out);
+/* attention with a sliding window and first keys that stay visible: queries at positions pos0 … pos0 + n_q − 1, the one at
+ * p over the cache rows j ≤ p with j < n_sink or j > p − window (window ≥ 1: itself at least) → d_out [n_q][n_head·128].
+ * Otherwise as htr_tree_attention. n_q = 1 is a decode step's. */
+int htr_window_attention(htr_device *dev, const float *d_q, size_t q_stride, int n_q, int pos0, int window, int n_sink,
+                         const htr_kv *kv, int n_head, float scale, float *d_out);
 /* the GPU token choice of a greedy preset on n_vocab logits (choose_pen → choose_max → choose_pick,
  * text.rs:222-231; semantics of ocr-decode sampling.rs:38-62, bit-exact): the repetition penalty rp over the distinct
  * ids of d_hist[len − window … len) applied in place (< 0: × rp, else ÷ rp, IEEE round-to-nearest), the frequency
