@@ -33,8 +33,8 @@ struct htr_device {
     void *pinned = nullptr;
     size_t pinned_bytes = 0;
     // scratch of the standalone kernel entry points, grown on demand (zero-filled when (re)allocated)
-    void *scratch[8] = {nullptr};
-    size_t scratch_bytes[8] = {0};
+    void *scratch[9] = {nullptr};
+    size_t scratch_bytes[9] = {0};
     // the measurement timer's events
     hipEvent_t t0 = nullptr, t1 = nullptr;
     // decode steps replayed as captured HIP graphs (HTR_GRAPHS=0 at open: launched one by one)
@@ -73,6 +73,7 @@ enum {
     SCR_GEMM_PART = 5,  // split-K products [split][M][N]
     SCR_HANDOVER = 6,   // htr_debug_handover's words
     SCR_KV_ATTN = 7,    // the tree and window attention's partial sums (one size)
+    SCR_KV_TICKET = 8,  // their tickets (one size; zero, self-resetting)
 };
 // the device's scratch buffer `slot` with at least `bytes` bytes (a larger one replaces it: the tickets' and best
 // keys' slots zero-filled, the others as htr_dev_alloc fills)

@@ -350,7 +350,8 @@ int htr_scratch(htr_device *dev, int slot, size_t bytes, void **out) {
         dev->scratch[slot] = nullptr;
         dev->scratch_bytes[slot] = 0;
         // the self-resetting words (best keys, tickets) start at zero; the rest is written before it is read
-        const bool zero = slot == SCR_CHOOSE_PART || slot == SCR_CHOOSE_CNT || slot == SCR_ATTN_CNT;
+        const bool zero =
+            slot == SCR_CHOOSE_PART || slot == SCR_CHOOSE_CNT || slot == SCR_ATTN_CNT || slot == SCR_KV_TICKET;
         HTR_TRY(alloc_filled(dev, bytes, HTR_MEM_WORK, zero, &dev->scratch[slot]));
         dev->scratch_bytes[slot] = bytes;
     }
