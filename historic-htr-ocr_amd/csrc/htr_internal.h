@@ -33,8 +33,8 @@ struct htr_device {
     void *pinned = nullptr;
     size_t pinned_bytes = 0;
     // scratch of the standalone kernel entry points, grown on demand (zero-filled when (re)allocated)
-    void *scratch[9] = {nullptr};
-    size_t scratch_bytes[9] = {0};
+    void *scratch[10] = {nullptr};
+    size_t scratch_bytes[10] = {0};
     // the measurement timer's events
     hipEvent_t t0 = nullptr, t1 = nullptr;
     // decode steps replayed as captured HIP graphs (HTR_GRAPHS=0 at open: launched one by one)
@@ -74,10 +74,14 @@ enum {
     SCR_HANDOVER = 6,   // htr_debug_handover's words
     SCR_KV_ATTN = 7,    // the tree and window attention's partial sums (one size)
     SCR_KV_TICKET = 8,  // their tickets (one size; zero, self-resetting)
+    SCR_KV_ROWS = 9,    // q8_0 rows read back for the window attention (htr_scratch_kept)
 };
 // the device's scratch buffer `slot` with at least `bytes` bytes (a larger one replaces it: the tickets' and best
 // keys' slots zero-filled, the others as htr_dev_alloc fills)
 int htr_scratch(htr_device *dev, int slot, size_t bytes, void **out);
+// the same for scratch that recorded graphs may hold: at least doubled when it grows, and what it was before stays
+// allocated until the device is closed
+int htr_scratch_kept(htr_device *dev, int slot, size_t bytes, void **out);
 
 // the device is dead: latch the first reason and fire the hook once; returns -1
 int htr_latch(htr_device *dev, const char *kind, const char *msg);

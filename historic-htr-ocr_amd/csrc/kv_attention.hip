@@ -4,9 +4,8 @@
 //   out[t][h] = Σ_j p_j·v_j / Σ_j p_j,  p_j = e^(scale·q·k_j − m)  over the keys j that query t sees (zeros if none)
 //
 // The q heads of a KV head share its keys, so a KV head's queries are rows (t, head of the group), packed: row r is query
-// r / group. A workgroup takes 32·WR rows and a run of key blocks of 32; its four waves are WR row tiles by KP = 4 / WR
-// parts of the blocks, whose sums are merged through LDS. Where the rows are few, the blocks are also split over
-// workgroups, whose sums a second launch joins.
+// r / group. A wave works on 32 rows, a block of 32 keys at a time. Few rows: the blocks are split over workgroups
+// (k_kv_attn_split); many: a workgroup takes 64 rows and all their blocks (k_kv_attn).
 //
 // On the f16 matrix cores (v_mfma_f32_32x32x16_f16) with f32-grade operands: q and p are pairs of f16 values, 22 bits; K
 // and V are f16 (a q8_0 element stands for f16(q·d): rounded once, 2^-11 of it, beside the block's own step of 2^-8 of its
@@ -19,8 +18,8 @@
 //            below, and drops out with l, which carries it too;
 //   values   Oᵀ += Vᵀ·(ph + pl)ᵀ, V by transposing LDS reads, p straight from the lane's registers.
 // A key that a row does not see is as if it were not there, whatever the cache holds in it: its score becomes −∞ after the
-// product, and where a block that not every row sees holds a value of V that is not finite (0·∞ is NaN on the matrix
-// cores), its products are summed one by one, with those that are not seen left out.
+// product, and values of V that are not finite are taken out of the product of a block that not every row sees, and make
+// NaN of the sums of the rows that do see them.
 #include <algorithm>
 #include <type_traits>
 
@@ -40,6 +39,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef float float2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef __fp16 fp16x4 __attribute__((ext_vector_type(4)));
 typedef int int2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
@@ -52,12 +52,14 @@ struct Args {
     HtrKvPlanes kv;
     int n, n_head, group;
     float scale;
+    int sink_rows, shift;      // keys from sink_rows on lie shift rows further up in memory
     int n_past;                // tree: the committed keys
     int pos0, window, n_sink;  // window
     int n_rg, n_split;         // row groups, parts of a row group's key blocks
     float *part;               // [n_kv·n_rg·n_split][32] rows of partial sums o[128], and each row's (m, l)
     uint64_t *part_ml;
     uint32_t *tickets;         // [n_kv·n_rg], TICKET words apart: zero, self-resetting
+    int xl;                    // a KV head's workgroups share an XCD, and its L2 shows them each other's stores
 };
 struct TreeMask {
     uint64_t of[HTR_TREE_MAX];
@@ -95,13 +97,21 @@ __device__ __forceinline__ void lds_load4(const void *base, uint32_t off, uint32
                  : "memory", "m0");
 }
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// v, as a value the compiler does not know: what is computed from it stays where it is used (a rare path's addresses and
+// offsets, moved out of the loop, would take registers from the loop)
+__device__ __forceinline__ int here(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 // this wave's LDS reads have their values
 __device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// partial sums between workgroups, through the coherence point
-__device__ __forceinline__ void put64(void *p, float a, float b) {
+// partial sums between workgroups: in the L2 of the XCD that they share (workgroup-scope stores, read by agent-scope loads
+// that find the L2's lines), or through the coherence point
+__device__ __forceinline__ void put64(void *p, float a, float b, bool xl) {
     const uint64_t v = (uint64_t)__float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32;
-    __hip_atomic_store((uint64_t *)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (xl) __hip_atomic_store((uint64_t *)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    else __hip_atomic_store((uint64_t *)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ float2 get64(const void *p) {
     const uint64_t v = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -149,6 +159,21 @@ template <bool TREE> struct Row {
     }
 };
 
+// p − (float)h for the low (0) or high (1) half of h: one mixed-precision fma
+template <int HI> __device__ __forceinline__ float minus_half(float p, uint32_t h) {
+    float r;
+    if constexpr (HI) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(p));
+    else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(p));
+    return r;
+}
+// two values as a pair of f16 values each
+__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const half2_t h = __builtin_convertvector((float2_t{a, b}), half2_t);
+    __builtin_memcpy(&hi, &h, 4);
+    const half2_t r = __builtin_convertvector((float2_t{minus_half<0>(a, hi), minus_half<1>(b, hi)}), half2_t);
+    __builtin_memcpy(&lo, &r, 4);
+}
+
 // a row's q·scale as f16 pairs, the B operand of step ks = dims 16ks + 8hf … + 7; the factor of its scores
 __device__ __forceinline__ float q_pairs(const float *qrow, float scale, half8 (&qh)[8], half8 (&ql)[8]) {
     float x[8][8], top = 0.0f;
@@ -170,35 +195,77 @@ __device__ __forceinline__ float q_pairs(const float *qrow, float scale, half8 (
     const int ex = max(__builtin_amdgcn_frexp_expf(pair_max<32>(top)), -100);
     const float up = ldexpf(1.0f, 10 - ex);
 #pragma unroll
-    for (int ks = 0; ks < 8; ks++)
+    for (int ks = 0; ks < 8; ks++) {
+        uint32_t h[4], r[4];
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float y = x[ks][e] * up;
-            const _Float16 hi = (_Float16)y;
-            qh[ks][e] = hi;
-            ql[ks][e] = (_Float16)(y - (float)hi);
-        }
+        for (int e = 0; e < 4; e++) split2(x[ks][2 * e] * up, x[ks][2 * e + 1] * up, h[e], r[e]);
+        __builtin_memcpy(&qh[ks], h, 16);
+        __builtin_memcpy(&ql[ks], r, 16);
+    }
     return ldexpf(LOG2E, ex - 10);
+}
+
+// values of V that are not finite, in blocks that not every row sees (0·∞ is NaN on the matrix cores, in rows too that do
+// not see them): taken as 0 in the product, and NaN put in afterwards where a row does see one, by a product of ones
+__device__ __forceinline__ half8 finite(half8 v, uint32_t &any) {
+    uint32_t w[4];
+    __builtin_memcpy(w, &v, 16);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const uint32_t b = ((w[e] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;  // a half whose exponent is all ones
+        any |= b;
+        w[e] &= ~((b >> 15) * 0xFFFFu);
+    }
+    __builtin_memcpy(&v, w, 16);
+    return v;
+}
+__device__ __forceinline__ half8 ones_of_not_finite(half8 v) {
+    uint32_t w[4];
+    __builtin_memcpy(w, &v, 16);
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = ((((w[e] & 0x7C007C00u) + 0x04000400u) & 0x80008000u) >> 15) * 0x3C00u;
+    __builtin_memcpy(&v, w, 16);
+    return v;
+}
+// o's sums of the rows that see one: NaN. seen: the lane's 16 keys; vread(u, ss): V's operand of tile u, step ss
+template <typename F> __device__ __forceinline__ void put_nan(f32x16 (&o)[4], uint32_t seen, F vread) {
+    half8 ind[2];
+#pragma unroll
+    for (int ss = 0; ss < 2; ss++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            w[e] = ((seen >> (8 * ss + 2 * e)) & 1) * 0x3C00u | ((seen >> (8 * ss + 2 * e + 1)) & 1) * 0x3C000000u;
+        __builtin_memcpy(&ind[ss], w, 16);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        f32x16 t = __builtin_amdgcn_mfma_f32_32x32x16_f16(ones_of_not_finite(vread(u, 0)), ind[0], f32x16{}, 0, 0, 0);
+        t = __builtin_amdgcn_mfma_f32_32x32x16_f16(ones_of_not_finite(vread(u, 1)), ind[1], t, 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < 16; x++) o[u][x] = t[x] > 0.0f ? NAN : o[u][x];
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 // ---- few rows: the blocks split over workgroups ----------------------------------------------------------------------------
 //
-// A workgroup takes 32 rows, each of its four waves every fourth block of its part. A wave loads its own blocks straight
+// A workgroup takes 32 rows, each of its eight waves every eighth block of its part. A wave loads its own blocks straight
 // into LDS of its own, so the waves wait for nobody until their sums are merged; f16 blocks with one buffer for K and one
 // for V, each filled again as soon as it is read (K under the softmax and the values, V under the next scores), q8_0 blocks,
-// half the size, with two, raw: a fragment's 8 quants become f16 in the registers of the one wave that uses them (7 VALU
-// instructions an operand register; V's by a transposing read of bytes).
+// half the size, with two, raw: a fragment's 8 quants become f16 in the registers of the one wave that uses them (14 VALU
+// instructions an operand; V's by a transposing read of bytes).
 //   f16   K and V [32 keys][16 chunks of 16 bytes], row r's chunk c at 16r + (c ^ r % 16), V's at 16r + (c ^ 2(r % 8));
 //   q8_0  K and V [32 keys][8 chunks], row r's chunk c at 8r + (c ^ r / 2 % 8); their scales [32 keys][4]; V's once more
 //         as [dims / 32][key / 16][hf][8], the order of an operand's slots.
 // Reads of 16 (32) lanes then fall on different bank groups.
 constexpr int QT = 256 + 256 + 16 + 16;  // 16-byte chunks of a q8_0 buffer: K, V, K scales, V scales
+constexpr int SW = 8;                    // waves
 
-template <bool Q8, bool TREE> __global__ __launch_bounds__(256, 2) void k_kv_attn_split(Args a, TreeMask tree) {
+template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv_attn_split(Args a, TreeMask tree) {
     constexpr int WAVE = Q8 ? 2 * QT + 16 : TILE;  // chunks of a wave's LDS
-    __shared__ __attribute__((aligned(16))) uint4_t s_kv[4][WAVE];
-    __shared__ float s_p[4][KB / 2][KB];  // weights, where they are summed one by one
-    __shared__ float s_ml[4][2][KB];
+    __shared__ __attribute__((aligned(16))) uint4_t s_kv[SW][WAVE];
+    __shared__ float s_ml[SW][2][KB];
     __shared__ float s_c[KB];
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -213,30 +280,45 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256, 2) void k_kv_att
 
     uint4_t *tile = s_kv[wave];
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4_t *)tile;
-    const uint32_t kx = 16 * ((lane & 15) ^ (lane >> 4)), vx = 16 * ((lane & 15) ^ (2 * (lane >> 4)));
-    const uint32_t bx = 16 * ((lane & 7) ^ (lane >> 4));
-    // block i's K or V (f16), or all of it into buffer b (q8_0); rows past the last key are the last key's, and are masked
+    // block i's K or V (f16), or all of it into buffer b (q8_0); a wave's instruction is 4 (8) whole rows. Rows past the last
+    // key are the last key's, and are masked
+    const uint32_t kx = 16 * ((lane & 15) ^ (lane >> 4)), vx = 16 * ((lane & 15) ^ (2 * (lane >> 4))), r4 = 2 * D * (lane >> 4);
+    const uint32_t bx = 16 * ((lane & 7) ^ (lane >> 4)), r8 = D * (lane >> 3);
     auto load = [&](int i, bool is_v) {
-        const int k0 = KB * blk.at(i);
+        const int k0 = KB * blk.at(i), last = n_keys - 1 - k0;
         const char *base = (const char *)(is_v ? a.kv.v : a.kv.k) + (head0 + k0) * (2 * D);
-        const uint32_t last = min(n_keys - 1 - k0, KB - 1);
+        const uint32_t to = lds + 16 * (is_v ? K_CHUNKS : 0);
+        if (last >= KB - 1) {
 #pragma unroll
-        for (int u = 0; u < 8; u++)
-            lds_load16(base, 2 * D * min((uint32_t)(4 * u + (lane >> 4)), last) + (is_v ? vx ^ (128 * (u & 1)) : kx ^ (64 * (u & 3))),
-                       lds + 16 * ((is_v ? K_CHUNKS : 0) + 64 * u));
+            for (int u = 0; u < 8; u++)
+                lds_load16(base + 2 * D * 4 * u, r4 + (is_v ? vx ^ (128 * (u & 1)) : kx ^ (64 * (u & 3))), to + 16 * 64 * u);
+        } else {
+            const int ln = here(lane);
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                lds_load16(base, 2 * D * min(4 * u + (ln >> 4), last) + (is_v ? vx ^ (128 * (u & 1)) : kx ^ (64 * (u & 3))), to + 16 * 64 * u);
+        }
     };
     auto load_q8 = [&](int i, int b) {
-        const int k0 = KB * blk.at(i);
+        const int k0 = KB * blk.at(i), last = n_keys - 1 - k0;
         const size_t row = head0 + k0;
-        const uint32_t last = min(n_keys - 1 - k0, KB - 1), to = lds + 16 * QT * b;
-        lds_load4(a.kv.kd + row * 4, 8 * min((uint32_t)lane >> 1, last) + 4 * (lane & 1), to + 16 * 512);
-        lds_load4(a.kv.vd + row * 4, 8 * min((uint32_t)lane >> 1, last) + 4 * (lane & 1), to + 16 * 528);
+        const uint32_t to = lds + 16 * QT * b;
+        const char *kb = (const char *)a.kv.k + row * D, *vb = (const char *)a.kv.v + row * D;
+        if (last >= KB - 1) {
+            lds_load4(a.kv.kd + row * 4, 4 * lane, to + 16 * 512);
+            lds_load4(a.kv.vd + row * 4, 4 * lane, to + 16 * 528);
 #pragma unroll
-        for (int u = 0; u < 8; u++)
-            lds_load16((const char *)(u < 4 ? a.kv.k : a.kv.v) + row * D,
-                       D * min((uint32_t)(8 * (u & 3) + (lane >> 3)), last) + (bx ^ (64 * (u & 1))), to + 16 * 64 * u);
+            for (int u = 0; u < 8; u++) lds_load16((u < 4 ? kb : vb) + D * 8 * (u & 3), r8 + (bx ^ (64 * (u & 1))), to + 16 * 64 * u);
+        } else {
+            const int ln = here(lane);
+            lds_load4(a.kv.kd + row * 4, 8 * min(ln >> 1, last) + 4 * (ln & 1), to + 16 * 512);
+            lds_load4(a.kv.vd + row * 4, 8 * min(ln >> 1, last) + 4 * (ln & 1), to + 16 * 528);
+#pragma unroll
+            for (int u = 0; u < 8; u++)
+                lds_load16(u < 4 ? kb : vb, D * min(8 * (u & 3) + (ln >> 3), last) + (bx ^ (64 * (u & 1))), to + 16 * 64 * u);
+        }
     };
-    int i = i0 + wave;
+    int i = i0 + wave, b = 0;
     if (i < i1) {
         if constexpr (Q8) {
             load_q8(i, 0);
@@ -266,13 +348,15 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256, 2) void k_kv_att
         for (int x = 0; x < 16; x++) o[u][x] = 0.0f;
     float m = M_NONE, l = 0.0f;
 
-    for (int b = 0; i < i1; i += 4, b ^= Q8) {
-        const bool more = i + 4 < i1;
+    // block i; MASK: not every row sees all of it
+    auto step = [&](auto is_masked) {
+        constexpr bool MASK = decltype(is_masked)::value;
+        const bool more = i + SW < i1;
         uint4_t *buf = tile + (Q8 ? QT * b : 0);
         if constexpr (Q8) {
             if (more) {
                 wait_reads();  // of the other buffer, a block ago
-                load_q8(i + 4, b ^ 1);
+                load_q8(i + SW, b ^ 1);
                 wait_loads<10>();
             } else {
                 wait_loads<0>();
@@ -307,7 +391,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256, 2) void k_kv_att
                 for (int ks = 0; ks < 4; ks++) f[ks] = *reinterpret_cast<const half8 *>(buf + 16 * c + ((8 * h + 2 * ks + hf) ^ (c & 15)));
                 if (h == 1) {
                     wait_reads();
-                    if (more) load(i + 4, false);
+                    if (more) load(i + SW, false);
                 }
 #pragma unroll
                 for (int ks = 0; ks < 4; ks++) {
@@ -316,14 +400,12 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256, 2) void k_kv_att
                 }
             }
         }
-        const int k0 = KB * blk.at(i);
-        const bool full = row.all_see(a, k0);
-        uint32_t seen = 0xffffu;
-        if (!full) {
-            seen = 0;
+        uint32_t seen = 0;
+        if constexpr (MASK) {
+            const int k0 = KB * blk.at(i) + here(4 * hf);
 #pragma unroll
             for (int x = 0; x < 16; x++) {
-                const bool v = row.sees(a, k0 + 8 * (x >> 2) + 4 * hf + (x & 3));
+                const bool v = row.sees(a, k0 + 8 * (x >> 2) + (x & 3));
                 seen |= (uint32_t)v << x;
                 s[x] = v ? s[x] : -INFINITY;
             }
@@ -340,97 +422,67 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256, 2) void k_kv_att
             for (int u = 0; u < 4; u++) o[u] *= corr;
         }
         float ls = 0.0f;
-        half8 ph[2], pl[2];
+        uint32_t ph[8], pl[8];
 #pragma unroll
-        for (int x = 0; x < 16; x++) {
-            s[x] = __builtin_amdgcn_exp2f(fmaf(s[x] - m, sc, P_SHIFT));  // not seen: 2^(−∞) = 0
-            ls += s[x];
-            const _Float16 hi = (_Float16)s[x];
-            ph[x >> 3][x & 7] = hi;
-            pl[x >> 3][x & 7] = (_Float16)(s[x] - (float)hi);
+        for (int x = 0; x < 8; x++) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * x] - m, sc, P_SHIFT));  // not seen: 2^(−∞) = 0
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * x + 1] - m, sc, P_SHIFT));
+            ls += p0;
+            ls += p1;
+            split2(p0, p1, ph[x], pl[x]);
         }
         l += ls;
         if constexpr (!Q8) {  // V
             if (more) wait_loads<8>();
             else wait_loads<0>();
         }
-        bool odd = false;  // a value of V that is not finite (or a scale that may make one)
-        if (!full) {
-            uint32_t any = 0;
+        auto vread = [&](int u, int ss) {
+            half8 v;
             if constexpr (Q8) {
-                const uint32_t w = reinterpret_cast<const uint32_t *>(buf + 528)[lane];
-                any = (w & 0x7FFFu) > 0x6007u || (w >> 16 & 0x7FFFu) > 0x6007u;  // past 515.5
+                const auto *p = (const __attribute__((address_space(3))) char *)buf + va[u] + 16 * 128 * ss;
+                const int2_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2_t *)p);
+                const half8 d = *reinterpret_cast<const half8 *>(tile + 2 * QT + 4 * u + 2 * ss + hf);
+                v = dequant8((uint32_t)w[0], (uint32_t)w[1], d);
             } else {
-#pragma unroll 2
-                for (int u = 0; u < 8; u++) {
-                    const uint4_t w = buf[K_CHUNKS + 64 * u + lane];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) any |= (w[e] & 0x7C00u) == 0x7C00u || (w[e] & 0x7C000000u) == 0x7C000000u;
-                }
+                const auto *p = (const __attribute__((address_space(3))) char *)buf + va[u] + 256 * 16 * ss;
+                const fp16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)p);
+                const fp16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)(p + 256 * 8));
+                __builtin_memcpy(&v, &lo, 8);
+                __builtin_memcpy((char *)&v + 8, &up, 8);
             }
-            odd = __builtin_amdgcn_ballot_w64(any != 0) != 0;
-        }
-        if (!odd) {
+            return v;
+        };
+        uint32_t odd = 0;
 #pragma unroll
-            for (int ss = 0; ss < 2; ss++)
+        for (int ss = 0; ss < 2; ss++) {
+            half8 h8, l8;
+            __builtin_memcpy(&h8, &ph[4 * ss], 16);
+            __builtin_memcpy(&l8, &pl[4 * ss], 16);
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    half8 v;
-                    if constexpr (Q8) {
-                        const auto *p = (const __attribute__((address_space(3))) char *)buf + va[u] + 16 * 128 * ss;
-                        const int2_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2_t *)p);
-                        const half8 d = *reinterpret_cast<const half8 *>(tile + 2 * QT + 4 * u + 2 * ss + hf);
-                        v = dequant8((uint32_t)w[0], (uint32_t)w[1], d);
-                    } else {
-                        const auto *p = (const __attribute__((address_space(3))) char *)buf + va[u] + 256 * 16 * ss;
-                        const fp16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)p);
-                        const fp16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)(p + 256 * 8));
-                        __builtin_memcpy(&v, &lo, 8);
-                        __builtin_memcpy((char *)&v + 8, &up, 8);
-                    }
-                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[ss], o[u], 0, 0, 0);
-                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[ss], o[u], 0, 0, 0);
-                }
-        } else {
-            // 16 keys' weights to LDS (−1: not seen), then key by key; the lane sums row c's dims 32u + 8(x / 4) + 4hf + x % 4
-#pragma unroll 1
-            for (int half = 0; half < 2; half++) {
-#pragma unroll
-                for (int x = 0; x < 8; x++)
-                    s_p[wave][8 * (x >> 2) + 4 * hf + (x & 3)][c] = (seen >> (8 * half + x)) & 1 ? (half ? s[8 + x] : s[x]) : -1.0f;
-                wait_reads();
-#pragma unroll 1
-                for (int k = 0; k < KB / 2; k++) {
-                    const int key = KB / 2 * half + k;
-                    const float p = s_p[wave][k][c];
-                    const bool v = !(p < 0.0f);
-#pragma unroll
-                    for (int u = 0; u < 4; u++)
-#pragma unroll
-                        for (int x = 0; x < 16; x++) {
-                            const int dim = 32 * u + 8 * (x >> 2) + 4 * hf + (x & 3);
-                            float w;
-                            if constexpr (Q8) {
-                                const int8_t q = reinterpret_cast<const int8_t *>(buf + 256 + 8 * key + ((dim >> 4) ^ ((key >> 1) & 7)))[dim & 15];
-                                w = (float)((_Float16)(float)q * reinterpret_cast<const _Float16 *>(buf + 528)[4 * key + u]);
-                            } else {
-                                w = (float)reinterpret_cast<const _Float16 *>(buf + K_CHUNKS + 16 * key + ((dim >> 3) ^ (2 * (key & 7))))[dim & 7];
-                            }
-                            o[u][x] = v ? fmaf(p, w, o[u][x]) : o[u][x];
-                            if ((x & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // (few values in registers at once)
-                        }
-                }
-                wait_reads();
+            for (int u = 0; u < 4; u++) {
+                half8 v = vread(u, ss);
+                if constexpr (MASK) v = finite(v, odd);
+                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, h8, o[u], 0, 0, 0);
+                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, l8, o[u], 0, 0, 0);
+                if constexpr (MASK) __builtin_amdgcn_sched_barrier(0);  // (few operands in registers at once)
             }
         }
+        if constexpr (MASK)
+            if (__builtin_amdgcn_ballot_w64(odd != 0)) put_nan(o, seen, vread);
         if constexpr (!Q8) {
             wait_reads();
-            if (more) load(i + 4, true);
+            if (more) load(i + SW, true);
         }
+        i += SW;
+        b ^= Q8;
+    };
+    while (i < i1) {
+        for (bool all = row.all_see(a, KB * blk.at(i)); all; all = i < i1 && row.all_see(a, KB * blk.at(i))) step(std::false_type{});
+        for (bool some = i < i1; some; some = i < i1 && !row.all_see(a, KB * blk.at(i))) step(std::true_type{});
     }
     l = pair_sum<32>(l);
 
-    // the waves' sums through LDS (each its own tile's place): wave u finishes dims 32u … of every row
+    // the waves' sums through LDS (each its own tile's place): thread (wave, lane) finishes 8 of the lane's 64 sums
     wait_reads();
     float4 *so = reinterpret_cast<float4 *>(tile);
 #pragma unroll
@@ -441,29 +493,31 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256, 2) void k_kv_att
     if (hf == 0) s_ml[wave][0][c] = m, s_ml[wave][1][c] = l;
     if (wave == 0 && hf == 0) s_c[c] = sc;
     __syncthreads();
-    m = fmaxf(fmaxf(s_ml[0][0][c], s_ml[1][0][c]), fmaxf(s_ml[2][0][c], s_ml[3][0][c]));
-    l = 0.0f;
-    float4 v[4];
+    m = M_NONE, l = 0.0f;
 #pragma unroll
-    for (int x = 0; x < 4; x++) v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p = 0; p < SW; p++) m = fmaxf(m, s_ml[p][0][c]);
+    float4 v[2];
 #pragma unroll
-    for (int p = 0; p < 4; p++) {
+    for (int x = 0; x < 2; x++) v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int p = 0; p < SW; p++) {
         const float w = __builtin_amdgcn_exp2f((s_ml[p][0][c] - m) * sc);
         l = fmaf(s_ml[p][1][c], w, l);
-        const float4 *from = reinterpret_cast<const float4 *>(s_kv[p]) + 4 * 64 * wave + lane;
+        const float4 *from = reinterpret_cast<const float4 *>(s_kv[p]) + 2 * 64 * wave + lane;
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
+        for (int x = 0; x < 2; x++) {
             const float4 y = from[64 * x];
             v[x].x = fmaf(y.x, w, v[x].x), v[x].y = fmaf(y.y, w, v[x].y);
             v[x].z = fmaf(y.z, w, v[x].z), v[x].w = fmaf(y.w, w, v[x].w);
         }
     }
+    const int dim0 = 16 * wave + 4 * hf;  // sums 8·wave … + 7 of the lane: dims 16·wave + 4hf … + 3, and 8 further
     if (a.n_split == 1) {
         if (row.r >= rows) return;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
-        float *orow = a.out + ((size_t)row.t * a.n_head + row.head) * D + 32 * wave + 4 * hf;
+        float *orow = a.out + ((size_t)row.t * a.n_head + row.head) * D + dim0;
 #pragma unroll
-        for (int x = 0; x < 4; x++)
+        for (int x = 0; x < 2; x++)
             *reinterpret_cast<float4 *>(orow + 8 * x) = make_float4(v[x].x * inv, v[x].y * inv, v[x].z * inv, v[x].w * inv);
         return;
     }
@@ -472,47 +526,49 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256, 2) void k_kv_att
     const size_t g0 = ((size_t)kvh * a.n_rg + rg) * a.n_split * KB;  // the row group's first row of partial sums
     if (row.r < rows) {
         const size_t pr = g0 + (size_t)split * KB + c;
-        float *prow = a.part + pr * D + 32 * wave + 4 * hf;
+        float *prow = a.part + pr * D + dim0;
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
-            put64(prow + 8 * x, v[x].x, v[x].y);
-            put64(prow + 8 * x + 2, v[x].z, v[x].w);
+        for (int x = 0; x < 2; x++) {
+            put64(prow + 8 * x, v[x].x, v[x].y, a.xl);
+            put64(prow + 8 * x + 2, v[x].z, v[x].w, a.xl);
         }
-        if (wave == 0 && hf == 0) put64(a.part_ml + pr, m, l);
+        if (wave == 0 && hf == 0) put64(a.part_ml + pr, m, l, a.xl);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's stores are performed
     __syncthreads();
     uint32_t *ticket = a.tickets + TICKET * ((size_t)kvh * a.n_rg + rg);
     if (tid == 0)
-        s_last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(a.n_split - 1);
+        s_last = (a.xl ? __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)
+                       : __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) ==
+                 (uint32_t)(a.n_split - 1);
     __syncthreads();
     if (!s_last) return;
     const int nr = min(KB, rows - r0), ns = a.n_split;
     float2 *s_w = reinterpret_cast<float2 *>(&s_kv[0][0]);  // [row][part]: (m, l), then (weight, l)
-    for (int id = tid; id < KB * MAX_SPLIT; id += 256) {
-        const int r = id / MAX_SPLIT, p = id % MAX_SPLIT;
-        if (r < nr && p < ns) s_w[id] = get64(a.part_ml + g0 + (size_t)p * KB + r);
+    for (int id = tid; id < nr * MAX_SPLIT; id += 64 * SW) {
+        const int p = id % MAX_SPLIT;
+        if (p < ns) s_w[id] = get64(a.part_ml + g0 + (size_t)p * KB + id / MAX_SPLIT);
     }
     __syncthreads();
     {
-        const int r = tid >> 3, p0 = tid & 7;
+        const int r = tid >> 4, p0 = tid & 15;
         float top = M_NONE, sum = 0.0f;
         if (r < nr)
-            for (int p = p0; p < ns; p += 8) top = fmaxf(top, s_w[MAX_SPLIT * r + p].x);
-        top = group_max<4>(top, lane);
+            for (int p = p0; p < ns; p += 16) top = fmaxf(top, s_w[MAX_SPLIT * r + p].x);
+        top = group_max<8>(top, lane);
         if (r < nr)
-            for (int p = p0; p < ns; p += 8) {
+            for (int p = p0; p < ns; p += 16) {
                 const float2 ml = s_w[MAX_SPLIT * r + p];
                 const float w = __builtin_amdgcn_exp2f((ml.x - top) * s_c[r]);
                 sum = fmaf(ml.y, w, sum);
                 s_w[MAX_SPLIT * r + p].x = w;
             }
-        sum = group_sum<4>(sum, lane);
+        sum = group_sum<8>(sum, lane);
         if (p0 == 0) s_ml[0][0][r] = sum == 0.0f ? 0.0f : 1.0f / sum;
     }
     __syncthreads();
-    // 32 threads of 4 dims a row; rows fewer than 8: a row's parts to 2, 4 or 8 such groups
-    const int gr = tid >> 5, d4 = tid & 31, lg = nr > 4 ? 3 : nr > 2 ? 2 : nr > 1 ? 1 : 0, groups = 8 >> lg;
+    // 32 threads of 4 dims a row; rows fewer than 16: a row's parts to 2, 4, 8 or 16 such groups
+    const int gr = tid >> 5, d4 = tid & 31, lg = nr > 8 ? 4 : nr > 4 ? 3 : nr > 2 ? 2 : nr > 1 ? 1 : 0, groups = 16 >> lg;
     float4 *s_g = reinterpret_cast<float4 *>(s_w + KB * MAX_SPLIT);
     for (int rb = 0; rb < nr; rb += 1 << lg) {
         const int r = min(rb + (gr & ((1 << lg) - 1)), nr - 1), g = gr >> lg;
@@ -532,7 +588,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256, 2) void k_kv_att
                 y.z = fmaf(in[e][1].x, w, y.z), y.w = fmaf(in[e][1].y, w, y.w);
             }
         }
-        if (groups > 1) {
+        if (groups > 1) {  // (fewer than 16 rows: one pass)
             s_g[tid] = y;
             __syncthreads();
             if (g == 0)
@@ -548,80 +604,56 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256, 2) void k_kv_att
                 make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
         }
     }
-    if (tid == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+    if (tid == 0) {  // for the next call
+        if (a.xl) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        else __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
 }
 
 // ---- many rows ---------------------------------------------------------------------------------------------------------------
+//
+// A workgroup takes 64 rows of a KV head: 4 waves = 2 row tiles × the even / odd key blocks, the two parts merged through
+// LDS at the end. A stage is 2 blocks (32 KB), K and V each double-buffered, K a stage ahead of V: the score MFMAs of the
+// next stage run under the softmax of this one. The cache is f16 (q8_0 rows are read back first: each is used by many
+// workgroups, and 112 VALU instructions a block and wave would be as many as the softmax's).
+constexpr int WR = 2, WP = 2;  // row tiles, key parts
 
-template <bool Q8, bool TREE, int WR>
-__global__ __launch_bounds__(256) void k_kv_attn(Args a, TreeMask tree) {
-    constexpr int KP = 4 / WR;
-    __shared__ __attribute__((aligned(16))) uint4_t s_kv[KP][TILE];  // K, then V
-    __shared__ float s_p[4][KB][KB];                                 // the weights, where they are summed one by one
-    __shared__ float s_ml[4][2][KB];
+template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_attn(Args a, TreeMask tree) {
+    __shared__ __attribute__((aligned(16))) uint4_t s_kv[2][WP][TILE];  // [buffer][part][K, V chunks]
+    __shared__ float s_ml[WR * WP][2][KB];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hf = lane >> 5, c = lane & 31, rt = wave % WR, kp = wave / WR;
-    const int kvh = blockIdx.x % a.kv.n_kv, rest = blockIdx.x / a.kv.n_kv;
-    const int split = rest % a.n_split, rg = a.n_rg - 1 - rest / a.n_split;
-    const int rows = a.n * a.group, r0 = rg * 32 * WR, r = r0 + 32 * rt + c, rc = min(r, rows - 1);
-    const int t = rc / a.group, head = kvh * a.group + rc % a.group;
+    const int hf = lane >> 5, c = lane & 31, rt = wave & 1, kp = wave >> 1;
+    const int kvh = blockIdx.x % a.kv.n_kv, rg = a.n_rg - 1 - blockIdx.x / a.kv.n_kv;  // (the longest rows first)
+    const int rows = a.n * a.group, r0 = rg * KB * WR;
     const int n_keys = TREE ? a.n_past + a.n : a.pos0 + a.n;
+    const Blocks blk = blocks_of<TREE>(a, r0 / a.group, min(r0 + KB * WR - 1, rows - 1) / a.group);
+    const int nb = blk.count(), n_stage = (nb + WP - 1) / WP;
+    const char *kh = (const char *)a.kv.k + (size_t)kvh * a.kv.n_ctx * (2 * D);
+    const char *vh = (const char *)a.kv.v + (size_t)kvh * a.kv.n_ctx * (2 * D);
 
-    // the row's keys, and those that every row of the wave's tile sees
-    const int qpos = a.pos0 + t;
-    uint64_t mask = 0;
-    if constexpr (TREE) mask = tree.of[t];
-    const int tile_a = min(r0 + 32 * rt, rows - 1) / a.group, tile_b = min(r0 + 32 * rt + 31, rows - 1) / a.group;
-    auto all_see = [&](int k0) {
-        if constexpr (TREE) return k0 + KB <= a.n_past;
-        else return k0 + KB - 1 <= a.pos0 + tile_a && (k0 + KB <= a.n_sink || k0 > a.pos0 + tile_b - a.window);
-    };
-    auto sees = [&](int key) {
-        if constexpr (TREE) {
-            const unsigned j = (unsigned)(key - a.n_past);
-            return key < a.n_past || (j < 64u && ((mask >> j) & 1) != 0);
-        } else {
-            return key <= qpos && (key < a.n_sink || key > qpos - a.window);
+    // a stage's K or V → buffer st % 2: 4 direct loads a wave, each of the 4 waves 4 rows of 16 (keys past the last: the last)
+    const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4_t *)&s_kv[0][0][64 * wave];
+    const int lrow = 4 * wave + (lane >> 4), lc = lane & 15;
+    const uint32_t koff = 16 * (lc ^ (lrow & 15)), voff = 16 * (lc ^ (2 * (lrow & 7)));  // the same for row lrow + 16
+    auto issue = [&](int st, bool is_v) {
+#pragma unroll
+        for (int p = 0; p < WP; p++) {
+            const int k0 = KB * blk.at(min(WP * st + p, nb - 1));
+            const char *base = (is_v ? vh : kh) + (size_t)(k0 < a.sink_rows ? k0 : k0 - a.shift) * (2 * D);
+            const uint32_t off = is_v ? voff : koff, last = 2 * D * min(n_keys - 1 - k0, KB - 1) + off;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                lds_load16(base, min(2 * D * (16 * h + lrow) + off, last),
+                           lds + 16u * (((st & 1) * WP + p) * TILE + (is_v ? K_CHUNKS : 0) + 256 * h));
         }
     };
+    issue(0, false);
+    issue(0, true);
+    if (n_stage > 1) issue(1, false);
 
-    const Blocks blk = blocks_of<TREE>(a, r0 / a.group, min(r0 + 32 * WR - 1, rows - 1) / a.group);
-    const int nb = blk.count(), i0 = (int)((int64_t)nb * split / a.n_split), i1 = (int)((int64_t)nb * (split + 1) / a.n_split);
-
-    // q·scale as f16 pairs: B operand of step ks = dims 16ks + 8hf … + 7 of row c
+    const Row<TREE> row(a, tree, kvh, r0 + KB * rt, c);
     half8 qh[8], ql[8];
-    float sc;
-    {
-        const float *qrow = a.q + (size_t)t * a.q_stride + (size_t)head * D + 8 * hf;
-        float x[8][8], top = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < 8; ks++) {
-            const float4 a0 = *reinterpret_cast<const float4 *>(qrow + 16 * ks);
-            const float4 a1 = *reinterpret_cast<const float4 *>(qrow + 16 * ks + 4);
-            x[ks][0] = a0.x, x[ks][1] = a0.y, x[ks][2] = a0.z, x[ks][3] = a0.w;
-            x[ks][4] = a1.x, x[ks][5] = a1.y, x[ks][6] = a1.z, x[ks][7] = a1.w;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                x[ks][e] *= a.scale;
-                top = fmaxf(top, fabsf(x[ks][e]));
-            }
-        }
-        // (a row of nothing but tiny values: its scores are 0 to f32 either way, and c stays a normal number)
-        const int ex = max(__builtin_amdgcn_frexp_expf(pair_max<32>(top)), -100);
-        sc = ldexpf(LOG2E, ex - 10);
-#pragma unroll
-        for (int ks = 0; ks < 8; ks++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float y = ldexpf(x[ks][e], 10 - ex);
-                const _Float16 hi = (_Float16)y;
-                qh[ks][e] = hi;
-                ql[ks][e] = (_Float16)(y - (float)hi);
-            }
-    }
-    // the lane's fragment slots in a block (K row r's 16-byte chunk c is at 16r + (c ^ r % 16), V's at 16r + (c ^ 2(r % 8)):
-    // the reads of 16 lanes fall on different bank groups): K step ks (key c, dims 16ks + 8hf …), V tile u (16-lane group:
-    // dims 32u + 16(lane / 16 % 2) …, keys 4hf + (lane % 16) / 4 of each group of 8)
+    const float sc = q_pairs(a.q + (size_t)row.t * a.q_stride + (size_t)row.head * D + 8 * hf, a.scale, qh, ql);
     int ka[8], va[4];
 #pragma unroll
     for (int ks = 0; ks < 8; ks++) ka[ks] = 16 * c + ((2 * ks + hf) ^ (c & 15));
@@ -634,212 +666,204 @@ __global__ __launch_bounds__(256) void k_kv_attn(Args a, TreeMask tree) {
 #pragma unroll
     for (int u = 0; u < 4; u++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) o[u][i] = 0.0f;
+        for (int x = 0; x < 16; x++) o[u][x] = 0.0f;
     float m = M_NONE, l = 0.0f;
 
-    const int n_stage = (i1 - i0 + KP - 1) / KP;
-    const int lt = rt * 64 + lane;  // the thread among those that load the part's block
-    for (int st = 0; st < n_stage; st++) {
-        const int i = i0 + st * KP + kp;
-        const bool live = i < i1;
-        const int k0 = KB * blk.at(min(i, i1 - 1));
-        // K and V → LDS (rows past the last key are the last key's, and are masked)
-        if constexpr (Q8) {
-#pragma unroll
-            for (int u = 0; u < 8 / WR; u++) {
-                const int id = lt + 64 * WR * u, is_v = id >> 8, row = (id >> 3) & 31, ch = id & 7;
-                const size_t at = (size_t)kvh * a.kv.n_ctx + min(k0 + row, n_keys - 1);
-                const uint4_t w = *reinterpret_cast<const uint4_t *>((const char *)(is_v ? a.kv.v : a.kv.k) + at * D + 16 * ch);
-                const uint16_t db = (is_v ? a.kv.vd : a.kv.kd)[at * 4 + (ch >> 1)];
-                _Float16 d;
-                __builtin_memcpy(&d, &db, 2);
-                const int sw = is_v ? 2 * (row & 7) : row & 15;
-                uint4_t *to = s_kv[kp] + (is_v ? K_CHUNKS : 0) + 16 * row;
-                *reinterpret_cast<half8 *>(to + ((2 * ch) ^ sw)) = dequant8(w[0], w[1], half2_t{d, d});
-                *reinterpret_cast<half8 *>(to + ((2 * ch + 1) ^ sw)) = dequant8(w[2], w[3], half2_t{d, d});
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < 16 / WR; u++) {
-                const int id = lt + 64 * WR * u, is_v = id >> 9, row = (id >> 4) & 31, ch = id & 15;
-                const size_t at = (size_t)kvh * a.kv.n_ctx + min(k0 + row, n_keys - 1);
-                const uint4_t w = *reinterpret_cast<const uint4_t *>((const char *)(is_v ? a.kv.v : a.kv.k) + at * (2 * D) + 16 * ch);
-                s_kv[kp][(is_v ? K_CHUNKS : 0) + 16 * row + (ch ^ (is_v ? 2 * (row & 7) : row & 15))] = w;
-            }
-        }
-        __syncthreads();
-        if (live) {
-            f32x16 s;
-#pragma unroll
-            for (int ks = 0; ks < 8; ks++) {
-                const half8 f = *reinterpret_cast<const half8 *>(s_kv[kp] + ka[ks]);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qh[ks], ks ? s : f32x16{}, 0, 0, 0);
-                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, ql[ks], s, 0, 0, 0);
-            }
-            const bool full = all_see(k0);
-            uint32_t seen = 0xffffu;
-            if (!full) {
-                seen = 0;
-#pragma unroll
-                for (int x = 0; x < 16; x++) {
-                    const bool v = sees(k0 + 8 * (x >> 2) + 4 * hf + (x & 3));
-                    seen |= (uint32_t)v << x;
-                    s[x] = v ? s[x] : -INFINITY;
-                }
-            }
-            float mx = s[0];
-#pragma unroll
-            for (int x = 1; x < 16; x++) mx = fmaxf(mx, s[x]);
-            mx = pair_max<32>(mx);
-            if (__builtin_amdgcn_ballot_w64((mx - m) * sc > P_ROOM)) {
-                const float to = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f((m - to) * sc);
-                m = to;
-                l *= corr;
-#pragma unroll
-                for (int u = 0; u < 4; u++) o[u] *= corr;
-            }
-            float ls = 0.0f;
+    // stage st in buffer b: its scores are in s; the next stage's are computed into sn under the softmax's VALU work
+    auto step = [&](int st, int b, f32x16 &s, f32x16 &sn, auto is_masked) {
+        constexpr bool MASK = decltype(is_masked)::value;
+        // this wave's loads of K stage st + 1 and V stage st are in, its reads of K stage st and V stage st − 1 have their
+        // values; behind the barrier everyone's, and the two buffers are free
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (st + 2 < n_stage) issue(st + 2, false);
+        if (st + 1 < n_stage) issue(st + 1, true);
+        uint32_t seen = 0;
+        if constexpr (MASK) {
+            const int i = WP * st + kp, k0 = KB * blk.at(min(i, nb - 1)) + here(4 * hf);
 #pragma unroll
             for (int x = 0; x < 16; x++) {
-                s[x] = __builtin_amdgcn_exp2f(fmaf(s[x] - m, sc, P_SHIFT));  // not seen: 2^(−∞) = 0
-                ls += s[x];
-            }
-            l += ls;
-            bool odd = false;
-            if (!full) {
-                uint32_t any = 0;
-#pragma unroll
-                for (int u = 0; u < 8; u++) {
-                    const uint4_t w = s_kv[kp][K_CHUNKS + 64 * u + lane];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        any |= (w[e] & 0x7C00u) == 0x7C00u;
-                        any |= (w[e] & 0x7C000000u) == 0x7C000000u;
-                    }
-                }
-                odd = __builtin_amdgcn_ballot_w64(any != 0) != 0;
-            }
-            if (!odd) {
-                half8 ph[2], pl[2];
-#pragma unroll
-                for (int x = 0; x < 16; x++) {
-                    const _Float16 hi = (_Float16)s[x];
-                    ph[x >> 3][x & 7] = hi;
-                    pl[x >> 3][x & 7] = (_Float16)(s[x] - (float)hi);
-                }
-                const auto *vb = (const __attribute__((address_space(3))) char *)s_kv[kp];
-#pragma unroll
-                for (int ss = 0; ss < 2; ss++)
-#pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        // slots 8hf … + 7 are keys 16ss + 4hf … + 3, then 16ss + 8 + 4hf … + 3: the lane's scores 8ss …
-                        const auto *p = vb + va[u] + 256 * 16 * ss;
-                        const fp16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)p);
-                        const fp16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)(p + 256 * 8));
-                        half8 v;
-                        __builtin_memcpy(&v, &lo, 8);
-                        __builtin_memcpy((char *)&v + 8, &up, 8);
-                        o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[ss], o[u], 0, 0, 0);
-                        o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[ss], o[u], 0, 0, 0);
-                    }
-            } else {
-                // the weights to LDS (−1: not seen), then key by key; lane 32hf + c sums row c's dims 32u + 8(x / 4) + 4hf + x % 4
-#pragma unroll
-                for (int x = 0; x < 16; x++)
-                    s_p[wave][8 * (x >> 2) + 4 * hf + (x & 3)][c] = (seen >> x) & 1 ? s[x] : -1.0f;
-                __builtin_amdgcn_wave_barrier();
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                const _Float16 *vt = reinterpret_cast<const _Float16 *>(s_kv[kp] + K_CHUNKS);
-#pragma unroll 1
-                for (int key = 0; key < KB; key++) {
-                    const float p = s_p[wave][key][c];
-                    const bool v = !(p < 0.0f);
-#pragma unroll
-                    for (int u = 0; u < 4; u++)
-#pragma unroll
-                        for (int x = 0; x < 16; x++) {
-                            const int dim = 32 * u + 8 * (x >> 2) + 4 * hf + (x & 3);
-                            const float w = (float)vt[8 * (16 * key + ((dim >> 3) ^ (2 * (key & 7)))) + (dim & 7)];
-                            o[u][x] = v ? fmaf(p, w, o[u][x]) : o[u][x];
-                        }
-                }
+                const bool v = i < nb && row.sees(a, k0 + 8 * (x >> 2) + (x & 3));
+                seen |= (uint32_t)v << x;
+                s[x] = v ? s[x] : -INFINITY;
             }
         }
-        __syncthreads();
+        float mx = s[0];
+#pragma unroll
+        for (int x = 1; x < 16; x++) mx = fmaxf(mx, s[x]);
+        mx = pair_max<32>(mx);
+        if (__builtin_amdgcn_ballot_w64((mx - m) * sc > P_ROOM)) {
+            const float to = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f((m - to) * sc);
+            m = to;
+            l *= corr;
+#pragma unroll
+            for (int u = 0; u < 4; u++) o[u] *= corr;
+        }
+        // the order pinned: behind each score MFMA of the next stage its share of this stage's softmax (left to itself the
+        // compiler issues the MFMAs back to back and the softmax behind them)
+        // (past the last stage: scores of what the buffer holds, not used)
+        const uint4_t *kb = s_kv[b ^ 1][kp];
+        const auto *vb = (const __attribute__((address_space(3))) char *)s_kv[b][kp];
+        auto vread = [&](int u, int ss) {
+            const auto *p = vb + va[u] + 256 * 16 * ss;
+            const fp16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)p);
+            const fp16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)(p + 256 * 8));
+            half8 v;
+            __builtin_memcpy(&v, &lo, 8);
+            __builtin_memcpy((char *)&v + 8, &up, 8);
+            return v;
+        };
+        uint32_t ph[8], pl[8];
+        float ls;
+        half8 f[8], v[4];
+#pragma unroll
+        for (int ks = 0; ks < 3; ks++) f[ks] = *reinterpret_cast<const half8 *>(kb + ka[ks]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int ks = 0; ks < 8; ks++) {
+            sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[ks], qh[ks], ks ? sn : f32x16{}, 0, 0, 0);
+            if (ks + 3 < 8) f[ks + 3] = *reinterpret_cast<const half8 *>(kb + ka[ks + 3]);
+            else v[ks - 5] = vread(ks - 5, 0);
+            const float2_t p = {__builtin_amdgcn_exp2f(fmaf(s[2 * ks] - m, sc, P_SHIFT)),
+                                __builtin_amdgcn_exp2f(fmaf(s[2 * ks + 1] - m, sc, P_SHIFT))};  // not seen: 2^(−∞) = 0
+            const half2_t hi = __builtin_convertvector(p, half2_t);
+            __builtin_memcpy(&ph[ks], &hi, 4);
+            asm volatile("" : "+v"(ph[ks]));  // holds the conversion here
+            __builtin_amdgcn_sched_barrier(0);
+            sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[ks], ql[ks], sn, 0, 0, 0);
+            ls = ks ? ls + p[0] : p[0];
+            ls += p[1];
+            const half2_t lo = __builtin_convertvector((float2_t{minus_half<0>(p[0], ph[ks]), minus_half<1>(p[1], ph[ks])}), half2_t);
+            __builtin_memcpy(&pl[ks], &lo, 4);
+            asm volatile("" : "+v"(pl[ks]));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        v[3] = vread(3, 0);
+        l += ls;
+        uint32_t odd = 0;
+#pragma unroll
+        for (int ss = 0; ss < 2; ss++) {
+            half8 h8, l8;
+            __builtin_memcpy(&h8, &ph[4 * ss], 16);
+            __builtin_memcpy(&l8, &pl[4 * ss], 16);
+            half8 vn[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                if constexpr (MASK) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    v[u] = finite(v[u], odd);
+                }
+                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[u], h8, o[u], 0, 0, 0);
+                if (ss == 0) vn[u] = vread(u, 1);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[u], l8, o[u], 0, 0, 0);
+                if (ss == 0) v[u] = vn[u];
+            }
+        }
+        if constexpr (MASK)
+            if (__builtin_amdgcn_ballot_w64(odd != 0)) put_nan(o, seen, vread);
+    };
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // K and V stage 0, K stage 1
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    f32x16 s0, s1;
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++) {
+        const half8 f = *reinterpret_cast<const half8 *>(s_kv[0][kp] + ka[ks]);
+        s0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qh[ks], ks ? s0 : f32x16{}, 0, 0, 0);
+        s0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, ql[ks], s0, 0, 0, 0);
+    }
+    // two stages at a time, both kinds of step passing one barrier a stage: a wave's blocks may be masked where another's
+    // are not
+    auto whole = [&](int st) { return WP * st + kp < nb && row.all_see(a, KB * blk.at(WP * st + kp)); };
+    for (int st = 0; st < n_stage;) {
+        for (; st + 1 < n_stage && whole(st) && whole(st + 1); st += 2) {
+            step(st, 0, s0, s1, std::false_type{});
+            step(st + 1, 1, s1, s0, std::false_type{});
+        }
+        for (int e = st + 2; st < min(e, n_stage); st++) {
+            step(st, st & 1, s0, s1, std::true_type{});
+            s0 = s1;
+        }
     }
     l = pair_sum<32>(l);
 
-    // the parts' sums through LDS, tile by tile of 32 dims: wave (rt, kp) leaves its tile u, then every wave adds its share
-    // (8 / KP … of the tile's dims) of its row tile's rows
-    if constexpr (KP > 1) {
-        if (hf == 0) s_ml[wave][0][c] = m, s_ml[wave][1][c] = l;
-        __syncthreads();
-        float w[KP], lsum = 0.0f, top = M_NONE;
+    // the key parts of each row tile through LDS (the stage buffers, once every wave is done with them): every wave leaves
+    // its sums as its lanes hold them, then wave (rt, kp) finishes dims 64kp … of its tile's rows
+    __syncthreads();
+    float4 *so = reinterpret_cast<float4 *>(&s_kv[0][0][0]);  // [wave][tile][register / 4][lane]
 #pragma unroll
-        for (int p = 0; p < KP; p++) top = fmaxf(top, s_ml[p * WR + rt][0][c]);
+    for (int u = 0; u < 4; u++)
 #pragma unroll
-        for (int p = 0; p < KP; p++) {
-            w[p] = __builtin_amdgcn_exp2f((s_ml[p * WR + rt][0][c] - top) * sc);
-            lsum = fmaf(s_ml[p * WR + rt][1][c], w[p], lsum);
+        for (int x = 0; x < 4; x++)
+            so[((wave * 4 + u) * 4 + x) * 64 + lane] = make_float4(o[u][4 * x], o[u][4 * x + 1], o[u][4 * x + 2], o[u][4 * x + 3]);
+    if (hf == 0) s_ml[wave][0][c] = m, s_ml[wave][1][c] = l;
+    __syncthreads();
+    if (row.r >= rows) return;
+    const float m0 = s_ml[rt][0][c], m1 = s_ml[WR + rt][0][c], top = fmaxf(m0, m1);
+    float w0 = __builtin_amdgcn_exp2f((m0 - top) * sc), w1 = __builtin_amdgcn_exp2f((m1 - top) * sc);
+    const float sum = fmaf(s_ml[rt][1][c], w0, s_ml[WR + rt][1][c] * w1), inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key: zeros
+    float *orow = a.out + ((size_t)row.t * a.n_head + row.head) * D + 64 * kp + 4 * hf;
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const float4 y0 = so[((rt * 4 + 2 * kp + u) * 4 + x) * 64 + lane], y1 = so[(((WR + rt) * 4 + 2 * kp + u) * 4 + x) * 64 + lane];
+            *reinterpret_cast<float4 *>(orow + 32 * u + 8 * x) =
+                make_float4(fmaf(y0.x, w0, y1.x * w1) * inv, fmaf(y0.y, w0, y1.y * w1) * inv,
+                            fmaf(y0.z, w0, y1.z * w1) * inv, fmaf(y0.w, w0, y1.w * w1) * inv);
         }
-        m = top, l = lsum;
-        const float mine = w[kp];
-        float *s_o = reinterpret_cast<float *>(&s_kv[0][0]);  // [wave][register][lane], one dim tile at a time
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-#pragma unroll
-            for (int x = 0; x < 16; x++) s_o[(wave * 16 + x) * 64 + lane] = o[u][x] * mine;
-            __syncthreads();
-#pragma unroll
-            for (int x = 0; x < 16; x++) {
-                float v = 0.0f;
-#pragma unroll
-                for (int p = 0; p < KP; p++) v += s_o[((p * WR + rt) * 16 + x) * 64 + lane];
-                o[u][x] = v;
-            }
-            __syncthreads();
-        }
-    }
-    if (kp != 0 || r >= rows) return;
-    {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
-        float *orow = a.out + ((size_t)t * a.n_head + head) * D + 4 * hf;
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-#pragma unroll
-            for (int x = 0; x < 4; x++)
-                *reinterpret_cast<float4 *>(orow + 32 * u + 8 * x) =
-                    make_float4(o[u][4 * x] * inv, o[u][4 * x + 1] * inv, o[u][4 * x + 2] * inv, o[u][4 * x + 3] * inv);
-    }
 }
 
-template <bool TREE> int launch(htr_device *dev, Args &a, const TreeMask &tree, int max_blocks) {
+// the rows that the queries see, read back into room of the device's: from_row on after the first sink_rows
+int read_back(htr_device *dev, Args &a, int n_keys, int sink_rows, int from_row) {
+    const int first = std::min(sink_rows, n_keys), rest = std::max(0, n_keys - from_row);
+    const size_t rows = (size_t)sink_rows + rest, bytes = rows * a.kv.n_kv * D * 2;
+    void *p;
+    HTR_TRY(htr_scratch_kept(dev, SCR_KV_ROWS, 2 * bytes, &p));
+    const HtrKvPlanes src = a.kv, dst{p, (char *)p + bytes, nullptr, nullptr, src.n_kv, (int)rows, false};
+    if (from_row == sink_rows) {
+        HTR_TRY(htr_kv_read_back(dev, src, 0, dst, 0, n_keys));
+    } else {
+        if (first) HTR_TRY(htr_kv_read_back(dev, src, 0, dst, 0, first));
+        if (rest) HTR_TRY(htr_kv_read_back(dev, src, from_row, dst, sink_rows, rest));
+    }
+    a.kv = dst, a.sink_rows = sink_rows, a.shift = from_row - sink_rows;
+    return 0;
+}
+
+// max_blocks: the most key blocks that 32 rows see; sink_rows, from_row: the rows 0 … sink_rows − 1 and from_row … (both
+// multiples of 32) hold all that is seen
+template <bool TREE> int launch(htr_device *dev, Args &a, const TreeMask &tree, int max_blocks, int sink_rows, int from_row) {
     const int rows = a.n * a.group;
     const int64_t groups = (int64_t)((rows + KB - 1) / KB) * a.kv.n_kv;
     if (groups >= 2 * dev->n_cu) {
-        constexpr int WR = 4;
         a.n_rg = (rows + KB * WR - 1) / (KB * WR), a.n_split = 1;
         const int64_t wide = (int64_t)a.n_rg * a.kv.n_kv;
         if (wide > INT32_MAX) return htr_fail("attention: %d rows of %d KV heads", rows, a.kv.n_kv);
-        if (a.kv.q8) hipLaunchKernelGGL((k_kv_attn<true, TREE, WR>), dim3((unsigned)wide), dim3(256), 0, dev->stream, a, tree);
-        else hipLaunchKernelGGL((k_kv_attn<false, TREE, WR>), dim3((unsigned)wide), dim3(256), 0, dev->stream, a, tree);
+        if (a.kv.q8) HTR_TRY(read_back(dev, a, TREE ? a.n_past + a.n : a.pos0 + a.n, sink_rows, from_row));
+        hipLaunchKernelGGL((k_kv_attn<TREE>), dim3((unsigned)wide), dim3(64 * WR * WP), 0, dev->stream, a, tree);
         return htr_launched(dev, "k_kv_attn");
     }
     a.n_rg = (rows + KB - 1) / KB;
-    // two workgroups a CU, no more parts than a wave has blocks
-    a.n_split = (int)std::max<int64_t>(1, std::min<int64_t>({2 * dev->n_cu / groups, (max_blocks + 3) / 4, MAX_SPLIT}));
+    // a workgroup a CU, no more parts than a wave has blocks
+    a.n_split = (int)std::max<int64_t>(1, std::min<int64_t>({dev->n_cu / groups, (max_blocks + SW - 1) / SW, MAX_SPLIT}));
+    a.xl = a.kv.n_kv % 8 == 0 && dev->xcd_round_robin == 1;
     if (a.n_split > 1) {
         void *p;
-        HTR_TRY(htr_scratch(dev, SCR_KV_TICKET, (size_t)2 * dev->n_cu * TICKET * 4, &p));
+        HTR_TRY(htr_scratch(dev, SCR_KV_TICKET, (size_t)dev->n_cu * TICKET * 4, &p));
         a.tickets = (uint32_t *)p;
-        HTR_TRY(htr_scratch(dev, SCR_KV_ATTN, (size_t)2 * dev->n_cu * KB * (D + 2) * 4, &p));
+        HTR_TRY(htr_scratch(dev, SCR_KV_ATTN, (size_t)dev->n_cu * KB * (D + 2) * 4, &p));
         a.part = (float *)p;
-        a.part_ml = (uint64_t *)(a.part + (size_t)2 * dev->n_cu * KB * D);
+        a.part_ml = (uint64_t *)(a.part + (size_t)dev->n_cu * KB * D);
     }
-    const dim3 g((unsigned)(groups * a.n_split)), b(256);
+    const dim3 g((unsigned)(groups * a.n_split)), b(64 * SW);
     if (a.kv.q8) hipLaunchKernelGGL((k_kv_attn_split<true, TREE>), g, b, 0, dev->stream, a, tree);
     else hipLaunchKernelGGL((k_kv_attn_split<false, TREE>), g, b, 0, dev->stream, a, tree);
-    return htr_launched(dev, "k_kv_attn_split");
+    return htr_launched(dev, a.kv.q8 ? "k_kv_attn_split<q8_0>" : "k_kv_attn_split<f16>");
 }
 
 int check_rows(const char *me, const float *d_q, size_t q_stride, const htr_kv *kv, int n_head, float *d_out, int64_t n) {
@@ -879,7 +903,7 @@ extern "C" int htr_tree_attention(htr_device *dev, const float *d_q, size_t q_st
     const HtrOnDevice on(dev);
     a.q = d_q, a.q_stride = q_stride, a.out = d_out, a.n = n, a.n_head = n_head, a.group = n_head / kv->n_kv;
     a.scale = scale, a.n_past = n_past;
-    return launch<true>(dev, a, tree, (n_past + n + KB - 1) / KB);
+    return launch<true>(dev, a, tree, (n_past + n + KB - 1) / KB, 0, 0);
 }
 
 extern "C" int htr_window_attention(htr_device *dev, const float *d_q, size_t q_stride, int n_q, int pos0, int window,
@@ -895,7 +919,8 @@ extern "C" int htr_window_attention(htr_device *dev, const float *d_q, size_t q_
     const HtrOnDevice on(dev);
     a.q = d_q, a.q_stride = q_stride, a.out = d_out, a.n = n_q, a.n_head = n_head, a.group = n_head / kv->n_kv;
     a.scale = scale, a.pos0 = pos0, a.window = window, a.n_sink = n_sink;
-    // the most blocks that a tile of 32 rows sees
-    const int64_t n_keys = pos0 + n_q, span = std::min<int64_t>(n_keys, (int64_t)window + std::min(n_sink, pos0 + n_q) + 96);
-    return launch<false>(dev, a, TreeMask{}, (int)((span + KB - 1) / KB));
+    const int n_keys = pos0 + n_q, sink = std::min(n_sink, n_keys), sink_rows = (sink + KB - 1) / KB * KB;
+    const int from = window > pos0 ? 0 : (pos0 - window + 1) / KB * KB;
+    const int64_t span = std::min<int64_t>(n_keys, (int64_t)window + sink + 3 * KB);  // of 32 rows' queries
+    return launch<false>(dev, a, TreeMask{}, (int)((span + KB - 1) / KB), sink_rows, std::max(from, sink_rows));
 }

@@ -328,6 +328,16 @@ int htr_kv_check(const char *what, const htr_kv *kv, HtrKvPlanes *out) {
     return 0;
 }
 
+namespace {
+dim3 copy_grid(const CopyArgs &a) { return dim3((unsigned)((a.n + COPY_ROWS - 1) / COPY_ROWS), (unsigned)(2 * a.src.n_kv)); }
+}  // namespace
+
+int htr_kv_read_back(htr_device *dev, const HtrKvPlanes &src, int src_row, const HtrKvPlanes &dst, int dst_row, int n) {
+    const CopyArgs a{src, dst, src_row, dst_row, n};
+    hipLaunchKernelGGL(k_kv_read_back, copy_grid(a), dim3(256), 0, dev->stream, a);
+    return htr_launched(dev, "k_kv_read_back");
+}
+
 extern "C" int htr_tree_masks(const int32_t *h_parent, int n, uint64_t *h_mask, int32_t *h_depth) {
     if (!h_parent || !h_mask || !h_depth) return htr_fail("htr_tree_masks: null argument");
     if (n < 1 || n > HTR_TREE_MAX) return htr_fail("htr_tree_masks: %d nodes (1 … %d)", n, HTR_TREE_MAX);
@@ -425,15 +435,12 @@ extern "C" int htr_kv_copy(htr_device *dev, const htr_kv *src, int src_row, cons
     if (n == 0) return 0;
     const HtrOnDevice on(dev);
     a.src_row = src_row, a.dst_row = dst_row, a.n = n;
-    const dim3 g((unsigned)((n + COPY_ROWS - 1) / COPY_ROWS), (unsigned)(2 * src->n_kv)), b(256);
+    const dim3 g = copy_grid(a), b(256);
     if (!a.src.q8 && a.dst.q8) {
         hipLaunchKernelGGL(k_kv_quantise, g, b, 0, dev->stream, a);
         return htr_launched(dev, "k_kv_quantise");
     }
-    if (a.src.q8 && !a.dst.q8) {
-        hipLaunchKernelGGL(k_kv_read_back, g, b, 0, dev->stream, a);
-        return htr_launched(dev, "k_kv_read_back");
-    }
+    if (a.src.q8 && !a.dst.q8) return htr_kv_read_back(dev, a.src, src_row, a.dst, dst_row, n);
     if (a.src.q8) hipLaunchKernelGGL(k_kv_copy<true>, g, b, 0, dev->stream, a);
     else hipLaunchKernelGGL(k_kv_copy<false>, g, b, 0, dev->stream, a);
     return htr_launched(dev, a.src.q8 ? "k_kv_copy<q8_0>" : "k_kv_copy<f16>");

@@ -359,6 +359,18 @@ int htr_scratch(htr_device *dev, int slot, size_t bytes, void **out) {
     return 0;
 }
 
+int htr_scratch_kept(htr_device *dev, int slot, size_t bytes, void **out) {
+    if (dev->scratch_bytes[slot] < bytes) {
+        const size_t b = std::max({bytes, 2 * dev->scratch_bytes[slot], (size_t)32 << 20});
+        void *p;
+        HTR_TRY(alloc_filled(dev, b, HTR_MEM_WORK, false, &p));
+        dev->scratch[slot] = p;
+        dev->scratch_bytes[slot] = b;
+    }
+    *out = dev->scratch[slot];
+    return 0;
+}
+
 extern "C" int htr_mem_live(htr_device *dev, htr_gpu_bytes *out) {
     if (!dev || !out) return htr_fail("htr_mem_live: null argument");
     *out = dev->live;
