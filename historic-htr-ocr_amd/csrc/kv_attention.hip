@@ -38,6 +38,7 @@ constexpr int MAX_SPLIT = 64, TICKET = 32;     // parts of a row group's blocks;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float float2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef __fp16 fp16x4 __attribute__((ext_vector_type(4)));
@@ -56,9 +57,9 @@ struct Args {
     int n_past;                // tree: the committed keys
     int pos0, window, n_sink;  // window
     int n_rg, n_split;         // row groups, parts of a row group's key blocks
-    float *part;               // [n_kv·n_rg·n_split][32] rows of partial sums o[128], and each row's (m, l)
-    uint64_t *part_ml;
-    uint32_t *tickets;         // [n_kv·n_rg], TICKET words apart: zero, self-resetting
+    float *part;               // [n_kv·n_rg·n_split][16·RT] rows of partial sums o[128], and each row's (m, l, c)
+    float4 *part_ml;
+    uint32_t *tickets;         // [n_kv·n_rg], TICKET words apart: zero, self-resetting; NULL: joined by a second launch
     int xl;                    // a KV head's workgroups share an XCD, and its L2 shows them each other's stores
 };
 struct TreeMask {
@@ -118,46 +119,46 @@ __device__ __forceinline__ float2 get64(const void *p) {
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
-// the key blocks that some row of queries ta … tb sees: the blocks 0 … first − 1, then from … to − 1
+// the blocks of U keys that some row of queries ta … tb sees: the blocks 0 … first − 1, then from … to − 1
 struct Blocks {
     int first, from, to;
     __device__ __forceinline__ int count() const { return first + max(0, to - from); }
     __device__ __forceinline__ int at(int i) const { return i < first ? i : from + (i - first); }
 };
-template <bool TREE> __device__ __forceinline__ Blocks blocks_of(const Args &a, int ta, int tb) {
+template <bool TREE, int U> __device__ __forceinline__ Blocks blocks_of(const Args &a, int ta, int tb) {
     if constexpr (TREE) {
-        return Blocks{0, 0, (a.n_past + a.n + KB - 1) / KB};
+        return Blocks{0, 0, (a.n_past + a.n + U - 1) / U};
     } else {
-        const int pa = a.pos0 + ta, pb = a.pos0 + tb, to = pb / KB + 1;
-        const int first = min((min(a.n_sink, pb + 1) + KB - 1) / KB, to), lo = a.window > pa ? 0 : (pa - a.window + 1) / KB;
+        const int pa = a.pos0 + ta, pb = a.pos0 + tb, to = pb / U + 1;
+        const int first = min((min(a.n_sink, pb + 1) + U - 1) / U, to), lo = a.window > pa ? 0 : (pa - a.window + 1) / U;
         return Blocks{first, max(first, lo), to};
     }
 }
 
-// one lane's row: query t, its head, and the keys it sees; and what every row of its wave's tile of 32 sees
+// one row: query t, its head, and the keys it sees
 template <bool TREE> struct Row {
-    int r, t, head, pos, tile_a, tile_b;
+    int r, t, head, pos;
     uint64_t mask;
-    __device__ __forceinline__ Row(const Args &a, const TreeMask &tree, int kvh, int r0, int c) {
-        const int last = a.n * a.group - 1, rc = min(r0 + c, last);
-        r = r0 + c, t = rc / a.group, head = kvh * a.group + rc % a.group, pos = a.pos0 + t;
-        tile_a = min(r0, last) / a.group, tile_b = min(r0 + 31, last) / a.group;
+    __device__ __forceinline__ Row(const Args &a, const TreeMask &tree, int kvh, int row) {
+        const int rc = min(row, a.n * a.group - 1);
+        r = row, t = rc / a.group, head = kvh * a.group + rc % a.group, pos = a.pos0 + t;
         mask = 0;
         if constexpr (TREE) mask = tree.of[t];
     }
-    __device__ __forceinline__ bool sees(const Args &a, int key) const {
-        if constexpr (TREE) {
-            const unsigned j = (unsigned)(key - a.n_past);
-            return key < a.n_past || (j < 64u && ((mask >> j) & 1) != 0);
-        } else {
-            return key <= pos && (key < a.n_sink || key > pos - a.window);
-        }
-    }
-    __device__ __forceinline__ bool all_see(const Args &a, int k0) const {
-        if constexpr (TREE) return k0 + KB <= a.n_past;
-        else return k0 + KB - 1 <= a.pos0 + tile_a && (k0 + KB <= a.n_sink || k0 > a.pos0 + tile_b - a.window);
-    }
 };
+template <bool TREE> __device__ __forceinline__ bool sees(const Args &a, int pos, uint64_t mask, int key) {
+    if constexpr (TREE) {
+        const unsigned j = (unsigned)(key - a.n_past);
+        return key < a.n_past || (j < 64u && ((mask >> j) & 1) != 0);
+    } else {
+        return key <= pos && (key < a.n_sink || key > pos - a.window);
+    }
+}
+// whether the queries ta … tb all see the keys k0 … k0 + U − 1
+template <bool TREE, int U> __device__ __forceinline__ bool all_see(const Args &a, int ta, int tb, int k0) {
+    if constexpr (TREE) return k0 + U <= a.n_past;
+    else return k0 + U - 1 <= a.pos0 + ta && (k0 + U <= a.n_sink || k0 > a.pos0 + tb - a.window);
+}
 
 // p − (float)h for the low (0) or high (1) half of h: one mixed-precision fma
 template <int HI> __device__ __forceinline__ float minus_half(float p, uint32_t h) {
@@ -174,28 +175,30 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     __builtin_memcpy(&lo, &r, 4);
 }
 
-// a row's q·scale as f16 pairs, the B operand of step ks = dims 16ks + 8hf … + 7; the factor of its scores
-__device__ __forceinline__ float q_pairs(const float *qrow, float scale, half8 (&qh)[8], half8 (&ql)[8]) {
-    float x[8][8], top = 0.0f;
+// a row's q·scale as f16 pairs, the B operand of steps of 128 / N dims (the lane's first 8 dims at qrow, of `G` lanes that
+// hold the row); the factor of its scores
+template <int N, int G> __device__ __forceinline__ float q_pairs(const float *qrow, float scale, half8 (&qh)[N], half8 (&ql)[N]) {
+    float x[N][8], top = 0.0f;
 #pragma unroll
-    for (int ks = 0; ks < 8; ks++) {
-        const float4 a0 = *reinterpret_cast<const float4 *>(qrow + 16 * ks);
-        const float4 a1 = *reinterpret_cast<const float4 *>(qrow + 16 * ks + 4);
+    for (int ks = 0; ks < N; ks++) {
+        const float4 a0 = *reinterpret_cast<const float4 *>(qrow + D / N * ks);
+        const float4 a1 = *reinterpret_cast<const float4 *>(qrow + D / N * ks + 4);
         x[ks][0] = a0.x, x[ks][1] = a0.y, x[ks][2] = a0.z, x[ks][3] = a0.w;
         x[ks][4] = a1.x, x[ks][5] = a1.y, x[ks][6] = a1.z, x[ks][7] = a1.w;
     }
 #pragma unroll
-    for (int ks = 0; ks < 8; ks++)
+    for (int ks = 0; ks < N; ks++)
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             x[ks][e] *= scale;
             top = fmaxf(top, fabsf(x[ks][e]));
         }
+    if constexpr (G == 4) top = pair_max<16>(top);
     // (a row of nothing but tiny values: its scores are 0 to f32 either way, and the factor stays a normal number)
     const int ex = max(__builtin_amdgcn_frexp_expf(pair_max<32>(top)), -100);
     const float up = ldexpf(1.0f, 10 - ex);
 #pragma unroll
-    for (int ks = 0; ks < 8; ks++) {
+    for (int ks = 0; ks < N; ks++) {
         uint32_t h[4], r[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) split2(x[ks][2 * e] * up, x[ks][2 * e + 1] * up, h[e], r[e]);
@@ -248,6 +251,400 @@ template <typename F> __device__ __forceinline__ void put_nan(f32x16 (&o)[4], ui
     }
 }
 
+// ---- few rows: the keys split over workgroups --------------------------------------------------------------------------------
+//
+// A workgroup takes 16·RT rows (RT 1 or 2) and a run of units of 16 keys, eight a round, one to each of its eight waves:
+//   scores   a wave's own unit against all rows, Sᵀ = K·(qh + ql)ᵀ by v_mfma_f32_16x16x32_f16: lane 16g + c holds row c's
+//            scores of keys 4g … 4g + 3; the rows' largest over the waves through LDS (barrier);
+//   weights  p = 2^((s − m)·c + 3) as f16 pairs to LDS, in the order of the next products' operands (barrier);
+//   values   Oᵀ += Vᵀ·(ph + pl)ᵀ over the round's 128 keys, a wave's own 16 dims. So every K and V value is loaded, and made
+//            f16, once for all the rows, no sums of O are merged between waves, and O is 8 registers at most.
+// K and V come straight into LDS, a wave's own unit each: K into one buffer (read by that wave alone, filled again once the
+// scores are taken), V into one of two (filled again when all waves are past the values of the round before). q8_0 units as
+// they are, int8: an operand's 8 quants become f16 in registers (14 VALU instructions), V's by a transposing read of bytes,
+// their scales from LDS in the order of the operand's slots.
+//   f16   [16 keys][16 chunks of 16 bytes], K row r's chunk c at 16r + (c ^ r), V's at 16r + (c ^ 2(r % 8));
+//   q8_0  [16 keys][8 chunks], row r's chunk c at 8r + (c ^ r / 2); the scales [16 keys][4]:
+// reads of 16 (32) lanes fall on different bank groups.
+// Where the keys are split, a part's (m, l, c) and O go to memory; few of them are joined by the row group's workgroup that is
+// the last there (a ticket), many by a second launch.
+constexpr int SW = 8, UK = 16, ST = SW / 2;  // waves; keys of a unit; steps of 32 keys of a round
+constexpr int JOIN_HERE = 256;               // rows × parts that the last workgroup joins itself
+
+struct JoinArgs {
+    const float *part;
+    const float4 *part_ml;
+    float *out;
+    int n_split, n_head, group, rows, n_kv, n_rg, tile;  // tile: rows of a row group's part
+};
+
+// one row's parts g, g + G, … joined by 32 lanes of 4 dims each; s_w: 64 words of the group's own. Returns Σ l
+__device__ __forceinline__ float join_row(const float *part, const float4 *part_ml, size_t first, size_t step, int ns, int g, int G,
+                                          float *s_w, int lane, float4 &y) {
+    const int j = lane & 31;
+    const float *from = part + first * D + 4 * j;
+    float2 in[8][2];
+    auto fetch = [&](int p0) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float *at = from + (size_t)min(p0 + e * G, ns - 1) * step * D;
+            in[e][0] = get64(at), in[e][1] = get64(at + 2);
+        }
+    };
+    fetch(g);
+    float m[2], l[2], top = M_NONE, sum = 0.0f, c = 1.0f;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const float4 *at = part_ml + first + (size_t)min(j + 32 * e, ns - 1) * step;
+        const float2 ml = get64(at);
+        c = get64(&at->z).x;
+        m[e] = j + 32 * e < ns ? ml.x : M_NONE, l[e] = j + 32 * e < ns ? ml.y : 0.0f;
+        top = fmaxf(top, m[e]);
+    }
+    top = group_max<16>(top, lane);
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const float w = __builtin_amdgcn_exp2f((m[e] - top) * c);
+        sum = fmaf(l[e], w, sum);
+        s_w[j + 32 * e] = j + 32 * e < ns ? w : 0.0f;
+    }
+    sum = group_sum<16>(sum, lane);
+    __builtin_amdgcn_wave_barrier();
+    y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p = g;;) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float w = p + e * G < ns ? s_w[p + e * G] : 0.0f;
+            y.x = fmaf(in[e][0].x, w, y.x), y.y = fmaf(in[e][0].y, w, y.y);
+            y.z = fmaf(in[e][1].x, w, y.z), y.w = fmaf(in[e][1].y, w, y.w);
+        }
+        p += 8 * G;
+        if (p >= ns) break;
+        fetch(p);
+    }
+    __builtin_amdgcn_wave_barrier();
+    return sum;
+}
+__device__ __forceinline__ void put_row(float *out, int n_head, int group, int kvh, int r, int j, float4 y, float sum) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
+    const int t = r / group, head = kvh * group + r % group;
+    *reinterpret_cast<float4 *>(out + ((size_t)t * n_head + head) * D + 4 * j) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+}
+
+// the second launch: two rows a workgroup, four groups of 32 lanes to a row's parts
+__global__ __launch_bounds__(256) void k_kv_attn_join(JoinArgs a) {
+    __shared__ float s_w[8][MAX_SPLIT];
+    __shared__ float4 s_y[8][32];
+    const int gr = threadIdx.x >> 5, j = threadIdx.x & 31, g = gr & 3;
+    const int id = min((int)blockIdx.x * 2 + (gr >> 2), a.rows * a.n_kv - 1);
+    const int kvh = id / a.rows, r = id % a.rows, rg = r / a.tile;
+    float4 y;
+    const float sum = join_row(a.part, a.part_ml, ((size_t)kvh * a.n_rg + rg) * a.n_split * a.tile + r % a.tile, a.tile, a.n_split, g, 4,
+                               s_w[gr], threadIdx.x & 63, y);
+    s_y[gr][j] = y;
+    __syncthreads();
+    if (g != 0 || (int)blockIdx.x * 2 + (gr >> 2) >= a.rows * a.n_kv) return;
+#pragma unroll
+    for (int e = 1; e < 4; e++) {
+        const float4 z = s_y[gr + e][j];
+        y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+    }
+    put_row(a.out, a.n_head, a.group, kvh, r, j, y, sum);
+}
+
+// the last workgroup of a row group to have stored its part joins them all (tile: rows of a part, the group's first at g0);
+// s_y: room for a float4 a thread
+__device__ __forceinline__ void join_last(const Args &a, int kvh, int rg, int r0, int rows, int tile, size_t g0, int *s_last,
+                                          float (&s_w)[2 * SW][MAX_SPLIT], float4 *s_y) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's stores are performed
+    __syncthreads();
+    uint32_t *ticket = a.tickets + TICKET * ((size_t)kvh * a.n_rg + rg);
+    if (tid == 0)
+        *s_last = (a.xl ? __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)
+                        : __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) ==
+                  (uint32_t)(a.n_split - 1);
+    __syncthreads();
+    if (!*s_last) return;
+    // 32 lanes a row; where the rows are fewer than the groups of lanes, several groups to a row's parts
+    const int nr = min(tile, rows - r0), gr = tid >> 5, j = tid & 31;
+    const int lg = nr > 8 ? 4 : nr > 4 ? 3 : nr > 2 ? 2 : nr > 1 ? 1 : 0, G = 16 >> lg;
+    for (int rb = 0; rb < nr; rb += 1 << lg) {
+        const int ri = rb + (gr & ((1 << lg) - 1)), part = gr >> lg;
+        float4 y;
+        const float sum = join_row(a.part, a.part_ml, g0 + min(ri, nr - 1), tile, a.n_split, part, G, s_w[gr], lane, y);
+        if (G > 1) {  // (one pass)
+            s_y[tid] = y;
+            __syncthreads();
+            if (part == 0)
+                for (int e = 1; e < G; e++) {
+                    const float4 z = s_y[tid + 32 * (e << lg)];
+                    y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+                }
+        }
+        if (part == 0 && ri < nr) put_row(a.out, a.n_head, a.group, kvh, r0 + ri, j, y, sum);
+    }
+    if (tid == 0) {  // for the next call
+        if (a.xl) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        else __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+
+template <bool Q8, bool TREE, int RT> __global__ __launch_bounds__(64 * SW, 2) void k_kv_attn_few(Args a, TreeMask tree) {
+    constexpr int UC = Q8 ? 8 * UK : 16 * UK;                        // 16-byte chunks of a unit's K or V
+    constexpr int NL = Q8 ? UK / 8 + 1 : UK / 4;                     // loads of a unit's K or V
+    __shared__ __attribute__((aligned(16))) uint4_t s_k[SW][UC], s_v[2][SW][UC];
+    __shared__ __attribute__((aligned(16))) uint4_t s_p[2][RT][ST][64];  // weights' high and low halves
+    __shared__ __attribute__((aligned(16))) uint32_t s_kd[Q8 ? SW : 1][64], s_vd[2][Q8 ? SW : 1][64];
+    __shared__ __attribute__((aligned(16))) uint16_t s_vt[4][ST][4][8];  // V's scales by dims / 32, step, lane group, slot
+    __shared__ float s_mx[SW][16 * RT], s_l[SW][16 * RT];
+    __shared__ float s_w[SW * 2][MAX_SPLIT];
+    __shared__ int s_last;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, c = lane & 15;
+    const int kvh = blockIdx.x % a.kv.n_kv, rest = blockIdx.x / a.kv.n_kv;
+    const int split = rest % a.n_split, rg = rest / a.n_split;
+    const int rows = a.n * a.group, r0 = rg * 16 * RT;
+    const int n_keys = TREE ? a.n_past + a.n : a.pos0 + a.n;
+    const int ta = r0 / a.group, tb = min(r0 + 16 * RT - 1, rows - 1) / a.group;
+    const Blocks blk = blocks_of<TREE, UK>(a, ta, tb);
+    const int nu = blk.count(), i0 = (int)((int64_t)nu * split / a.n_split), i1 = (int)((int64_t)nu * (split + 1) / a.n_split);
+    const int n_round = (i1 - i0 + SW - 1) / SW;
+    const size_t head0 = (size_t)kvh * a.kv.n_ctx;
+
+    // the unit i (one past the part's end: the last's, masked) of K, or of V into buffer b; a wave's instruction is 4 (8) whole
+    // rows. Rows past the last key are the last key's, and masked
+    const uint32_t kx = 16 * ((lane & 15) ^ (lane >> 4)), vx = 16 * ((lane & 15) ^ (2 * (lane >> 4))), r4 = 2 * D * (lane >> 4);
+    const uint32_t bx = 16 * ((lane & 7) ^ (lane >> 4)), r8 = D * (lane >> 3);
+    auto lds_of = [](auto &x) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)(char *)&x; };
+    auto load = [&](int i, bool is_v, int b) {
+        const int k0 = UK * blk.at(min(i, i1 - 1)), last = min(n_keys - 1 - k0, UK - 1);
+        const size_t row = head0 + k0;
+        const uint32_t to = is_v ? lds_of(s_v[b][wave]) : lds_of(s_k[wave]);
+        const char *base = (const char *)(is_v ? a.kv.v : a.kv.k) + row * (Q8 ? D : 2 * D);
+        if constexpr (Q8) {
+            lds_load4((is_v ? a.kv.vd : a.kv.kd) + row * 4, 8 * min((lane & 31) >> 1, last) + 4 * (lane & 1),
+                      is_v ? lds_of(s_vd[b][wave]) : lds_of(s_kd[wave]));
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                lds_load16(base, min(r8 + 8 * D * u, (uint32_t)(D * last)) + (bx ^ (64 * (u & 1))), to + 16 * 64 * u);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                lds_load16(base, min(r4 + 4 * 2 * D * u, (uint32_t)(2 * D * last)) + (is_v ? vx ^ (128 * (u & 1)) : kx ^ (64 * (u & 3))),
+                           to + 16 * 64 * u);
+        }
+    };
+    if (n_round > 0) {
+        load(i0 + wave, false, 0);
+        load(i0 + wave, true, 0);
+    }
+
+    half8 qh[RT][4], ql[RT][4];
+    float sc[RT], m[RT], l[RT];
+    int pos[RT];
+    uint64_t mask[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const Row<TREE> row(a, tree, kvh, r0 + 16 * rt + c);
+        pos[rt] = row.pos, mask[rt] = row.mask;
+        sc[rt] = q_pairs<4, 4>(a.q + (size_t)row.t * a.q_stride + (size_t)row.head * D + 8 * g, a.scale, qh[rt], ql[rt]);
+        m[rt] = M_NONE, l[rt] = 0.0f;
+    }
+    // the lane's place in V's units: slots 8g … are keys 4g … 4g + 3 of a step's first unit, then of its second
+    const int vrow = Q8 ? 4 * g + ((c >> 1) & 3) : 4 * g + (c >> 2);
+    f32x4 o[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) o[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    auto round = [&](int rd, auto is_masked) {
+        constexpr bool MASK = decltype(is_masked)::value;
+        const int i = i0 + SW * rd + wave, b = rd & 1;
+        const bool more = rd + 1 < n_round;
+        wait_loads<NL>();  // K; V is still on its way
+        f32x4 s[RT];
+        {
+            half8 f[4];
+            if constexpr (Q8) {
+                const uint2_t dk = reinterpret_cast<const uint2_t *>(s_kd[wave])[c];
+                half2_t d2[2];
+                __builtin_memcpy(d2, &dk, 8);
+#pragma unroll
+                for (int ks = 0; ks < 4; ks++) {
+                    const uint2_t w = *reinterpret_cast<const uint2_t *>((const char *)(s_k[wave] + 8 * c + ((2 * ks + (g >> 1)) ^ (c >> 1))) + 8 * (g & 1));
+                    const _Float16 d = d2[ks >> 1][ks & 1];
+                    f[ks] = dequant8(w[0], w[1], half2_t{d, d});
+                }
+            } else {
+#pragma unroll
+                for (int ks = 0; ks < 4; ks++) f[ks] = *reinterpret_cast<const half8 *>(s_k[wave] + 16 * c + ((4 * ks + g) ^ c));
+            }
+            wait_reads();
+            if (more) load(i + SW, false, 0);
+#pragma unroll
+            for (int ks = 0; ks < 4; ks++)
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[ks], qh[rt][ks], ks ? s[rt] : f32x4{}, 0, 0, 0);
+                    s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[ks], ql[rt][ks], s[rt], 0, 0, 0);
+                }
+        }
+        uint32_t seen[RT];
+        if constexpr (MASK) {
+            const int k0 = UK * blk.at(min(i, i1 - 1)) + here(4 * g);
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                seen[rt] = 0;
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const bool v = i < i1 && sees<TREE>(a, pos[rt], mask[rt], k0 + x);
+                    seen[rt] |= (uint32_t)v << x;
+                    s[rt][x] = v ? s[rt][x] : -INFINITY;
+                }
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const float mx = pair_max<32>(pair_max<16>(fmaxf(fmaxf(s[rt][0], s[rt][1]), fmaxf(s[rt][2], s[rt][3]))));
+            if (g == 0) s_mx[wave][16 * rt + c] = mx;
+        }
+        wait_reads();
+        __builtin_amdgcn_s_barrier();  // everyone's largest scores; everyone is past the values of the round before
+        asm volatile("" ::: "memory");
+        if (more) load(i + SW, true, b ^ 1);
+        float mx[RT];
+        bool far = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            mx[rt] = s_mx[0][16 * rt + c];
+#pragma unroll
+            for (int w = 1; w < SW; w++) mx[rt] = fmaxf(mx[rt], s_mx[w][16 * rt + c]);
+            far |= (mx[rt] - m[rt]) * sc[rt] > P_ROOM;
+        }
+        if (__builtin_amdgcn_ballot_w64(far)) {  // (alike in every wave)
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                const float to = fmaxf(m[rt], mx[rt]), corr = __builtin_amdgcn_exp2f((m[rt] - to) * sc[rt]);
+                m[rt] = to;
+                l[rt] *= corr;
+                o[rt] *= corr;
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            float p[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) p[x] = __builtin_amdgcn_exp2f(fmaf(s[rt][x] - m[rt], sc[rt], P_SHIFT));  // not seen: 2^(−∞) = 0
+            l[rt] += (p[0] + p[1]) + (p[2] + p[3]);
+            uint32_t h[2], r[2];
+            split2(p[0], p[1], h[0], r[0]);
+            split2(p[2], p[3], h[1], r[1]);
+            if constexpr (MASK) {  // (a weight's sign: not seen)
+                h[0] |= (seen[rt] & 1 ? 0u : 0x8000u) | (seen[rt] & 2 ? 0u : 0x80000000u);
+                h[1] |= (seen[rt] & 4 ? 0u : 0x8000u) | (seen[rt] & 8 ? 0u : 0x80000000u);
+            }
+            reinterpret_cast<uint2_t *>(&s_p[0][rt][wave >> 1][lane])[wave & 1] = uint2_t{h[0], h[1]};
+            reinterpret_cast<uint2_t *>(&s_p[1][rt][wave >> 1][lane])[wave & 1] = uint2_t{r[0], r[1]};
+        }
+        if (more) wait_loads<2 * NL>();  // V
+        else wait_loads<0>();
+        if constexpr (Q8)
+            if (lane < 32) {  // V's scales into the order of the operands' slots
+                const uint32_t d2 = s_vd[b][wave][lane];
+                const int key = lane >> 1, at = 4 * (wave & 1) + (key & 3);
+                s_vt[2 * (lane & 1)][wave >> 1][key >> 2][at] = (uint16_t)d2;
+                s_vt[2 * (lane & 1) + 1][wave >> 1][key >> 2][at] = (uint16_t)(d2 >> 16);
+            }
+        wait_reads();
+        __builtin_amdgcn_s_barrier();  // everyone's weights and V
+        asm volatile("" ::: "memory");
+        auto vread = [&](int st) {  // Vᵀ of step st, the wave's dims
+            half8 v;
+            if constexpr (Q8) {
+                const uint4_t *unit = s_v[b][2 * st] + UC * ((c >> 3) & 1);
+                const auto *p = (const __attribute__((address_space(3))) char *)(unit + 8 * vrow + (wave ^ (vrow >> 1))) + 8 * (c & 1);
+                const int2_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2_t *)p);
+                v = dequant8((uint32_t)w[0], (uint32_t)w[1], *reinterpret_cast<const half8 *>(s_vt[wave >> 1][st][g]));
+            } else {
+                const int at = 16 * vrow + ((2 * wave + ((c >> 1) & 1)) ^ (2 * (vrow & 7)));
+                const auto *p = (const __attribute__((address_space(3))) char *)(s_v[b][2 * st] + at) + 8 * (c & 1);
+                const fp16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)p);
+                const fp16x4 up = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)(p + 16 * UC));
+                __builtin_memcpy(&v, &lo, 8);
+                __builtin_memcpy((char *)&v + 8, &up, 8);
+            }
+            return v;
+        };
+        uint32_t odd = 0;
+#pragma unroll
+        for (int st = 0; st < ST; st++) {
+            half8 v = vread(st);
+            if constexpr (MASK) v = finite(v, odd);
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, *reinterpret_cast<const half8 *>(&s_p[0][rt][st][lane]), o[rt], 0, 0, 0);
+                o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, *reinterpret_cast<const half8 *>(&s_p[1][rt][st][lane]), o[rt], 0, 0, 0);
+            }
+        }
+        if constexpr (MASK)
+            if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+                // NaN into the sums of the rows that see a value that is not finite: a product of ones
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int st = 0; st < ST; st++) {
+                        uint4_t h = s_p[0][rt][st][lane];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) h[e] = ((~h[e] >> 15) & 0x00010001u) * 0x3C00u;
+                        half8 ind;
+                        __builtin_memcpy(&ind, &h, 16);
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones_of_not_finite(vread(st)), ind, t, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; x++) o[rt][x] = t[x] > 0.0f ? NAN : o[rt][x];
+                }
+            }
+    };
+    // whether every row sees all keys of the round's units
+    auto whole = [&](int rd) {
+        const int i = i0 + SW * rd + (lane & 7);
+        return __builtin_amdgcn_ballot_w64(!(i < i1 && all_see<TREE, UK>(a, ta, tb, UK * blk.at(min(i, i1 - 1))))) == 0;
+    };
+    for (int rd = 0; rd < n_round;) {
+        for (bool all = whole(rd); all; all = rd < n_round && whole(rd)) round(rd++, std::false_type{});
+        for (bool some = rd < n_round; some; some = rd < n_round && !whole(rd)) round(rd++, std::true_type{});
+    }
+    // Σ l over the lanes and waves (m is the same in every wave)
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        l[rt] = pair_sum<32>(pair_sum<16>(l[rt]));
+        if (g == 0) s_l[wave][16 * rt + c] = l[rt];
+    }
+    __syncthreads();
+    const size_t g0 = ((size_t)kvh * a.n_rg + rg) * a.n_split * (16 * RT);  // the row group's first row of partial sums
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int r = r0 + 16 * rt + c;
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < SW; w++) sum += s_l[w][16 * rt + c];
+        if (r >= rows) continue;
+        if (a.n_split == 1) {
+            put_row(a.out, a.n_head, a.group, kvh, r, 4 * wave + g, make_float4(o[rt][0], o[rt][1], o[rt][2], o[rt][3]), sum);
+            continue;
+        }
+        const size_t pr = g0 + (size_t)split * (16 * RT) + 16 * rt + c;
+        float *to = a.part + pr * D + 16 * wave + 4 * g;
+        put64(to, o[rt][0], o[rt][1], a.xl);
+        put64(to + 2, o[rt][2], o[rt][3], a.xl);
+        if (wave == 0 && g == 0) {
+            put64(a.part_ml + pr, m[rt], sum, a.xl);
+            put64(&a.part_ml[pr].z, sc[rt], 0.0f, a.xl);
+        }
+    }
+    if (a.tickets) join_last(a, kvh, rg, r0, rows, 16 * RT, g0, &s_last, s_w, reinterpret_cast<float4 *>(&s_k[0][0]));
+}
+
 // ---- few rows: the blocks split over workgroups ----------------------------------------------------------------------------
 //
 // A workgroup takes 32 rows, each of its eight waves every eighth block of its part. A wave loads its own blocks straight
@@ -260,13 +657,13 @@ template <typename F> __device__ __forceinline__ void put_nan(f32x16 (&o)[4], ui
 //         as [dims / 32][key / 16][hf][8], the order of an operand's slots.
 // Reads of 16 (32) lanes then fall on different bank groups.
 constexpr int QT = 256 + 256 + 16 + 16;  // 16-byte chunks of a q8_0 buffer: K, V, K scales, V scales
-constexpr int SW = 8;                    // waves
 
 template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv_attn_split(Args a, TreeMask tree) {
     constexpr int WAVE = Q8 ? 2 * QT + 16 : TILE;  // chunks of a wave's LDS
+    static_assert(WAVE >= 1024, "a wave's sums fit");
     __shared__ __attribute__((aligned(16))) uint4_t s_kv[SW][WAVE];
     __shared__ float s_ml[SW][2][KB];
-    __shared__ float s_c[KB];
+    __shared__ float s_w[2 * SW][MAX_SPLIT];
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hf = lane >> 5, c = lane & 31;
@@ -274,7 +671,8 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     const int split = rest % a.n_split, rg = rest / a.n_split;
     const int rows = a.n * a.group, r0 = rg * KB;
     const int n_keys = TREE ? a.n_past + a.n : a.pos0 + a.n;
-    const Blocks blk = blocks_of<TREE>(a, r0 / a.group, min(r0 + KB - 1, rows - 1) / a.group);
+    const int ta = r0 / a.group, tb = min(r0 + KB - 1, rows - 1) / a.group;
+    const Blocks blk = blocks_of<TREE, KB>(a, ta, tb);
     const int nb = blk.count(), i0 = (int)((int64_t)nb * split / a.n_split), i1 = (int)((int64_t)nb * (split + 1) / a.n_split);
     const size_t head0 = (size_t)kvh * a.kv.n_ctx;
 
@@ -328,9 +726,15 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
         }
     }
 
-    const Row<TREE> row(a, tree, kvh, r0, c);
     half8 qh[8], ql[8];
-    const float sc = q_pairs(a.q + (size_t)row.t * a.q_stride + (size_t)row.head * D + 8 * hf, a.scale, qh, ql);
+    const Row<TREE> row(a, tree, kvh, r0 + c);
+    const float sc = q_pairs<8, 2>(a.q + (size_t)row.t * a.q_stride + (size_t)row.head * D + 8 * hf, a.scale, qh, ql);
+    float m = M_NONE, l = 0.0f;
+    f32x16 o[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int x = 0; x < 16; x++) o[u][x] = 0.0f;
 
     // the lane's places in a block: K step ks is key c, dims 16ks + 8hf …; V tile u, step ss, slots 8hf … + 7 are the keys
     // 16ss + 4hf … + 3, then 16ss + 8 + 4hf … + 3 (the lane's scores 8ss …) of dims 32u + 16(lane / 16 % 2) …
@@ -340,13 +744,6 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     for (int u = 0; u < 4; u++)
         va[u] = Q8 ? 16 * (256 + 8 * vrow + ((2 * u + ((lane >> 4) & 1)) ^ (vrow >> 1))) + 8 * (lane & 1)
                    : 16 * (K_CHUNKS + 16 * vrow + ((4 * u + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (2 * vrow))) + 8 * (lane & 1);
-
-    f32x16 o[4];
-#pragma unroll
-    for (int u = 0; u < 4; u++)
-#pragma unroll
-        for (int x = 0; x < 16; x++) o[u][x] = 0.0f;
-    float m = M_NONE, l = 0.0f;
 
     // block i; MASK: not every row sees all of it
     auto step = [&](auto is_masked) {
@@ -405,7 +802,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
             const int k0 = KB * blk.at(i) + here(4 * hf);
 #pragma unroll
             for (int x = 0; x < 16; x++) {
-                const bool v = row.sees(a, k0 + 8 * (x >> 2) + (x & 3));
+                const bool v = sees<TREE>(a, row.pos, row.mask, k0 + 8 * (x >> 2) + (x & 3));
                 seen |= (uint32_t)v << x;
                 s[x] = v ? s[x] : -INFINITY;
             }
@@ -477,12 +874,14 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
         b ^= Q8;
     };
     while (i < i1) {
-        for (bool all = row.all_see(a, KB * blk.at(i)); all; all = i < i1 && row.all_see(a, KB * blk.at(i))) step(std::false_type{});
-        for (bool some = i < i1; some; some = i < i1 && !row.all_see(a, KB * blk.at(i))) step(std::true_type{});
+        for (bool all = all_see<TREE, KB>(a, ta, tb, KB * blk.at(i)); all; all = i < i1 && all_see<TREE, KB>(a, ta, tb, KB * blk.at(i)))
+            step(std::false_type{});
+        for (bool some = i < i1; some; some = i < i1 && !all_see<TREE, KB>(a, ta, tb, KB * blk.at(i))) step(std::true_type{});
     }
+
     l = pair_sum<32>(l);
 
-    // the waves' sums through LDS (each its own tile's place): thread (wave, lane) finishes 8 of the lane's 64 sums
+    // the waves' sums through LDS (each its own tile's place): wave w finishes dims 16w … of every row
     wait_reads();
     float4 *so = reinterpret_cast<float4 *>(tile);
 #pragma unroll
@@ -491,7 +890,6 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
         for (int x = 0; x < 4; x++)
             so[(4 * u + x) * 64 + lane] = make_float4(o[u][4 * x], o[u][4 * x + 1], o[u][4 * x + 2], o[u][4 * x + 3]);
     if (hf == 0) s_ml[wave][0][c] = m, s_ml[wave][1][c] = l;
-    if (wave == 0 && hf == 0) s_c[c] = sc;
     __syncthreads();
     m = M_NONE, l = 0.0f;
 #pragma unroll
@@ -511,103 +909,26 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
             v[x].z = fmaf(y.z, w, v[x].z), v[x].w = fmaf(y.w, w, v[x].w);
         }
     }
-    const int dim0 = 16 * wave + 4 * hf;  // sums 8·wave … + 7 of the lane: dims 16·wave + 4hf … + 3, and 8 further
-    if (a.n_split == 1) {
-        if (row.r >= rows) return;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
-        float *orow = a.out + ((size_t)row.t * a.n_head + row.head) * D + dim0;
-#pragma unroll
-        for (int x = 0; x < 2; x++)
-            *reinterpret_cast<float4 *>(orow + 8 * x) = make_float4(v[x].x * inv, v[x].y * inv, v[x].z * inv, v[x].w * inv);
-        return;
-    }
-
-    // the part's sums to memory; the last workgroup of the row group to get there joins them
     const size_t g0 = ((size_t)kvh * a.n_rg + rg) * a.n_split * KB;  // the row group's first row of partial sums
     if (row.r < rows) {
-        const size_t pr = g0 + (size_t)split * KB + c;
-        float *prow = a.part + pr * D + dim0;
+        if (a.n_split == 1) {
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-            put64(prow + 8 * x, v[x].x, v[x].y, a.xl);
-            put64(prow + 8 * x + 2, v[x].z, v[x].w, a.xl);
-        }
-        if (wave == 0 && hf == 0) put64(a.part_ml + pr, m, l, a.xl);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's stores are performed
-    __syncthreads();
-    uint32_t *ticket = a.tickets + TICKET * ((size_t)kvh * a.n_rg + rg);
-    if (tid == 0)
-        s_last = (a.xl ? __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)
-                       : __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) ==
-                 (uint32_t)(a.n_split - 1);
-    __syncthreads();
-    if (!s_last) return;
-    const int nr = min(KB, rows - r0), ns = a.n_split;
-    float2 *s_w = reinterpret_cast<float2 *>(&s_kv[0][0]);  // [row][part]: (m, l), then (weight, l)
-    for (int id = tid; id < nr * MAX_SPLIT; id += 64 * SW) {
-        const int p = id % MAX_SPLIT;
-        if (p < ns) s_w[id] = get64(a.part_ml + g0 + (size_t)p * KB + id / MAX_SPLIT);
-    }
-    __syncthreads();
-    {
-        const int r = tid >> 4, p0 = tid & 15;
-        float top = M_NONE, sum = 0.0f;
-        if (r < nr)
-            for (int p = p0; p < ns; p += 16) top = fmaxf(top, s_w[MAX_SPLIT * r + p].x);
-        top = group_max<8>(top, lane);
-        if (r < nr)
-            for (int p = p0; p < ns; p += 16) {
-                const float2 ml = s_w[MAX_SPLIT * r + p];
-                const float w = __builtin_amdgcn_exp2f((ml.x - top) * s_c[r]);
-                sum = fmaf(ml.y, w, sum);
-                s_w[MAX_SPLIT * r + p].x = w;
+            for (int x = 0; x < 2; x++) put_row(a.out, a.n_head, a.group, kvh, row.r, 4 * wave + hf + 2 * x, v[x], l);
+        } else {
+            const size_t pr = g0 + (size_t)split * KB + c;
+            float *to = a.part + pr * D + 16 * wave + 4 * hf;
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                put64(to + 8 * x, v[x].x, v[x].y, a.xl);
+                put64(to + 8 * x + 2, v[x].z, v[x].w, a.xl);
             }
-        sum = group_sum<8>(sum, lane);
-        if (p0 == 0) s_ml[0][0][r] = sum == 0.0f ? 0.0f : 1.0f / sum;
-    }
-    __syncthreads();
-    // 32 threads of 4 dims a row; rows fewer than 16: a row's parts to 2, 4, 8 or 16 such groups
-    const int gr = tid >> 5, d4 = tid & 31, lg = nr > 8 ? 4 : nr > 4 ? 3 : nr > 2 ? 2 : nr > 1 ? 1 : 0, groups = 16 >> lg;
-    float4 *s_g = reinterpret_cast<float4 *>(s_w + KB * MAX_SPLIT);
-    for (int rb = 0; rb < nr; rb += 1 << lg) {
-        const int r = min(rb + (gr & ((1 << lg) - 1)), nr - 1), g = gr >> lg;
-        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float *from = a.part + (g0 + r) * D + 4 * d4;
-        for (int p = g; p < ns; p += 8 * groups) {
-            float2 in[8][2];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float *at = from + (size_t)min(p + e * groups, ns - 1) * (KB * D);
-                in[e][0] = get64(at), in[e][1] = get64(at + 2);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float w = p + e * groups < ns ? s_w[MAX_SPLIT * r + p + e * groups].x : 0.0f;
-                y.x = fmaf(in[e][0].x, w, y.x), y.y = fmaf(in[e][0].y, w, y.y);
-                y.z = fmaf(in[e][1].x, w, y.z), y.w = fmaf(in[e][1].y, w, y.w);
+            if (wave == 0 && hf == 0) {
+                put64(a.part_ml + pr, m, l, a.xl);
+                put64(&a.part_ml[pr].z, sc, 0.0f, a.xl);
             }
         }
-        if (groups > 1) {  // (fewer than 16 rows: one pass)
-            s_g[tid] = y;
-            __syncthreads();
-            if (g == 0)
-                for (int e = 1; e < groups; e++) {
-                    const float4 z = s_g[tid + 32 * (e << lg)];
-                    y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
-                }
-        }
-        if (g == 0 && rb + (gr & ((1 << lg) - 1)) < nr) {
-            const float inv = s_ml[0][0][r];
-            const int t = (r0 + r) / a.group, head = kvh * a.group + (r0 + r) % a.group;
-            *reinterpret_cast<float4 *>(a.out + ((size_t)t * a.n_head + head) * D + 4 * d4) =
-                make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
-        }
     }
-    if (tid == 0) {  // for the next call
-        if (a.xl) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        else __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    if (a.tickets) join_last(a, kvh, rg, r0, rows, KB, g0, &s_last, s_w, reinterpret_cast<float4 *>(&s_kv[0][0]));
 }
 
 // ---- many rows ---------------------------------------------------------------------------------------------------------------
@@ -626,7 +947,7 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
     const int kvh = blockIdx.x % a.kv.n_kv, rg = a.n_rg - 1 - blockIdx.x / a.kv.n_kv;  // (the longest rows first)
     const int rows = a.n * a.group, r0 = rg * KB * WR;
     const int n_keys = TREE ? a.n_past + a.n : a.pos0 + a.n;
-    const Blocks blk = blocks_of<TREE>(a, r0 / a.group, min(r0 + KB * WR - 1, rows - 1) / a.group);
+    const Blocks blk = blocks_of<TREE, KB>(a, r0 / a.group, min(r0 + KB * WR - 1, rows - 1) / a.group);
     const int nb = blk.count(), n_stage = (nb + WP - 1) / WP;
     const char *kh = (const char *)a.kv.k + (size_t)kvh * a.kv.n_ctx * (2 * D);
     const char *vh = (const char *)a.kv.v + (size_t)kvh * a.kv.n_ctx * (2 * D);
@@ -651,9 +972,10 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
     issue(0, true);
     if (n_stage > 1) issue(1, false);
 
-    const Row<TREE> row(a, tree, kvh, r0 + KB * rt, c);
+    const Row<TREE> row(a, tree, kvh, r0 + KB * rt + c);
+    const int ta = min(r0 + KB * rt, rows - 1) / a.group, tb = min(r0 + KB * rt + KB - 1, rows - 1) / a.group;
     half8 qh[8], ql[8];
-    const float sc = q_pairs(a.q + (size_t)row.t * a.q_stride + (size_t)row.head * D + 8 * hf, a.scale, qh, ql);
+    const float sc = q_pairs<8, 2>(a.q + (size_t)row.t * a.q_stride + (size_t)row.head * D + 8 * hf, a.scale, qh, ql);
     int ka[8], va[4];
 #pragma unroll
     for (int ks = 0; ks < 8; ks++) ka[ks] = 16 * c + ((2 * ks + hf) ^ (c & 15));
@@ -684,7 +1006,7 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
             const int i = WP * st + kp, k0 = KB * blk.at(min(i, nb - 1)) + here(4 * hf);
 #pragma unroll
             for (int x = 0; x < 16; x++) {
-                const bool v = i < nb && row.sees(a, k0 + 8 * (x >> 2) + (x & 3));
+                const bool v = i < nb && sees<TREE>(a, row.pos, row.mask, k0 + 8 * (x >> 2) + (x & 3));
                 seen |= (uint32_t)v << x;
                 s[x] = v ? s[x] : -INFINITY;
             }
@@ -778,7 +1100,7 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
     }
     // two stages at a time, both kinds of step passing one barrier a stage: a wave's blocks may be masked where another's
     // are not
-    auto whole = [&](int st) { return WP * st + kp < nb && row.all_see(a, KB * blk.at(WP * st + kp)); };
+    auto whole = [&](int st) { return WP * st + kp < nb && all_see<TREE, KB>(a, ta, tb, KB * blk.at(WP * st + kp)); };
     for (int st = 0; st < n_stage;) {
         for (; st + 1 < n_stage && whole(st) && whole(st + 1); st += 2) {
             step(st, 0, s0, s1, std::false_type{});
@@ -835,35 +1157,56 @@ int read_back(htr_device *dev, Args &a, int n_keys, int sink_rows, int from_row)
     return 0;
 }
 
-// max_blocks: the most key blocks that 32 rows see; sink_rows, from_row: the rows 0 … sink_rows − 1 and from_row … (both
-// multiples of 32) hold all that is seen
-template <bool TREE> int launch(htr_device *dev, Args &a, const TreeMask &tree, int max_blocks, int sink_rows, int from_row) {
-    const int rows = a.n * a.group;
-    const int64_t groups = (int64_t)((rows + KB - 1) / KB) * a.kv.n_kv;
-    if (groups >= 2 * dev->n_cu) {
-        a.n_rg = (rows + KB * WR - 1) / (KB * WR), a.n_split = 1;
-        const int64_t wide = (int64_t)a.n_rg * a.kv.n_kv;
-        if (wide > INT32_MAX) return htr_fail("attention: %d rows of %d KV heads", rows, a.kv.n_kv);
-        if (a.kv.q8) HTR_TRY(read_back(dev, a, TREE ? a.n_past + a.n : a.pos0 + a.n, sink_rows, from_row));
-        hipLaunchKernelGGL((k_kv_attn<TREE>), dim3((unsigned)wide), dim3(64 * WR * WP), 0, dev->stream, a, tree);
-        return htr_launched(dev, "k_kv_attn");
-    }
-    a.n_rg = (rows + KB - 1) / KB;
-    // a workgroup a CU, no more parts than a wave has blocks
-    a.n_split = (int)std::max<int64_t>(1, std::min<int64_t>({dev->n_cu / groups, (max_blocks + SW - 1) / SW, MAX_SPLIT}));
+// RT: 16·RT rows a workgroup in rounds of 128 keys; 0: 32 rows, each of the waves its own blocks of 32 keys
+template <bool TREE, int RT> int launch_split(htr_device *dev, Args &a, const TreeMask &tree, int max_keys) {
+    const int rows = a.n * a.group, tile = RT ? 16 * RT : KB, run = (RT ? UK : KB) * SW;
+    a.n_rg = (rows + tile - 1) / tile;
+    const int groups = a.n_rg * a.kv.n_kv, max_run = (max_keys + run - 1) / run;
+    // a workgroup a CU, no more parts than rounds; no parts where they would save less than they cost
+    a.n_split = std::max(1, std::min({dev->n_cu / groups, max_run, MAX_SPLIT}));
+    if (max_run <= 2) a.n_split = 1;
     a.xl = a.kv.n_kv % 8 == 0 && dev->xcd_round_robin == 1;
+    const bool here = std::min(rows, tile) * a.n_split <= JOIN_HERE;
     if (a.n_split > 1) {
         void *p;
         HTR_TRY(htr_scratch(dev, SCR_KV_TICKET, (size_t)dev->n_cu * TICKET * 4, &p));
-        a.tickets = (uint32_t *)p;
-        HTR_TRY(htr_scratch(dev, SCR_KV_ATTN, (size_t)dev->n_cu * KB * (D + 2) * 4, &p));
+        if (here) a.tickets = (uint32_t *)p;
+        const size_t most = (size_t)dev->n_cu * KB;  // rows of partial sums
+        HTR_TRY(htr_scratch(dev, SCR_KV_ATTN, most * (D + 4) * 4, &p));
         a.part = (float *)p;
-        a.part_ml = (uint64_t *)(a.part + (size_t)dev->n_cu * KB * D);
+        a.part_ml = (float4 *)(a.part + most * D);
+        if (!here) a.xl = 0;  // (the second launch runs on any XCD)
     }
     const dim3 g((unsigned)(groups * a.n_split)), b(64 * SW);
-    if (a.kv.q8) hipLaunchKernelGGL((k_kv_attn_split<true, TREE>), g, b, 0, dev->stream, a, tree);
-    else hipLaunchKernelGGL((k_kv_attn_split<false, TREE>), g, b, 0, dev->stream, a, tree);
-    return htr_launched(dev, a.kv.q8 ? "k_kv_attn_split<q8_0>" : "k_kv_attn_split<f16>");
+    if constexpr (RT != 0) {
+        if (a.kv.q8) hipLaunchKernelGGL((k_kv_attn_few<true, TREE, RT>), g, b, 0, dev->stream, a, tree);
+        else hipLaunchKernelGGL((k_kv_attn_few<false, TREE, RT>), g, b, 0, dev->stream, a, tree);
+    } else {
+        if (a.kv.q8) hipLaunchKernelGGL((k_kv_attn_split<true, TREE>), g, b, 0, dev->stream, a, tree);
+        else hipLaunchKernelGGL((k_kv_attn_split<false, TREE>), g, b, 0, dev->stream, a, tree);
+    }
+    HTR_TRY(htr_launched(dev, RT ? "k_kv_attn_few" : "k_kv_attn_split"));
+    if (a.n_split == 1 || here) return 0;
+    const JoinArgs ja{a.part, a.part_ml, a.out, a.n_split, a.n_head, a.group, rows, a.kv.n_kv, a.n_rg, tile};
+    hipLaunchKernelGGL(k_kv_attn_join, dim3((unsigned)((rows * a.kv.n_kv + 1) / 2)), dim3(256), 0, dev->stream, ja);
+    return htr_launched(dev, "k_kv_attn_join");
+}
+
+// max_keys: the most keys that the queries of a row group see; sink_rows, from_row: the rows 0 … sink_rows − 1 and from_row …
+// (both multiples of 32) hold all that is seen
+template <bool TREE> int launch(htr_device *dev, Args &a, const TreeMask &tree, int max_keys, int sink_rows, int from_row) {
+    const int rows = a.n * a.group;
+    const int64_t groups = (int64_t)((rows + KB * WR - 1) / (KB * WR)) * a.kv.n_kv;
+    if (groups >= dev->n_cu) {
+        a.n_rg = (rows + KB * WR - 1) / (KB * WR), a.n_split = 1;
+        if (groups > INT32_MAX) return htr_fail("attention: %d rows of %d KV heads", rows, a.kv.n_kv);
+        if (a.kv.q8) HTR_TRY(read_back(dev, a, TREE ? a.n_past + a.n : a.pos0 + a.n, sink_rows, from_row));
+        hipLaunchKernelGGL((k_kv_attn<TREE>), dim3((unsigned)groups), dim3(64 * WR * WP), 0, dev->stream, a, tree);
+        return htr_launched(dev, "k_kv_attn");
+    }
+    if (rows <= 16) return launch_split<TREE, 1>(dev, a, tree, max_keys);
+    if (rows <= 32) return launch_split<TREE, 2>(dev, a, tree, max_keys);
+    return launch_split<TREE, 0>(dev, a, tree, max_keys);
 }
 
 int check_rows(const char *me, const float *d_q, size_t q_stride, const htr_kv *kv, int n_head, float *d_out, int64_t n) {
@@ -903,7 +1246,7 @@ extern "C" int htr_tree_attention(htr_device *dev, const float *d_q, size_t q_st
     const HtrOnDevice on(dev);
     a.q = d_q, a.q_stride = q_stride, a.out = d_out, a.n = n, a.n_head = n_head, a.group = n_head / kv->n_kv;
     a.scale = scale, a.n_past = n_past;
-    return launch<true>(dev, a, tree, (n_past + n + KB - 1) / KB, 0, 0);
+    return launch<true>(dev, a, tree, n_past + n, 0, 0);
 }
 
 extern "C" int htr_window_attention(htr_device *dev, const float *d_q, size_t q_stride, int n_q, int pos0, int window,
@@ -921,6 +1264,6 @@ extern "C" int htr_window_attention(htr_device *dev, const float *d_q, size_t q_
     a.scale = scale, a.pos0 = pos0, a.window = window, a.n_sink = n_sink;
     const int n_keys = pos0 + n_q, sink = std::min(n_sink, n_keys), sink_rows = (sink + KB - 1) / KB * KB;
     const int from = window > pos0 ? 0 : (pos0 - window + 1) / KB * KB;
-    const int64_t span = std::min<int64_t>(n_keys, (int64_t)window + sink + 3 * KB);  // of 32 rows' queries
-    return launch<false>(dev, a, TreeMask{}, (int)((span + KB - 1) / KB), sink_rows, std::max(from, sink_rows));
+    const int64_t span = (int64_t)window + sink + 64;  // of 64 rows' queries
+    return launch<false>(dev, a, TreeMask{}, (int)std::min<int64_t>(n_keys, span), sink_rows, std::max(from, sink_rows));
 }
