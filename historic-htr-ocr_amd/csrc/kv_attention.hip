@@ -52,6 +52,7 @@ struct Args {
     float *out;
     HtrKvPlanes kv;
     int n, n_head, group;
+    uint32_t per_group;        // ⌈2^32 / group⌉ (group > 1): the quotient of a row below 2^32 / group by one product
     float scale;
     int sink_rows, shift;      // keys from sink_rows on lie shift rows further up in memory
     int n_past;                // tree: the committed keys
@@ -135,13 +136,26 @@ template <bool TREE, int U> __device__ __forceinline__ Blocks blocks_of(const Ar
     }
 }
 
+// part `split` of n blocks in n_split even parts
+struct Part {
+    int i0, i1;
+};
+__device__ __forceinline__ Part part_of(int n, int split, int n_split) {
+    const int per = n / n_split, more = n - per * n_split, i0 = split * per + min(split, more);
+    return Part{i0, i0 + per + (split < more ? 1 : 0)};
+}
+// row r's query
+__device__ __forceinline__ int query_of(int group, uint32_t per_group, int r) {
+    return group == 1 ? r : (int)__umulhi((uint32_t)r, per_group);
+}
+
 // one row: query t, its head, and the keys it sees
 template <bool TREE> struct Row {
     int r, t, head, pos;
     uint64_t mask;
     __device__ __forceinline__ Row(const Args &a, const TreeMask &tree, int kvh, int row) {
         const int rc = min(row, a.n * a.group - 1);
-        r = row, t = rc / a.group, head = kvh * a.group + rc % a.group, pos = a.pos0 + t;
+        r = row, t = query_of(a.group, a.per_group, rc), head = kvh * a.group + (rc - t * a.group), pos = a.pos0 + t;
         mask = 0;
         if constexpr (TREE) mask = tree.of[t];
     }
@@ -222,6 +236,10 @@ __device__ __forceinline__ half8 finite(half8 v, uint32_t &any) {
     __builtin_memcpy(&v, w, 16);
     return v;
 }
+__device__ __forceinline__ half8 finite(half8 v) {
+    uint32_t any = 0;
+    return finite(v, any);
+}
 __device__ __forceinline__ half8 ones_of_not_finite(half8 v) {
     uint32_t w[4];
     __builtin_memcpy(w, &v, 16);
@@ -275,6 +293,7 @@ struct JoinArgs {
     const float *part;
     const float4 *part_ml;
     float *out;
+    uint32_t per_group;
     int n_split, n_head, group, rows, n_kv, n_rg, tile;  // tile: rows of a row group's part
 };
 
@@ -325,9 +344,9 @@ __device__ __forceinline__ float join_row(const float *part, const float4 *part_
     __builtin_amdgcn_wave_barrier();
     return sum;
 }
-__device__ __forceinline__ void put_row(float *out, int n_head, int group, int kvh, int r, int j, float4 y, float sum) {
+__device__ __forceinline__ void put_row(float *out, int n_head, int group, uint32_t per_group, int kvh, int r, int j, float4 y, float sum) {
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
-    const int t = r / group, head = kvh * group + r % group;
+    const int t = query_of(group, per_group, r), head = kvh * group + (r - t * group);
     *reinterpret_cast<float4 *>(out + ((size_t)t * n_head + head) * D + 4 * j) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
 }
 
@@ -349,7 +368,7 @@ __global__ __launch_bounds__(256) void k_kv_attn_join(JoinArgs a) {
         const float4 z = s_y[gr + e][j];
         y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
     }
-    put_row(a.out, a.n_head, a.group, kvh, r, j, y, sum);
+    put_row(a.out, a.n_head, a.group, a.per_group, kvh, r, j, y, sum);
 }
 
 // the last workgroup of a row group to have stored its part joins them all (tile: rows of a part, the group's first at g0);
@@ -366,9 +385,10 @@ __device__ __forceinline__ void join_last(const Args &a, int kvh, int rg, int r0
                   (uint32_t)(a.n_split - 1);
     __syncthreads();
     if (!*s_last) return;
-    // 32 lanes a row; where the rows are fewer than the groups of lanes, several groups to a row's parts
+    // 32 lanes a row; where the rows are fewer than the groups of lanes, several groups (of 8 parts at once each) to a row
     const int nr = min(tile, rows - r0), gr = tid >> 5, j = tid & 31;
-    const int lg = nr > 8 ? 4 : nr > 4 ? 3 : nr > 2 ? 2 : nr > 1 ? 1 : 0, G = 16 >> lg;
+    const int few = nr > 8 ? 0 : nr > 4 ? 1 : nr > 2 ? 2 : nr > 1 ? 3 : 4;  // log2 of the groups that there are for a row
+    const int ns8 = (a.n_split + 7) / 8, lg = 4 - min(few, ns8 > 4 ? 3 : ns8 > 2 ? 2 : ns8 > 1 ? 1 : 0), G = 16 >> lg;
     for (int rb = 0; rb < nr; rb += 1 << lg) {
         const int ri = rb + (gr & ((1 << lg) - 1)), part = gr >> lg;
         float4 y;
@@ -382,7 +402,7 @@ __device__ __forceinline__ void join_last(const Args &a, int kvh, int rg, int r0
                     y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
                 }
         }
-        if (part == 0 && ri < nr) put_row(a.out, a.n_head, a.group, kvh, r0 + ri, j, y, sum);
+        if (part == 0 && ri < nr) put_row(a.out, a.n_head, a.group, a.per_group, kvh, r0 + ri, j, y, sum);
     }
     if (tid == 0) {  // for the next call
         if (a.xl) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
@@ -399,16 +419,15 @@ template <bool Q8, bool TREE, int RT> __global__ __launch_bounds__(64 * SW, 2) v
     __shared__ __attribute__((aligned(16))) uint16_t s_vt[4][ST][4][8];  // V's scales by dims / 32, step, lane group, slot
     __shared__ float s_mx[SW][16 * RT], s_l[SW][16 * RT];
     __shared__ float s_w[SW * 2][MAX_SPLIT];
-    __shared__ int s_last;
+    __shared__ int s_odd[SW], s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c = lane & 15;
-    const int kvh = blockIdx.x % a.kv.n_kv, rest = blockIdx.x / a.kv.n_kv;
-    const int split = rest % a.n_split, rg = rest / a.n_split;
+    const int kvh = blockIdx.x, split = blockIdx.y, rg = blockIdx.z;
     const int rows = a.n * a.group, r0 = rg * 16 * RT;
     const int n_keys = TREE ? a.n_past + a.n : a.pos0 + a.n;
-    const int ta = r0 / a.group, tb = min(r0 + 16 * RT - 1, rows - 1) / a.group;
+    const int ta = query_of(a.group, a.per_group, r0), tb = query_of(a.group, a.per_group, min(r0 + 16 * RT - 1, rows - 1));
     const Blocks blk = blocks_of<TREE, UK>(a, ta, tb);
-    const int nu = blk.count(), i0 = (int)((int64_t)nu * split / a.n_split), i1 = (int)((int64_t)nu * (split + 1) / a.n_split);
+    const auto [i0, i1] = part_of(blk.count(), split, a.n_split);
     const int n_round = (i1 - i0 + SW - 1) / SW;
     const size_t head0 = (size_t)kvh * a.kv.n_ctx;
 
@@ -457,8 +476,13 @@ template <bool Q8, bool TREE, int RT> __global__ __launch_bounds__(64 * SW, 2) v
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) o[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    auto round = [&](int rd, auto is_masked) {
-        constexpr bool MASK = decltype(is_masked)::value;
+    // whether every row sees all keys of the round's units
+    auto whole = [&](int rd) {
+        const int i = i0 + SW * rd + (lane & 7);
+        return __builtin_amdgcn_ballot_w64(!(i < i1 && all_see<TREE, UK>(a, ta, tb, UK * blk.at(min(i, i1 - 1))))) == 0;
+    };
+    for (int rd = 0; rd < n_round; rd++) {
+        const bool masked = !whole(rd);  // (what only a masked round does stands behind uniform branches, and is not fetched else)
         const int i = i0 + SW * rd + wave, b = rd & 1;
         const bool more = rd + 1 < n_round;
         wait_loads<NL>();  // K; V is still on its way
@@ -490,7 +514,9 @@ template <bool Q8, bool TREE, int RT> __global__ __launch_bounds__(64 * SW, 2) v
                 }
         }
         uint32_t seen[RT];
-        if constexpr (MASK) {
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) seen[rt] = 15u;
+        if (masked) {
             const int k0 = UK * blk.at(min(i, i1 - 1)) + here(4 * g);
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
@@ -539,10 +565,9 @@ template <bool Q8, bool TREE, int RT> __global__ __launch_bounds__(64 * SW, 2) v
             uint32_t h[2], r[2];
             split2(p[0], p[1], h[0], r[0]);
             split2(p[2], p[3], h[1], r[1]);
-            if constexpr (MASK) {  // (a weight's sign: not seen)
-                h[0] |= (seen[rt] & 1 ? 0u : 0x8000u) | (seen[rt] & 2 ? 0u : 0x80000000u);
-                h[1] |= (seen[rt] & 4 ? 0u : 0x8000u) | (seen[rt] & 8 ? 0u : 0x80000000u);
-            }
+            // a weight's sign: not seen
+            h[0] |= (~seen[rt] & 1u) << 15 | (~seen[rt] & 2u) << 30;
+            h[1] |= (~seen[rt] & 4u) << 13 | (~seen[rt] & 8u) << 28;
             reinterpret_cast<uint2_t *>(&s_p[0][rt][wave >> 1][lane])[wave & 1] = uint2_t{h[0], h[1]};
             reinterpret_cast<uint2_t *>(&s_p[1][rt][wave >> 1][lane])[wave & 1] = uint2_t{r[0], r[1]};
         }
@@ -555,6 +580,22 @@ template <bool Q8, bool TREE, int RT> __global__ __launch_bounds__(64 * SW, 2) v
                 s_vt[2 * (lane & 1)][wave >> 1][key >> 2][at] = (uint16_t)d2;
                 s_vt[2 * (lane & 1) + 1][wave >> 1][key >> 2][at] = (uint16_t)(d2 >> 16);
             }
+        if (masked) {  // does the wave's unit hold a value of V that is not finite (a scale that may make one: past 515.5)?
+            uint32_t any = 0;
+            if constexpr (Q8) {
+                const uint32_t w = s_vd[b][wave][here(lane)];
+                any = (w & 0x7FFFu) > 0x6007u || (w >> 16 & 0x7FFFu) > 0x6007u;
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const uint4_t w = s_v[b][wave][64 * u + here(lane)];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) any |= ((w[e] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+                }
+            }
+            if (lane == 0) s_odd[wave] = 0;
+            if (any) s_odd[wave] = 1;
+        }
         wait_reads();
         __builtin_amdgcn_s_barrier();  // everyone's weights and V
         asm volatile("" ::: "memory");
@@ -575,44 +616,39 @@ template <bool Q8, bool TREE, int RT> __global__ __launch_bounds__(64 * SW, 2) v
             }
             return v;
         };
-        uint32_t odd = 0;
+        bool odd = false;
+        if (masked) odd = __builtin_amdgcn_ballot_w64(s_odd[here(lane & 7)] != 0) != 0;
+        if (!odd) {
 #pragma unroll
-        for (int st = 0; st < ST; st++) {
-            half8 v = vread(st);
-            if constexpr (MASK) v = finite(v, odd);
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, *reinterpret_cast<const half8 *>(&s_p[0][rt][st][lane]), o[rt], 0, 0, 0);
-                o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, *reinterpret_cast<const half8 *>(&s_p[1][rt][st][lane]), o[rt], 0, 0, 0);
-            }
-        }
-        if constexpr (MASK)
-            if (__builtin_amdgcn_ballot_w64(odd != 0)) {
-                // NaN into the sums of the rows that see a value that is not finite: a product of ones
+            for (int st = 0; st < ST; st++) {
+                const half8 v = vread(st);
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) {
-                    f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
-                    for (int st = 0; st < ST; st++) {
-                        uint4_t h = s_p[0][rt][st][lane];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) h[e] = ((~h[e] >> 15) & 0x00010001u) * 0x3C00u;
-                        half8 ind;
-                        __builtin_memcpy(&ind, &h, 16);
-                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones_of_not_finite(vread(st)), ind, t, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int x = 0; x < 4; x++) o[rt][x] = t[x] > 0.0f ? NAN : o[rt][x];
+                    o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, *reinterpret_cast<const half8 *>(&s_p[0][rt][st][lane]), o[rt], 0, 0, 0);
+                    o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, *reinterpret_cast<const half8 *>(&s_p[1][rt][st][lane]), o[rt], 0, 0, 0);
                 }
             }
-    };
-    // whether every row sees all keys of the round's units
-    auto whole = [&](int rd) {
-        const int i = i0 + SW * rd + (lane & 7);
-        return __builtin_amdgcn_ballot_w64(!(i < i1 && all_see<TREE, UK>(a, ta, tb, UK * blk.at(min(i, i1 - 1))))) == 0;
-    };
-    for (int rd = 0; rd < n_round;) {
-        for (bool all = whole(rd); all; all = rd < n_round && whole(rd)) round(rd++, std::false_type{});
-        for (bool some = rd < n_round; some; some = rd < n_round && !whole(rd)) round(rd++, std::true_type{});
+        } else {
+            // such values as 0, and NaN into the sums of the rows that see one: a product of ones
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+                for (int st = 0; st < ST; st++) {
+                    const half8 v = vread(st), z = finite(v);
+                    uint4_t h = s_p[0][rt][st][lane];
+                    half8 ind;
+                    o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(z, *reinterpret_cast<const half8 *>(&h), o[rt], 0, 0, 0);
+                    o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(z, *reinterpret_cast<const half8 *>(&s_p[1][rt][st][lane]), o[rt], 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) h[e] = ((~h[e] >> 15) & 0x00010001u) * 0x3C00u;
+                    __builtin_memcpy(&ind, &h, 16);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones_of_not_finite(v), ind, t, 0, 0, 0);
+                }
+#pragma unroll
+                for (int x = 0; x < 4; x++) o[rt][x] = t[x] > 0.0f ? NAN : o[rt][x];
+            }
+        }
     }
     // Σ l over the lanes and waves (m is the same in every wave)
 #pragma unroll
@@ -630,7 +666,7 @@ template <bool Q8, bool TREE, int RT> __global__ __launch_bounds__(64 * SW, 2) v
         for (int w = 0; w < SW; w++) sum += s_l[w][16 * rt + c];
         if (r >= rows) continue;
         if (a.n_split == 1) {
-            put_row(a.out, a.n_head, a.group, kvh, r, 4 * wave + g, make_float4(o[rt][0], o[rt][1], o[rt][2], o[rt][3]), sum);
+            put_row(a.out, a.n_head, a.group, a.per_group, kvh, r, 4 * wave + g, make_float4(o[rt][0], o[rt][1], o[rt][2], o[rt][3]), sum);
             continue;
         }
         const size_t pr = g0 + (size_t)split * (16 * RT) + 16 * rt + c;
@@ -667,13 +703,12 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hf = lane >> 5, c = lane & 31;
-    const int kvh = blockIdx.x % a.kv.n_kv, rest = blockIdx.x / a.kv.n_kv;
-    const int split = rest % a.n_split, rg = rest / a.n_split;
+    const int kvh = blockIdx.x, split = blockIdx.y, rg = blockIdx.z;
     const int rows = a.n * a.group, r0 = rg * KB;
     const int n_keys = TREE ? a.n_past + a.n : a.pos0 + a.n;
-    const int ta = r0 / a.group, tb = min(r0 + KB - 1, rows - 1) / a.group;
+    const int ta = query_of(a.group, a.per_group, r0), tb = query_of(a.group, a.per_group, min(r0 + KB - 1, rows - 1));
     const Blocks blk = blocks_of<TREE, KB>(a, ta, tb);
-    const int nb = blk.count(), i0 = (int)((int64_t)nb * split / a.n_split), i1 = (int)((int64_t)nb * (split + 1) / a.n_split);
+    const auto [i0, i1] = part_of(blk.count(), split, a.n_split);
     const size_t head0 = (size_t)kvh * a.kv.n_ctx;
 
     uint4_t *tile = s_kv[wave];
@@ -913,7 +948,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     if (row.r < rows) {
         if (a.n_split == 1) {
 #pragma unroll
-            for (int x = 0; x < 2; x++) put_row(a.out, a.n_head, a.group, kvh, row.r, 4 * wave + hf + 2 * x, v[x], l);
+            for (int x = 0; x < 2; x++) put_row(a.out, a.n_head, a.group, a.per_group, kvh, row.r, 4 * wave + hf + 2 * x, v[x], l);
         } else {
             const size_t pr = g0 + (size_t)split * KB + c;
             float *to = a.part + pr * D + 16 * wave + 4 * hf;
@@ -947,7 +982,8 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
     const int kvh = blockIdx.x % a.kv.n_kv, rg = a.n_rg - 1 - blockIdx.x / a.kv.n_kv;  // (the longest rows first)
     const int rows = a.n * a.group, r0 = rg * KB * WR;
     const int n_keys = TREE ? a.n_past + a.n : a.pos0 + a.n;
-    const Blocks blk = blocks_of<TREE, KB>(a, r0 / a.group, min(r0 + KB * WR - 1, rows - 1) / a.group);
+    const Blocks blk = blocks_of<TREE, KB>(a, query_of(a.group, a.per_group, r0),
+                                             query_of(a.group, a.per_group, min(r0 + KB * WR - 1, rows - 1)));
     const int nb = blk.count(), n_stage = (nb + WP - 1) / WP;
     const char *kh = (const char *)a.kv.k + (size_t)kvh * a.kv.n_ctx * (2 * D);
     const char *vh = (const char *)a.kv.v + (size_t)kvh * a.kv.n_ctx * (2 * D);
@@ -973,7 +1009,8 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
     if (n_stage > 1) issue(1, false);
 
     const Row<TREE> row(a, tree, kvh, r0 + KB * rt + c);
-    const int ta = min(r0 + KB * rt, rows - 1) / a.group, tb = min(r0 + KB * rt + KB - 1, rows - 1) / a.group;
+    const int ta = query_of(a.group, a.per_group, min(r0 + KB * rt, rows - 1));
+    const int tb = query_of(a.group, a.per_group, min(r0 + KB * rt + KB - 1, rows - 1));
     half8 qh[8], ql[8];
     const float sc = q_pairs<8, 2>(a.q + (size_t)row.t * a.q_stride + (size_t)row.head * D + 8 * hf, a.scale, qh, ql);
     int ka[8], va[4];
@@ -1164,7 +1201,7 @@ template <bool TREE, int RT> int launch_split(htr_device *dev, Args &a, const Tr
     const int groups = a.n_rg * a.kv.n_kv, max_run = (max_keys + run - 1) / run;
     // a workgroup a CU, no more parts than rounds; no parts where they would save less than they cost
     a.n_split = std::max(1, std::min({dev->n_cu / groups, max_run, MAX_SPLIT}));
-    if (max_run <= 2) a.n_split = 1;
+    if (max_run <= 3) a.n_split = 1;
     a.xl = a.kv.n_kv % 8 == 0 && dev->xcd_round_robin == 1;
     const bool here = std::min(rows, tile) * a.n_split <= JOIN_HERE;
     if (a.n_split > 1) {
@@ -1177,7 +1214,7 @@ template <bool TREE, int RT> int launch_split(htr_device *dev, Args &a, const Tr
         a.part_ml = (float4 *)(a.part + most * D);
         if (!here) a.xl = 0;  // (the second launch runs on any XCD)
     }
-    const dim3 g((unsigned)(groups * a.n_split)), b(64 * SW);
+    const dim3 g((unsigned)a.kv.n_kv, (unsigned)a.n_split, (unsigned)a.n_rg), b(64 * SW);
     if constexpr (RT != 0) {
         if (a.kv.q8) hipLaunchKernelGGL((k_kv_attn_few<true, TREE, RT>), g, b, 0, dev->stream, a, tree);
         else hipLaunchKernelGGL((k_kv_attn_few<false, TREE, RT>), g, b, 0, dev->stream, a, tree);
@@ -1187,7 +1224,7 @@ template <bool TREE, int RT> int launch_split(htr_device *dev, Args &a, const Tr
     }
     HTR_TRY(htr_launched(dev, RT ? "k_kv_attn_few" : "k_kv_attn_split"));
     if (a.n_split == 1 || here) return 0;
-    const JoinArgs ja{a.part, a.part_ml, a.out, a.n_split, a.n_head, a.group, rows, a.kv.n_kv, a.n_rg, tile};
+    const JoinArgs ja{a.part, a.part_ml, a.out, a.per_group, a.n_split, a.n_head, a.group, rows, a.kv.n_kv, a.n_rg, tile};
     hipLaunchKernelGGL(k_kv_attn_join, dim3((unsigned)((rows * a.kv.n_kv + 1) / 2)), dim3(256), 0, dev->stream, ja);
     return htr_launched(dev, "k_kv_attn_join");
 }
@@ -1216,7 +1253,8 @@ int check_rows(const char *me, const float *d_q, size_t q_stride, const htr_kv *
     if (q_stride < qd || (q_stride & 3))
         return htr_fail("%s: rows %zu floats apart (a multiple of 4, at least %zu)", me, q_stride, qd);
     if (((uintptr_t)d_q | (uintptr_t)d_out) & 15) return htr_fail("%s: pointers must be 16-byte aligned", me);
-    if (n * (n_head / kv->n_kv) > (1 << 30)) return htr_fail("%s: %lld queries of %d heads", me, (long long)n, n_head);
+    const int64_t group = n_head / kv->n_kv;  // (rows · group < 2^32: the kernels' quotients)
+    if (n * group > 1 << 30 || n * group * group >= 1ll << 32) return htr_fail("%s: %lld queries of %d heads", me, (long long)n, n_head);
     const uintptr_t q0 = (uintptr_t)d_q, q1 = q0 + 4 * (q_stride * (n - 1) + qd), o0 = (uintptr_t)d_out, o1 = o0 + 4 * qd * n;
     if (q0 < o1 && o0 < q1) return htr_fail("%s: the output overlaps the queries", me);
     return 0;
@@ -1245,6 +1283,7 @@ extern "C" int htr_tree_attention(htr_device *dev, const float *d_q, size_t q_st
     HTR_TRY(htr_check_alive(dev));
     const HtrOnDevice on(dev);
     a.q = d_q, a.q_stride = q_stride, a.out = d_out, a.n = n, a.n_head = n_head, a.group = n_head / kv->n_kv;
+    a.per_group = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
     a.scale = scale, a.n_past = n_past;
     return launch<true>(dev, a, tree, n_past + n, 0, 0);
 }
@@ -1261,6 +1300,7 @@ extern "C" int htr_window_attention(htr_device *dev, const float *d_q, size_t q_
     HTR_TRY(htr_check_alive(dev));
     const HtrOnDevice on(dev);
     a.q = d_q, a.q_stride = q_stride, a.out = d_out, a.n = n_q, a.n_head = n_head, a.group = n_head / kv->n_kv;
+    a.per_group = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
     a.scale = scale, a.pos0 = pos0, a.window = window, a.n_sink = n_sink;
     const int n_keys = pos0 + n_q, sink = std::min(n_sink, n_keys), sink_rows = (sink + KB - 1) / KB * KB;
     const int from = window > pos0 ? 0 : (pos0 - window + 1) / KB * KB;
