@@ -42,27 +42,47 @@ __device__ __forceinline__ float half_bits(uint32_t b) {
     return (float)h;
 }
 
-// x / d rounded to the nearest integer, ties to even, for |x| ≤ 127·d (inv ≈ 1 / d, 0 where d is 0): the quotient in f32
-// is within 2^-16, so r is the nearest or, beside a border, its neighbour; x − r·d is exact
+// x / d rounded to the nearest integer, ties to even, for |x| ≤ 127·d and d > 0 (inv ≈ 1 / d): the quotient in f32 is within
+// 2^-16, so r is the nearest integer or, beside a border, its neighbour; x − r·d is exact in f32
 __device__ __forceinline__ int quant(float x, float d, float inv) {
     float r = rintf(x * inv);
     const float e = fmaf(-r, d, x), hd = 0.5f * d;
-    if (fabsf(e) >= hd && d > 0.0f) {
-        const bool odd = ((int)r & 1) != 0;
-        if (e > hd || (e == hd && odd)) r += 1.0f;
-        else if (e < -hd || (e == -hd && odd)) r -= 1.0f;
-    }
+    const bool odd = ((int)r & 1) != 0;
+    if (e > hd || (e == hd && odd)) r += 1.0f;
+    else if (e < -hd || (e == -hd && odd)) r -= 1.0f;
     return (int)r;
 }
-// 8 of a block's values, its scale's bits → 8 quants
+// 8 of a block's values (|x| ≤ 127·d, or not where the block is not finite), its scale's bits → 8 quants. x / d + 1.5·2^23 is
+// rounded to an integer, two's complement in its low byte; where no remainder reaches half a scale those are the quants
 __device__ __forceinline__ uint2_t quant8(const float (&x)[8], uint32_t db) {
-    if (db > 0x7C00u) return uint2_t{0u, 0u};
-    const float d = half_bits(db), inv = d > 0.0f ? 1.0f / d : 0.0f;
-    uint32_t w[2] = {0u, 0u};
+    if (db == 0u || db > 0x7C00u) return uint2_t{0u, 0u};
+    const float d = half_bits(db), inv = 1.0f / d, big = 12582912.0f;
+    uint32_t t[8], w[2];
+    float far = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-        w[e >> 2] |= ((uint32_t)quant(fminf(fmaxf(x[e], -Q8_MAX), Q8_MAX), d, inv) & 0xffu) << (8 * (e & 3));
+    for (int e = 0; e < 8; e++) {
+        const float y = fmaf(x[e], inv, big);
+        t[e] = __float_as_uint(y);
+        far = fmaxf(far, fabsf(fmaf(big - y, d, x[e])));
+    }
+    if (far >= 0.5f * d) {  // (4e-5 of the values)
+#pragma unroll
+        for (int e = 0; e < 8; e++) t[e] = (uint32_t)quant(x[e], d, inv);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++)  // the low bytes of four words
+        w[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(t[4 * h + 3], t[4 * h + 2], 0x0c0c0400u),
+                                     __builtin_amdgcn_perm(t[4 * h + 1], t[4 * h], 0x0c0c0400u), 0x05040100u);
     return uint2_t{w[0], w[1]};
+}
+typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max2_u16(uint32_t a, uint32_t b) {
+    ushort2_t x, y;
+    __builtin_memcpy(&x, &a, 4);
+    __builtin_memcpy(&y, &b, 4);
+    x = __builtin_elementwise_max(x, y);
+    __builtin_memcpy(&a, &x, 4);
+    return a;
 }
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 // the largest over the 4 lanes of a block (lanes 4b … 4b + 3 hold 8 values each)
@@ -176,6 +196,8 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256) void k_post_rows
         for (int e = 0; e < 8; e++) top = max(top, abs_bits(y[e]));
         const uint32_t db = block_scale(block_max(top, lane));
         if (id >= count) return;
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = fminf(fmaxf(y[e], -Q8_MAX), Q8_MAX);
         *reinterpret_cast<uint2_t *>((char *)(is_v ? a.kv.v : a.kv.k) + row * D + 8 * j) = quant8(y, db);
         if ((j & 3) == 0) (is_v ? a.kv.vd : a.kv.kd)[row * (D / KV_BLOCK) + (j >> 2)] = (uint16_t)db;
     } else {
@@ -195,56 +217,74 @@ struct CopyArgs {
 };
 constexpr int COPY_ROWS = 64;  // rows a workgroup
 
-// blockIdx.y: K and V of each KV head. Quantise: 16 lanes of 8 values to a row
-__global__ __launch_bounds__(256) void k_kv_quantise(CopyArgs a) {
-    const int lane = threadIdx.x & 63, j = lane & 15, head = blockIdx.y >> 1, is_v = blockIdx.y & 1;
-    const _Float16 *src = (const _Float16 *)(is_v ? a.src.v : a.src.k) + ((size_t)head * a.src.n_ctx + a.src_row) * D;
-    const size_t to = (size_t)head * a.dst.n_ctx + a.dst_row;
-    const int r0 = blockIdx.x * COPY_ROWS + (threadIdx.x >> 4);
-    half8 in[COPY_ROWS / 16];
-#pragma unroll
-    for (int i = 0; i < COPY_ROWS / 16; i++)
-        in[i] = *reinterpret_cast<const half8 *>(src + (size_t)min(r0 + 16 * i, a.n - 1) * D + 8 * j);
-#pragma unroll
-    for (int i = 0; i < COPY_ROWS / 16; i++) {
-        float x[8];
-        uint32_t top = 0;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            x[e] = (float)in[i][e];
-            top = max(top, abs_bits(x[e]));
-        }
-        const uint32_t db = block_scale(block_max(top, lane));
-        const uint2_t q = quant8(x, db);
-        if (r0 + 16 * i < a.n) {
-            const size_t row = to + r0 + 16 * i;
-            *reinterpret_cast<uint2_t *>((char *)(is_v ? a.dst.v : a.dst.k) + row * D + 8 * j) = q;
-            if ((j & 3) == 0) (is_v ? a.dst.vd : a.dst.kd)[row * (D / KV_BLOCK) + (j >> 2)] = (uint16_t)db;
-        }
-    }
+// 16 bytes that are read once
+__device__ __forceinline__ uint4_t load_once(const void *p) {
+    return __builtin_nontemporal_load((const __attribute__((address_space(1))) uint4_t *)(uintptr_t)p);
 }
 
-// read back: 8 lanes of 16 values to a row
+// blockIdx.y: K and V of each KV head. Quantise: 8 lanes of 16 values to a row, 2 lanes to a block; the workgroup's scales
+// through LDS, so that they leave as whole lines too
+__global__ __launch_bounds__(256) void k_kv_quantise(CopyArgs a) {
+    __shared__ __attribute__((aligned(8))) uint16_t s_d[COPY_ROWS][4];
+    const int tid = threadIdx.x, lane = tid & 63, j = tid & 7, head = blockIdx.y >> 1, is_v = blockIdx.y & 1;
+    const _Float16 *src = (const _Float16 *)(is_v ? a.src.v : a.src.k) + ((size_t)head * a.src.n_ctx + a.src_row) * D;
+    const size_t to = (size_t)head * a.dst.n_ctx + a.dst_row;
+    const int r0 = blockIdx.x * COPY_ROWS, r = tid >> 3;
+    uint4_t in[COPY_ROWS / 32][2];
+#pragma unroll
+    for (int i = 0; i < COPY_ROWS / 32; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            in[i][h] = load_once(src + (size_t)min(r0 + r + 32 * i, a.n - 1) * D + 16 * j + 8 * h);
+#pragma unroll
+    for (int i = 0; i < COPY_ROWS / 32; i++) {
+        // (f16's largest, 65504, is 127.07 of the largest scale: its quant is 127 without being saturated first)
+        uint32_t top = 0;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = max2_u16(top, in[i][h][e] & 0x7FFF7FFFu);
+        top = max(top & 0xFFFFu, top >> 16);  // as f16 bits: those of an infinity and past are the largest too
+        top = max(top, lane_swap_u32<1>(top, lane));
+        const uint32_t db = block_scale(abs_bits(half_bits(top)));
+        uint4_t q;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            half8 v;
+            __builtin_memcpy(&v, &in[i][h], 16);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = (float)v[e];
+            const uint2_t w = quant8(x, db);
+            q[2 * h] = w[0], q[2 * h + 1] = w[1];
+        }
+        if (r0 + r + 32 * i < a.n)
+            *reinterpret_cast<uint4_t *>((char *)(is_v ? a.dst.v : a.dst.k) + (to + r0 + r + 32 * i) * D + 16 * j) = q;
+        if ((j & 1) == 0) s_d[r + 32 * i][j >> 1] = (uint16_t)db;
+    }
+    __syncthreads();
+    if (tid < COPY_ROWS && r0 + tid < a.n)
+        reinterpret_cast<uint2_t *>((is_v ? a.dst.vd : a.dst.kd) + to * (D / KV_BLOCK))[r0 + tid] = *reinterpret_cast<const uint2_t *>(s_d[tid]);
+}
+
+// read back: 16 lanes of 8 values to a row (whole lines leave a wave at once)
 __global__ __launch_bounds__(256) void k_kv_read_back(CopyArgs a) {
-    const int j = threadIdx.x & 7, head = blockIdx.y >> 1, is_v = blockIdx.y & 1;
+    const int j = threadIdx.x & 15, head = blockIdx.y >> 1, is_v = blockIdx.y & 1;
     const size_t from = (size_t)head * a.src.n_ctx + a.src_row, to = (size_t)head * a.dst.n_ctx + a.dst_row;
-    const int r0 = blockIdx.x * COPY_ROWS + (threadIdx.x >> 3);
-    uint4_t q[COPY_ROWS / 32];
-    uint16_t d[COPY_ROWS / 32];
+    const int r0 = blockIdx.x * COPY_ROWS + (threadIdx.x >> 4);
+    uint2_t q[COPY_ROWS / 16];
+    uint16_t d[COPY_ROWS / 16];
 #pragma unroll
-    for (int i = 0; i < COPY_ROWS / 32; i++) {
-        const size_t row = from + min(r0 + 32 * i, a.n - 1);
-        q[i] = *reinterpret_cast<const uint4_t *>((const char *)(is_v ? a.src.v : a.src.k) + row * D + 16 * j);
-        d[i] = (is_v ? a.src.vd : a.src.kd)[row * (D / KV_BLOCK) + (j >> 1)];
+    for (int i = 0; i < COPY_ROWS / 16; i++) {
+        const size_t row = from + min(r0 + 16 * i, a.n - 1);
+        q[i] = __builtin_nontemporal_load((const __attribute__((address_space(1))) uint2_t *)(uintptr_t)(
+            (const char *)(is_v ? a.src.v : a.src.k) + row * D + 8 * j));
+        d[i] = (is_v ? a.src.vd : a.src.kd)[row * (D / KV_BLOCK) + (j >> 2)];
     }
 #pragma unroll
-    for (int i = 0; i < COPY_ROWS / 32; i++) {
-        if (r0 + 32 * i >= a.n) continue;
-        _Float16 *o = (_Float16 *)(is_v ? a.dst.v : a.dst.k) + (to + r0 + 32 * i) * D + 16 * j;
-        const half2_t s = scale_pair(d[i]);
-        *reinterpret_cast<half8 *>(o) = dequant8(uint2_t{q[i][0], q[i][1]}, s);
-        *reinterpret_cast<half8 *>(o + 8) = dequant8(uint2_t{q[i][2], q[i][3]}, s);
-    }
+    for (int i = 0; i < COPY_ROWS / 16; i++)
+        if (r0 + 16 * i < a.n)
+            *reinterpret_cast<half8 *>((_Float16 *)(is_v ? a.dst.v : a.dst.k) + (to + r0 + 16 * i) * D + 8 * j) = dequant8(q[i], scale_pair(d[i]));
 }
 
 // the same type on both sides: a row's bytes (16 or 8 units of 16), its 8 bytes of scales
