@@ -1232,7 +1232,7 @@ template <bool TREE, int RT> int launch_split(htr_device *dev, Args &a, const Tr
 template <bool TREE> int launch(htr_device *dev, Args &a, const TreeMask &tree, int max_keys, int sink_rows, int from_row) {
     const int rows = a.n * a.group;
     const int64_t groups = (int64_t)((rows + KB * WR - 1) / (KB * WR)) * a.kv.n_kv;
-    if (groups >= dev->n_cu) {
+    if (rows > KB && groups >= dev->n_cu) {
         a.n_rg = (rows + KB * WR - 1) / (KB * WR), a.n_split = 1;
         if (groups > INT32_MAX) return htr_fail("attention: %d rows of %d KV heads", rows, a.kv.n_kv);
         if (a.kv.q8) HTR_TRY(read_back(dev, a, TREE ? a.n_past + a.n : a.pos0 + a.n, sink_rows, from_row));
@@ -1244,7 +1244,8 @@ template <bool TREE> int launch(htr_device *dev, Args &a, const TreeMask &tree, 
     return launch_split<TREE, 0>(dev, a, tree, max_keys);
 }
 
-int check_rows(const char *me, const float *d_q, size_t q_stride, const htr_kv *kv, int n_head, float *d_out, int64_t n) {
+int check_rows(const char *me, const float *d_q, size_t q_stride, const htr_kv *kv, const HtrKvPlanes &planes, int n_head,
+               float *d_out, int64_t n) {
     if (!d_q || !d_out) return htr_fail("%s: null argument", me);
     if (n_head < 1 || n_head % kv->n_kv) return htr_fail("%s: %d q heads on %d KV heads", me, n_head, kv->n_kv);
     const size_t qd = (size_t)n_head * D;
@@ -1255,6 +1256,7 @@ int check_rows(const char *me, const float *d_q, size_t q_stride, const htr_kv *
     if (n * group > 1 << 30 || n * group * group >= 1ll << 32) return htr_fail("%s: %lld queries of %d heads", me, (long long)n, n_head);
     const uintptr_t q0 = (uintptr_t)d_q, q1 = q0 + 4 * (q_stride * (n - 1) + qd), o0 = (uintptr_t)d_out, o1 = o0 + 4 * qd * n;
     if (q0 < o1 && o0 < q1) return htr_fail("%s: the output overlaps the queries", me);
+    if (htr_kv_overlaps(planes, d_out, 4 * qd * n)) return htr_fail("%s: the output overlaps the cache", me);
     return 0;
 }
 
@@ -1270,7 +1272,7 @@ extern "C" int htr_tree_attention(htr_device *dev, const float *d_q, size_t q_st
     if (n < 1 || n > HTR_TREE_MAX) return htr_fail("%s: %d nodes (1 … %d)", me, n, HTR_TREE_MAX);
     if (n_past < 0 || n_past > kv->n_ctx - n)
         return htr_fail("%s: %d keys and %d nodes in a %d-row cache", me, n_past, n, kv->n_ctx);
-    HTR_TRY(check_rows(me, d_q, q_stride, kv, n_head, d_out, n));
+    HTR_TRY(check_rows(me, d_q, q_stride, kv, a.kv, n_head, d_out, n));
     TreeMask tree{};
     const uint64_t all = n == 64 ? ~0ull : (1ull << n) - 1;
     for (int t = 0; t < n; t++) {
@@ -1294,7 +1296,7 @@ extern "C" int htr_window_attention(htr_device *dev, const float *d_q, size_t q_
     if (n_q < 1 || pos0 < 0 || pos0 > kv->n_ctx - n_q)
         return htr_fail("%s: %d queries from position %d in a %d-row cache", me, n_q, pos0, kv->n_ctx);
     if (window < 1 || n_sink < 0) return htr_fail("%s: a window of %d keys and %d first ones", me, window, n_sink);
-    HTR_TRY(check_rows(me, d_q, q_stride, kv, n_head, d_out, n_q));
+    HTR_TRY(check_rows(me, d_q, q_stride, kv, a.kv, n_head, d_out, n_q));
     HTR_TRY(htr_check_alive(dev));
     const HtrOnDevice on(dev);
     a.q = d_q, a.q_stride = q_stride, a.out = d_out, a.n = n_q, a.n_head = n_head, a.group = n_head / kv->n_kv;

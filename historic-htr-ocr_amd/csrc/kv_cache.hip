@@ -378,6 +378,16 @@ int htr_kv_read_back(htr_device *dev, const HtrKvPlanes &src, int src_row, const
     return htr_launched(dev, "k_kv_read_back");
 }
 
+namespace {
+size_t row_bytes(const HtrKvPlanes &c) { return (size_t)c.n_kv * c.n_ctx * D * (c.q8 ? 1 : 2); }
+size_t scale_bytes(const HtrKvPlanes &c) { return c.q8 ? (size_t)c.n_kv * c.n_ctx * 8 : 0; }
+}  // namespace
+
+bool htr_kv_overlaps(const HtrKvPlanes &kv, const void *p, size_t n) {
+    return overlap(p, n, kv.k, row_bytes(kv)) || overlap(p, n, kv.v, row_bytes(kv)) ||
+           (kv.q8 && (overlap(p, n, kv.kd, scale_bytes(kv)) || overlap(p, n, kv.vd, scale_bytes(kv))));
+}
+
 extern "C" int htr_tree_masks(const int32_t *h_parent, int n, uint64_t *h_mask, int32_t *h_depth) {
     if (!h_parent || !h_mask || !h_depth) return htr_fail("htr_tree_masks: null argument");
     if (n < 1 || n > HTR_TREE_MAX) return htr_fail("htr_tree_masks: %d nodes (1 … %d)", n, HTR_TREE_MAX);
@@ -428,6 +438,9 @@ extern "C" int htr_qkv_post_rows(htr_device *dev, const float *d_q, size_t q_str
     if ((overlap(d_q, q_bytes, d_q_out, out_bytes) && !(d_q == d_q_out && (n == 1 || q_stride == qd))) ||
         overlap(d_k, kv_bytes, d_q_out, out_bytes) || overlap(d_v, kv_bytes, d_q_out, out_bytes))
         return htr_fail("%s: the q output overlaps the input rows", me);
+    if (htr_kv_overlaps(a.kv, d_q, q_bytes) || htr_kv_overlaps(a.kv, d_k, kv_bytes) || htr_kv_overlaps(a.kv, d_v, kv_bytes) ||
+        htr_kv_overlaps(a.kv, d_q_out, out_bytes))
+        return htr_fail("%s: the rows or the q output overlap the cache", me);
     const size_t grid = ((size_t)n * (n_head + 2 * kv->n_kv) + 15) / 16;
     if (grid > (size_t)INT32_MAX) return htr_fail("%s: %d rows of %d heads", me, n, n_head);
     HTR_TRY(htr_check_alive(dev));
@@ -454,16 +467,14 @@ extern "C" int htr_kv_copy(htr_device *dev, const htr_kv *src, int src_row, cons
     if (n < 0 || src_row < 0 || src_row > src->n_ctx - n || dst_row < 0 || dst_row > dst->n_ctx - n)
         return htr_fail("%s: %d rows from row %d of %d to row %d of %d", me, n, src_row, src->n_ctx, dst_row, dst->n_ctx);
     // the caches' planes: apart, or the same ones with rows apart
-    auto bytes = [](const htr_kv *c) { return (size_t)c->n_kv * c->n_ctx * D * (c->type == HTR_GGML_Q8_0 ? 1 : 2); };
-    auto scale_bytes = [](const htr_kv *c) { return (size_t)c->n_kv * c->n_ctx * 8; };
     struct Plane {
         const void *p;
         size_t n;
     };
-    const Plane s[4] = {{a.src.k, bytes(src)}, {a.src.v, bytes(src)}, {a.src.kd, a.src.q8 ? scale_bytes(src) : 0},
-                        {a.src.vd, a.src.q8 ? scale_bytes(src) : 0}};
-    const Plane d[4] = {{a.dst.k, bytes(dst)}, {a.dst.v, bytes(dst)}, {a.dst.kd, a.dst.q8 ? scale_bytes(dst) : 0},
-                        {a.dst.vd, a.dst.q8 ? scale_bytes(dst) : 0}};
+    const Plane s[4] = {{a.src.k, row_bytes(a.src)}, {a.src.v, row_bytes(a.src)}, {a.src.kd, scale_bytes(a.src)},
+                        {a.src.vd, scale_bytes(a.src)}};
+    const Plane d[4] = {{a.dst.k, row_bytes(a.dst)}, {a.dst.v, row_bytes(a.dst)}, {a.dst.kd, scale_bytes(a.dst)},
+                        {a.dst.vd, scale_bytes(a.dst)}};
     const bool apart = src_row + n <= dst_row || dst_row + n <= src_row;
     for (int i = 0; i < 4; i++)
         for (int j = 0; j < 4; j++) {

@@ -13,6 +13,8 @@ struct HtrKvPlanes {
 // 0 with *out filled, or -1 with the message of what is wrong with the cache
 int htr_kv_check(const char *what, const htr_kv *kv, HtrKvPlanes *out);
 
+// whether [p, p + n) touches the cache's memory
+bool htr_kv_overlaps(const HtrKvPlanes &kv, const void *p, size_t n);
 // rows of a q8_0 cache as f16 into another's (n ≥ 1, in range: not checked)
 int htr_kv_read_back(htr_device *dev, const HtrKvPlanes &src, int src_row, const HtrKvPlanes &dst, int dst_row, int n);
 

@@ -1,6 +1,7 @@
 """The operators on a layer's KV cache without a GPU: the tree's masks and depths, and the refusals, which the entry points
 give before they look at the device (a null one here, so that nothing can be launched)."""
 import ctypes as C
+import re
 
 import numpy as np
 import pytest
@@ -90,7 +91,8 @@ def test_good_arguments_reach_the_device_and_bad_caches_do_not(name):
     ("post", dict(depth=[0, 63, 1], pos0=137), "positions 137 … 200"), ("post", dict(n_pos=0), "0-position"),
     ("post", dict(n=65, row0=0, depth=[0] * 65), "65 drafted rows"),
     ("post", dict(qs=516, out=16 << 20), "overlaps"), ("post", dict(out=(16 << 20) + 1024), "overlaps"),
-    ("post", dict(out=32 << 20), "overlaps"),
+    ("post", dict(out=32 << 20), "overlaps"), ("post", dict(out=1 << 20), "overlap the cache"),
+    ("post", dict(v=(2 << 20) - 256), "overlap the cache"),
     ("copy", dict(src_row=96), "from row 96"), ("copy", dict(dst_row=-1), "row -1"), ("copy", dict(n=-1), "-1 rows"),
     ("copy", dict(dst=_kv(n_kv=1, k=5 << 20, v=6 << 20)), "2 KV heads into 1"), ("copy", dict(dst=_kv(), dst_row=4), "overlap"),
     ("copy", dict(dst=_kv(k=(1 << 20) + 256, v=6 << 20), dst_row=50), "overlap"),
@@ -104,6 +106,7 @@ def test_good_arguments_reach_the_device_and_bad_caches_do_not(name):
     ("tree", dict(mask=[1, 2, 8]), "node 2's mask 0x8"), ("tree", dict(out=(16 << 20) + 4096), "overlaps"),
     ("window", dict(out=0), "null argument"), ("window", dict(n=0), "0 queries"), ("window", dict(pos0=98), "position 98"),
     ("window", dict(pos0=-1), "position -1"), ("window", dict(w=0), "window of 0"), ("window", dict(sink=-1), "-1 first"),
+    ("tree", dict(out=(2 << 20) + 64), "overlaps the cache"), ("window", dict(out=(1 << 20) - 2048), "overlaps the cache"),
     ("window", dict(n_head=-2), "-2 q heads"), ("window", dict(qs=0), "0 floats"), ("window", dict(out=16 << 20), "overlaps"),
 ])
 def test_refusals(name, change, match):
@@ -124,3 +127,25 @@ def test_cache_object_takes_scales_of_both():
 
     with pytest.raises(ValueError, match="scales of both"):
         htr.KvCache.of(1, 1, B, B, B)
+
+
+def test_no_lds_access_in_flight_at_a_barrier(tmp_path):
+    """the attention's kernels fill LDS by loads that the compiler does not know and wait for their reads themselves: at each
+    of their barriers, over all paths, no LDS access of the wave is in flight; and the loops that wait for a number of loads
+    have no memory accesses but those loads, so that the number is theirs alone"""
+    from test_kernel_waits import _assembly, _functions, _pending_at_barriers
+
+    seen = 0
+    for name, body in _functions(_assembly("kv_attention", tmp_path)):
+        if "k_kv_attn" not in name or "join" in name:
+            continue
+        at = _pending_at_barriers(body)
+        seen += len(at)
+        assert not any(at.values()), (name, sorted(at.items()))
+        if not re.search("attn_few|attn_split", name):
+            continue  # waits for all of them
+        last = max(i for i, s in enumerate(body) if "_load_lds_" in s)
+        first = min(i for i, s in enumerate(body) if "v_mfma" in s)
+        between = [s for s in body[first:last] if s.startswith(("global_", "buffer_", "flat_", "scratch_"))]
+        assert between and all("_load_lds_" in s for s in between), (name, [s for s in between if "_load_lds_" not in s])
+    assert seen >= 40

@@ -511,6 +511,112 @@ def test_queries_of_any_size(dev, size):
     c.free()
 
 
+# (queries, q heads to a KV head, KV heads): each of the kernels that a call may take
+WAYS = [(3, 2, 2), (11, 2, 8), (40, 3, 2), (128, 2, 64)]
+
+
+@pytest.mark.parametrize("n,group,n_kv", WAYS)
+@pytest.mark.parametrize("q8_0", [False, True], ids=["f16", "q8_0"])
+def test_scores_that_grow_and_fall(dev, n, group, n_kv, q8_0):
+    """the largest score moves with almost every block, up and down by hundreds, so that every sum is taken again and again to
+    another reference: a score of size s errs by 2^-21·s (see the sizes below), and as much its weight"""
+    rows, window = 900, 700
+    k = normal(1, n_kv, rows, 128, std=0.3)
+    k[..., 0] = np.float32(40.0) * np.sin(np.arange(rows) / 37.0).astype(np.float32)
+    c = Cache(dev, k.astype(np.float16), normal(2, n_kv, rows, 128, std=4.0).astype(np.float16), q8_0)
+    q = normal(3, n, n_kv * group, 128)
+    q[..., 0] = np.where(np.arange(n) % 2, 6.0, -6.0)[:, None]
+    pos0 = rows - n
+    got = run_window(dev, q, c, pos0, window, 20, 1.0)
+    heads_seen = slice(0, 2) if n_kv == 64 else slice(0, n_kv)  # (the plain form is slow)
+    keep = q.reshape(n, n_kv, group, 128)[:, heads_seen].reshape(n, -1, 128)
+    want = attention(keep, c.k[heads_seen], c.v[heads_seen], window_seen(n, pos0, window, 20, rows), 1.0)
+    assert rel_rows(got.reshape(n, n_kv, group * 128)[:, heads_seen].reshape(n, -1), want) < BAR * 250 / 8
+    c.free()
+
+
+@pytest.mark.parametrize("n,group,n_kv", WAYS)
+@pytest.mark.parametrize("q8_0", [False, True], ids=["f16", "q8_0"])
+def test_values_that_are_not_finite_in_every_kernel(dev, n, group, n_kv, q8_0):
+    """a row of V with a NaN that the first queries do not see yet, one that has left the last ones' window, and one among the
+    first keys: those that see none of them are as the plain form, the others not finite in those dims alone"""
+    rows, window, sink = n + 300, 150, 3
+    k, v = normal(1, n_kv, rows, 128).astype(np.float16), normal(2, n_kv, rows, 128).astype(np.float16)
+    pos0 = rows - n
+    bad = [(rows - 2, 5), (pos0 - window + 2, 70), (rows - n // 2 - 1, 100)]
+    vv = v.copy()
+    for r, d in bad:
+        vv[:, r, d] = np.nan
+    c = Cache(dev, k, vv, q8_0)
+    kk, clean = (values(*blocks(x)) if q8_0 else x for x in (k, v))
+    q = normal(3, n, n_kv * group, 128)
+    got = run_window(dev, q, c, pos0, window, sink).reshape(n, n_kv * group, 128)
+    seen = window_seen(n, pos0, window, sink, rows)
+    hs = min(n_kv, 2)
+    want = attention(q[:, :hs * group], kk[:hs], clean[:hs], seen, SCALE).reshape(n, hs * group, 128)
+    for t in range(n):
+        hit = {d2 for r, d in bad if seen[t, r] for d2 in (range(d // 32 * 32, d // 32 * 32 + 32) if q8_0 else (d,))}
+        fine = [d for d in range(128) if d not in hit]
+        assert not hit or not np.any(np.isfinite(got[t][:, sorted(hit)])), t
+        assert np.all(np.isfinite(got[t][:, fine])), t
+        if t % 7 == 0 or n < 20:
+            e = np.linalg.norm(got[t, :hs * group][:, fine] - want[t][:, fine], axis=1) / np.linalg.norm(want[t][:, fine], axis=1)
+            assert np.all(e < BAR), t
+    c.free()
+
+
+@pytest.mark.parametrize("q8_0", [False, True], ids=["f16", "q8_0"])
+def test_trees_of_very_many_heads(dev, q8_0):
+    """256 q heads on 64: the kernel of many rows, on a tree"""
+    n, past, n_kv = 64, 77, 64
+    t = random_tree(5, n)
+    c, q = cache(dev, 121, n_kv, past + n, q8_0), normal(122, n, 256, 128)
+    got = run_tree(dev, q, c, t, past).reshape(n, n_kv, 512)
+    want = attention(q[:, 8:16], c.k[2:4], c.v[2:4], tree_seen(t.masks, past, past + n), SCALE)
+    assert rel_rows(got[:, 2:4].reshape(n, -1), want) < BAR
+    c.free()
+
+
+def test_calls_of_changing_shapes_share_the_scratch(dev):
+    """one call after another over caches of 8, 2 and 16 KV heads (partial sums and tickets in an XCD's L2, and through the
+    coherence point), of one to 64 nodes: each as alone"""
+    for i, (n, past, n_kv, group) in enumerate([(1, 3000, 8, 2), (1, 3000, 2, 2), (20, 2000, 8, 1), (64, 900, 16, 1), (1, 1000, 16, 3), (9, 5000, 8, 1),
+                                                (1, 4000, 8, 2), (30, 3000, 1, 2), (1, 700, 8, 4)]):
+        t = random_tree(i, n)
+        c, q = cache(dev, 130 + i, n_kv, past + n, i % 2 == 1), normal(140 + i, n, n_kv * group, 128)
+        assert rel_rows(run_tree(dev, q, c, t, past), attention(q, c.k, c.v, tree_seen(t.masks, past, past + n), SCALE)) < BAR, i
+        c.free()
+
+
+def test_graphs_outlive_the_scratch_they_were_recorded_over(dev):
+    """many queries over a q8_0 cache read rows back into scratch: a graph recorded over it replays right after a larger call
+    has made it anew, and a call that would make it cannot be recorded"""
+    d = htr.Device(0)
+    n_kv, n = 64, 128
+    c, q = cache(d, 151, n_kv, 700, True), normal(152, n, 2 * n_kv, 128)
+    qb, out = d.upload(q), d.alloc(q.nbytes)
+    call = lambda cc, pos0: htr.window_attention(d, qb, n, pos0, 300, 4, cc.kv, 2 * n_kv, SCALE, out)  # noqa: E731
+    d.capture_begin()
+    with pytest.raises(htr.HtrError, match="captured"):
+        call(c, 500)
+    d.capture_end().free()
+    call(c, 500)
+    want = out.download(np.float32)
+    d.capture_begin()
+    call(c, 500)
+    g = d.capture_end()
+    big = Cache(d, *(np.zeros((n_kv, 9000, 128), np.float16) for _ in range(2)), True)
+    before = d.mem_live()["work"]
+    htr.window_attention(d, qb, n, 8000, 9000, 4, big.kv, 2 * n_kv, SCALE, out)
+    assert d.mem_live()["work"] > before
+    for _ in range(3):
+        out.upload(np.zeros(q.size, np.float32))
+        g.launch()
+        assert np.array_equal(bits(out.download(np.float32)), bits(want))
+    g.free()
+    d.close()
+
+
 def test_negative_and_zero_scale(dev):
     c, q = cache(dev, 71, 1, 80), normal(72, 3, 2, 128)
     seen = tree_seen(htr.Tree(np.arange(3) - 1).masks, 77, 80)
