@@ -297,26 +297,29 @@ struct JoinArgs {
     int n_split, n_head, group, rows, n_kv, n_rg, tile;  // tile: rows of a row group's part
 };
 
-// one row's parts g, g + G, … joined by 32 lanes of 4 dims each; s_w: 64 words of the group's own. Returns Σ l
+// one row's parts g, g + G, … joined by 32 lanes of 4 dims each; s_w: 64 words of the group's own. LATER: the parts are an
+// earlier launch's. Returns Σ l
+template <bool LATER>
 __device__ __forceinline__ float join_row(const float *part, const float4 *part_ml, size_t first, size_t step, int ns, int g, int G,
                                           float *s_w, int lane, float4 &y) {
     const int j = lane & 31;
     const float *from = part + first * D + 4 * j;
-    float2 in[8][2];
+    float4 in[8];
+    auto get = [](const float *at) {
+        if constexpr (LATER) return *reinterpret_cast<const float4 *>(at);
+        const float2 a = get64(at), b = get64(at + 2);
+        return make_float4(a.x, a.y, b.x, b.y);
+    };
     auto fetch = [&](int p0) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float *at = from + (size_t)min(p0 + e * G, ns - 1) * step * D;
-            in[e][0] = get64(at), in[e][1] = get64(at + 2);
-        }
+        for (int e = 0; e < 8; e++) in[e] = get(from + (size_t)min(p0 + e * G, ns - 1) * step * D);
     };
     fetch(g);
     float m[2], l[2], top = M_NONE, sum = 0.0f, c = 1.0f;
 #pragma unroll
     for (int e = 0; e < 2; e++) {
-        const float4 *at = part_ml + first + (size_t)min(j + 32 * e, ns - 1) * step;
-        const float2 ml = get64(at);
-        c = get64(&at->z).x;
+        const float4 ml = get(reinterpret_cast<const float *>(part_ml + first + (size_t)min(j + 32 * e, ns - 1) * step));
+        c = ml.z;
         m[e] = j + 32 * e < ns ? ml.x : M_NONE, l[e] = j + 32 * e < ns ? ml.y : 0.0f;
         top = fmaxf(top, m[e]);
     }
@@ -334,8 +337,7 @@ __device__ __forceinline__ float join_row(const float *part, const float4 *part_
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float w = p + e * G < ns ? s_w[p + e * G] : 0.0f;
-            y.x = fmaf(in[e][0].x, w, y.x), y.y = fmaf(in[e][0].y, w, y.y);
-            y.z = fmaf(in[e][1].x, w, y.z), y.w = fmaf(in[e][1].y, w, y.w);
+            y.x = fmaf(in[e].x, w, y.x), y.y = fmaf(in[e].y, w, y.y), y.z = fmaf(in[e].z, w, y.z), y.w = fmaf(in[e].w, w, y.w);
         }
         p += 8 * G;
         if (p >= ns) break;
@@ -358,7 +360,7 @@ __global__ __launch_bounds__(256) void k_kv_attn_join(JoinArgs a) {
     const int id = min((int)blockIdx.x * 2 + (gr >> 2), a.rows * a.n_kv - 1);
     const int kvh = id / a.rows, r = id % a.rows, rg = r / a.tile;
     float4 y;
-    const float sum = join_row(a.part, a.part_ml, ((size_t)kvh * a.n_rg + rg) * a.n_split * a.tile + r % a.tile, a.tile, a.n_split, g, 4,
+    const float sum = join_row<true>(a.part, a.part_ml, ((size_t)kvh * a.n_rg + rg) * a.n_split * a.tile + r % a.tile, a.tile, a.n_split, g, 4,
                                s_w[gr], threadIdx.x & 63, y);
     s_y[gr][j] = y;
     __syncthreads();
@@ -392,7 +394,7 @@ __device__ __forceinline__ void join_last(const Args &a, int kvh, int rg, int r0
     for (int rb = 0; rb < nr; rb += 1 << lg) {
         const int ri = rb + (gr & ((1 << lg) - 1)), part = gr >> lg;
         float4 y;
-        const float sum = join_row(a.part, a.part_ml, g0 + min(ri, nr - 1), tile, a.n_split, part, G, s_w[gr], lane, y);
+        const float sum = join_row<false>(a.part, a.part_ml, g0 + min(ri, nr - 1), tile, a.n_split, part, G, s_w[gr], lane, y);
         if (G > 1) {  // (one pass)
             s_y[tid] = y;
             __syncthreads();
@@ -1210,7 +1212,7 @@ template <bool TREE, int RT> int launch_split(htr_device *dev, Args &a, const Tr
         HTR_TRY(htr_scratch(dev, SCR_KV_ATTN, most * (D + 4) * 4, &p));
         a.part = (float *)p;
         a.part_ml = (float4 *)(a.part + most * D);
-        if (!here) a.xl = 0;  // (the second launch runs on any XCD)
+        if (!here) a.xl = 1;  // (the launch's end hands its stores on)
     }
     const dim3 g((unsigned)a.kv.n_kv, (unsigned)a.n_split, (unsigned)a.n_rg), b(64 * SW);
     if constexpr (RT != 0) {

@@ -26,6 +26,11 @@ typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 
+// 16 bytes that are read once
+__device__ __forceinline__ uint4_t load_once(const void *p) {
+    return __builtin_nontemporal_load((const __attribute__((address_space(1))) uint4_t *)(uintptr_t)p);
+}
+
 // the f16 scale (as bits) of a block whose largest |x| has the f32 bits `top`
 __device__ __forceinline__ uint32_t block_scale(uint32_t top) {
     if (top >= F32_INF) return 0x7E00u;  // a NaN or an infinity
@@ -162,8 +167,8 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256) void k_post_rows
                        : is_v ? a.v + t * a.kv_stride + (size_t)(kvh - a.kv.n_kv) * D
                               : a.k + t * a.kv_stride + (size_t)kvh * D;
     float x[8], y[8];
-    const float4 x0 = *reinterpret_cast<const float4 *>(src + 8 * j), x1 = *reinterpret_cast<const float4 *>(src + 8 * j + 4);
-    x[0] = x0.x, x[1] = x0.y, x[2] = x0.z, x[3] = x0.w, x[4] = x1.x, x[5] = x1.y, x[6] = x1.z, x[7] = x1.w;
+#pragma unroll
+    for (int i = 0; i < 2; i++) *reinterpret_cast<float4 *>(x + 4 * i) = *reinterpret_cast<const float4 *>(src + 8 * j + 4 * i);
     const float *w = is_q ? a.qn : a.kn, *cs = a.rope + (size_t)(a.pos0 + (TREE ? depth.at[t] : t)) * D + 16 * (j & 7);
     float wf[8], c[16];
 #pragma unroll
@@ -216,11 +221,6 @@ struct CopyArgs {
     int src_row, dst_row, n;
 };
 constexpr int COPY_ROWS = 64;  // rows a workgroup
-
-// 16 bytes that are read once
-__device__ __forceinline__ uint4_t load_once(const void *p) {
-    return __builtin_nontemporal_load((const __attribute__((address_space(1))) uint4_t *)(uintptr_t)p);
-}
 
 // blockIdx.y: K and V of each KV head. Quantise: 8 lanes of 16 values to a row, 2 lanes to a block; the workgroup's scales
 // through LDS, so that they leave as whole lines too
