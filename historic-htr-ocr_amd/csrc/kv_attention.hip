@@ -207,9 +207,11 @@ template <int N, int G> __device__ __forceinline__ float q_pairs(const float *qr
             x[ks][e] *= scale;
             top = fmaxf(top, fabsf(x[ks][e]));
         }
-    if constexpr (G == 4) top = pair_max<16>(top);
+    if constexpr (G == 16) top = group_max<8>(top, threadIdx.x & 63);  // 16 lanes in a row
+    if constexpr (G == 4) top = pair_max<16>(top);                     // every 16th lane
+    if constexpr (G <= 4) top = pair_max<32>(top);                     // every 32nd
     // (a row of nothing but tiny values: its scores are 0 to f32 either way, and the factor stays a normal number)
-    const int ex = max(__builtin_amdgcn_frexp_expf(pair_max<32>(top)), -100);
+    const int ex = max(__builtin_amdgcn_frexp_expf(top), -100);
     const float up = ldexpf(1.0f, 10 - ex);
 #pragma unroll
     for (int ks = 0; ks < N; ks++) {
@@ -287,7 +289,11 @@ template <typename F> __device__ __forceinline__ void put_nan(f32x16 (&o)[4], ui
 // Where the keys are split, a part's (m, l, c) and O go to memory; few of them are joined by the row group's workgroup that is
 // the last there (a ticket), many by a second launch.
 constexpr int SW = 8, UK = 16, ST = SW / 2;  // waves; keys of a unit; steps of 32 keys of a round
-constexpr int JOIN_HERE = 256;               // rows × parts that the last workgroup joins itself
+// Rows × parts that the last workgroup joins itself, its parts in the L2 of its XCD or through the coherence point. In the L2
+// (16 q heads on 8 KV heads) both ways take the same time from 100 to 256: 7 tokens over 1000 … 2000 keys 7.5 … 8.6 µs, as many
+// or 1 µs more by a second launch, which costs the host 4 µs too; with 500 14.1 and 11.9. Through the coherence point 60 tokens
+// on 4 KV heads over 1000 … 4500 keys (128 … 256) take 12.7 … 16.1 and 11.2 … 14.2; one token (16 … 64) 7.6 … 8.7 both ways.
+constexpr int JOIN_L2 = 256, JOIN_FAR = 64;
 
 struct JoinArgs {
     const float *part;
@@ -700,8 +706,9 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     constexpr int WAVE = Q8 ? 2 * QT + 16 : TILE;  // chunks of a wave's LDS
     static_assert(WAVE >= 1024, "a wave's sums fit");
     __shared__ __attribute__((aligned(16))) uint4_t s_kv[SW][WAVE];
-    __shared__ float s_ml[SW][2][KB];
-    __shared__ float s_w[2 * SW][MAX_SPLIT];
+    __shared__ __attribute__((aligned(16))) uint4_t s_q[2][16 * KB];  // the rows' pairs; then the join's
+    __shared__ float s_ml[SW][2][KB], s_c[KB];
+    auto &s_w = *reinterpret_cast<float(*)[2 * SW][MAX_SPLIT]>(&s_q[0][0]);
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hf = lane >> 5, c = lane & 31;
@@ -764,8 +771,26 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     }
 
     half8 qh[8], ql[8];
+    {
+        // each thread makes the pairs of 8 dims of a row; the operands come back from LDS (dims 8j … of row c at 32j + (c ^ j):
+        // 16 threads' writes and 32 lanes' reads fall on different bank groups)
+        const int j = tid & 15, rq = tid >> 4;
+        const Row<TREE> mine(a, tree, kvh, r0 + rq);
+        half8 h[1], r[1];
+        const float f = q_pairs<1, 16>(a.q + (size_t)mine.t * a.q_stride + (size_t)mine.head * D + 8 * j, a.scale, h, r);
+        *reinterpret_cast<half8 *>(&s_q[0][KB * j + (rq ^ j)]) = h[0];
+        *reinterpret_cast<half8 *>(&s_q[1][KB * j + (rq ^ j)]) = r[0];
+        if (j == 0) s_c[rq] = f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++) {
+        const int j = 2 * ks + hf, at = KB * j + (c ^ j);
+        qh[ks] = *reinterpret_cast<const half8 *>(&s_q[0][at]);
+        ql[ks] = *reinterpret_cast<const half8 *>(&s_q[1][at]);
+    }
     const Row<TREE> row(a, tree, kvh, r0 + c);
-    const float sc = q_pairs<8, 2>(a.q + (size_t)row.t * a.q_stride + (size_t)row.head * D + 8 * hf, a.scale, qh, ql);
+    const float sc = s_c[c];
     float m = M_NONE, l = 0.0f;
     f32x16 o[4];
 #pragma unroll
@@ -1203,7 +1228,7 @@ template <bool TREE, int RT> int launch_split(htr_device *dev, Args &a, const Tr
     a.n_split = std::max(1, std::min({dev->n_cu / groups, max_run, MAX_SPLIT}));
     if (max_run <= 3) a.n_split = 1;
     a.xl = a.kv.n_kv % 8 == 0 && dev->xcd_round_robin == 1;
-    const bool here = std::min(rows, tile) * a.n_split <= JOIN_HERE;
+    const bool here = std::min(rows, tile) * a.n_split <= (a.xl ? JOIN_L2 : JOIN_FAR);
     if (a.n_split > 1) {
         void *p;
         HTR_TRY(htr_scratch(dev, SCR_KV_TICKET, (size_t)dev->n_cu * TICKET * 4, &p));
