@@ -1228,16 +1228,16 @@ template <bool TREE, int RT> int launch_split(htr_device *dev, Args &a, const Tr
     a.n_split = std::max(1, std::min({dev->n_cu / groups, max_run, MAX_SPLIT}));
     if (max_run <= 3) a.n_split = 1;
     a.xl = a.kv.n_kv % 8 == 0 && dev->xcd_round_robin == 1;
-    const bool here = std::min(rows, tile) * a.n_split <= (a.xl ? JOIN_L2 : JOIN_FAR);
+    const bool same = std::min(rows, tile) * a.n_split <= (a.xl ? JOIN_L2 : JOIN_FAR);
     if (a.n_split > 1) {
         void *p;
         HTR_TRY(htr_scratch(dev, SCR_KV_TICKET, (size_t)dev->n_cu * TICKET * 4, &p));
-        if (here) a.tickets = (uint32_t *)p;
+        if (same) a.tickets = (uint32_t *)p;
         const size_t most = (size_t)dev->n_cu * KB;  // rows of partial sums
         HTR_TRY(htr_scratch(dev, SCR_KV_ATTN, most * (D + 4) * 4, &p));
         a.part = (float *)p;
         a.part_ml = (float4 *)(a.part + most * D);
-        if (!here) a.xl = 1;  // (the launch's end hands its stores on)
+        if (!same) a.xl = 1;  // (the launch's end hands its stores on)
     }
     const dim3 g((unsigned)a.kv.n_kv, (unsigned)a.n_split, (unsigned)a.n_rg), b(64 * SW);
     if constexpr (RT != 0) {
@@ -1248,7 +1248,7 @@ template <bool TREE, int RT> int launch_split(htr_device *dev, Args &a, const Tr
         else hipLaunchKernelGGL((k_kv_attn_split<false, TREE>), g, b, 0, dev->stream, a, tree);
     }
     HTR_TRY(htr_launched(dev, RT ? "k_kv_attn_few" : "k_kv_attn_split"));
-    if (a.n_split == 1 || here) return 0;
+    if (a.n_split == 1 || same) return 0;
     const JoinArgs ja{a.part, a.part_ml, a.out, a.per_group, a.n_split, a.n_head, a.group, rows, a.kv.n_kv, a.n_rg, tile};
     hipLaunchKernelGGL(k_kv_attn_join, dim3((unsigned)((rows * a.kv.n_kv + 1) / 2)), dim3(256), 0, dev->stream, ja);
     return htr_launched(dev, "k_kv_attn_join");

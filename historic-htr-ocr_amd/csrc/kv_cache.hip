@@ -381,11 +381,30 @@ int htr_kv_read_back(htr_device *dev, const HtrKvPlanes &src, int src_row, const
 namespace {
 size_t row_bytes(const HtrKvPlanes &c) { return (size_t)c.n_kv * c.n_ctx * D * (c.q8 ? 1 : 2); }
 size_t scale_bytes(const HtrKvPlanes &c) { return c.q8 ? (size_t)c.n_kv * c.n_ctx * 8 : 0; }
+struct Plane {
+    const void *p;
+    size_t n;
+};
+struct Planes {
+    Plane of[4];
+    explicit Planes(const HtrKvPlanes &c)
+        : of{{c.k, row_bytes(c)}, {c.v, row_bytes(c)}, {c.kd, scale_bytes(c)}, {c.vd, scale_bytes(c)}} {}
+};
+// a cache that is written to: its planes lie apart
+int check_apart(const char *what, const HtrKvPlanes &kv) {
+    const Planes c(kv);
+    for (int i = 0; i < 4; i++)
+        for (int j = 0; j < i; j++)
+            if (c.of[i].n && c.of[j].n && overlap(c.of[i].p, c.of[i].n, c.of[j].p, c.of[j].n))
+                return htr_fail("%s: the cache's planes overlap", what);
+    return 0;
+}
 }  // namespace
 
 bool htr_kv_overlaps(const HtrKvPlanes &kv, const void *p, size_t n) {
-    return overlap(p, n, kv.k, row_bytes(kv)) || overlap(p, n, kv.v, row_bytes(kv)) ||
-           (kv.q8 && (overlap(p, n, kv.kd, scale_bytes(kv)) || overlap(p, n, kv.vd, scale_bytes(kv))));
+    for (const Plane &c : Planes(kv).of)
+        if (c.n && overlap(p, n, c.p, c.n)) return true;
+    return false;
 }
 
 extern "C" int htr_tree_masks(const int32_t *h_parent, int n, uint64_t *h_mask, int32_t *h_depth) {
@@ -407,6 +426,7 @@ extern "C" int htr_qkv_post_rows(htr_device *dev, const float *d_q, size_t q_str
     const char *me = "htr_qkv_post_rows";
     PostRowsArgs a{};
     HTR_TRY(htr_kv_check(me, kv, &a.kv));
+    HTR_TRY(check_apart(me, a.kv));
     if (!d_q || !d_k || !d_v || !d_q_norm || !d_k_norm || !d_rope || !d_q_out) return htr_fail("%s: null argument", me);
     if (n_head < 1 || n_head % kv->n_kv) return htr_fail("%s: %d q heads on %d KV heads", me, n_head, kv->n_kv);
     const size_t qd = (size_t)n_head * D, kvd = (size_t)kv->n_kv * D;
@@ -441,6 +461,10 @@ extern "C" int htr_qkv_post_rows(htr_device *dev, const float *d_q, size_t q_str
     if (htr_kv_overlaps(a.kv, d_q, q_bytes) || htr_kv_overlaps(a.kv, d_k, kv_bytes) || htr_kv_overlaps(a.kv, d_v, kv_bytes) ||
         htr_kv_overlaps(a.kv, d_q_out, out_bytes))
         return htr_fail("%s: the rows or the q output overlap the cache", me);
+    const Plane read[3] = {{d_q_norm, 4 * D}, {d_k_norm, 4 * D}, {d_rope, (size_t)n_pos * D * 4}};
+    for (const auto &w : read)
+        if (overlap(w.p, w.n, d_q_out, out_bytes) || htr_kv_overlaps(a.kv, w.p, w.n))
+            return htr_fail("%s: the q output or the cache overlaps the norms' weights or the rope table", me);
     const size_t grid = ((size_t)n * (n_head + 2 * kv->n_kv) + 15) / 16;
     if (grid > (size_t)INT32_MAX) return htr_fail("%s: %d rows of %d heads", me, n, n_head);
     HTR_TRY(htr_check_alive(dev));
@@ -467,14 +491,9 @@ extern "C" int htr_kv_copy(htr_device *dev, const htr_kv *src, int src_row, cons
     if (n < 0 || src_row < 0 || src_row > src->n_ctx - n || dst_row < 0 || dst_row > dst->n_ctx - n)
         return htr_fail("%s: %d rows from row %d of %d to row %d of %d", me, n, src_row, src->n_ctx, dst_row, dst->n_ctx);
     // the caches' planes: apart, or the same ones with rows apart
-    struct Plane {
-        const void *p;
-        size_t n;
-    };
-    const Plane s[4] = {{a.src.k, row_bytes(a.src)}, {a.src.v, row_bytes(a.src)}, {a.src.kd, scale_bytes(a.src)},
-                        {a.src.vd, scale_bytes(a.src)}};
-    const Plane d[4] = {{a.dst.k, row_bytes(a.dst)}, {a.dst.v, row_bytes(a.dst)}, {a.dst.kd, scale_bytes(a.dst)},
-                        {a.dst.vd, scale_bytes(a.dst)}};
+    HTR_TRY(check_apart(me, a.dst));
+    const Planes src_planes(a.src), dst_planes(a.dst);
+    const Plane *s = src_planes.of, *d = dst_planes.of;
     const bool apart = src_row + n <= dst_row || dst_row + n <= src_row;
     for (int i = 0; i < 4; i++)
         for (int j = 0; j < 4; j++) {
@@ -501,6 +520,7 @@ extern "C" int htr_kv_keep(htr_device *dev, const htr_kv *kv, int row0, const in
     const char *me = "htr_kv_keep";
     KeepArgs a{};
     HTR_TRY(htr_kv_check(me, kv, &a.kv));
+    HTR_TRY(check_apart(me, a.kv));
     if (n < 0 || n > HTR_TREE_MAX) return htr_fail("%s: %d rows (at most %d)", me, n, HTR_TREE_MAX);
     if (n && !h_idx) return htr_fail("%s: null rows", me);
     if (row0 < 0 || row0 > kv->n_ctx - n) return htr_fail("%s: %d rows from row %d of %d", me, n, row0, kv->n_ctx);

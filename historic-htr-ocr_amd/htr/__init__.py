@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+from array import array
 from dataclasses import dataclass
 
 import numpy as np
@@ -549,8 +550,8 @@ def kv_copy(dev: Device, src: KvCache, src_row: int, dst: KvCache, dst_row: int,
 
 def kv_keep(dev: Device, kv: KvCache, row0: int, rows) -> None:
     """rows row0 + rows[i] to row0 + i, all read before any is written"""
-    n = len(rows)
-    _check(lib().htr_kv_keep(dev.h, kv.ref, row0, (C.c_int32 * max(n, 1))(*rows), n))
+    idx = array("i", rows)
+    _check(lib().htr_kv_keep(dev.h, kv.ref, row0, idx.buffer_info()[0] if idx else None, len(idx)))
 
 
 def tree_attention(dev: Device, q, tree: Tree | int, n_past: int, kv: KvCache, n_head: int, scale: float, out,

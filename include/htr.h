@@ -197,9 +197,10 @@ int htr_tree_masks(const int32_t *h_parent, int n, uint64_t *h_mask, int32_t *h_
  * RoPE at position pos0 + h_depth[t] (row t of a draft: n ≤ 64, depths 0 … 63; h_depth NULL: pos0 + t) from the table
  * d_rope [n_pos][64] × (cos, sin); q to d_q_out [n][n_head·128], k and v to the cache's rows row0 + t. The norm and the
  * turn are computed in f64 and rounded to f32, then to f16 or q8_0 (a block's scale the smallest f16 number d with
- * 127·d ≥ max |x|, its quants x / d to the nearest integer, ties to even; finite values saturate at ±65468.5 = 127·515.5, a block with a
- * NaN or an infinity is NaN). Strides multiples of 4, pointers 16-byte aligned; d_q_out may be d_q where its rows are
- * n_head·128 apart, and overlaps the inputs in no other way; the cache is apart from both (else refused). */
+ * 127·d ≥ max |x|, its quants x / d to the nearest integer, ties to even; finite values saturate at ±65468.5 = 127·515.5,
+ * a block with a NaN or an infinity is NaN). Strides multiples of 4, pointers 16-byte aligned; d_q_out may be d_q where its rows are
+ * n_head·128 apart, and overlaps the inputs in no other way; the cache is apart from both, and its planes from each other
+ * (else refused). */
 int htr_qkv_post_rows(htr_device *dev, const float *d_q, size_t q_stride, const float *d_k, const float *d_v,
                       size_t kv_stride, int n, const float *d_q_norm, const float *d_k_norm, const float *d_rope,
                       int n_pos, int pos0, const int32_t *h_depth, int n_head, float eps, const htr_kv *kv, int row0,
@@ -218,15 +219,15 @@ int htr_kv_keep(htr_device *dev, const htr_kv *kv, int row0, const int32_t *h_id
  * A row that a query does not see does not touch its output, whatever it holds; one that it sees with a value that is not
  * finite gives values that are not. All sums in f32, q and the weights held to 22 bits; over a q8_0 cache the same bits as
  * over its read-back, and the same bits every time. Scratch: 4.4 MB, the same for every size, made at the first call that
- * splits a query's keys (that call cannot be one that is being captured). The output is apart from the queries and the
- * cache (else refused); strides multiples of 4, pointers 16-byte aligned. */
+ * splits a query's keys; and for a q8_0 cache that many rows read (over 8000 rows of q heads), its rows in f16: at
+ * least 32 MB, doubled when it grows, what it was before kept until the device is closed, so that graphs recorded over it
+ * stay good. A call that makes or grows scratch cannot be one that is being captured. The output is apart from the queries
+ * and the cache (else refused); strides multiples of 4, pointers 16-byte aligned. */
 int htr_tree_attention(htr_device *dev, const float *d_q, size_t q_stride, int n, const uint64_t *h_mask, int n_past,
                        const htr_kv *kv, int n_head, float scale, float *d_out);
 /* attention with a sliding window and first keys that stay visible: queries at positions pos0 … pos0 + n_q − 1, the one at
  * p over the cache rows j ≤ p with j < n_sink or j > p − window (window ≥ 1: itself at least) → d_out [n_q][n_head·128].
- * Otherwise as htr_tree_attention; n_q = 1 is a decode step's. Many queries over a q8_0 cache read the rows that they see
- * back into scratch first: at least 32 MB, doubled when it grows, what it was before kept until the device is closed, so
- * that graphs recorded over it stay good (a call that makes or grows it cannot be one that is being captured). */
+ * Otherwise as htr_tree_attention; n_q = 1 is a decode step's, and of a q8_0 cache only the rows that are seen are read. */
 int htr_window_attention(htr_device *dev, const float *d_q, size_t q_stride, int n_q, int pos0, int window, int n_sink,
                          const htr_kv *kv, int n_head, float scale, float *d_out);
 /* the GPU token choice of a greedy preset on n_vocab logits (choose_pen → choose_max → choose_pick,

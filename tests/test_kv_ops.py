@@ -93,6 +93,8 @@ def test_good_arguments_reach_the_device_and_bad_caches_do_not(name):
     ("post", dict(qs=516, out=16 << 20), "overlaps"), ("post", dict(out=(16 << 20) + 1024), "overlaps"),
     ("post", dict(out=32 << 20), "overlaps"), ("post", dict(out=1 << 20), "overlap the cache"),
     ("post", dict(v=(2 << 20) - 256), "overlap the cache"),
+    ("post", dict(out=(64 << 20) + 256), "overlaps the norms"), ("post", dict(qn=(112 << 20) + 4096), "overlaps the norms"),
+    ("post", dict(out=(96 << 20) + 64 * 1024), "overlaps the norms"), ("post", dict(rope=(1 << 20) - 512), "overlaps the norms"),
     ("copy", dict(src_row=96), "from row 96"), ("copy", dict(dst_row=-1), "row -1"), ("copy", dict(n=-1), "-1 rows"),
     ("copy", dict(dst=_kv(n_kv=1, k=5 << 20, v=6 << 20)), "2 KV heads into 1"), ("copy", dict(dst=_kv(), dst_row=4), "overlap"),
     ("copy", dict(dst=_kv(k=(1 << 20) + 256, v=6 << 20), dst_row=50), "overlap"),
@@ -111,6 +113,37 @@ def test_good_arguments_reach_the_device_and_bad_caches_do_not(name):
 ])
 def test_refusals(name, change, match):
     _refused(_calls(_kv())[name](**change), match)
+
+
+@pytest.mark.parametrize("change", [dict(v=1 << 20), dict(v=(1 << 20) + 2 * 100 * 256 - 16), dict(Q8, vd=3 << 20),
+                                    dict(Q8, kd=(2 << 20) + 128)])
+def test_a_cache_that_is_written_to_has_planes_apart(change):
+    kv = _kv(**change)
+    for name in ("post", "keep"):
+        _refused(_calls(kv)[name](), "planes overlap")
+    _refused(_calls(_kv(k=32 << 20, v=33 << 20))["copy"](dst=kv), "planes overlap")
+    for name in ("tree", "window"):
+        _refused(_calls(kv)[name](), "null device")  # read only
+
+
+def test_kv_keep_takes_any_integers_and_no_others():
+    class Dev:
+        h = None
+
+    class B:
+        ptr = 1 << 20
+
+    class V:
+        ptr = 2 << 20
+
+    kv = htr.KvCache.of(2, 100, B, V)
+    for rows in ([], [0, 3], (1,), range(4), np.array([2, 1]), np.array([5], np.int32)):
+        with pytest.raises(htr.HtrError, match="null device"):
+            htr.kv_keep(Dev, kv, 90, rows)
+    with pytest.raises(OverflowError):
+        htr.kv_keep(Dev, kv, 90, [1 << 32])
+    with pytest.raises(TypeError):
+        htr.kv_keep(Dev, kv, 90, [0.5])
 
 
 def test_copy_between_rows_of_one_cache_and_in_place_rows_are_allowed():
