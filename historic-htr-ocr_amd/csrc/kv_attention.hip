@@ -58,7 +58,7 @@ struct Args {
     int n_past;                // tree: the committed keys
     int pos0, window, n_sink;  // window
     int n_rg, n_split;         // row groups, parts of a row group's key blocks
-    float *part;               // [n_kv·n_rg·n_split][16·RT] rows of partial sums o[128], and each row's (m, l, c)
+    float *part;               // [n_kv·n_rg·n_split][rows of a part] sums o[128], and each row's (m, l, c)
     float4 *part_ml;
     uint32_t *tickets;         // [n_kv·n_rg], TICKET words apart: zero, self-resetting; NULL: joined by a second launch
     int xl;                    // a KV head's workgroups share an XCD, and its L2 shows them each other's stores
@@ -273,7 +273,7 @@ template <typename F> __device__ __forceinline__ void put_nan(f32x16 (&o)[4], ui
 
 // ---- few rows: the keys split over workgroups --------------------------------------------------------------------------------
 //
-// A workgroup takes 16·RT rows (RT 1 or 2) and a run of units of 16 keys, eight a round, one to each of its eight waves:
+// A workgroup takes 16 rows and a run of units of 16 keys, eight a round, one to each of its eight waves:
 //   scores   a wave's own unit against all rows, Sᵀ = K·(qh + ql)ᵀ by v_mfma_f32_16x16x32_f16: lane 16g + c holds row c's
 //            scores of keys 4g … 4g + 3; the rows' largest over the waves through LDS (barrier);
 //   weights  p = 2^((s − m)·c + 3) as f16 pairs to LDS, in the order of the next products' operands (barrier);
@@ -288,7 +288,7 @@ template <typename F> __device__ __forceinline__ void put_nan(f32x16 (&o)[4], ui
 // reads of 16 (32) lanes fall on different bank groups.
 // Where the keys are split, a part's (m, l, c) and O go to memory; few of them are joined by the row group's workgroup that is
 // the last there (a ticket), many by a second launch.
-constexpr int SW = 8, UK = 16, ST = SW / 2;  // waves; keys of a unit; steps of 32 keys of a round
+constexpr int SW = 8, UK = 16, ST = SW / 2, FR = 16;  // waves; keys of a unit; steps of 32 keys of a round; rows
 // Rows × parts that the last workgroup joins itself, its parts in the L2 of its XCD or through the coherence point. In the L2
 // (16 q heads on 8 KV heads) both ways take the same time from 100 to 256: 7 tokens over 1000 … 2000 keys 7.5 … 8.6 µs, as many
 // or 1 µs more by a second launch, which costs the host 4 µs too; with 500 14.1 and 11.9. Through the coherence point 60 tokens
@@ -418,22 +418,22 @@ __device__ __forceinline__ void join_last(const Args &a, int kvh, int rg, int r0
     }
 }
 
-template <bool Q8, bool TREE, int RT> __global__ __launch_bounds__(64 * SW, 2) void k_kv_attn_few(Args a, TreeMask tree) {
+template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv_attn_few(Args a, TreeMask tree) {
     constexpr int UC = Q8 ? 8 * UK : 16 * UK;                        // 16-byte chunks of a unit's K or V
     constexpr int NL = Q8 ? UK / 8 + 1 : UK / 4;                     // loads of a unit's K or V
     __shared__ __attribute__((aligned(16))) uint4_t s_k[SW][UC], s_v[2][SW][UC];
-    __shared__ __attribute__((aligned(16))) uint4_t s_p[2][RT][ST][64];  // weights' high and low halves
+    __shared__ __attribute__((aligned(16))) uint4_t s_p[2][ST][64];  // weights' high and low halves
     __shared__ __attribute__((aligned(16))) uint32_t s_kd[Q8 ? SW : 1][64], s_vd[2][Q8 ? SW : 1][64];
     __shared__ __attribute__((aligned(16))) uint16_t s_vt[4][ST][4][8];  // V's scales by dims / 32, step, lane group, slot
-    __shared__ float s_mx[SW][16 * RT], s_l[SW][16 * RT];
+    __shared__ float s_mx[SW][UK], s_l[SW][UK];
     __shared__ float s_w[SW * 2][MAX_SPLIT];
     __shared__ int s_odd[SW], s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c = lane & 15;
     const int kvh = blockIdx.x, split = blockIdx.y, rg = blockIdx.z;
-    const int rows = a.n * a.group, r0 = rg * 16 * RT;
+    const int rows = a.n * a.group, r0 = rg * FR;
     const int n_keys = TREE ? a.n_past + a.n : a.pos0 + a.n;
-    const int ta = query_of(a.group, a.per_group, r0), tb = query_of(a.group, a.per_group, min(r0 + 16 * RT - 1, rows - 1));
+    const int ta = query_of(a.group, a.per_group, r0), tb = query_of(a.group, a.per_group, min(r0 + FR - 1, rows - 1));
     const Blocks blk = blocks_of<TREE, UK>(a, ta, tb);
     const auto [i0, i1] = part_of(blk.count(), split, a.n_split);
     const int n_round = (i1 - i0 + SW - 1) / SW;
@@ -467,22 +467,13 @@ template <bool Q8, bool TREE, int RT> __global__ __launch_bounds__(64 * SW, 2) v
         load(i0 + wave, true, 0);
     }
 
-    half8 qh[RT][4], ql[RT][4];
-    float sc[RT], m[RT], l[RT];
-    int pos[RT];
-    uint64_t mask[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        const Row<TREE> row(a, tree, kvh, r0 + 16 * rt + c);
-        pos[rt] = row.pos, mask[rt] = row.mask;
-        sc[rt] = q_pairs<4, 4>(a.q + (size_t)row.t * a.q_stride + (size_t)row.head * D + 8 * g, a.scale, qh[rt], ql[rt]);
-        m[rt] = M_NONE, l[rt] = 0.0f;
-    }
+    half8 qh[4], ql[4];
+    const Row<TREE> row(a, tree, kvh, r0 + c);
+    const float sc = q_pairs<4, 4>(a.q + (size_t)row.t * a.q_stride + (size_t)row.head * D + 8 * g, a.scale, qh, ql);
+    float m = M_NONE, l = 0.0f;
     // the lane's place in V's units: slots 8g … are keys 4g … 4g + 3 of a step's first unit, then of its second
     const int vrow = Q8 ? 4 * g + ((c >> 1) & 3) : 4 * g + (c >> 2);
-    f32x4 o[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) o[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 
     // whether every row sees all keys of the round's units
     auto whole = [&](int rd) {
@@ -494,7 +485,7 @@ template <bool Q8, bool TREE, int RT> __global__ __launch_bounds__(64 * SW, 2) v
         const int i = i0 + SW * rd + wave, b = rd & 1;
         const bool more = rd + 1 < n_round;
         wait_loads<NL>();  // K; V is still on its way
-        f32x4 s[RT];
+        f32x4 s;
         {
             half8 f[4];
             if constexpr (Q8) {
@@ -514,70 +505,50 @@ template <bool Q8, bool TREE, int RT> __global__ __launch_bounds__(64 * SW, 2) v
             wait_reads();
             if (more) load(i + SW, false, 0);
 #pragma unroll
-            for (int ks = 0; ks < 4; ks++)
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[ks], qh[rt][ks], ks ? s[rt] : f32x4{}, 0, 0, 0);
-                    s[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[ks], ql[rt][ks], s[rt], 0, 0, 0);
-                }
-        }
-        uint32_t seen[RT];
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) seen[rt] = 15u;
-        if (masked) {
-            const int k0 = UK * blk.at(min(i, i1 - 1)) + here(4 * g);
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                seen[rt] = 0;
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const bool v = i < i1 && sees<TREE>(a, pos[rt], mask[rt], k0 + x);
-                    seen[rt] |= (uint32_t)v << x;
-                    s[rt][x] = v ? s[rt][x] : -INFINITY;
-                }
+            for (int ks = 0; ks < 4; ks++) {
+                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[ks], qh[ks], ks ? s : f32x4{}, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[ks], ql[ks], s, 0, 0, 0);
             }
         }
+        uint32_t seen = 15u;
+        if (masked) {
+            const int k0 = UK * blk.at(min(i, i1 - 1)) + here(4 * g);
+            seen = 0;
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            const float mx = pair_max<32>(pair_max<16>(fmaxf(fmaxf(s[rt][0], s[rt][1]), fmaxf(s[rt][2], s[rt][3]))));
-            if (g == 0) s_mx[wave][16 * rt + c] = mx;
+            for (int x = 0; x < 4; x++) {
+                const bool v = i < i1 && sees<TREE>(a, row.pos, row.mask, k0 + x);
+                seen |= (uint32_t)v << x;
+                s[x] = v ? s[x] : -INFINITY;
+            }
         }
+        float mx = pair_max<32>(pair_max<16>(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))));
+        if (g == 0) s_mx[wave][c] = mx;
         wait_reads();
         __builtin_amdgcn_s_barrier();  // everyone's largest scores; everyone is past the values of the round before
         asm volatile("" ::: "memory");
         if (more) load(i + SW, true, b ^ 1);
-        float mx[RT];
-        bool far = false;
+        mx = s_mx[0][c];
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-            mx[rt] = s_mx[0][16 * rt + c];
-#pragma unroll
-            for (int w = 1; w < SW; w++) mx[rt] = fmaxf(mx[rt], s_mx[w][16 * rt + c]);
-            far |= (mx[rt] - m[rt]) * sc[rt] > P_ROOM;
+        for (int w = 1; w < SW; w++) mx = fmaxf(mx, s_mx[w][c]);
+        if (__builtin_amdgcn_ballot_w64((mx - m) * sc > P_ROOM)) {  // (alike in every wave)
+            const float to = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f((m - to) * sc);
+            m = to;
+            l *= corr;
+            o *= corr;
         }
-        if (__builtin_amdgcn_ballot_w64(far)) {  // (alike in every wave)
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                const float to = fmaxf(m[rt], mx[rt]), corr = __builtin_amdgcn_exp2f((m[rt] - to) * sc[rt]);
-                m[rt] = to;
-                l[rt] *= corr;
-                o[rt] *= corr;
-            }
-        }
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
+        {
             float p[4];
 #pragma unroll
-            for (int x = 0; x < 4; x++) p[x] = __builtin_amdgcn_exp2f(fmaf(s[rt][x] - m[rt], sc[rt], P_SHIFT));  // not seen: 2^(−∞) = 0
-            l[rt] += (p[0] + p[1]) + (p[2] + p[3]);
+            for (int x = 0; x < 4; x++) p[x] = __builtin_amdgcn_exp2f(fmaf(s[x] - m, sc, P_SHIFT));  // not seen: 2^(−∞) = 0
+            l += (p[0] + p[1]) + (p[2] + p[3]);
             uint32_t h[2], r[2];
             split2(p[0], p[1], h[0], r[0]);
             split2(p[2], p[3], h[1], r[1]);
             // a weight's sign: not seen
-            h[0] |= (~seen[rt] & 1u) << 15 | (~seen[rt] & 2u) << 30;
-            h[1] |= (~seen[rt] & 4u) << 13 | (~seen[rt] & 8u) << 28;
-            reinterpret_cast<uint2_t *>(&s_p[0][rt][wave >> 1][lane])[wave & 1] = uint2_t{h[0], h[1]};
-            reinterpret_cast<uint2_t *>(&s_p[1][rt][wave >> 1][lane])[wave & 1] = uint2_t{r[0], r[1]};
+            h[0] |= (~seen & 1u) << 15 | (~seen & 2u) << 30;
+            h[1] |= (~seen & 4u) << 13 | (~seen & 8u) << 28;
+            reinterpret_cast<uint2_t *>(&s_p[0][wave >> 1][lane])[wave & 1] = uint2_t{h[0], h[1]};
+            reinterpret_cast<uint2_t *>(&s_p[1][wave >> 1][lane])[wave & 1] = uint2_t{r[0], r[1]};
         }
         if (more) wait_loads<2 * NL>();  // V
         else wait_loads<0>();
@@ -630,63 +601,51 @@ template <bool Q8, bool TREE, int RT> __global__ __launch_bounds__(64 * SW, 2) v
 #pragma unroll
             for (int st = 0; st < ST; st++) {
                 const half8 v = vread(st);
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, *reinterpret_cast<const half8 *>(&s_p[0][rt][st][lane]), o[rt], 0, 0, 0);
-                    o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, *reinterpret_cast<const half8 *>(&s_p[1][rt][st][lane]), o[rt], 0, 0, 0);
-                }
+                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, *reinterpret_cast<const half8 *>(&s_p[0][st][lane]), o, 0, 0, 0);
+                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, *reinterpret_cast<const half8 *>(&s_p[1][st][lane]), o, 0, 0, 0);
             }
         } else {
             // such values as 0, and NaN into the sums of the rows that see one: a product of ones
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
+            f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-                for (int st = 0; st < ST; st++) {
-                    const half8 v = vread(st), z = finite(v);
-                    uint4_t h = s_p[0][rt][st][lane];
-                    half8 ind;
-                    o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(z, *reinterpret_cast<const half8 *>(&h), o[rt], 0, 0, 0);
-                    o[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(z, *reinterpret_cast<const half8 *>(&s_p[1][rt][st][lane]), o[rt], 0, 0, 0);
+            for (int st = 0; st < ST; st++) {
+                const half8 v = vread(st), z = finite(v);
+                uint4_t h = s_p[0][st][lane];
+                half8 ind;
+                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(z, *reinterpret_cast<const half8 *>(&h), o, 0, 0, 0);
+                o = __builtin_amdgcn_mfma_f32_16x16x32_f16(z, *reinterpret_cast<const half8 *>(&s_p[1][st][lane]), o, 0, 0, 0);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) h[e] = ((~h[e] >> 15) & 0x00010001u) * 0x3C00u;
-                    __builtin_memcpy(&ind, &h, 16);
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones_of_not_finite(v), ind, t, 0, 0, 0);
-                }
-#pragma unroll
-                for (int x = 0; x < 4; x++) o[rt][x] = t[x] > 0.0f ? NAN : o[rt][x];
+                for (int e = 0; e < 4; e++) h[e] = ((~h[e] >> 15) & 0x00010001u) * 0x3C00u;
+                __builtin_memcpy(&ind, &h, 16);
+                t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones_of_not_finite(v), ind, t, 0, 0, 0);
             }
+#pragma unroll
+            for (int x = 0; x < 4; x++) o[x] = t[x] > 0.0f ? NAN : o[x];
         }
     }
     // Σ l over the lanes and waves (m is the same in every wave)
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        l[rt] = pair_sum<32>(pair_sum<16>(l[rt]));
-        if (g == 0) s_l[wave][16 * rt + c] = l[rt];
-    }
+    l = pair_sum<32>(pair_sum<16>(l));
+    if (g == 0) s_l[wave][c] = l;
     __syncthreads();
-    const size_t g0 = ((size_t)kvh * a.n_rg + rg) * a.n_split * (16 * RT);  // the row group's first row of partial sums
+    const size_t g0 = ((size_t)kvh * a.n_rg + rg) * a.n_split * FR;  // the row group's first row of partial sums
+    l = 0.0f;
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        const int r = r0 + 16 * rt + c;
-        float sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < SW; w++) sum += s_l[w][16 * rt + c];
-        if (r >= rows) continue;
+    for (int w = 0; w < SW; w++) l += s_l[w][c];
+    if (row.r < rows) {
         if (a.n_split == 1) {
-            put_row(a.out, a.n_head, a.group, a.per_group, kvh, r, 4 * wave + g, make_float4(o[rt][0], o[rt][1], o[rt][2], o[rt][3]), sum);
-            continue;
-        }
-        const size_t pr = g0 + (size_t)split * (16 * RT) + 16 * rt + c;
-        float *to = a.part + pr * D + 16 * wave + 4 * g;
-        put64(to, o[rt][0], o[rt][1], a.xl);
-        put64(to + 2, o[rt][2], o[rt][3], a.xl);
-        if (wave == 0 && g == 0) {
-            put64(a.part_ml + pr, m[rt], sum, a.xl);
-            put64(&a.part_ml[pr].z, sc[rt], 0.0f, a.xl);
+            put_row(a.out, a.n_head, a.group, a.per_group, kvh, row.r, 4 * wave + g, make_float4(o[0], o[1], o[2], o[3]), l);
+        } else {
+            const size_t pr = g0 + (size_t)split * FR + c;
+            float *to = a.part + pr * D + 16 * wave + 4 * g;
+            put64(to, o[0], o[1], a.xl);
+            put64(to + 2, o[2], o[3], a.xl);
+            if (wave == 0 && g == 0) {
+                put64(a.part_ml + pr, m, l, a.xl);
+                put64(&a.part_ml[pr].z, sc, 0.0f, a.xl);
+            }
         }
     }
-    if (a.tickets) join_last(a, kvh, rg, r0, rows, 16 * RT, g0, &s_last, s_w, reinterpret_cast<float4 *>(&s_k[0][0]));
+    if (a.tickets) join_last(a, kvh, rg, r0, rows, FR, g0, &s_last, s_w, reinterpret_cast<float4 *>(&s_k[0][0]));
 }
 
 // ---- few rows: the blocks split over workgroups ----------------------------------------------------------------------------
@@ -1219,9 +1178,9 @@ int read_back(htr_device *dev, Args &a, int n_keys, int sink_rows, int from_row)
     return 0;
 }
 
-// RT: 16·RT rows a workgroup in rounds of 128 keys; 0: 32 rows, each of the waves its own blocks of 32 keys
-template <bool TREE, int RT> int launch_split(htr_device *dev, Args &a, const TreeMask &tree, int max_keys) {
-    const int rows = a.n * a.group, tile = RT ? 16 * RT : KB, run = (RT ? UK : KB) * SW;
+// FEW: 16 rows a workgroup in rounds of 128 keys; else 32 rows, each of the waves its own blocks of 32 keys
+template <bool TREE, bool FEW> int launch_split(htr_device *dev, Args &a, const TreeMask &tree, int max_keys) {
+    const int rows = a.n * a.group, tile = FEW ? FR : KB, run = (FEW ? UK : KB) * SW;
     a.n_rg = (rows + tile - 1) / tile;
     const int groups = a.n_rg * a.kv.n_kv, max_run = (max_keys + run - 1) / run;
     // a workgroup a CU, no more parts than rounds; no parts where they would save less than they cost
@@ -1240,14 +1199,14 @@ template <bool TREE, int RT> int launch_split(htr_device *dev, Args &a, const Tr
         if (!same) a.xl = 1;  // (the launch's end hands its stores on)
     }
     const dim3 g((unsigned)a.kv.n_kv, (unsigned)a.n_split, (unsigned)a.n_rg), b(64 * SW);
-    if constexpr (RT != 0) {
-        if (a.kv.q8) hipLaunchKernelGGL((k_kv_attn_few<true, TREE, RT>), g, b, 0, dev->stream, a, tree);
-        else hipLaunchKernelGGL((k_kv_attn_few<false, TREE, RT>), g, b, 0, dev->stream, a, tree);
+    if constexpr (FEW) {
+        if (a.kv.q8) hipLaunchKernelGGL((k_kv_attn_few<true, TREE>), g, b, 0, dev->stream, a, tree);
+        else hipLaunchKernelGGL((k_kv_attn_few<false, TREE>), g, b, 0, dev->stream, a, tree);
     } else {
         if (a.kv.q8) hipLaunchKernelGGL((k_kv_attn_split<true, TREE>), g, b, 0, dev->stream, a, tree);
         else hipLaunchKernelGGL((k_kv_attn_split<false, TREE>), g, b, 0, dev->stream, a, tree);
     }
-    HTR_TRY(htr_launched(dev, RT ? "k_kv_attn_few" : "k_kv_attn_split"));
+    HTR_TRY(htr_launched(dev, FEW ? "k_kv_attn_few" : "k_kv_attn_split"));
     if (a.n_split == 1 || same) return 0;
     const JoinArgs ja{a.part, a.part_ml, a.out, a.per_group, a.n_split, a.n_head, a.group, rows, a.kv.n_kv, a.n_rg, tile};
     hipLaunchKernelGGL(k_kv_attn_join, dim3((unsigned)((rows * a.kv.n_kv + 1) / 2)), dim3(256), 0, dev->stream, ja);
@@ -1258,17 +1217,16 @@ template <bool TREE, int RT> int launch_split(htr_device *dev, Args &a, const Tr
 // (both multiples of 32) hold all that is seen
 template <bool TREE> int launch(htr_device *dev, Args &a, const TreeMask &tree, int max_keys, int sink_rows, int from_row) {
     const int rows = a.n * a.group;
-    const int64_t groups = (int64_t)((rows + KB * WR - 1) / (KB * WR)) * a.kv.n_kv;
-    if (rows > KB && groups >= dev->n_cu) {
+    if (rows > KB && (int64_t)((rows + KB - 1) / KB) * a.kv.n_kv > 3 * dev->n_cu) {
         a.n_rg = (rows + KB * WR - 1) / (KB * WR), a.n_split = 1;
+        const int64_t groups = (int64_t)a.n_rg * a.kv.n_kv;
         if (groups > INT32_MAX) return htr_fail("attention: %d rows of %d KV heads", rows, a.kv.n_kv);
         if (a.kv.q8) HTR_TRY(read_back(dev, a, TREE ? a.n_past + a.n : a.pos0 + a.n, sink_rows, from_row));
         hipLaunchKernelGGL((k_kv_attn<TREE>), dim3((unsigned)groups), dim3(64 * WR * WP), 0, dev->stream, a, tree);
         return htr_launched(dev, "k_kv_attn");
     }
-    if (rows <= 16) return launch_split<TREE, 1>(dev, a, tree, max_keys);
-    if (rows <= 32) return launch_split<TREE, 2>(dev, a, tree, max_keys);
-    return launch_split<TREE, 0>(dev, a, tree, max_keys);
+    if (rows <= FR) return launch_split<TREE, true>(dev, a, tree, max_keys);
+    return launch_split<TREE, false>(dev, a, tree, max_keys);
 }
 
 int check_rows(const char *me, const float *d_q, size_t q_stride, const htr_kv *kv, const HtrKvPlanes &planes, int n_head,

@@ -393,7 +393,8 @@ def test_tree_masks_of_any_kind(dev, past):
 @pytest.mark.parametrize("n,pos0,window,sink,n_kv,group,gap", [
     (1, 0, 1, 0, 1, 1, 0), (1, 0, 5, 3, 2, 2, 0), (1, 500, 64, 4, 8, 2, 128), (1, 500, 1, 0, 2, 1, 0), (3, 29, 2, 40, 2, 2, 0),
     (33, 0, 8, 0, 2, 2, 0), (40, 100, 33, 1, 1, 5, 0), (65, 31, 32, 64, 2, 2, 4), (130, 0, 1000, 0, 8, 2, 0), (200, 70, 50, 33, 1, 3, 0),
-    (300, 11, 97, 5, 2, 4, 0), (257, 0, 2 ** 31 - 1, 2 ** 31 - 1, 1, 2, 0), (70, 40, 1, 2, 2, 2, 0)])
+    (300, 11, 97, 5, 2, 4, 0), (257, 0, 2 ** 31 - 1, 2 ** 31 - 1, 1, 2, 0), (70, 40, 1, 2, 2, 2, 0),
+    (150, 100, 33, 40, 64, 3, 4), (131, 0, 2 ** 31 - 1, 0, 128, 2, 0), (99, 7, 50, 0, 128, 2, 0)])
 def test_window_attention(dev, q8_0, n, pos0, window, sink, n_kv, group, gap):
     rows = pos0 + n + 2
     c = cache(dev, 200 + n, n_kv, rows, q8_0)
@@ -415,11 +416,12 @@ def test_attention_over_q8_0_is_that_over_its_read_back(dev):
     c = cache(dev, 31, 8, 3000, True)
     back = cache(dev, 33, 8, 3000)
     htr.kv_copy(dev, c.kv, 0, back.kv, 0, 3000)
-    q = normal(34, 700, 16, 128)
+    q = normal(34, 2000, 16, 128)
     for n, past in ((1, 2900), (64, 2900), (13, 7)):
         t = random_tree(n, n)
         assert np.array_equal(bits(run_tree(dev, q[:n], c, t, past)), bits(run_tree(dev, q[:n], back, t, past)))
-    for n, pos0, w, s in ((1, 2000, 500, 4), (700, 1000, 300, 4), (700, 2300, 2 ** 20, 0)):
+    for n, pos0, w, s in ((1, 2000, 500, 4), (700, 1000, 300, 4), (700, 2300, 2 ** 20, 0),
+                          (2000, 1000, 300, 4), (2000, 1000, 2 ** 20, 0)):
         assert np.array_equal(bits(run_window(dev, q[:n], c, pos0, w, s)), bits(run_window(dev, q[:n], back, pos0, w, s)))
     c.free()
     back.free()
@@ -512,7 +514,7 @@ def test_queries_of_any_size(dev, size):
 
 
 # (queries, q heads to a KV head, KV heads): each of the kernels that a call may take
-WAYS = [(3, 2, 2), (11, 2, 8), (40, 3, 2), (128, 2, 64)]
+WAYS = [(3, 2, 2), (11, 2, 8), (40, 3, 2), (200, 2, 64)]
 
 
 @pytest.mark.parametrize("n,group,n_kv", WAYS)
@@ -567,10 +569,10 @@ def test_values_that_are_not_finite_in_every_kernel(dev, n, group, n_kv, q8_0):
 
 @pytest.mark.parametrize("q8_0", [False, True], ids=["f16", "q8_0"])
 def test_trees_of_very_many_heads(dev, q8_0):
-    """256 q heads on 64: the kernel of many rows, on a tree"""
-    n, past, n_kv = 64, 77, 64
+    """512 q heads on 128: the kernel of many rows, on a tree"""
+    n, past, n_kv = 64, 77, 128
     t = random_tree(5, n)
-    c, q = cache(dev, 121, n_kv, past + n, q8_0), normal(122, n, 256, 128)
+    c, q = cache(dev, 121, n_kv, past + n, q8_0), normal(122, n, 512, 128)
     got = run_tree(dev, q, c, t, past).reshape(n, n_kv, 512)
     want = attention(q[:, 8:16], c.k[2:4], c.v[2:4], tree_seen(t.masks, past, past + n), SCALE)
     assert rel_rows(got[:, 2:4].reshape(n, -1), want) < BAR
@@ -592,7 +594,7 @@ def test_graphs_outlive_the_scratch_they_were_recorded_over(dev):
     """many queries over a q8_0 cache read rows back into scratch: a graph recorded over it replays right after a larger call
     has made it anew, and a call that would make it cannot be recorded"""
     d = htr.Device(0)
-    n_kv, n = 64, 128
+    n_kv, n = 64, 200
     c, q = cache(d, 151, n_kv, 700, True), normal(152, n, 2 * n_kv, 128)
     qb, out = d.upload(q), d.alloc(q.nbytes)
     call = lambda cc, pos0: htr.window_attention(d, qb, n, pos0, 300, 4, cc.kv, 2 * n_kv, SCALE, out)  # noqa: E731
