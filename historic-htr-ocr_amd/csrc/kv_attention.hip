@@ -4,22 +4,26 @@
 //   out[t][h] = Σ_j p_j·v_j / Σ_j p_j,  p_j = e^(scale·q·k_j − m)  over the keys j that query t sees (zeros if none)
 //
 // The q heads of a KV head share its keys, so a KV head's queries are rows (t, head of the group), packed: row r is query
-// r / group. A wave works on 32 rows, a block of 32 keys at a time. Few rows: the blocks are split over workgroups
-// (k_kv_attn_split); many: a workgroup takes 64 rows and all their blocks (k_kv_attn).
+// r / group. Up to 16 rows: workgroups of 16 rows and a part of the keys, which share every key (k_kv_attn_few); more:
+// workgroups of 32 rows and a part of the keys, whose waves take blocks of their own (k_kv_attn_split); many: workgroups of
+// 64 rows and all their keys (k_kv_attn). Parts are joined by the last workgroup that is there, or by a second launch.
 //
-// On the f16 matrix cores (v_mfma_f32_32x32x16_f16) with f32-grade operands: q and p are pairs of f16 values, 22 bits; K
-// and V are f16 (a q8_0 element stands for f16(q·d): rounded once, 2^-11 of it, beside the block's own step of 2^-8 of its
-// largest); all sums are f32.
+// On the f16 matrix cores with f32-grade operands: q and p are pairs of f16 values, 22 bits, so that both products are two
+// instructions each; K and V are f16 (a q8_0 element stands for f16(q·d): rounded once, 2^-11 of it, beside the block's own
+// step of 2^-8 of its largest); all sums are f32.
 //   q        x = q·scale is rounded to f32 once, and a row is held times 2^(10 − e), e the exponent of its largest, so that
 //            the pair neither overflows nor loses bits whatever the row's size; a score is s·c, c = log2(e)·2^(e − 10);
-//   scores   Sᵀ = K·(qh + ql)ᵀ: lane 32·hf + c holds row c's scores of keys 8(i / 4) + 4hf + i % 4, i < 16;
+//   scores   Sᵀ = K·(qh + ql)ᵀ, keys by rows, so that a lane holds scores of one row (of v_mfma_f32_32x32x16_f16 lane
+//            32·hf + c row c's of keys 8(i / 4) + 4hf + i % 4, i < 16);
 //   softmax  p = 2^((s − m)·c + 3): the difference first, so p is right for scores of any size. m, the row's reference, is
 //            moved to the largest score only when some p would pass 2^8 (O and l are rescaled then); the 3 leaves room
 //            below, and drops out with l, which carries it too;
-//   values   Oᵀ += Vᵀ·(ph + pl)ᵀ, V by transposing LDS reads, p straight from the lane's registers.
+//   values   Oᵀ += Vᵀ·(ph + pl)ᵀ, V by transposing LDS reads, p in the lanes that it was made in.
 // A key that a row does not see is as if it were not there, whatever the cache holds in it: its score becomes −∞ after the
 // product, and values of V that are not finite are taken out of the product of a block that not every row sees, and make
 // NaN of the sums of the rows that do see them.
+//
+// Times below are of calls one after another on an MI355X, 16 q heads on 8 KV heads if nothing else is said.
 #include <algorithm>
 #include <type_traits>
 
@@ -189,14 +193,15 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     __builtin_memcpy(&lo, &r, 4);
 }
 
-// a row's q·scale as f16 pairs, the B operand of steps of 128 / N dims (the lane's first 8 dims at qrow, of `G` lanes that
-// hold the row); the factor of its scores
+// a row's q·scale as f16 pairs, the B operand of N steps (the lane's 8 dims of step 0 at qrow, of `G` lanes that hold the
+// row); the factor of its scores
 template <int N, int G> __device__ __forceinline__ float q_pairs(const float *qrow, float scale, half8 (&qh)[N], half8 (&ql)[N]) {
+    auto dim = [](int ks) { return N == 4 ? 64 * (ks >> 1) + 8 * (ks & 1) : D / N * ks; };
     float x[N][8], top = 0.0f;
 #pragma unroll
     for (int ks = 0; ks < N; ks++) {
-        const float4 a0 = *reinterpret_cast<const float4 *>(qrow + D / N * ks);
-        const float4 a1 = *reinterpret_cast<const float4 *>(qrow + D / N * ks + 4);
+        const float4 a0 = *reinterpret_cast<const float4 *>(qrow + dim(ks));
+        const float4 a1 = *reinterpret_cast<const float4 *>(qrow + dim(ks) + 4);
         x[ks][0] = a0.x, x[ks][1] = a0.y, x[ks][2] = a0.z, x[ks][3] = a0.w;
         x[ks][4] = a1.x, x[ks][5] = a1.y, x[ks][6] = a1.z, x[ks][7] = a1.w;
     }
@@ -271,28 +276,32 @@ template <typename F> __device__ __forceinline__ void put_nan(f32x16 (&o)[4], ui
     }
 }
 
-// ---- few rows: the keys split over workgroups --------------------------------------------------------------------------------
+// ---- up to 16 rows: the keys split over workgroups, shared by the rows --------------------------------------------------------
 //
 // A workgroup takes 16 rows and a run of units of 16 keys, eight a round, one to each of its eight waves:
 //   scores   a wave's own unit against all rows, Sᵀ = K·(qh + ql)ᵀ by v_mfma_f32_16x16x32_f16: lane 16g + c holds row c's
 //            scores of keys 4g … 4g + 3; the rows' largest over the waves through LDS (barrier);
 //   weights  p = 2^((s − m)·c + 3) as f16 pairs to LDS, in the order of the next products' operands (barrier);
 //   values   Oᵀ += Vᵀ·(ph + pl)ᵀ over the round's 128 keys, a wave's own 16 dims. So every K and V value is loaded, and made
-//            f16, once for all the rows, no sums of O are merged between waves, and O is 8 registers at most.
+//            f16, once for all the rows, no sums of O are merged between waves, and O is 4 registers.
 // K and V come straight into LDS, a wave's own unit each: K into one buffer (read by that wave alone, filled again once the
 // scores are taken), V into one of two (filled again when all waves are past the values of the round before). q8_0 units as
 // they are, int8: an operand's 8 quants become f16 in registers (14 VALU instructions), V's by a transposing read of bytes,
 // their scales from LDS in the order of the operand's slots.
 //   f16   [16 keys][16 chunks of 16 bytes], K row r's chunk c at 16r + (c ^ r), V's at 16r + (c ^ 2(r % 8));
-//   q8_0  [16 keys][8 chunks], row r's chunk c at 8r + (c ^ r / 2); the scales [16 keys][4]:
+//   q8_0  [16 keys][8 chunks], row r's chunk c at 8r + (c ^ r / 2), V's of odd units with c ^ 4 too; the scales [16 keys][4]:
 // reads of 16 (32) lanes fall on different bank groups.
-// Where the keys are split, a part's (m, l, c) and O go to memory; few of them are joined by the row group's workgroup that is
-// the last there (a ticket), many by a second launch.
+//
+// Bound: latency. A call takes 5.0 µs up to 128 keys and 0.95 (f16) or 1.2 µs (q8_0) a further round; splitting the keys
+// costs 2.4. One token over 2000 f16 keys 7.8 µs, over 8000 q8_0 keys 10.3 (17.4 MB: 3.5 at a copy's rate). The waves'
+// own blocks of k_kv_attn_split take 9.2 over 1000 keys (here 7.3) and 11.8 over the 8000 (their 32-row products are half or
+// more empty, and their sums have to be merged); at 16 rows the two are as fast, above this way is slower (24 rows over 1300
+// keys 11.6 and 10.7, over 6000 q8_0 keys 15.1 and 12.5).
 constexpr int SW = 8, UK = 16, ST = SW / 2, FR = 16;  // waves; keys of a unit; steps of 32 keys of a round; rows
-// Rows × parts that the last workgroup joins itself, its parts in the L2 of its XCD or through the coherence point. In the L2
-// (16 q heads on 8 KV heads) both ways take the same time from 100 to 256: 7 tokens over 1000 … 2000 keys 7.5 … 8.6 µs, as many
-// or 1 µs more by a second launch, which costs the host 4 µs too; with 500 14.1 and 11.9. Through the coherence point 60 tokens
-// on 4 KV heads over 1000 … 4500 keys (128 … 256) take 12.7 … 16.1 and 11.2 … 14.2; one token (16 … 64) 7.6 … 8.7 both ways.
+// Rows × parts that the last workgroup joins itself, in the L2 of its XCD or through the coherence point; more are joined by a
+// second launch. In the L2 the two are as fast up to 256 (7 tokens over 1300 keys, 154: 9.4 and 8.8 µs; over 400, 56: 7.6 and
+// 8.6), and a launch costs the host 4 µs; with 448 (3000 and more keys) 14.1 and 11.9. Through the coherence point 60 tokens on
+// 4 KV heads over 1000 … 4500 keys (128 … 256) take 12.7 … 16.1 and 11.2 … 14.2, one token (16 … 64) 7.6 … 8.7 both ways.
 constexpr int JOIN_L2 = 256, JOIN_FAR = 64;
 
 struct JoinArgs {
@@ -442,7 +451,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     // the unit i (one past the part's end: the last's, masked) of K, or of V into buffer b; a wave's instruction is 4 (8) whole
     // rows. Rows past the last key are the last key's, and masked
     const uint32_t kx = 16 * ((lane & 15) ^ (lane >> 4)), vx = 16 * ((lane & 15) ^ (2 * (lane >> 4))), r4 = 2 * D * (lane >> 4);
-    const uint32_t bx = 16 * ((lane & 7) ^ (lane >> 4)), r8 = D * (lane >> 3);
+    const uint32_t bx = 16 * ((lane & 7) ^ (lane >> 4)), wx = bx ^ (64 * (wave & 1)), r8 = D * (lane >> 3);
     auto lds_of = [](auto &x) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)(char *)&x; };
     auto load = [&](int i, bool is_v, int b) {
         const int k0 = UK * blk.at(min(i, i1 - 1)), last = min(n_keys - 1 - k0, UK - 1);
@@ -454,7 +463,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
                       is_v ? lds_of(s_vd[b][wave]) : lds_of(s_kd[wave]));
 #pragma unroll
             for (int u = 0; u < 2; u++)
-                lds_load16(base, min(r8 + 8 * D * u, (uint32_t)(D * last)) + (bx ^ (64 * (u & 1))), to + 16 * 64 * u);
+                lds_load16(base, min(r8 + 8 * D * u, (uint32_t)(D * last)) + ((is_v ? wx : bx) ^ (64 * (u & 1))), to + 16 * 64 * u);
         } else {
 #pragma unroll
             for (int u = 0; u < 4; u++)
@@ -469,7 +478,8 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
 
     half8 qh[4], ql[4];
     const Row<TREE> row(a, tree, kvh, r0 + c);
-    const float sc = q_pairs<4, 4>(a.q + (size_t)row.t * a.q_stride + (size_t)row.head * D + 8 * g, a.scale, qh, ql);
+    // (the 8 dims of the lane's operand: of two steps 16 in a row, 16 bytes of quants)
+    const float sc = q_pairs<4, 4>(a.q + (size_t)row.t * a.q_stride + (size_t)row.head * D + 16 * g, a.scale, qh, ql);
     float m = M_NONE, l = 0.0f;
     // the lane's place in V's units: slots 8g … are keys 4g … 4g + 3 of a step's first unit, then of its second
     const int vrow = Q8 ? 4 * g + ((c >> 1) & 3) : 4 * g + (c >> 2);
@@ -493,14 +503,15 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
                 half2_t d2[2];
                 __builtin_memcpy(d2, &dk, 8);
 #pragma unroll
-                for (int ks = 0; ks < 4; ks++) {
-                    const uint2_t w = *reinterpret_cast<const uint2_t *>((const char *)(s_k[wave] + 8 * c + ((2 * ks + (g >> 1)) ^ (c >> 1))) + 8 * (g & 1));
-                    const _Float16 d = d2[ks >> 1][ks & 1];
-                    f[ks] = dequant8(w[0], w[1], half2_t{d, d});
+                for (int h = 0; h < 2; h++) {
+                    const uint4_t w = s_k[wave][8 * c + ((4 * h + g) ^ (c >> 1))];
+                    const _Float16 d = g < 2 ? d2[h][0] : d2[h][1];
+                    f[2 * h] = dequant8(w[0], w[1], half2_t{d, d});
+                    f[2 * h + 1] = dequant8(w[2], w[3], half2_t{d, d});
                 }
             } else {
 #pragma unroll
-                for (int ks = 0; ks < 4; ks++) f[ks] = *reinterpret_cast<const half8 *>(s_k[wave] + 16 * c + ((4 * ks + g) ^ c));
+                for (int ks = 0; ks < 4; ks++) f[ks] = *reinterpret_cast<const half8 *>(s_k[wave] + 16 * c + ((8 * (ks >> 1) + 2 * g + (ks & 1)) ^ c));
             }
             wait_reads();
             if (more) load(i + SW, false, 0);
@@ -582,7 +593,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
             half8 v;
             if constexpr (Q8) {
                 const uint4_t *unit = s_v[b][2 * st] + UC * ((c >> 3) & 1);
-                const auto *p = (const __attribute__((address_space(3))) char *)(unit + 8 * vrow + (wave ^ (vrow >> 1))) + 8 * (c & 1);
+                const auto *p = (const __attribute__((address_space(3))) char *)(unit + 8 * vrow + (wave ^ (vrow >> 1) ^ ((c & 8) >> 1))) + 8 * (c & 1);
                 const int2_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2_t *)p);
                 v = dequant8((uint32_t)w[0], (uint32_t)w[1], *reinterpret_cast<const half8 *>(s_vt[wave >> 1][st][g]));
             } else {
@@ -648,17 +659,24 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     if (a.tickets) join_last(a, kvh, rg, r0, rows, FR, g0, &s_last, s_w, reinterpret_cast<float4 *>(&s_k[0][0]));
 }
 
-// ---- few rows: the blocks split over workgroups ----------------------------------------------------------------------------
+// ---- more rows: the keys split over workgroups, blocks of its own to a wave -----------------------------------------------------
 //
-// A workgroup takes 32 rows, each of its eight waves every eighth block of its part. A wave loads its own blocks straight
-// into LDS of its own, so the waves wait for nobody until their sums are merged; f16 blocks with one buffer for K and one
-// for V, each filled again as soon as it is read (K under the softmax and the values, V under the next scores), q8_0 blocks,
-// half the size, with two, raw: a fragment's 8 quants become f16 in the registers of the one wave that uses them (14 VALU
-// instructions an operand; V's by a transposing read of bytes).
-//   f16   K and V [32 keys][16 chunks of 16 bytes], row r's chunk c at 16r + (c ^ r % 16), V's at 16r + (c ^ 2(r % 8));
-//   q8_0  K and V [32 keys][8 chunks], row r's chunk c at 8r + (c ^ r / 2 % 8); their scales [32 keys][4]; V's once more
-//         as [dims / 32][key / 16][hf][8], the order of an operand's slots.
+// A workgroup takes 32 rows, each of its eight waves every eighth block of 32 keys of its part. A wave loads its own blocks
+// straight into LDS of its own, so the waves wait for nobody until their sums are merged; f16 blocks with one buffer for K
+// and one for V, each filled again as soon as it is read (K under the softmax and the values, V under the next scores), q8_0
+// blocks, half the size, with two, raw: a fragment's 8 quants become f16 in the registers of the one wave that uses them (14
+// VALU instructions an operand; V's by a transposing read of bytes).
+//   f16   K and V [32 keys][16 chunks of 16 bytes], K row r's chunk c at 16r + (c ^ r % 16), V's at 16r + (c ^ 4(r % 4));
+//   q8_0  K and V [32 keys][8 chunks], K row r's chunk c at 8r + (c ^ r / 2 % 8), V's at 8r + (c ^ (r & 2) ^ (r & 8) / 2); their
+//         scales [32 keys][4]; V's once more as [dims / 32][key / 16][hf][8], the order of an operand's slots.
 // Reads of 16 (32) lanes then fall on different bank groups.
+//
+// Bound: of few keys latency (8 µs a call up to 300 keys: 2 until the first block is there, 2 for the merge), of many the
+// instructions of its two waves a SIMD: a block of f16 is 32 MFMA and 256 VALU instructions, 16 of them exponentials, one of
+// q8_0 224 VALU instructions more (MFMA busy 33 %, VALU 56 % over 40013 keys). 64 tokens over 6001 f16 keys 16.2 µs
+// (27 MB: 5.5 at a copy's rate), 27 over 40013 q8_0 keys 30.6 (88 MB: 17.8). With four waves a workgroup the
+// kernels alone took 30.9 and 54.9 for 21.2 and 30. Two row tiles to a wave, which halves the conversions, cost 6.7 µs of the
+// 27 tokens' call: half as many waves, and each longer.
 constexpr int QT = 256 + 256 + 16 + 16;  // 16-byte chunks of a q8_0 buffer: K, V, K scales, V scales
 
 template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv_attn_split(Args a, TreeMask tree) {
@@ -683,8 +701,8 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4_t *)tile;
     // block i's K or V (f16), or all of it into buffer b (q8_0); a wave's instruction is 4 (8) whole rows. Rows past the last
     // key are the last key's, and are masked
-    const uint32_t kx = 16 * ((lane & 15) ^ (lane >> 4)), vx = 16 * ((lane & 15) ^ (2 * (lane >> 4))), r4 = 2 * D * (lane >> 4);
-    const uint32_t bx = 16 * ((lane & 7) ^ (lane >> 4)), r8 = D * (lane >> 3);
+    const uint32_t kx = 16 * ((lane & 15) ^ (lane >> 4)), vx = 16 * ((lane & 15) ^ (4 * (lane >> 4))), r4 = 2 * D * (lane >> 4);
+    const uint32_t bx = 16 * ((lane & 7) ^ (lane >> 4)), wx = 16 * ((lane & 7) ^ (2 * ((lane >> 4) & 1))), r8 = D * (lane >> 3);
     auto load = [&](int i, bool is_v) {
         const int k0 = KB * blk.at(i), last = n_keys - 1 - k0;
         const char *base = (const char *)(is_v ? a.kv.v : a.kv.k) + (head0 + k0) * (2 * D);
@@ -692,12 +710,12 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
         if (last >= KB - 1) {
 #pragma unroll
             for (int u = 0; u < 8; u++)
-                lds_load16(base + 2 * D * 4 * u, r4 + (is_v ? vx ^ (128 * (u & 1)) : kx ^ (64 * (u & 3))), to + 16 * 64 * u);
+                lds_load16(base + 2 * D * 4 * u, r4 + (is_v ? vx : kx ^ (64 * (u & 3))), to + 16 * 64 * u);
         } else {
             const int ln = here(lane);
 #pragma unroll
             for (int u = 0; u < 8; u++)
-                lds_load16(base, 2 * D * min(4 * u + (ln >> 4), last) + (is_v ? vx ^ (128 * (u & 1)) : kx ^ (64 * (u & 3))), to + 16 * 64 * u);
+                lds_load16(base, 2 * D * min(4 * u + (ln >> 4), last) + (is_v ? vx : kx ^ (64 * (u & 3))), to + 16 * 64 * u);
         }
     };
     auto load_q8 = [&](int i, int b) {
@@ -709,14 +727,14 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
             lds_load4(a.kv.kd + row * 4, 4 * lane, to + 16 * 512);
             lds_load4(a.kv.vd + row * 4, 4 * lane, to + 16 * 528);
 #pragma unroll
-            for (int u = 0; u < 8; u++) lds_load16((u < 4 ? kb : vb) + D * 8 * (u & 3), r8 + (bx ^ (64 * (u & 1))), to + 16 * 64 * u);
+            for (int u = 0; u < 8; u++) lds_load16((u < 4 ? kb : vb) + D * 8 * (u & 3), r8 + ((u < 4 ? bx : wx) ^ (64 * (u & 1))), to + 16 * 64 * u);
         } else {
             const int ln = here(lane);
             lds_load4(a.kv.kd + row * 4, 8 * min(ln >> 1, last) + 4 * (ln & 1), to + 16 * 512);
             lds_load4(a.kv.vd + row * 4, 8 * min(ln >> 1, last) + 4 * (ln & 1), to + 16 * 528);
 #pragma unroll
             for (int u = 0; u < 8; u++)
-                lds_load16(u < 4 ? kb : vb, D * min(8 * (u & 3) + (ln >> 3), last) + (bx ^ (64 * (u & 1))), to + 16 * 64 * u);
+                lds_load16(u < 4 ? kb : vb, D * min(8 * (u & 3) + (ln >> 3), last) + ((u < 4 ? bx : wx) ^ (64 * (u & 1))), to + 16 * 64 * u);
         }
     };
     int i = i0 + wave, b = 0;
@@ -729,6 +747,8 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
         }
     }
 
+    // the 8 dims of the lane's operand of a step: of two steps 16 in a row, 16 bytes of quants
+    auto dims8 = [&](int ks) { return 4 * (ks >> 1) + 2 * hf + (ks & 1); };
     half8 qh[8], ql[8];
     {
         // each thread makes the pairs of 8 dims of a row; the operands come back from LDS (dims 8j … of row c at 32j + (c ^ j):
@@ -744,7 +764,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     __syncthreads();
 #pragma unroll
     for (int ks = 0; ks < 8; ks++) {
-        const int j = 2 * ks + hf, at = KB * j + (c ^ j);
+        const int j = dims8(ks), at = KB * j + (c ^ j);
         qh[ks] = *reinterpret_cast<const half8 *>(&s_q[0][at]);
         ql[ks] = *reinterpret_cast<const half8 *>(&s_q[1][at]);
     }
@@ -757,14 +777,14 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
 #pragma unroll
         for (int x = 0; x < 16; x++) o[u][x] = 0.0f;
 
-    // the lane's places in a block: K step ks is key c, dims 16ks + 8hf …; V tile u, step ss, slots 8hf … + 7 are the keys
+    // the lane's places in a block: K step ks is key c, dims 8·dims8 …; V tile u, step ss, slots 8hf … + 7 are the keys
     // 16ss + 4hf … + 3, then 16ss + 8 + 4hf … + 3 (the lane's scores 8ss …) of dims 32u + 16(lane / 16 % 2) …
     const int vrow = Q8 ? 8 * ((lane >> 3) & 1) + 4 * hf + ((lane >> 1) & 3) : 4 * hf + ((lane & 15) >> 2);
     int va[4];
 #pragma unroll
     for (int u = 0; u < 4; u++)
-        va[u] = Q8 ? 16 * (256 + 8 * vrow + ((2 * u + ((lane >> 4) & 1)) ^ (vrow >> 1))) + 8 * (lane & 1)
-                   : 16 * (K_CHUNKS + 16 * vrow + ((4 * u + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (2 * vrow))) + 8 * (lane & 1);
+        va[u] = Q8 ? 16 * (256 + 8 * vrow + ((2 * u + ((lane >> 4) & 1)) ^ (vrow & 2) ^ ((vrow & 8) >> 1))) + 8 * (lane & 1)
+                   : 16 * (K_CHUNKS + 16 * vrow + ((4 * u + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (4 * (vrow & 3)))) + 8 * (lane & 1);
 
     // block i; MASK: not every row sees all of it
     auto step = [&](auto is_masked) {
@@ -793,11 +813,12 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
             const uint2_t dk = reinterpret_cast<const uint2_t *>(buf + 512)[c];
             half2_t d4[2];
             __builtin_memcpy(d4, &dk, 8);
+            uint4_t w;
 #pragma unroll
             for (int ks = 0; ks < 8; ks++) {
-                const uint2_t w = *reinterpret_cast<const uint2_t *>((const char *)(buf + 8 * c + (ks ^ ((c >> 1) & 7))) + 8 * hf);
+                if (ks % 2 == 0) w = buf[8 * c + ((ks + hf) ^ ((c >> 1) & 7))];
                 const _Float16 d = d4[ks >> 2][(ks >> 1) & 1];
-                const half8 f = dequant8(w[0], w[1], half2_t{d, d});
+                const half8 f = dequant8(w[2 * (ks & 1)], w[2 * (ks & 1) + 1], half2_t{d, d});
                 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qh[ks], ks ? s : f32x16{}, 0, 0, 0);
                 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, ql[ks], s, 0, 0, 0);
             }
@@ -806,7 +827,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
 #pragma unroll
             for (int h = 0; h < 2; h++) {
 #pragma unroll
-                for (int ks = 0; ks < 4; ks++) f[ks] = *reinterpret_cast<const half8 *>(buf + 16 * c + ((8 * h + 2 * ks + hf) ^ (c & 15)));
+                for (int ks = 0; ks < 4; ks++) f[ks] = *reinterpret_cast<const half8 *>(buf + 16 * c + (dims8(4 * h + ks) ^ (c & 15)));
                 if (h == 1) {
                     wait_reads();
                     if (more) load(i + SW, false);
@@ -952,12 +973,17 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     if (a.tickets) join_last(a, kvh, rg, r0, rows, KB, g0, &s_last, s_w, reinterpret_cast<float4 *>(&s_kv[0][0]));
 }
 
-// ---- many rows ---------------------------------------------------------------------------------------------------------------
+// ---- many rows -----------------------------------------------------------------------------------------------------------------
 //
 // A workgroup takes 64 rows of a KV head: 4 waves = 2 row tiles × the even / odd key blocks, the two parts merged through
 // LDS at the end. A stage is 2 blocks (32 KB), K and V each double-buffered, K a stage ahead of V: the score MFMAs of the
 // next stage run under the softmax of this one. The cache is f16 (q8_0 rows are read back first: each is used by many
-// workgroups, and 112 VALU instructions a block and wave would be as many as the softmax's).
+// workgroups, and 224 VALU instructions a block and wave would be as many as the softmax's).
+//
+// Bound: the matrix cores' work and the softmax's instructions on the same two waves a SIMD, and the power of the two: 6001
+// queries with a window of 1500 of a q8_0 cache, 149 GFLOP as pairs, 180 µs with 13 of reading back (MFMA busy 50 %, VALU
+// 45 %; of zeros, at the full clock, 147). 1925 with a window of 512 28 µs. 128 rows a workgroup, 8 waves: 198 (their barriers
+// hold twice as many).
 constexpr int WR = 2, WP = 2;  // row tiles, key parts
 
 template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_attn(Args a, TreeMask tree) {
@@ -977,7 +1003,7 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
     // a stage's K or V → buffer st % 2: 4 direct loads a wave, each of the 4 waves 4 rows of 16 (keys past the last: the last)
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4_t *)&s_kv[0][0][64 * wave];
     const int lrow = 4 * wave + (lane >> 4), lc = lane & 15;
-    const uint32_t koff = 16 * (lc ^ (lrow & 15)), voff = 16 * (lc ^ (2 * (lrow & 7)));  // the same for row lrow + 16
+    const uint32_t koff = 16 * (lc ^ (lrow & 15)), voff = 16 * (lc ^ (4 * (lrow & 3)));  // the same for row lrow + 16
     auto issue = [&](int st, bool is_v) {
 #pragma unroll
         for (int p = 0; p < WP; p++) {
@@ -1005,7 +1031,7 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
     const int vrow = 4 * hf + ((lane & 15) >> 2);
 #pragma unroll
     for (int u = 0; u < 4; u++)
-        va[u] = 16 * (K_CHUNKS + 16 * vrow + ((4 * u + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (2 * vrow))) + 8 * (lane & 1);
+        va[u] = 16 * (K_CHUNKS + 16 * vrow + ((4 * u + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (4 * (vrow & 3)))) + 8 * (lane & 1);
 
     f32x16 o[4];
 #pragma unroll
@@ -1164,7 +1190,8 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
 }
 
 // the rows that the queries see, read back into room of the device's: from_row on after the first sink_rows, or all of them
-// where what lies between is less than a quarter (one launch, 3 µs less than two)
+// where what lies between is at most a quarter: one launch, 3 µs less than two (2000 queries with a window of 4096 from 4500 on
+// 121.5 and 124.9 µs, from 16000 on, three quarters between, 124.3 and 122.2)
 int read_back(htr_device *dev, Args &a, int n_keys, int sink_rows, int from_row) {
     if (from_row - sink_rows <= n_keys / 4) sink_rows = from_row = 0;
     const int first = std::min(sink_rows, n_keys), rest = std::max(0, n_keys - from_row);
@@ -1178,12 +1205,13 @@ int read_back(htr_device *dev, Args &a, int n_keys, int sink_rows, int from_row)
     return 0;
 }
 
-// FEW: 16 rows a workgroup in rounds of 128 keys; else 32 rows, each of the waves its own blocks of 32 keys
+// FEW: 16 rows a workgroup in rounds of 128 keys; else 32 rows in rounds of 256, each of the waves its own blocks of 32
 template <bool TREE, bool FEW> int launch_split(htr_device *dev, Args &a, const TreeMask &tree, int max_keys) {
     const int rows = a.n * a.group, tile = FEW ? FR : KB, run = (FEW ? UK : KB) * SW;
     a.n_rg = (rows + tile - 1) / tile;
     const int groups = a.n_rg * a.kv.n_kv, max_run = (max_keys + run - 1) / run;
-    // a workgroup a CU, no more parts than rounds; no parts where they would save less than they cost
+    // a workgroup a CU, no more parts than rounds; no parts where they would save less than they cost: 64 tokens over 700 keys
+    // (3 rounds) 9.0 µs, in parts 11.3; one over 380 keys (3) 6.8 and 7.3, over 500 (4) 7.9 and 7.4
     a.n_split = std::max(1, std::min({dev->n_cu / groups, max_run, MAX_SPLIT}));
     if (max_run <= 3) a.n_split = 1;
     a.xl = a.kv.n_kv % 8 == 0 && dev->xcd_round_robin == 1;
@@ -1217,6 +1245,9 @@ template <bool TREE, bool FEW> int launch_split(htr_device *dev, Args &a, const 
 // (both multiples of 32) hold all that is seen
 template <bool TREE> int launch(htr_device *dev, Args &a, const TreeMask &tree, int max_keys, int sink_rows, int from_row) {
     const int rows = a.n * a.group;
+    // from more than three rounds of 32-row workgroups on the kernel of many rows: with a window of 4096 f16 keys 1000 queries (two
+    // rounds) take 61 µs by workgroups of 32 rows and 72 by it, 1500 (three) 88 and 106, 1750 (four) 117 and 107, 4000 233 and 201;
+    // of q8_0 80 and 90, 117 and 123, 153 and 122; 1500 from position 0 without a window 35 and 35, 2000 52 and 43
     if (rows > KB && (int64_t)((rows + KB - 1) / KB) * a.kv.n_kv > 3 * dev->n_cu) {
         a.n_rg = (rows + KB * WR - 1) / (KB * WR), a.n_split = 1;
         const int64_t groups = (int64_t)a.n_rg * a.kv.n_kv;
