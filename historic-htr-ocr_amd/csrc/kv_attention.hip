@@ -65,7 +65,7 @@ struct Args {
     float *part;               // [n_kv·n_rg·n_split][rows of a part] sums o[128], and each row's (m, l, c)
     float4 *part_ml;
     uint32_t *tickets;         // [n_kv·n_rg], TICKET words apart: zero, self-resetting; NULL: joined by a second launch
-    int xl;                    // a KV head's workgroups share an XCD, and its L2 shows them each other's stores
+    int xl;                    // a row group's workgroups share an XCD, and its L2 shows them each other's stores
 };
 struct TreeMask {
     uint64_t of[HTR_TREE_MAX];
@@ -439,7 +439,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     __shared__ int s_odd[SW], s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c = lane & 15;
-    const int kvh = blockIdx.x, split = blockIdx.y, rg = blockIdx.z;
+    const int kvh = blockIdx.x, rg = blockIdx.y, split = blockIdx.z;
     const int rows = a.n * a.group, r0 = rg * FR;
     const int n_keys = TREE ? a.n_past + a.n : a.pos0 + a.n;
     const int ta = query_of(a.group, a.per_group, r0), tb = query_of(a.group, a.per_group, min(r0 + FR - 1, rows - 1));
@@ -689,7 +689,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hf = lane >> 5, c = lane & 31;
-    const int kvh = blockIdx.x, split = blockIdx.y, rg = blockIdx.z;
+    const int kvh = blockIdx.x, rg = blockIdx.y, split = blockIdx.z;
     const int rows = a.n * a.group, r0 = rg * KB;
     const int n_keys = TREE ? a.n_past + a.n : a.pos0 + a.n;
     const int ta = query_of(a.group, a.per_group, r0), tb = query_of(a.group, a.per_group, min(r0 + KB - 1, rows - 1));
@@ -1214,7 +1214,7 @@ template <bool TREE, bool FEW> int launch_split(htr_device *dev, Args &a, const 
     // (3 rounds) 9.0 µs, in parts 11.3; one over 380 keys (3) 6.8 and 7.3, over 500 (4) 7.9 and 7.4
     a.n_split = std::max(1, std::min({dev->n_cu / groups, max_run, MAX_SPLIT}));
     if (max_run <= 3) a.n_split = 1;
-    a.xl = a.kv.n_kv % 8 == 0 && dev->xcd_round_robin == 1;
+    a.xl = groups % 8 == 0 && dev->xcd_round_robin == 1;  // (a launch's workgroups go to the 8 XCDs in turn)
     const bool same = std::min(rows, tile) * a.n_split <= (a.xl ? JOIN_L2 : JOIN_FAR);
     if (a.n_split > 1) {
         void *p;
@@ -1226,7 +1226,7 @@ template <bool TREE, bool FEW> int launch_split(htr_device *dev, Args &a, const 
         a.part_ml = (float4 *)(a.part + most * D);
         if (!same) a.xl = 1;  // (the launch's end hands its stores on)
     }
-    const dim3 g((unsigned)a.kv.n_kv, (unsigned)a.n_split, (unsigned)a.n_rg), b(64 * SW);
+    const dim3 g((unsigned)a.kv.n_kv, (unsigned)a.n_rg, (unsigned)a.n_split), b(64 * SW);
     if constexpr (FEW) {
         if (a.kv.q8) hipLaunchKernelGGL((k_kv_attn_few<true, TREE>), g, b, 0, dev->stream, a, tree);
         else hipLaunchKernelGGL((k_kv_attn_few<false, TREE>), g, b, 0, dev->stream, a, tree);
