@@ -164,12 +164,16 @@ template <bool TREE> struct Row {
         if constexpr (TREE) mask = tree.of[t];
     }
 };
-template <bool TREE> __device__ __forceinline__ bool sees(const Args &a, int pos, uint64_t mask, int key) {
+// the lowest n bits (none for n ≤ 0, all from 32 on)
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? ~0u : (1u << max(n, 0)) - 1; }
+// the keys k0 … k0 + 31 that the row sees, a bit each
+template <bool TREE> __device__ __forceinline__ uint32_t sees(const Args &a, int pos, uint64_t mask, int k0) {
+    const int n = (TREE ? a.n_past : pos + 1) - k0;  // the committed keys among them; those that are not ahead
     if constexpr (TREE) {
-        const unsigned j = (unsigned)(key - a.n_past);
-        return key < a.n_past || (j < 64u && ((mask >> j) & 1) != 0);
+        const uint32_t drafted = n < 0 ? (n > -64 ? (uint32_t)(mask >> -n) : 0u) : n < 32 ? (uint32_t)mask << n : 0u;
+        return low_bits(n) | drafted;
     } else {
-        return key <= pos && (key < a.n_sink || key > pos - a.window);
+        return low_bits(n) & (~low_bits(n - a.window) | low_bits(a.n_sink - k0));
     }
 }
 // whether the queries ta … tb all see the keys k0 … k0 + U − 1
@@ -255,7 +259,7 @@ __device__ __forceinline__ half8 ones_of_not_finite(half8 v) {
     __builtin_memcpy(&v, w, 16);
     return v;
 }
-// o's sums of the rows that see one: NaN. seen: the lane's 16 keys; vread(u, ss): V's operand of tile u, step ss
+// o's sums of the rows that see one: NaN. seen: the lane's 16 keys (bits 0 … 3, 8 … 11, 16 …, 24 …); vread(u, ss): V's operand of tile u, step ss
 template <typename F> __device__ __forceinline__ void put_nan(f32x16 (&o)[4], uint32_t seen, F vread) {
     half8 ind[2];
 #pragma unroll
@@ -263,7 +267,8 @@ template <typename F> __device__ __forceinline__ void put_nan(f32x16 (&o)[4], ui
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            w[e] = ((seen >> (8 * ss + 2 * e)) & 1) * 0x3C00u | ((seen >> (8 * ss + 2 * e + 1)) & 1) * 0x3C000000u;
+            w[e] = ((seen >> (16 * ss + 4 * (e & 2) + 2 * (e & 1))) & 1) * 0x3C00u |
+                   ((seen >> (16 * ss + 4 * (e & 2) + 2 * (e & 1) + 1)) & 1) * 0x3C000000u;
         __builtin_memcpy(&ind[ss], w, 16);
     }
 #pragma unroll
@@ -524,13 +529,9 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
         uint32_t seen = 15u;
         if (masked) {
             const int k0 = UK * blk.at(min(i, i1 - 1)) + here(4 * g);
-            seen = 0;
+            seen = i < i1 ? sees<TREE>(a, row.pos, row.mask, k0) : 0u;
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const bool v = i < i1 && sees<TREE>(a, row.pos, row.mask, k0 + x);
-                seen |= (uint32_t)v << x;
-                s[x] = v ? s[x] : -INFINITY;
-            }
+            for (int x = 0; x < 4; x++) s[x] = seen >> x & 1 ? s[x] : -INFINITY;
         }
         float mx = pair_max<32>(pair_max<16>(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))));
         if (g == 0) s_mx[wave][c] = mx;
@@ -841,13 +842,9 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
         }
         uint32_t seen = 0;
         if constexpr (MASK) {
-            const int k0 = KB * blk.at(i) + here(4 * hf);
+            seen = sees<TREE>(a, row.pos, row.mask, KB * blk.at(i) + here(4 * hf));
 #pragma unroll
-            for (int x = 0; x < 16; x++) {
-                const bool v = sees<TREE>(a, row.pos, row.mask, k0 + 8 * (x >> 2) + (x & 3));
-                seen |= (uint32_t)v << x;
-                s[x] = v ? s[x] : -INFINITY;
-            }
+            for (int x = 0; x < 16; x++) s[x] = seen >> (8 * (x >> 2) + (x & 3)) & 1 ? s[x] : -INFINITY;
         }
         float mx = s[0];
 #pragma unroll
@@ -1052,13 +1049,10 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
         if (st + 1 < n_stage) issue(st + 1, true);
         uint32_t seen = 0;
         if constexpr (MASK) {
-            const int i = WP * st + kp, k0 = KB * blk.at(min(i, nb - 1)) + here(4 * hf);
+            const int i = WP * st + kp;
+            seen = i < nb ? sees<TREE>(a, row.pos, row.mask, KB * blk.at(i) + here(4 * hf)) : 0u;
 #pragma unroll
-            for (int x = 0; x < 16; x++) {
-                const bool v = i < nb && sees<TREE>(a, row.pos, row.mask, k0 + 8 * (x >> 2) + (x & 3));
-                seen |= (uint32_t)v << x;
-                s[x] = v ? s[x] : -INFINITY;
-            }
+            for (int x = 0; x < 16; x++) s[x] = seen >> (8 * (x >> 2) + (x & 3)) & 1 ? s[x] : -INFINITY;
         }
         float mx = s[0];
 #pragma unroll
@@ -1317,7 +1311,7 @@ extern "C" int htr_window_attention(htr_device *dev, const float *d_q, size_t q_
     const HtrOnDevice on(dev);
     a.q = d_q, a.q_stride = q_stride, a.out = d_out, a.n = n_q, a.n_head = n_head, a.group = n_head / kv->n_kv;
     a.per_group = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
-    a.scale = scale, a.pos0 = pos0, a.window = window, a.n_sink = n_sink;
+    a.scale = scale, a.pos0 = pos0, a.window = std::min(window, pos0 + n_q), a.n_sink = n_sink;
     const int n_keys = pos0 + n_q, sink = std::min(n_sink, n_keys), sink_rows = (sink + KB - 1) / KB * KB;
     const int from = window > pos0 ? 0 : (pos0 - window + 1) / KB * KB;
     const int64_t span = (int64_t)window + sink + 64;  // of 64 rows' queries
