@@ -48,6 +48,7 @@ typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef __fp16 fp16x4 __attribute__((ext_vector_type(4)));
 typedef int int2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
+typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 
 struct Args {
@@ -235,22 +236,37 @@ template <int N, int G> __device__ __forceinline__ float q_pairs(const float *qr
 
 // values of V that are not finite, in blocks that not every row sees (0·∞ is NaN on the matrix cores, in rows too that do
 // not see them): taken as 0 in the product, and NaN put in afterwards where a row does see one, by a product of ones
-__device__ __forceinline__ half8 finite(half8 v, uint32_t &any) {
+__device__ __forceinline__ half8 finite(half8 v) {
     uint32_t w[4];
     __builtin_memcpy(w, &v, 16);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         const uint32_t b = ((w[e] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;  // a half whose exponent is all ones
-        any |= b;
         w[e] &= ~((b >> 15) * 0xFFFFu);
     }
     __builtin_memcpy(&v, w, 16);
     return v;
 }
-__device__ __forceinline__ half8 finite(half8 v) {
-    uint32_t any = 0;
-    return finite(v, any);
+// the largest |v| so far, as bits by halves; whether a lane of the wave has met one that is not finite
+__device__ __forceinline__ void largest(half8 v, uint32_t &top) {
+    ushort2_t t;
+    uint32_t w[4];
+    __builtin_memcpy(w, &v, 16);
+    __builtin_memcpy(&t, &top, 4);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        ushort2_t x;
+        w[e] &= 0x7FFF7FFFu;
+        __builtin_memcpy(&x, &w[e], 4);
+        t = __builtin_elementwise_max(t, x);
+    }
+    __builtin_memcpy(&top, &t, 4);
 }
+__device__ __forceinline__ bool any_not_finite(uint32_t top) {
+    return __builtin_amdgcn_ballot_w64((((top & 0x7C007C00u) + 0x04000400u) & 0x80008000u) != 0) != 0;
+}
+// of two scales of a q8_0 cache one that may make such a value: NaN, or past 515.5
+__device__ __forceinline__ bool scale_past(uint32_t d) { return (d & 0x7FFFu) > 0x6007u || (d >> 16 & 0x7FFFu) > 0x6007u; }
 __device__ __forceinline__ half8 ones_of_not_finite(half8 v) {
     uint32_t w[4];
     __builtin_memcpy(w, &v, 16);
@@ -574,8 +590,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
         if (masked) {  // does the wave's unit hold a value of V that is not finite (a scale that may make one: past 515.5)?
             uint32_t any = 0;
             if constexpr (Q8) {
-                const uint32_t w = s_vd[b][wave][here(lane)];
-                any = (w & 0x7FFFu) > 0x6007u || (w >> 16 & 0x7FFFu) > 0x6007u;
+                any = scale_past(s_vd[b][wave][here(lane)]);
             } else {
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
@@ -888,7 +903,15 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
             }
             return v;
         };
-        uint32_t odd = 0;
+        bool odd = false;
+        if constexpr (MASK && Q8) {
+            odd = __builtin_amdgcn_ballot_w64(scale_past(reinterpret_cast<const uint32_t *>(buf + 528)[here(lane)])) != 0;
+        } else if constexpr (MASK) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int u = 0; u < 4; u++) largest(vread(u, 0), top), largest(vread(u, 1), top);
+            odd = any_not_finite(top);
+        }
 #pragma unroll
         for (int ss = 0; ss < 2; ss++) {
             half8 h8, l8;
@@ -897,14 +920,14 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 half8 v = vread(u, ss);
-                if constexpr (MASK) v = finite(v, odd);
+                if (odd) v = finite(v);
                 o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, h8, o[u], 0, 0, 0);
                 o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, l8, o[u], 0, 0, 0);
                 if constexpr (MASK) __builtin_amdgcn_sched_barrier(0);  // (few operands in registers at once)
             }
         }
         if constexpr (MASK)
-            if (__builtin_amdgcn_ballot_w64(odd != 0)) put_nan(o, seen, vread);
+            if (odd) put_nan(o, seen, vread);
         if constexpr (!Q8) {
             wait_reads();
             if (more) load(i + SW, true);
@@ -978,8 +1001,8 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
 // workgroups, and 224 VALU instructions a block and wave would be as many as the softmax's).
 //
 // Bound: the matrix cores' work and the softmax's instructions on the same two waves a SIMD, and the power of the two: 6001
-// queries with a window of 1500 of a q8_0 cache, 149 GFLOP as pairs, 180 µs with 13 of reading back (MFMA busy 50 %, VALU
-// 45 %; of zeros, at the full clock, 147). 1925 with a window of 512 28 µs. 128 rows a workgroup, 8 waves: 198 (their barriers
+// queries with a window of 1500 of a q8_0 cache, 149 GFLOP as pairs, 178 µs with 13 of reading back (MFMA busy 50 %, VALU
+// 45 %; of zeros, at the full clock, 145). 1925 with a window of 512 27.3 µs. 128 rows a workgroup, 8 waves: 198 (their barriers
 // hold twice as many).
 constexpr int WR = 2, WP = 2;  // row tiles, key parts
 
@@ -1106,7 +1129,13 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
         }
         v[3] = vread(3, 0);
         l += ls;
-        uint32_t odd = 0;
+        bool odd = false;
+        if constexpr (MASK) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int u = 0; u < 4; u++) largest(v[u], top), largest(vread(u, 1), top);
+            odd = any_not_finite(top);
+        }
 #pragma unroll
         for (int ss = 0; ss < 2; ss++) {
             half8 h8, l8;
@@ -1115,10 +1144,7 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
             half8 vn[4];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                if constexpr (MASK) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    v[u] = finite(v[u], odd);
-                }
+                if (odd) v[u] = finite(v[u]);
                 o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[u], h8, o[u], 0, 0, 0);
                 if (ss == 0) vn[u] = vread(u, 1);
             }
@@ -1129,7 +1155,7 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
             }
         }
         if constexpr (MASK)
-            if (__builtin_amdgcn_ballot_w64(odd != 0)) put_nan(o, seen, vread);
+            if (odd) put_nan(o, seen, vread);
     };
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // K and V stage 0, K stage 1
     __builtin_amdgcn_s_barrier();
