@@ -141,6 +141,14 @@ __device__ __forceinline__ double row_sum(double v, int lane) {
     return v + swap_f64<1>(v, lane);
 }
 
+// 1 / √t: the hardware's estimate (2^-23 or better), squared twice by Newton's step
+__device__ __forceinline__ double inv_sqrt(double t) {
+    double r = __builtin_amdgcn_rsq(t);
+#pragma unroll
+    for (int i = 0; i < 2; i++) r = fma(0.5 * r, fma(-t * r, r, 1.0), r);
+    return t == INFINITY ? 0.0 : r;
+}
+
 struct PostRowsArgs {
     const float *q, *k, *v;
     size_t q_stride, kv_stride;
@@ -157,9 +165,9 @@ struct TreeDepth {
 // One head of one row to 16 lanes of dims 4j … 4j + 3 and 64 + 4j …, a turn's pairs in one lane. The norm and the turn are in
 // f64: what they give is rounded to f32, then to the cache's type, and lies next to a border of that type often enough (4e-4
 // of f16 values for f32 sums, an f16 ulp off each, and as many q8_0 quants a step off) that f32 sums would give each order of
-// summation a cache of its own. It costs nothing here: 70 f64 operations a lane for 100 bytes of traffic.
-// 1925 rows of 16 + 2·8 heads into q8_0 (51 MB) 12.1 µs, into f16 (55 MB) 11.1; with 8 dims in a row to a lane, whose loads
-// skip every other 16 bytes, 13.5 and 13.4. One row: 4 µs, a launch.
+// summation a cache of its own. Its 70 operations a lane hide behind the lane's 100 bytes: 1925 rows of 16 + 2·8 heads into
+// q8_0 (51 MB) 10.5 µs, 4.9 TB/s, into f16 (55 MB) 10.1; with the library's 1 / sqrt, and V's heads taken through it all too,
+// 11.9 and 11.2; with 8 dims in a row to a lane, whose loads skip every other 16 bytes, 13.5 and 13.4. One row: 4 µs, a launch.
 template <bool Q8, bool TREE> __global__ __launch_bounds__(256) void k_post_rows(PostRowsArgs a, TreeDepth depth) {
     const int lane = threadIdx.x & 63, j = lane & 15, heads = a.n_head + 2 * a.kv.n_kv;
     const uint32_t id = blockIdx.x * 16u + (threadIdx.x >> 4), count = (uint32_t)a.n * heads, at = min(id, count - 1);
@@ -168,26 +176,29 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256) void k_post_rows
     const float *src = is_q   ? a.q + t * a.q_stride + (size_t)h * D
                        : is_v ? a.v + t * a.kv_stride + (size_t)(kvh - a.kv.n_kv) * D
                               : a.k + t * a.kv_stride + (size_t)kvh * D;
-    float x[2][4], y[2][4], wf[2][4], cs[8];
-    const float *w = is_q ? a.qn : a.kn, *turn = a.rope + (size_t)(a.pos0 + (TREE ? depth.at[t] : t)) * D + 8 * j;
+    float y[2][4];
 #pragma unroll
-    for (int u = 0; u < 2; u++) *reinterpret_cast<float4 *>(x[u]) = *reinterpret_cast<const float4 *>(src + 64 * u + 4 * j);
+    for (int u = 0; u < 2; u++) *reinterpret_cast<float4 *>(y[u]) = *reinterpret_cast<const float4 *>(src + 64 * u + 4 * j);
+    if (!is_v) {
+        const float *w = is_q ? a.qn : a.kn, *turn = a.rope + (size_t)(a.pos0 + (TREE ? depth.at[t] : t)) * D + 8 * j;
+        float wf[2][4], cs[8];
 #pragma unroll
-    for (int u = 0; u < 2; u++) *reinterpret_cast<float4 *>(wf[u]) = *reinterpret_cast<const float4 *>(w + 64 * u + 4 * j);
+        for (int u = 0; u < 2; u++) *reinterpret_cast<float4 *>(wf[u]) = *reinterpret_cast<const float4 *>(w + 64 * u + 4 * j);
 #pragma unroll
-    for (int u = 0; u < 2; u++) *reinterpret_cast<float4 *>(cs + 4 * u) = *reinterpret_cast<const float4 *>(turn + 4 * u);
-    double ss = 0.0;
+        for (int u = 0; u < 2; u++) *reinterpret_cast<float4 *>(cs + 4 * u) = *reinterpret_cast<const float4 *>(turn + 4 * u);
+        double ss = 0.0;
 #pragma unroll
-    for (int u = 0; u < 2; u++)
+        for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) ss = fma((double)x[u][e], (double)x[u][e], ss);
-    const double inv = 1.0 / sqrt(row_sum(ss, lane) / (double)D + a.eps);
+            for (int e = 0; e < 4; e++) ss = fma((double)y[u][e], (double)y[u][e], ss);
+        const double inv = inv_sqrt(fma(row_sum(ss, lane), 1.0 / D, a.eps));
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const double lo = (double)x[0][e] * inv * (double)wf[0][e], up = (double)x[1][e] * inv * (double)wf[1][e];
-        const double c = (double)cs[2 * e], s = (double)cs[2 * e + 1];
-        y[0][e] = is_v ? x[0][e] : (float)(lo * c - up * s);
-        y[1][e] = is_v ? x[1][e] : (float)(lo * s + up * c);
+        for (int e = 0; e < 4; e++) {
+            const double lo = (double)y[0][e] * inv * (double)wf[0][e], up = (double)y[1][e] * inv * (double)wf[1][e];
+            const double c = (double)cs[2 * e], s = (double)cs[2 * e + 1];
+            y[0][e] = (float)(lo * c - up * s);
+            y[1][e] = (float)(lo * s + up * c);
+        }
     }
     if (is_q) {
         if (id >= count) return;
