@@ -177,11 +177,19 @@ template <bool TREE> __device__ __forceinline__ uint32_t sees(const Args &a, int
         return low_bits(n) & (~low_bits(n - a.window) | low_bits(a.n_sink - k0));
     }
 }
-// whether the queries ta … tb all see the keys k0 … k0 + U − 1
-template <bool TREE, int U> __device__ __forceinline__ bool all_see(const Args &a, int ta, int tb, int k0) {
-    if constexpr (TREE) return k0 + U <= a.n_past;
-    else return k0 + U - 1 <= a.pos0 + ta && (k0 + U <= a.n_sink || k0 > a.pos0 + tb - a.window);
-}
+// the blocks of U keys that the queries ta … tb all see the whole of: those before `to` that are among the first keys or in
+// the last one's window
+template <bool TREE, int U> struct Whole {
+    int to, sink, from;
+    __device__ __forceinline__ Whole(const Args &a, int ta, int tb) {
+        const int out = a.pos0 + tb - a.window;  // the last key that the last query does not see any more
+        to = (TREE ? a.n_past : a.pos0 + ta + 1) / U, sink = a.n_sink / U, from = out < 0 ? 0 : out / U + 1;
+    }
+    __device__ __forceinline__ bool block(int k) const {
+        if constexpr (TREE) return k < to;
+        else return k < to && (k < sink || k >= from);
+    }
+};
 
 // p − (float)h for the low (0) or high (1) half of h: one mixed-precision fma
 template <int HI> __device__ __forceinline__ float minus_half(float p, uint32_t h) {
@@ -507,9 +515,10 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 
     // whether every row sees all keys of the round's units
+    const Whole<TREE, UK> full(a, ta, tb);
     auto whole = [&](int rd) {
         const int i = i0 + SW * rd + (lane & 7);
-        return __builtin_amdgcn_ballot_w64(!(i < i1 && all_see<TREE, UK>(a, ta, tb, UK * blk.at(min(i, i1 - 1))))) == 0;
+        return __builtin_amdgcn_ballot_w64(!(i < i1 && full.block(blk.at(i)))) == 0;
     };
     for (int rd = 0; rd < n_round; rd++) {
         const bool masked = !whole(rd);  // (what only a masked round does stands behind uniform branches, and is not fetched else)
@@ -802,6 +811,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
         va[u] = Q8 ? 16 * (256 + 8 * vrow + ((2 * u + ((lane >> 4) & 1)) ^ (vrow & 2) ^ ((vrow & 8) >> 1))) + 8 * (lane & 1)
                    : 16 * (K_CHUNKS + 16 * vrow + ((4 * u + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (4 * (vrow & 3)))) + 8 * (lane & 1);
 
+    const Whole<TREE, KB> full(a, ta, tb);
     // block i; MASK: not every row sees all of it
     auto step = [&](auto is_masked) {
         constexpr bool MASK = decltype(is_masked)::value;
@@ -936,9 +946,8 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
         b ^= Q8;
     };
     while (i < i1) {
-        for (bool all = all_see<TREE, KB>(a, ta, tb, KB * blk.at(i)); all; all = i < i1 && all_see<TREE, KB>(a, ta, tb, KB * blk.at(i)))
-            step(std::false_type{});
-        for (bool some = i < i1; some; some = i < i1 && !all_see<TREE, KB>(a, ta, tb, KB * blk.at(i))) step(std::true_type{});
+        for (bool all = full.block(blk.at(i)); all; all = i < i1 && full.block(blk.at(i))) step(std::false_type{});
+        for (bool some = i < i1; some; some = i < i1 && !full.block(blk.at(i))) step(std::true_type{});
     }
 
     l = pair_sum<32>(l);
@@ -1001,8 +1010,8 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
 // workgroups, and 224 VALU instructions a block and wave would be as many as the softmax's).
 //
 // Bound: the matrix cores' work and the softmax's instructions on the same two waves a SIMD, and the power of the two: 6001
-// queries with a window of 1500 of a q8_0 cache, 149 GFLOP as pairs, 178 µs with 13 of reading back (MFMA busy 50 %, VALU
-// 45 %; of zeros, at the full clock, 145). 1925 with a window of 512 27.3 µs. 128 rows a workgroup, 8 waves: 198 (their barriers
+// queries with a window of 1500 of a q8_0 cache, 149 GFLOP as pairs, 176 µs with 13 of reading back (MFMA busy 51 %, VALU
+// 44 %; of zeros, at the full clock, 143). 1925 with a window of 512 27.2 µs. 128 rows a workgroup, 8 waves: 198 (their barriers
 // hold twice as many).
 constexpr int WR = 2, WP = 2;  // row tiles, key parts
 
@@ -1020,25 +1029,41 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
     const char *kh = (const char *)a.kv.k + (size_t)kvh * a.kv.n_ctx * (2 * D);
     const char *vh = (const char *)a.kv.v + (size_t)kvh * a.kv.n_ctx * (2 * D);
 
-    // a stage's K or V → buffer st % 2: 4 direct loads a wave, each of the 4 waves 4 rows of 16 (keys past the last: the last)
+    // a stage's K or V → buffer b: 4 direct loads a wave, each of the 4 waves 4 rows of 16 (keys past the last: the last). A
+    // stage's place is worked out once, for its K, and kept for its V a stage later
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4_t *)&s_kv[0][0][64 * wave];
     const int lrow = 4 * wave + (lane >> 4), lc = lane & 15;
     const uint32_t koff = 16 * (lc ^ (lrow & 15)), voff = 16 * (lc ^ (4 * (lrow & 3)));  // the same for row lrow + 16
-    auto issue = [&](int st, bool is_v) {
+    struct Place {
+        size_t at[WP];  // the blocks' first byte
+        int last[WP];   // their last row of a key
+    };
+    const int skip = blk.from - blk.first, skip_mem = skip - a.shift / KB;
+    auto place = [&](int st) {
+        Place x;
 #pragma unroll
         for (int p = 0; p < WP; p++) {
-            const int k0 = KB * blk.at(min(WP * st + p, nb - 1));
-            const char *base = (is_v ? vh : kh) + (size_t)(k0 < a.sink_rows ? k0 : k0 - a.shift) * (2 * D);
-            const uint32_t off = is_v ? voff : koff, last = 2 * D * min(n_keys - 1 - k0, KB - 1) + off;
+            const int i = min(WP * st + p, nb - 1), past = i >= blk.first ? 1 : 0;
+            x.at[p] = (size_t)(uint32_t)(i + past * skip_mem) * (KB * 2 * D);
+            x.last[p] = min(n_keys - 1 - KB * (i + past * skip), KB - 1);
+        }
+        return x;
+    };
+    auto issue = [&](const Place &x, int b, bool is_v) {
+#pragma unroll
+        for (int p = 0; p < WP; p++) {
+            const char *base = (is_v ? vh : kh) + x.at[p];
+            const uint32_t off = is_v ? voff : koff, last = 2 * D * x.last[p] + off;
 #pragma unroll
             for (int h = 0; h < 2; h++)
                 lds_load16(base, min(2 * D * (16 * h + lrow) + off, last),
-                           lds + 16u * (((st & 1) * WP + p) * TILE + (is_v ? K_CHUNKS : 0) + 256 * h));
+                           lds + 16u * ((b * WP + p) * TILE + (is_v ? K_CHUNKS : 0) + 256 * h));
         }
     };
-    issue(0, false);
-    issue(0, true);
-    if (n_stage > 1) issue(1, false);
+    Place next = place(0);  // of stage st + 1
+    issue(next, 0, false);
+    issue(next, 0, true);
+    if (n_stage > 1) issue(next = place(1), 1, false);
 
     const Row<TREE> row(a, tree, kvh, r0 + KB * rt + c);
     const int ta = query_of(a.group, a.per_group, min(r0 + KB * rt, rows - 1));
@@ -1068,8 +1093,11 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (st + 2 < n_stage) issue(st + 2, false);
-        if (st + 1 < n_stage) issue(st + 1, true);
+        if (st + 1 < n_stage) {
+            const Place now = next;
+            if (st + 2 < n_stage) issue(next = place(st + 2), b, false);
+            issue(now, b ^ 1, true);
+        }
         uint32_t seen = 0;
         if constexpr (MASK) {
             const int i = WP * st + kp;
@@ -1169,7 +1197,8 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
     }
     // two stages at a time, both kinds of step passing one barrier a stage: a wave's blocks may be masked where another's
     // are not
-    auto whole = [&](int st) { return WP * st + kp < nb && all_see<TREE, KB>(a, ta, tb, KB * blk.at(WP * st + kp)); };
+    const Whole<TREE, KB> full(a, ta, tb);
+    auto whole = [&](int st) { return WP * st + kp < nb && full.block(blk.at(WP * st + kp)); };
     for (int st = 0; st < n_stage;) {
         for (; st + 1 < n_stage && whole(st) && whole(st + 1); st += 2) {
             step(st, 0, s0, s1, std::false_type{});
