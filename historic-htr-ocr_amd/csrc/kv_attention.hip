@@ -697,9 +697,10 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
 // Reads of 16 (32) lanes then fall on different bank groups.
 //
 // Bound: of few keys latency (8 µs a call up to 300 keys: 2 until the first block is there, 2 for the merge), of many the
-// instructions of its two waves a SIMD: a block of f16 is 32 MFMA and 256 VALU instructions, 16 of them exponentials, one of
-// q8_0 224 VALU instructions more (MFMA busy 33 %, VALU 56 % over 40013 keys). 64 tokens over 6001 f16 keys 16.2 µs
-// (27 MB: 5.5 at a copy's rate), 27 over 40013 q8_0 keys 30.6 (88 MB: 17.8). With four waves a workgroup the
+// instructions of its two waves a SIMD: a block of f16 is 32 MFMA and some 130 VALU instructions, 16 of them exponentials,
+// one of q8_0 224 VALU instructions more (MFMA busy 33 %, VALU 58 % over 40013 keys). 64 tokens over 6001 f16 keys 16.0 µs (27
+// MB: 5.5 at a copy's rate), 27 over 40013 q8_0 keys 29.8 (88 MB: 17.8), of real values, whose products lower the clock, 33 …
+// 36. With four waves a workgroup the
 // kernels alone took 30.9 and 54.9 for 21.2 and 30. Two row tiles to a wave, which halves the conversions, cost 6.7 µs of the
 // 27 tokens' call: half as many waves, and each longer.
 constexpr int QT = 256 + 256 + 16 + 16;  // 16-byte chunks of a q8_0 buffer: K, V, K scales, V scales
@@ -848,6 +849,16 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
                 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qh[ks], ks ? s : f32x16{}, 0, 0, 0);
                 s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, ql[ks], s, 0, 0, 0);
             }
+            // the next operand's conversion in the shadow of this one's products, half a conversion to each (as compiled both
+            // products went first, and the conversion behind them: 30.4 µs for 29.8 over 40013 keys)
+            __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 22, 0);
+#pragma unroll
+            for (int e = 0; e < 14; e++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 7, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
         } else {
             half8 f[4];
 #pragma unroll
