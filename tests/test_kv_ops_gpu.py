@@ -579,11 +579,26 @@ def test_trees_of_very_many_heads(dev, q8_0):
     c.free()
 
 
+@pytest.mark.parametrize("n,group,n_kv", WAYS)
+def test_queries_that_are_not_finite(dev, n, group, n_kv):
+    """a query with a NaN and one with an infinity: their outputs are not finite, every other bit for bit as without them"""
+    rows = 400
+    c, q = cache(dev, 161, n_kv, rows), normal(162, n, n_kv * group, 128)
+    want = run_window(dev, q, c, rows - n, 170, 3).reshape(n, -1, 128)
+    q[1, 0, 5], q[n - 1, -1, 127] = np.nan, -np.inf
+    got = run_window(dev, q, c, rows - n, 170, 3).reshape(n, -1, 128)
+    assert not np.any(np.isfinite(got[1, 0])) and not np.any(np.isfinite(got[n - 1, -1]))
+    got[1, 0], got[n - 1, -1] = want[1, 0], want[n - 1, -1]
+    assert np.array_equal(bits(got), bits(want))
+    c.free()
+
+
 def test_calls_of_changing_shapes_share_the_scratch(dev):
     """one call after another over caches of 8, 2 and 16 KV heads (partial sums and tickets in an XCD's L2, and through the
     coherence point), of one to 64 nodes: each as alone"""
     for i, (n, past, n_kv, group) in enumerate([(1, 3000, 8, 2), (1, 3000, 2, 2), (20, 2000, 8, 1), (64, 900, 16, 1), (1, 1000, 16, 3), (9, 5000, 8, 1),
-                                                (1, 4000, 8, 2), (30, 3000, 1, 2), (1, 700, 8, 4)]):
+                                                (1, 4000, 8, 2), (30, 3000, 1, 2), (1, 700, 8, 4), (60, 1500, 4, 4), (64, 3000, 2, 2),
+                                                (33, 900, 1, 8), (60, 1100, 4, 4), (2, 900, 3, 2)]):
         t = random_tree(i, n)
         c, q = cache(dev, 130 + i, n_kv, past + n, i % 2 == 1), normal(140 + i, n, n_kv * group, 128)
         assert rel_rows(run_tree(dev, q, c, t, past), attention(q, c.k, c.v, tree_seen(t.masks, past, past + n), SCALE)) < BAR, i
