@@ -217,17 +217,19 @@ int htr_kv_keep(htr_device *dev, const htr_kv *kv, int row0, const int32_t *h_id
  * host array of htr_tree_masks, or any other: read before the call returns; NULL: a chain, j ≤ t) →
  * d_out [n][n_head·128] = softmax(scale·q·Kᵀ)·V, zeros for a query that sees no row. n = 1 is a decode step's attention.
  * A row that a query does not see does not touch its output, whatever it holds; of one that it sees a V value that is not
- * finite gives one that is not, a K value that is not a score of NaN or of an infinity (−∞: no weight). All sums in f32, q and the weights held to 22 bits; over a q8_0 cache the same bits as
- * over its read-back, and the same bits every time. Scratch: 4.4 MB, the same for every size, made at the first call that
- * splits a query's keys; and for a q8_0 cache that many rows read (over 8000 rows of q heads), its rows in f16: at
- * least 32 MB, doubled when it grows, what it was before kept until the device is closed, so that graphs recorded over it
- * stay good. A call that makes or grows scratch cannot be one that is being captured. The output is apart from the queries
- * and the cache (else refused); strides multiples of 4, pointers 16-byte aligned. */
+ * finite gives one that is not, a K value that is not a score of NaN or of an infinity (−∞: no weight). All sums in f32,
+ * q and the weights held to 22 bits; over a q8_0 cache the same bits as over its read-back, and the same bits every time.
+ * Scratch: 4.4 MB, the same for every size, made at the first call that splits a query's keys; and for a q8_0 cache that
+ * many rows read (over 12000 rows of q heads), its rows in f16: at least 32 MB, doubled when it grows, what it was before
+ * kept until the device is closed, so that graphs recorded over it stay good. A call that makes or grows scratch cannot be
+ * one that is being captured. The output is apart from the queries and the cache (else refused); strides multiples of 4,
+ * pointers 16-byte aligned. */
 int htr_tree_attention(htr_device *dev, const float *d_q, size_t q_stride, int n, const uint64_t *h_mask, int n_past,
                        const htr_kv *kv, int n_head, float scale, float *d_out);
 /* attention with a sliding window and first keys that stay visible: queries at positions pos0 … pos0 + n_q − 1, the one at
  * p over the cache rows j ≤ p with j < n_sink or j > p − window (window ≥ 1: itself at least) → d_out [n_q][n_head·128].
- * Otherwise as htr_tree_attention; n_q = 1 is a decode step's, and of a q8_0 cache only the rows that are seen are read. */
+ * Otherwise as htr_tree_attention; n_q = 1 is a decode step's. Of a cache only the blocks of rows that some query sees are
+ * read (read back first: also a gap of up to a quarter of the rows). */
 int htr_window_attention(htr_device *dev, const float *d_q, size_t q_stride, int n_q, int pos0, int window, int n_sink,
                          const htr_kv *kv, int n_head, float scale, float *d_out);
 /* the GPU token choice of a greedy preset on n_vocab logits (choose_pen → choose_max → choose_pick,
