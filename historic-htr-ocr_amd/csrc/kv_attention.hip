@@ -40,8 +40,6 @@ constexpr float M_NONE = -3.0e38f;             // m before the first key: finite
 constexpr int MAX_SPLIT = 64, TICKET = 32;     // parts of a row group's blocks; words between tickets (128 bytes)
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float float2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
@@ -71,32 +69,6 @@ struct Args {
 struct TreeMask {
     uint64_t of[HTR_TREE_MAX];
 };
-
-// int8 quants → f16(q·d) (as kv_cache.hip's read-back)
-__device__ __forceinline__ half2_t dequant2(uint32_t w, uint32_t sel, half2_t d) {
-    const uint32_t p = __builtin_amdgcn_perm(0x64646464u, w, sel);
-    half2_t h;
-    __builtin_memcpy(&h, &p, 4);
-    return (h - half2_t{(_Float16)1152.0f, (_Float16)1152.0f}) * d;
-}
-__device__ __forceinline__ half8 dequant8(uint32_t q0, uint32_t q1, half2_t d) {
-    const uint32_t a = q0 ^ 0x80808080u, b = q1 ^ 0x80808080u;
-    half2_t r[4] = {dequant2(a, 0x07010700u, d), dequant2(a, 0x07030702u, d), dequant2(b, 0x07010700u, d),
-                    dequant2(b, 0x07030702u, d)};
-    half8 o;
-    __builtin_memcpy(&o, r, 16);
-    return o;
-}
-
-// the same with a scale a value
-__device__ __forceinline__ half8 dequant8(uint32_t q0, uint32_t q1, half8 d) {
-    const uint32_t a = q0 ^ 0x80808080u, b = q1 ^ 0x80808080u;
-    half2_t r[4] = {dequant2(a, 0x07010700u, half2_t{d[0], d[1]}), dequant2(a, 0x07030702u, half2_t{d[2], d[3]}),
-                    dequant2(b, 0x07010700u, half2_t{d[4], d[5]}), dequant2(b, 0x07030702u, half2_t{d[6], d[7]})};
-    half8 o;
-    __builtin_memcpy(&o, r, 16);
-    return o;
-}
 
 // 4 bytes a lane from base + off to LDS bytes lds + 4·lane (as lds_load16)
 __device__ __forceinline__ void lds_load4(const void *base, uint32_t off, uint32_t lds) {
@@ -283,7 +255,8 @@ __device__ __forceinline__ half8 ones_of_not_finite(half8 v) {
     __builtin_memcpy(&v, w, 16);
     return v;
 }
-// o's sums of the rows that see one: NaN. seen: the lane's 16 keys (bits 0 … 3, 8 … 11, 16 …, 24 …); vread(u, ss): V's operand of tile u, step ss
+// o's sums of the rows that see one: NaN. seen: the lane's 16 keys (bits 0 … 3, 8 … 11, 16 …, 24 …);
+// vread(u, ss): V's operand of tile u, step ss
 template <typename F> __device__ __forceinline__ void put_nan(f32x16 (&o)[4], uint32_t seen, F vread) {
     half8 ind[2];
 #pragma unroll
@@ -473,7 +446,8 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     const int n_keys = TREE ? a.n_past + a.n : a.pos0 + a.n;
     const int ta = query_of(a.group, a.per_group, r0), tb = query_of(a.group, a.per_group, min(r0 + FR - 1, rows - 1));
     const Blocks blk = blocks_of<TREE, UK>(a, ta, tb);
-    const auto [i0, i1] = part_of(blk.count(), split, a.n_split);
+    const Part part = part_of(blk.count(), split, a.n_split);
+    const int i0 = part.i0, i1 = part.i1;
     const int n_round = (i1 - i0 + SW - 1) / SW;
     const size_t head0 = (size_t)kvh * a.kv.n_ctx;
 
@@ -541,7 +515,10 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
                 }
             } else {
 #pragma unroll
-                for (int ks = 0; ks < 4; ks++) f[ks] = *reinterpret_cast<const half8 *>(s_k[wave] + 16 * c + ((8 * (ks >> 1) + 2 * g + (ks & 1)) ^ c));
+                for (int ks = 0; ks < 4; ks++) {
+                    const int chunk = 8 * (ks >> 1) + 2 * g + (ks & 1);
+                    f[ks] = *reinterpret_cast<const half8 *>(s_k[wave] + 16 * c + (chunk ^ c));
+                }
             }
             wait_reads();
             if (more) load(i + SW, false, 0);
@@ -618,7 +595,8 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
             half8 v;
             if constexpr (Q8) {
                 const uint4_t *unit = s_v[b][2 * st] + UC * ((c >> 3) & 1);
-                const auto *p = (const __attribute__((address_space(3))) char *)(unit + 8 * vrow + (wave ^ (vrow >> 1) ^ ((c & 8) >> 1))) + 8 * (c & 1);
+                const int at = 8 * vrow + (wave ^ (vrow >> 1) ^ ((c & 8) >> 1));
+                const auto *p = (const __attribute__((address_space(3))) char *)(unit + at) + 8 * (c & 1);
                 const int2_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2_t *)p);
                 v = dequant8((uint32_t)w[0], (uint32_t)w[1], *reinterpret_cast<const half8 *>(s_vt[wave >> 1][st][g]));
             } else {
@@ -720,7 +698,8 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
     const int n_keys = TREE ? a.n_past + a.n : a.pos0 + a.n;
     const int ta = query_of(a.group, a.per_group, r0), tb = query_of(a.group, a.per_group, min(r0 + KB - 1, rows - 1));
     const Blocks blk = blocks_of<TREE, KB>(a, ta, tb);
-    const auto [i0, i1] = part_of(blk.count(), split, a.n_split);
+    const Part part = part_of(blk.count(), split, a.n_split);
+    const int i0 = part.i0, i1 = part.i1;
     const size_t head0 = (size_t)kvh * a.kv.n_ctx;
 
     uint4_t *tile = s_kv[wave];

@@ -22,9 +22,7 @@ constexpr int D = 128, KV_BLOCK = 32;
 constexpr float Q8_MAX = 127.0f * 515.5f;  // 515.5: the largest scale whose 127-fold f16 holds
 constexpr uint32_t F32_INF = 0x7F800000u;
 
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 
@@ -100,22 +98,6 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, int lane) {
     return max(v, lane_swap_u32<1>(v, lane));
 }
 
-// int8 quants → f16(q·d): a byte q ^ 0x80 under the high byte 0x64 is the f16 number 1024 + 128 + q, so one packed
-// subtraction gives q exactly, and one packed product rounds q·d once
-__device__ __forceinline__ half2_t dequant2(uint32_t w, uint32_t sel, half2_t d) {
-    const uint32_t p = __builtin_amdgcn_perm(0x64646464u, w, sel);
-    half2_t h;
-    __builtin_memcpy(&h, &p, 4);
-    return (h - half2_t{(_Float16)1152.0f, (_Float16)1152.0f}) * d;
-}
-__device__ __forceinline__ half8 dequant8(uint2_t q, half2_t d) {
-    const uint32_t a = q[0] ^ 0x80808080u, b = q[1] ^ 0x80808080u;
-    half2_t r[4] = {dequant2(a, 0x07010700u, d), dequant2(a, 0x07030702u, d), dequant2(b, 0x07010700u, d),
-                    dequant2(b, 0x07030702u, d)};
-    half8 o;
-    __builtin_memcpy(&o, r, 16);
-    return o;
-}
 __device__ __forceinline__ half2_t scale_pair(uint16_t bits) {
     _Float16 h;
     __builtin_memcpy(&h, &bits, 2);
@@ -309,7 +291,7 @@ __global__ __launch_bounds__(256) void k_kv_read_back(CopyArgs a) {
 #pragma unroll
     for (int i = 0; i < BACK_ROWS / 16; i++)
         if (r0 + 16 * i < a.n)
-            __builtin_nontemporal_store(dequant8(q[i], scale_pair(d[i])),
+            __builtin_nontemporal_store(dequant8(q[i][0], q[i][1], scale_pair(d[i])),
                                         (__attribute__((address_space(1))) half8 *)(uintptr_t)(
                                             (_Float16 *)(is_v ? a.dst.v : a.dst.k) + (to + r0 + 16 * i) * D + 8 * j));
 }
