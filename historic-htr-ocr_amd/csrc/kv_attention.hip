@@ -245,8 +245,9 @@ __device__ __forceinline__ void largest(half8 v, uint32_t &top) {
 __device__ __forceinline__ bool any_not_finite(uint32_t top) {
     return __builtin_amdgcn_ballot_w64((((top & 0x7C007C00u) + 0x04000400u) & 0x80008000u) != 0) != 0;
 }
-// of two scales of a q8_0 cache one that may make such a value: NaN, or past 515.5
-__device__ __forceinline__ bool scale_past(uint32_t d) { return (d & 0x7FFFu) > 0x6007u || (d >> 16 & 0x7FFFu) > 0x6007u; }
+// of two scales of a q8_0 cache one that may make such a value: NaN, or 512 and past (of the quant −128, which is not written
+// here but may stand in a cache made elsewhere, −128·512 is f16's −∞; 511.75, the number before, gives −65504)
+__device__ __forceinline__ bool scale_past(uint32_t d) { return (d & 0x7FFFu) > 0x5FFFu || (d >> 16 & 0x7FFFu) > 0x5FFFu; }
 __device__ __forceinline__ half8 ones_of_not_finite(half8 v) {
     uint32_t w[4];
     __builtin_memcpy(w, &v, 16);
@@ -573,7 +574,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
                 s_vt[2 * (lane & 1)][wave >> 1][key >> 2][at] = (uint16_t)d2;
                 s_vt[2 * (lane & 1) + 1][wave >> 1][key >> 2][at] = (uint16_t)(d2 >> 16);
             }
-        if (masked) {  // does the wave's unit hold a value of V that is not finite (a scale that may make one: past 515.5)?
+        if (masked) {  // does the wave's unit hold a value of V that is not finite (a scale that may make one: 512 and past)?
             uint32_t any = 0;
             if constexpr (Q8) {
                 any = scale_past(s_vd[b][wave][here(lane)]);

@@ -854,3 +854,58 @@ def test_capture_before_the_scratch_exists_is_refused(dev):
     htr.tree_attention(d, qb, 1, 599, c.kv, 16, SCALE, out)
     assert rel_rows(out.download(np.float32), attention(q, c.k, c.v, np.ones((1, 600), bool), SCALE)) < BAR
     d.close()
+
+
+# ---- what a row sees, and nothing else, makes its output --------------------------------------------------------------------
+
+@pytest.mark.parametrize("n,group,n_kv", WAYS)
+@pytest.mark.parametrize("scale", [511.75, 512.0, 515.5, 65504.0])
+def test_quants_of_minus_128_at_scales_that_overflow(dev, n, group, n_kv, scale):
+    """a q8_0 cache may hold the quant -128 (this library writes none): with a scale of 512 and more f16(q·d) is an infinity.
+    V rows with such an element that the first queries do not see yet, and one just before every query's window: those that
+    see none of them get the clean cache's bits, and all of them those over the cache's read-back"""
+    rows, window, sink = n + 300, 150, 3
+    (qk, dk), (qv, dv) = (blocks(normal(s, n_kv, rows, 128).astype(np.float16)) for s in (1, 2))
+    pos0 = rows - n
+    at = [(rows - 2, 5), (pos0 - window, 70), (rows - n // 2 - 1, 100)]
+    bq, bd = qv.copy(), dv.copy()
+    for r, d in at:
+        bq[:, r, d // 32 * 32:d // 32 * 32 + 32], bq[:, r, d], bd[:, r, d // 32] = 1, -128, scale
+    q = normal(3, n, n_kv * group, 128)
+    got = []
+    for v, d in ((bq, bd), (qv, dv)):
+        bufs = [dev.upload(a) for a in (qk, v, dk, d)]
+        kv = htr.KvCache.of(n_kv, rows, *bufs)
+        back = htr.KvCache(dev, n_kv, rows)
+        htr.kv_copy(dev, kv, 0, back, 0, rows)
+        for c in (kv, back):
+            got.append(run_window(dev, q, type("c", (), {"kv": c}), pos0, window, sink))
+        for b in bufs + [back]:
+            b.free()
+    assert np.array_equal(got[0], got[1], equal_nan=True) and np.array_equal(bits(got[2]), bits(got[3]))
+    seen = window_seen(n, pos0, window, sink, rows)
+    free = ~seen[:, [r for r, _ in at]].any(axis=1)
+    assert 0 < free.sum() < n
+    assert np.array_equal(bits(got[0][free]), bits(got[2][free]))
+    for r, d in at:
+        hit = got[0][seen[:, r]].reshape(-1, 128)[:, d]
+        assert np.all(np.isfinite(hit)) if scale < 512 else not np.any(np.isfinite(hit))
+
+
+def test_a_quant_of_minus_128_in_a_draft(dev):
+    """the same in trees: of one node's row (few rows, and more), with the masks of its siblings without it"""
+    for n, n_kv, group in ((5, 2, 2), (40, 2, 3)):
+        past, hit = 50, 2
+        (qk, dk), (qv, dv) = (blocks(normal(s, n_kv, past + n, 128).astype(np.float16)) for s in (1, 2))
+        bq, bd = qv.copy(), dv.copy()
+        bq[:, past + hit, :32], bd[:, past + hit, 0] = -128, 513.5
+        masks = np.array([(2 << i) - 1 if i % 2 else ((2 << i) - 1) & ~(1 << hit) for i in range(n)], np.uint64)
+        q, got = normal(3, n, n_kv * group, 128), []
+        for v, d in ((bq, bd), (qv, dv)):
+            bufs = [dev.upload(a) for a in (qk, v, dk, d)]
+            got.append(run_tree(dev, q, type("c", (), {"kv": htr.KvCache.of(n_kv, past + n, *bufs)}), htr.Tree.of_masks(masks), past))
+            for b in bufs:
+                b.free()
+        sees = (masks >> np.uint64(hit)) & np.uint64(1) != 0
+        assert np.array_equal(bits(got[0][~sees]), bits(got[1][~sees])), n
+        assert not np.any(np.isfinite(got[0][sees].reshape(-1, 128)[:, :32])), n
