@@ -16,8 +16,9 @@
 //   scores   Sᵀ = K·(qh + ql)ᵀ, keys by rows, so that a lane holds scores of one row (of v_mfma_f32_32x32x16_f16 lane
 //            32·hf + c row c's of keys 8(i / 4) + 4hf + i % 4, i < 16);
 //   softmax  p = 2^((s − m)·c + 3): the difference first, so p is right for scores of any size. m, the row's reference, is
-//            moved to the largest score only when some p would pass 2^8 (O and l are rescaled then); the 3 leaves room
-//            below, and drops out with l, which carries it too;
+//            moved to the largest score only when one of its p would pass 2^8 (O and l are rescaled then), whatever the
+//            rows beside it do, so that a row's sums are those of the keys it sees; the 3 leaves room below, and drops out
+//            with l, which carries it too;
 //   values   Oᵀ += Vᵀ·(ph + pl)ᵀ, V by transposing LDS reads, p in the lanes that it was made in.
 // A key that a row does not see is as if it were not there, whatever the cache holds in it: its score becomes −∞ after the
 // product, and values of V that are not finite are taken out of the product of a block that not every row sees, and make
@@ -545,8 +546,9 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
         mx = s_mx[0][c];
 #pragma unroll
         for (int w = 1; w < SW; w++) mx = fmaxf(mx, s_mx[w][c]);
-        if (__builtin_amdgcn_ballot_w64((mx - m) * sc > P_ROOM)) {  // (alike in every wave)
-            const float to = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f((m - to) * sc);
+        const bool up = (mx - m) * sc > P_ROOM;  // (alike in every wave)
+        if (__builtin_amdgcn_ballot_w64(up)) {
+            const float to = up ? mx : m, corr = __builtin_amdgcn_exp2f((m - to) * sc);
             m = to;
             l *= corr;
             o *= corr;
@@ -866,8 +868,9 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
 #pragma unroll
         for (int x = 1; x < 16; x++) mx = fmaxf(mx, s[x]);
         mx = pair_max<32>(mx);
-        if (__builtin_amdgcn_ballot_w64((mx - m) * sc > P_ROOM)) {
-            const float to = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f((m - to) * sc);
+        const bool up = (mx - m) * sc > P_ROOM;
+        if (__builtin_amdgcn_ballot_w64(up)) {
+            const float to = up ? mx : m, corr = __builtin_amdgcn_exp2f((m - to) * sc);
             m = to;
             l *= corr;
 #pragma unroll
@@ -1100,8 +1103,9 @@ template <bool TREE> __global__ __launch_bounds__(64 * WR * WP, 2) void k_kv_att
 #pragma unroll
         for (int x = 1; x < 16; x++) mx = fmaxf(mx, s[x]);
         mx = pair_max<32>(mx);
-        if (__builtin_amdgcn_ballot_w64((mx - m) * sc > P_ROOM)) {
-            const float to = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f((m - to) * sc);
+        const bool up = (mx - m) * sc > P_ROOM;
+        if (__builtin_amdgcn_ballot_w64(up)) {
+            const float to = up ? mx : m, corr = __builtin_amdgcn_exp2f((m - to) * sc);
             m = to;
             l *= corr;
 #pragma unroll

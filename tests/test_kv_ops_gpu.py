@@ -909,3 +909,30 @@ def test_a_quant_of_minus_128_in_a_draft(dev):
         sees = (masks >> np.uint64(hit)) & np.uint64(1) != 0
         assert np.array_equal(bits(got[0][~sees]), bits(got[1][~sees])), n
         assert not np.any(np.isfinite(got[0][sees].reshape(-1, 128)[:, :32])), n
+
+
+@pytest.mark.parametrize("n,group,n_kv,window", [(3, 2, 8, 300), (11, 2, 8, 600), (40, 3, 2, 600), (200, 2, 64, 700)])
+@pytest.mark.parametrize("q8_0", [False, True], ids=["f16", "q8_0"])
+def test_a_key_moves_only_the_rows_that_see_it(dev, n, group, n_kv, window, q8_0):
+    """a key that the later queries see, with a score far above all others or an infinite one in some of them: the outputs of
+    the queries before it are bit for bit as with an ordinary key there, though the kernels take their rows together"""
+    rows, sink = 900, 20
+    pos0, r = rows - n, rows - 1 - n // 2
+    k, v = normal(1, n_kv, rows, 128).astype(np.float16), normal(2, n_kv, rows, 128).astype(np.float16)
+    q = normal(3, n, n_kv * group, 128)
+    c = Cache(dev, k, v, q8_0)
+    want = run_window(dev, q, c, pos0, window, sink)
+    c.free()
+    before = pos0 + np.arange(n) < r
+    assert 0 < before.sum() < n
+    for change in (2.0, np.inf):
+        kk = k.copy()
+        if change == 2.0:
+            kk[:, r] = change * q[n - 1].reshape(n_kv, group, 128)[:, 0]
+        else:
+            kk[:, r, 40] = change
+        c = Cache(dev, kk, v, q8_0)
+        got = run_window(dev, q, c, pos0, window, sink)
+        c.free()
+        assert np.array_equal(bits(got[before]), bits(want[before])), change
+        assert not np.array_equal(bits(got[~before]), bits(want[~before]))
