@@ -15,10 +15,12 @@
 //            the pair neither overflows nor loses bits whatever the row's size; a score is s·c, c = log2(e)·2^(e − 10);
 //   scores   Sᵀ = K·(qh + ql)ᵀ, keys by rows, so that a lane holds scores of one row (of v_mfma_f32_32x32x16_f16 lane
 //            32·hf + c row c's of keys 8(i / 4) + 4hf + i % 4, i < 16);
-//   softmax  p = 2^((s − m)·c + 3): the difference first, so p is right for scores of any size. m, the row's reference, is
-//            moved to the largest score only when one of its p would pass 2^8 (O and l are rescaled then), whatever the
-//            rows beside it do, so that a row's sums are those of the keys it sees; the 3 leaves room below, and drops out
-//            with l, which carries it too;
+//   softmax  p = 2^((s − m)·c + 10): the difference first, so p is right for scores of any size. m, the row's reference, is
+//            moved to the largest score only when one of its p would pass 2^15 (O and l are rescaled then), whatever the
+//            rows beside it do, so that a row's sums are those of the keys it sees. The 10 leaves room below, and drops out
+//            with l, which carries it too: the low half's last step is 2^-24, so a weight is held to 2^-22 of itself or 2^-35
+//            of the largest (with 3 in its place 2^-28: 2^15 keys at that below one lost 1e-4 of the output together), for
+//            an exponent of up to 10 whose own rounding takes the outputs from 2.3 … 3.6e-7 to 2.7 … 4.0e-7 of 64 bits;
 //   values   Oᵀ += Vᵀ·(ph + pl)ᵀ, V by transposing LDS reads, p in the lanes that it was made in.
 // A key that a row does not see is as if it were not there, whatever the cache holds in it: its score becomes −∞ after the
 // product, and values of V that are not finite are taken out of the product of a block that not every row sees, and make
@@ -35,7 +37,7 @@ namespace {
 
 constexpr int D = 128, KB = 32;                // head dim; keys a block
 constexpr int K_CHUNKS = 512, TILE = 1024;     // 16-byte chunks of a block's K, of its K and V
-constexpr float P_SHIFT = 3.0f, P_ROOM = 5.0f; // log2 of the largest p when m moves; its growth before m must move
+constexpr float P_SHIFT = 10.0f, P_ROOM = 5.0f; // log2 of the largest p when m moves; its growth before m must move
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float M_NONE = -3.0e38f;             // m before the first key: finite, so that s − m is never ∞ − ∞
 constexpr int MAX_SPLIT = 64, TICKET = 32;     // parts of a row group's blocks; words between tickets (128 bytes)
@@ -285,7 +287,7 @@ template <typename F> __device__ __forceinline__ void put_nan(f32x16 (&o)[4], ui
 // A workgroup takes 16 rows and a run of units of 16 keys, eight a round, one to each of its eight waves:
 //   scores   a wave's own unit against all rows, Sᵀ = K·(qh + ql)ᵀ by v_mfma_f32_16x16x32_f16: lane 16g + c holds row c's
 //            scores of keys 4g … 4g + 3; the rows' largest over the waves through LDS (barrier);
-//   weights  p = 2^((s − m)·c + 3) as f16 pairs to LDS, in the order of the next products' operands (barrier);
+//   weights  p = 2^((s − m)·c + 10) as f16 pairs to LDS, in the order of the next products' operands (barrier);
 //   values   Oᵀ += Vᵀ·(ph + pl)ᵀ over the round's 128 keys, a wave's own 16 dims. So every K and V value is loaded, and made
 //            f16, once for all the rows, no sums of O are merged between waves, and O is 4 registers.
 // K and V come straight into LDS, a wave's own unit each: K into one buffer (read by that wave alone, filled again once the

@@ -218,7 +218,8 @@ int htr_kv_keep(htr_device *dev, const htr_kv *kv, int row0, const int32_t *h_id
  * d_out [n][n_head·128] = softmax(scale·q·Kᵀ)·V, zeros for a query that sees no row. n = 1 is a decode step's attention.
  * A row that a query does not see does not touch its output, whatever it holds; of one that it sees a V value that is not
  * finite gives one that is not, a K value that is not a score of NaN or of an infinity (−∞: no weight). All sums in f32,
- * q and the weights held to 22 bits; over a q8_0 cache the same bits as over its read-back, and the same bits every time.
+ * q held to 22 bits of its row's largest value, a weight to 22 bits or 2^-35 of its row's largest weight; over a q8_0 cache
+ * the same bits as over its read-back, and the same bits every time.
  * Scratch: 4.4 MB, the same for every size, made at the first call that splits a query's keys; and for a q8_0 cache that
  * many rows read (over 12000 rows of q heads), its rows in f16: at least 32 MB, doubled when it grows, what it was before
  * kept until the device is closed, so that graphs recorded over it stay good. A call that makes or grows scratch cannot be

@@ -936,3 +936,47 @@ def test_a_key_moves_only_the_rows_that_see_it(dev, n, group, n_kv, window, q8_0
         c.free()
         assert np.array_equal(bits(got[before]), bits(want[before])), change
         assert not np.array_equal(bits(got[~before]), bits(want[~before]))
+
+
+@pytest.mark.parametrize("kind", ["few", "split", "many"])
+@pytest.mark.parametrize("q8_0", [False, True], ids=["f16", "q8_0"])
+def test_small_weights_of_many_keys_count(dev, kind, q8_0):
+    """a few first keys take the largest weights, 2^28 times those of the many others: each of those is nothing beside them,
+    2^13 … 2^15 of them in a wave's run are not. A weight is held to 2^-22 of itself or 2^-35 of the largest, so the values'
+    sum of N of them errs by N·2^-35 of the largest value (2^-20 at most here), beside the exponential's and the f32 sums'
+    2^-21: 2^-18 leaves room. The keys' scores are exact: the queries have one dim that is not 0"""
+    if kind == "few":  # one token; a part of 2^13 keys to a workgroup, a large key at each one's start
+        n, rows, large = 1, 2 ** 19, np.arange(0, 2 ** 19, 2 ** 13)
+    elif kind == "split":  # a wave takes every eighth block of 32 keys: one large key in each of the first eight
+        n, rows, large = 32 * 129, 2 ** 16 + 32 * 129, 32 * np.arange(8)
+    else:  # a wave takes every other block
+        n, rows, large = 32 * 3 * 256 + 64, 2 ** 15 + 32 * 3 * 256 + 64, 32 * np.arange(2)
+    x = np.ones((1, rows, 128), np.float16)  # K and V alike: dim 0 makes the scores, the others are the values
+    x[0, :, :32], x[0, large] = 0, 0
+    x[0, large, 0] = 16
+    scale = 28.03 / 16 / np.log2(np.e)
+    if q8_0:
+        qx, dx = blocks(x)
+        x = values(qx, dx)
+        bufs = [dev.upload(qx), dev.upload(dx)]
+        kv = htr.KvCache.of(1, rows, bufs[0], bufs[0], bufs[1], bufs[1])
+    else:
+        bufs = [dev.upload(x)]
+        kv = htr.KvCache.of(1, rows, bufs[0], bufs[0])
+    q = np.zeros((n, 1, 128), np.float32)
+    q[..., 0] = 1.0
+    c = type("c", (), {"kv": kv})
+    if kind == "few":
+        got = run_tree(dev, q, c, 1, rows - 1, scale)
+    else:
+        got = run_window(dev, q, c, rows - n, rows, 0, scale)
+    keys = rows - n + 1 + np.arange(n)
+    w = np.exp(-float(x[0, 0, 0]) * float(np.float32(scale)))
+    small = (keys - large.size) * w / (large.size + (keys - large.size) * w)
+    tail = float(x[0, 1, 127])
+    assert np.all(x[0, 1, 32:] == x[0, 1, 127]) and small.min() > 2.0 ** -17  # (more than the bar: that they count is seen)
+    off = np.abs(got[:, 32:].astype(np.float64) - small[:, None] * tail)
+    print(f"\n[{kind}] the small ones' share {small.max():.2e}, off by {off.max():.2e}", flush=True)
+    assert off.max() < 2.0 ** -18 * tail
+    for b in bufs:
+        b.free()
