@@ -79,8 +79,8 @@ enum {
 // the device's scratch buffer `slot` with at least `bytes` bytes (a larger one replaces it: the tickets' and best
 // keys' slots zero-filled, the others as htr_dev_alloc fills)
 int htr_scratch(htr_device *dev, int slot, size_t bytes, void **out);
-// the same for scratch that recorded graphs may hold: at least doubled when it grows, and what it was before stays
-// allocated until the device is closed
+// the same for scratch that recorded graphs may hold: at least doubled when it grows (where that finds no room, just
+// `bytes`), and what it was before stays allocated until the device is closed
 int htr_scratch_kept(htr_device *dev, int slot, size_t bytes, void **out);
 
 // the device is dead: latch the first reason and fire the hook once; returns -1

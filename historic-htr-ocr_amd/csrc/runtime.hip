@@ -303,13 +303,19 @@ static int fill_new(htr_device *dev, void *p, size_t b, bool zero) {
     return htr_hip(dev, hipMemsetAsync(p, zero || !dev->poison ? 0 : 0xFF, b, dev->stream), "hipMemsetAsync");
 }
 
-static int alloc_filled(htr_device *dev, size_t bytes, int kind, bool zero, void **out) {
+// or_less: where there is no room for `bytes` that is no failure of the device, *out is NULL
+static int alloc_filled(htr_device *dev, size_t bytes, int kind, bool zero, void **out, bool or_less = false) {
     HTR_TRY(htr_check_alive(dev));
     HTR_TRY(htr_check_not_capturing(dev, "device allocation"));
     if (kind < HTR_MEM_WEIGHTS || kind > HTR_MEM_READBACK) return htr_fail("memory kind %d: 0…3", kind);
     size_t b = std::max<size_t>(bytes, 4);
     void *p = nullptr;
     hipError_t e = hipMalloc(&p, b);
+    if (e == hipErrorOutOfMemory && or_less) {
+        (void)hipGetLastError();  // the runtime's per-thread error is this one: clear it for later launch checks
+        *out = nullptr;
+        return 0;
+    }
     if (e != hipSuccess) {
         char what[128];
         snprintf(what, sizeof what, "hipMalloc(%zu bytes)", b);
@@ -361,9 +367,10 @@ int htr_scratch(htr_device *dev, int slot, size_t bytes, void **out) {
 
 int htr_scratch_kept(htr_device *dev, int slot, size_t bytes, void **out) {
     if (dev->scratch_bytes[slot] < bytes) {
-        const size_t b = std::max({bytes, 2 * dev->scratch_bytes[slot], (size_t)32 << 20});
+        size_t b = std::max({bytes, 2 * dev->scratch_bytes[slot], (size_t)32 << 20});
         void *p;
-        HTR_TRY(alloc_filled(dev, b, HTR_MEM_WORK, false, &p));
+        HTR_TRY(alloc_filled(dev, b, HTR_MEM_WORK, false, &p, b > bytes));
+        if (!p) HTR_TRY(alloc_filled(dev, b = bytes, HTR_MEM_WORK, false, &p));
         dev->scratch[slot] = p;
         dev->scratch_bytes[slot] = b;
     }

@@ -221,10 +221,10 @@ int htr_kv_keep(htr_device *dev, const htr_kv *kv, int row0, const int32_t *h_id
  * q held to 22 bits of its row's largest value, a weight to 22 bits or 2^-35 of its row's largest weight; over a q8_0 cache
  * the same bits as over its read-back, and the same bits every time.
  * Scratch: 4.4 MB, the same for every size, made at the first call that splits a query's keys; and for a q8_0 cache that
- * many rows read (over 12000 rows of q heads), its rows in f16: at least 32 MB, doubled when it grows, what it was before
- * kept until the device is closed, so that graphs recorded over it stay good. A call that makes or grows scratch cannot be
- * one that is being captured. The output is apart from the queries and the cache (else refused); strides multiples of 4,
- * pointers 16-byte aligned. */
+ * many rows read (over 12000 rows of q heads), its rows in f16: at least 32 MB, doubled when it grows (where that finds no
+ * room, what the call needs), what it was before kept until the device is closed, so that graphs recorded over it stay
+ * good. A call that makes or grows scratch cannot be one that is being captured. The output is apart from the queries and
+ * the cache (else refused); strides multiples of 4, pointers 16-byte aligned. */
 int htr_tree_attention(htr_device *dev, const float *d_q, size_t q_stride, int n, const uint64_t *h_mask, int n_past,
                        const htr_kv *kv, int n_head, float scale, float *d_out);
 /* attention with a sliding window and first keys that stay visible: queries at positions pos0 … pos0 + n_q − 1, the one at

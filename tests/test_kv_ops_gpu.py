@@ -980,3 +980,34 @@ def test_small_weights_of_many_keys_count(dev, kind, q8_0):
     assert off.max() < 2.0 ** -18 * tail
     for b in bufs:
         b.free()
+
+
+def test_scratch_that_cannot_double_is_what_the_call_needs(dev):
+    """room for rows read back is doubled when it grows, and exactly what the call needs where the doubled size is not there:
+    the call goes on, and the device stays alive"""
+    n_kv, n, gib = 64, 200, 1 << 30
+    d = htr.Device(0)
+    try:
+        c = htr.KvCache(d, n_kv, 75000, q8_0=True)
+        some = cache(d, 171, n_kv, 300, True)
+        htr.kv_copy(d, some.kv, 0, c, 59700, 300)
+        htr.kv_copy(d, some.kv, 0, c, 74700, 300)
+        q = normal(172, n, 2 * n_kv, 128)
+        at = type("c", (), {"kv": c})
+        run_window(d, q, at, 60000 - n, 75000, 0)  # 2 · 64 · 60000 rows of 256 bytes: 1.83 GiB
+        need, doubled = 2 * n_kv * 75000 * 256, 2 * 2 * n_kv * 60000 * 256
+        free, total = C.c_size_t(), C.c_size_t()
+        assert htr.lib().hipMemGetInfo(C.byref(free), C.byref(total)) == 0
+        left = (need + doubled) // 2  # 0.7 GiB more than the call needs, as much less than it would like
+        held = free.value - left
+        while held > 0:
+            d.alloc(min(held, 8 * gib))
+            held -= 8 * gib
+        before = d.mem_live()["work"]
+        got = run_window(d, q, at, 75000 - n, 75000, 0)
+        d.alive()
+        assert d.mem_live()["work"] - before == need
+        few = run_window(d, q[n - 4:], at, 74996, 75000, 0)  # (by a kernel that reads no rows back)
+        assert rel_rows(got[n - 4:], few.astype(np.float64)) < 2 * BAR
+    finally:
+        d.close()
