@@ -471,11 +471,12 @@ def causal_attention(dev: Device, q: Buffer, kc: Buffer, vc: Buffer, n_q: int, p
 
 class KvCache:
     """One layer's KV cache (htr_kv): f16 rows, or q8_0 blocks as int8 quants and f16 scales. ``KvCache(dev, n_kv, n_ctx)``
-    allocates one (freed by ``free``); ``KvCache.of`` takes buffers that the caller holds."""
+    allocates one (freed by ``free``, and refused by every call from then on); ``KvCache.of`` takes buffers that the caller
+    holds for as long as the cache is used."""
 
     def __init__(self, dev: Device, n_kv: int, n_ctx: int, q8_0: bool = False):
         rows = n_kv * n_ctx
-        self.held = []
+        self.held, self.c = [], KvC()
         try:
             for nbytes in (rows * 128 * (1 if q8_0 else 2),) * 2 + (rows * 8,) * (2 if q8_0 else 0):
                 self.held.append(Buffer(dev, nbytes, MEM_KV_CACHE))
@@ -501,6 +502,8 @@ class KvCache:
         self.ref = C.addressof(self.c)
 
     def free(self) -> None:
+        if self.held:
+            self.c.d_k = self.c.d_v = self.c.d_kd = self.c.d_vd = None
         for b in self.held:
             b.free()
         self.held = []

@@ -182,3 +182,54 @@ def test_no_lds_access_in_flight_at_a_barrier(tmp_path):
         between = [s for s in body[first:last] if s.startswith(("global_", "buffer_", "flat_", "scratch_"))]
         assert between and all("_load_lds_" in s for s in between), (name, [s for s in between if "_load_lds_" not in s])
     assert seen >= 40
+
+
+class _Memory:
+    """stands in for a device's buffers: an address that no call follows"""
+    made = []
+
+    def __init__(self, dev, nbytes, kind):
+        if len(self.made) == dev.room:
+            raise htr.HtrError("no room")
+        self.ptr = (len(self.made) + 1) << 20
+        self.made.append(self)
+
+    def free(self):
+        self.ptr = None
+
+
+class _NoDevice:
+    h, room = None, 4
+
+
+def test_a_cache_that_was_freed_is_refused(monkeypatch):
+    """its addresses go with its memory: a call on it must not reach what another allocation has there by then"""
+    monkeypatch.setattr(htr, "Buffer", _Memory)
+    monkeypatch.setattr(_Memory, "made", [])
+    out = _Memory(_NoDevice, 0, 0)
+    for q8_0 in (False, True):
+        _Memory.made.clear()
+        kv = htr.KvCache(_NoDevice, 2, 50, q8_0)
+        calls = [lambda: htr.kv_keep(_NoDevice, kv, 0, [1]), lambda: htr.kv_copy(_NoDevice, kv, 0, kv, 9, 1),
+                 lambda: htr.tree_attention(_NoDevice, out, 1, 5, kv, 2, 1.0, type("B", (), {"ptr": 16 << 20})),
+                 lambda: htr.window_attention(_NoDevice, out, 1, 5, 3, 0, kv, 2, 1.0, type("B", (), {"ptr": 16 << 20}))]
+        for call in calls:
+            with pytest.raises(htr.HtrError, match="null device"):
+                call()
+        kv.free()
+        for call in calls:
+            with pytest.raises(htr.HtrError, match="null cache rows"):
+                call()
+        kv.free()
+    lent = htr.KvCache.of(2, 50, out, type("B", (), {"ptr": 9 << 20}))
+    lent.free()  # the caller's buffers: nothing to free
+    with pytest.raises(htr.HtrError, match="null device"):
+        htr.kv_keep(_NoDevice, lent, 0, [1])
+
+
+def test_a_cache_without_room_for_all_planes_frees_those_it_had(monkeypatch):
+    monkeypatch.setattr(htr, "Buffer", _Memory)
+    monkeypatch.setattr(_Memory, "made", [])
+    with pytest.raises(htr.HtrError, match="no room"):
+        htr.KvCache(type("D", (), {"h": None, "room": 3}), 2, 50, True)
+    assert len(_Memory.made) == 3 and all(b.ptr is None for b in _Memory.made)
