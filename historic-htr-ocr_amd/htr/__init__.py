@@ -475,6 +475,7 @@ class KvCache:
     holds for as long as the cache is used."""
 
     def __init__(self, dev: Device, n_kv: int, n_ctx: int, q8_0: bool = False):
+        self._check(n_kv, n_ctx)
         rows = n_kv * n_ctx
         self.held, self.c = [], KvC()
         try:
@@ -488,10 +489,16 @@ class KvCache:
     @classmethod
     def of(cls, n_kv: int, n_ctx: int, k, v, kd=None, vd=None) -> "KvCache":
         """a cache on buffers (anything with ``ptr``): f16 rows k, v, or int8 quants with the f16 scales kd, vd"""
+        cls._check(n_kv, n_ctx)
         self = cls.__new__(cls)
         self.held = []
         self._set(n_kv, n_ctx, k, v, kd, vd)
         return self
+
+    @staticmethod
+    def _check(n_kv: int, n_ctx: int) -> None:
+        if not (1 <= n_kv <= 4096 and 1 <= n_ctx < 2 ** 31):
+            raise ValueError(f"a cache of {n_kv} KV heads, {n_ctx} rows (1 … 4096 heads, 1 … 2^31 - 1 rows)")
 
     def _set(self, n_kv: int, n_ctx: int, k, v, kd=None, vd=None) -> None:
         if (kd is None) != (vd is None):

@@ -233,3 +233,16 @@ def test_a_cache_without_room_for_all_planes_frees_those_it_had(monkeypatch):
     with pytest.raises(htr.HtrError, match="no room"):
         htr.KvCache(type("D", (), {"h": None, "room": 3}), 2, 50, True)
     assert len(_Memory.made) == 3 and all(b.ptr is None for b in _Memory.made)
+
+
+@pytest.mark.parametrize("n_kv,n_ctx", [(0, 5), (-1, 5), (4097, 5), (2, 0), (2, -3), (2, 2 ** 31)])
+def test_a_cache_of_sizes_that_no_call_takes_asks_for_no_memory(monkeypatch, n_kv, n_ctx):
+    """(a negative size would be asked for as nearly 2^64 bytes, which leaves the device dead; one past 32 bits would reach
+    the library as another)"""
+    monkeypatch.setattr(htr, "Buffer", _Memory)
+    monkeypatch.setattr(_Memory, "made", [])
+    with pytest.raises(ValueError, match="KV heads"):
+        htr.KvCache(_NoDevice, n_kv, n_ctx)
+    assert not _Memory.made
+    with pytest.raises(ValueError, match="KV heads"):
+        htr.KvCache.of(n_kv, n_ctx, type("B", (), {"ptr": 1 << 20}), type("B", (), {"ptr": 2 << 20}))
