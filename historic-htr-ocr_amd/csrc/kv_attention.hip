@@ -1296,10 +1296,9 @@ template <bool TREE> int launch(htr_device *dev, Args &a, const TreeMask &tree, 
     // of q8_0 80 and 90, 117 and 123, 153 and 122; 1500 from position 0 without a window 35 and 35, 2000 52 and 43
     if (rows > KB && (int64_t)((rows + KB - 1) / KB) * a.kv.n_kv > 3 * dev->n_cu) {
         a.n_rg = (rows + KB * WR - 1) / (KB * WR), a.n_split = 1;
-        const int64_t groups = (int64_t)a.n_rg * a.kv.n_kv;
-        if (groups > INT32_MAX) return htr_fail("attention: %d rows of %d KV heads", rows, a.kv.n_kv);
+        const unsigned groups = (unsigned)a.n_rg * (unsigned)a.kv.n_kv;  // (check_rows: they fit)
         if (a.kv.q8) HTR_TRY(read_back(dev, a, TREE ? a.n_past + a.n : a.pos0 + a.n, sink_rows, from_row));
-        hipLaunchKernelGGL((k_kv_attn<TREE>), dim3((unsigned)groups), dim3(64 * WR * WP), 0, dev->stream, a, tree);
+        hipLaunchKernelGGL((k_kv_attn<TREE>), dim3(groups), dim3(64 * WR * WP), 0, dev->stream, a, tree);
         return htr_launched(dev, "k_kv_attn");
     }
     if (rows <= FR) return launch_split<TREE, true>(dev, a, tree, max_keys);
@@ -1315,7 +1314,9 @@ int check_rows(const char *me, const float *d_q, size_t q_stride, const htr_kv *
         return htr_fail("%s: rows %zu floats apart (a multiple of 4, at least %zu)", me, q_stride, qd);
     if (((uintptr_t)d_q | (uintptr_t)d_out) & 15) return htr_fail("%s: pointers must be 16-byte aligned", me);
     const int64_t group = n_head / kv->n_kv;  // (rows · group < 2^32: the kernels' quotients)
-    if (n * group > 1 << 30 || n * group * group >= 1ll << 32) return htr_fail("%s: %lld queries of %d heads", me, (long long)n, n_head);
+    if (n * group > 1 << 30 || n * group * group >= 1ll << 32 ||
+        (n * group + KB * WR - 1) / (KB * WR) * kv->n_kv > (int64_t)HTR_MAX_GROUPS)  // (those of the kernel of many rows)
+        return htr_fail("%s: %lld queries of %d heads", me, (long long)n, n_head);
     const uintptr_t q0 = (uintptr_t)d_q, q1 = q0 + 4 * (q_stride * (n - 1) + qd), o0 = (uintptr_t)d_out, o1 = o0 + 4 * qd * n;
     if (q0 < o1 && o0 < q1) return htr_fail("%s: the output overlaps the queries", me);
     if (htr_kv_overlaps(planes, d_out, 4 * qd * n)) return htr_fail("%s: the output overlaps the cache", me);

@@ -475,7 +475,9 @@ extern "C" int htr_qkv_post_rows(htr_device *dev, const float *d_q, size_t q_str
         if (overlap(w.p, w.n, d_q_out, out_bytes) || htr_kv_overlaps(a.kv, w.p, w.n))
             return htr_fail("%s: the q output or the cache overlaps the norms' weights or the rope table", me);
     const size_t count = (size_t)n * ((size_t)n_head + 2 * kv->n_kv), grid = (count + 15) / 16;
-    if (count > (size_t)INT32_MAX) return htr_fail("%s: %d rows of %d heads", me, n, n_head);
+    if (grid > HTR_MAX_GROUPS)
+        return htr_fail("%s: %d rows of %d + %d heads in one call (at most %zu heads' rows)", me, n, n_head, 2 * kv->n_kv,
+                        16 * HTR_MAX_GROUPS);
     HTR_TRY(htr_check_alive(dev));
     const HtrOnDevice on(dev);
     a.q = d_q, a.k = d_k, a.v = d_v, a.q_stride = q_stride, a.kv_stride = kv_stride;
@@ -499,6 +501,8 @@ extern "C" int htr_kv_copy(htr_device *dev, const htr_kv *src, int src_row, cons
     if (src->n_kv != dst->n_kv) return htr_fail("%s: %d KV heads into %d", me, src->n_kv, dst->n_kv);
     if (n < 0 || src_row < 0 || src_row > src->n_ctx - n || dst_row < 0 || dst_row > dst->n_ctx - n)
         return htr_fail("%s: %d rows from row %d of %d to row %d of %d", me, n, src_row, src->n_ctx, dst_row, dst->n_ctx);
+    if ((size_t)n > COPY_ROWS * HTR_MAX_GROUPS)
+        return htr_fail("%s: %d rows in one call (at most %zu)", me, n, COPY_ROWS * HTR_MAX_GROUPS);
     // the caches' planes: apart, or the same ones with rows apart
     HTR_TRY(check_apart(me, a.dst));
     const Planes src_planes(a.src), dst_planes(a.dst);

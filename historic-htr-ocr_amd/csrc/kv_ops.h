@@ -40,6 +40,9 @@ struct HtrKvPlanes {
     int n_kv, n_ctx;
     bool q8;
 };
+// the most workgroups of 256 threads along a grid's first dimension, which takes less than 2^32 threads (a launch of more
+// fails, and leaves the device dead)
+constexpr size_t HTR_MAX_GROUPS = (1u << 24) - 1;
 // 0 with *out filled, or -1 with the message of what is wrong with the cache
 int htr_kv_check(const char *what, const htr_kv *kv, HtrKvPlanes *out);
 

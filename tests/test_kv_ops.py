@@ -246,3 +246,19 @@ def test_a_cache_of_sizes_that_no_call_takes_asks_for_no_memory(monkeypatch, n_k
     assert not _Memory.made
     with pytest.raises(ValueError, match="KV heads"):
         htr.KvCache.of(n_kv, n_ctx, type("B", (), {"ptr": 1 << 20}), type("B", (), {"ptr": 2 << 20}))
+
+
+def test_more_rows_than_a_launch_takes_are_refused():
+    """a grid's first dimension holds less than 2^32 threads: a launch of more fails and leaves the device dead, so that such a
+    call is refused before, and the largest below is not"""
+    T = 1 << 40
+    big = dict(n_kv=4, n_ctx=2 ** 24, k=T, v=2 * T)
+    post = dict(q=3 * T, k=4 * T, v=5 * T, n_head=8, qs=1024, ks=512, row0=0, pos0=0, n_pos=2 ** 25, out=6 * T)  # 16 heads a row
+    _refused(_calls(_kv(**big))["post"](n=2 ** 24, **post), "16777216 rows of 8 + 8 heads in one call")
+    _refused(_calls(_kv(**big))["post"](n=2 ** 24 - 1, **post), "null device")
+    long = [_kv(n_kv=1, n_ctx=2 ** 30, k=i * T, v=(i + 1) * T) for i in (1, 3)]
+    _refused(_calls(long[0])["copy"](dst=long[1], n=2 ** 29), "536870912 rows in one call")
+    _refused(_calls(long[0])["copy"](dst=long[1], n=2 ** 29 - 32), "null device")
+    wide = _kv(n_kv=2, n_ctx=2 ** 28, k=T, v=2 * T)
+    _refused(_calls(wide)["window"](q=3 * T, out=4 * T, n=2 ** 28, pos0=0), "268435456 queries of 4 heads")
+    _refused(_calls(wide)["window"](q=3 * T, out=4 * T, n=2 ** 28 - 32, pos0=0), "null device")
