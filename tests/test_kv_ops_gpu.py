@@ -1011,3 +1011,113 @@ def test_scratch_that_cannot_double_is_what_the_call_needs(dev):
         assert rel_rows(got[n - 4:], few.astype(np.float64)) < 2 * BAR
     finally:
         d.close()
+
+
+@pytest.mark.parametrize("sink", [0, 1, 33, 64])
+@pytest.mark.parametrize("pos0,window", [(1500, 100), (1503, 1), (1520, 65)])
+def test_windows_read_back_as_two_ranges(dev, pos0, window, sink):
+    """many queries over a q8_0 cache whose first keys and window are far apart: the rows between are not read back, and the
+    blocks past them lie further down than their keys say. The first row group's window starts on the second range's first
+    block. What lies between is not finite, and what is seen as over the whole cache's read-back, bit for bit"""
+    n, n_kv, group = 200, 64, 2
+    rows = pos0 + n + 3
+    first, from_row = (sink + 31) // 32 * 32, (pos0 - window + 1) // 32 * 32
+    assert from_row - first > (pos0 + n) // 4
+    k, v = (normal(s, n_kv, rows, 128).astype(np.float16) for s in (1, 2))
+    c = Cache(dev, k, v, True)
+    back = cache(dev, 3, n_kv, rows)
+    htr.kv_copy(dev, c.kv, 0, back.kv, 0, rows)
+    for b in c.bufs[2:]:
+        d = b.download(np.float16).reshape(n_kv, rows, 4)
+        d[:, first:from_row] = np.nan
+        b.upload(d)
+    q = normal(4, n, n_kv * group, 128)
+    got, want = (run_window(dev, q, x, pos0, window, sink) for x in (c, back))
+    assert np.array_equal(bits(got), bits(want))
+    plain = attention(q[:, :4], c.k[:2], c.v[:2], window_seen(n, pos0, window, sink, rows), SCALE)
+    assert rel_rows(got.reshape(n, -1, 128)[:, :4].reshape(n, -1), plain) < BAR
+    c.free()
+    back.free()
+
+
+@pytest.mark.parametrize("n,group,n_kv", WAYS)
+@pytest.mark.parametrize("q8_0", [False, True], ids=["f16", "q8_0"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_rows_that_are_not_seen_leave_every_bit(dev, n, group, n_kv, q8_0, bad):
+    """K or V rows with a value that is not finite: the queries that do not see them are bit for bit as without, in every
+    kernel, and of V the other dims of those that do too. A V value gives one that is not finite in its dims; a K value a
+    score of NaN, and so outputs of NaN, or of an infinity, of which −∞ takes the key's weight"""
+    rows, window, sink = n + 300, 150, 3
+    k, v = normal(1, n_kv, rows, 128).astype(np.float16), normal(2, n_kv, rows, 128).astype(np.float16)
+    pos0, r, d = rows - n, rows - n // 2 - 1, 100
+    dims = list(range(96, 128)) if q8_0 else [d]
+    seen = window_seen(n, pos0, window, sink, rows)
+    sees = seen[:, r].copy()
+    assert 0 < sees.sum() < n
+    q = normal(3, n, n_kv * group, 128)
+    clean = Cache(dev, k, v, q8_0)
+    want = run_window(dev, q, clean, pos0, window, sink).reshape(n, -1, 128)
+    seen[:, r] = False
+    hs = min(n_kv, 2)
+    without = attention(q[:, :hs * group], clean.k[:hs], clean.v[:hs], seen, SCALE).reshape(n, -1, 128)
+    clean.free()
+    for which in (0, 1):
+        x = [k.copy(), v.copy()]
+        x[which][:, r, d] = bad
+        c = Cache(dev, *x, q8_0)
+        got = run_window(dev, q, c, pos0, window, sink).reshape(n, -1, 128)
+        c.free()
+        assert np.array_equal(bits(got[~sees]), bits(want[~sees]))
+        if which:
+            others = [i for i in range(128) if i not in dims]
+            assert not np.any(np.isfinite(got[sees][..., dims]))
+            assert np.array_equal(bits(got[sees][..., others]), bits(want[sees][..., others]))
+            continue
+        nan = np.isnan(got[sees]).all(axis=2)
+        if np.isnan(bad) or q8_0:  # (a q8_0 block with an infinity is NaN)
+            assert nan.all()
+            continue
+        assert np.array_equal(nan, ~np.isfinite(got[sees]).all(axis=2))
+        rest, plain, nan = got[sees][:, :hs * group], without[sees], nan[:, :hs * group]
+        off = np.linalg.norm(rest - plain, axis=2) / np.linalg.norm(plain, axis=2)
+        assert np.all(off[~nan] < BAR)
+
+
+def test_rows_beside_those_of_a_decode_step(dev):
+    """the same raw rows by htr_qkv_post, one at a time, and by htr_qkv_post_rows: V bit for bit; q and K within what the
+    step's f32 norm and turn err by, some 16 roundings, 2^-20 of the pair's size, and, of K, an f16 ulp where a border lies
+    between the two"""
+    n, n_head, n_kv, pos0, n_ctx = 37, 16, 8, 611, 700
+    x = normal(5, n, n_head + 2 * n_kv, 128, std=3.0)
+    qn, kn = normal(6, 128, std=0.1) + 1, normal(7, 128, std=0.1) + 1
+    cs = orc.rope_table(1e6, 128, n_ctx)
+    w = [dev.upload(a) for a in (qn, kn, cs)]
+    step, rows = cache(dev, 8, n_kv, n_ctx), cache(dev, 8, n_kv, n_ctx)
+    q_step = np.empty((n, n_head, 128), np.float32)
+    for t in range(n):
+        raw = dev.upload(x[t])
+        htr.qkv_post(dev, raw, *w, n_head, n_kv, pos0 + t, n_ctx, EPS, *step.bufs)
+        q_step[t] = raw.download(np.float32, n_head * 128).reshape(n_head, 128)
+        raw.free()
+    raw, q_out, width = dev.upload(x), dev.alloc(n * n_head * 512), (n_head + 2 * n_kv) * 128
+
+    class At:
+        def __init__(self, ptr):
+            self.ptr = ptr
+
+    htr.qkv_post_rows(dev, raw, At(raw.ptr + n_head * 512), At(raw.ptr + (n_head + n_kv) * 512), n, *w, n_ctx, pos0, n_head, EPS,
+                      rows.kv, pos0, q_out, q_stride=width, kv_stride=width)
+    assert np.array_equal(bits(step.rows("v")), bits(rows.rows("v")))
+
+    def pair(y):  # the size of each value's pair, a dim and the one 64 further on
+        s = np.abs(y[..., :64].astype(np.float64)) + np.abs(y[..., 64:])
+        return 2.0 ** -20 * np.concatenate([s, s], axis=-1)
+
+    q_rows = q_out.download(np.float32).reshape(n, n_head, 128)
+    assert np.all(np.abs(q_rows.astype(np.float64) - q_step) <= pair(q_rows))
+    a, b = step.rows("k").astype(np.float64), rows.rows("k").astype(np.float64)
+    ulp = 2.0 ** -10 * np.maximum(np.abs(a), np.abs(b)) + 2.0 ** -24
+    assert np.all(np.abs(a - b) <= ulp + pair(b))
+    print(f"\n[K rows that differ] {np.mean(a != b):.1e} of the cache's values", flush=True)
+    for y in (step, rows, raw, q_out, *w):
+        y.free()
