@@ -60,7 +60,7 @@ struct Args {
     int n, n_head, group;
     uint32_t per_group;        // ⌈2^32 / group⌉ (group > 1): the quotient of a row below 2^32 / group by one product
     float scale;
-    int sink_rows, shift;      // keys from sink_rows on lie shift rows further up in memory
+    int shift;                 // keys past the first ones' blocks lie this many rows further up in memory
     int n_past;                // tree: the committed keys
     int pos0, window, n_sink;  // window
     int n_rg, n_split;         // row groups, parts of a row group's key blocks
@@ -1247,7 +1247,7 @@ int read_back(htr_device *dev, Args &a, int n_keys, int sink_rows, int from_row)
     const HtrKvPlanes src = a.kv, dst{p, (char *)p + bytes, nullptr, nullptr, src.n_kv, (int)rows, false};
     if (first) HTR_TRY(htr_kv_read_back(dev, src, 0, dst, 0, first));
     if (rest) HTR_TRY(htr_kv_read_back(dev, src, from_row, dst, sink_rows, rest));
-    a.kv = dst, a.sink_rows = sink_rows, a.shift = from_row - sink_rows;
+    a.kv = dst, a.shift = from_row - sink_rows;
     return 0;
 }
 
