@@ -298,8 +298,11 @@ template <typename F> __device__ __forceinline__ void put_nan(f32x16 (&o)[4], ui
 //   q8_0  [16 keys][8 chunks], row r's chunk c at 8r + (c ^ r / 2), V's of odd units with c ^ 4 too; the scales [16 keys][4]:
 // reads of 16 (32) lanes fall on different bank groups.
 //
-// Bound: latency. A call takes 5.0 µs up to 128 keys and 0.95 (f16) or 1.2 µs (q8_0) a further round; splitting the keys
-// costs 2.4. One token over 2000 f16 keys 7.8 µs, over 8000 q8_0 keys 10.3 (17.4 MB: 3.5 at a copy's rate). The waves'
+// Bound: latency, of the loads and of a round's two barriers and exchanges. A call takes 5.0 µs up to 128 keys and 0.95 (f16)
+// or 1.2 µs (q8_0) a further round; splitting the keys costs 2.4. One token over 8000 q8_0 keys takes 10.2 µs (17.4 MB: 2.5 at
+// the 7.0 TB/s of a read). k_attn_decode, for one token, f16 rows and two q heads to a KV head alone, has all its keys' loads in
+// flight at once and exchanges between waves only at the end: over 512 / 2048 / 8192 keys 6.4 / 6.4 / 9.2 µs, this kernel
+// 7.2 / 7.7 / 9.4 (q8_0 rows 7.4 / 7.7 / 9.7). The waves'
 // own blocks of k_kv_attn_split take 9.2 over 1000 keys (here 7.3) and 11.8 over the 8000 (their 32-row products are half or
 // more empty, and their sums have to be merged); at 16 rows the two are as fast, above this way is slower (24 rows over 1300
 // keys 11.6 and 10.7, over 6000 q8_0 keys 15.1 and 12.5).
@@ -681,7 +684,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
 //
 // Bound: of few keys latency (8 µs a call up to 300 keys: 2 until the first block is there, 2 for the merge), of many the
 // instructions of its two waves a SIMD: a block of f16 is 32 MFMA and some 130 VALU instructions, 16 of them exponentials,
-// one of q8_0 224 VALU instructions more (MFMA busy 33 %, VALU 58 % over 40013 keys). 64 tokens over 6001 f16 keys 16.0 µs (27
+// one of q8_0 224 VALU instructions more (MFMA busy 34 %, VALU 59 % over 40013 keys). 64 tokens over 6001 f16 keys 16.0 µs (27
 // MB: 5.5 at a copy's rate), 27 over 40013 q8_0 keys 29.8 (88 MB: 17.8), of real values, whose products lower the clock, 33 …
 // 36. With four waves a workgroup the
 // kernels alone took 30.9 and 54.9 for 21.2 and 30. Two row tiles to a wave, which halves the conversions, cost 6.7 µs of the
@@ -1006,7 +1009,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(64 * SW, 2) void k_kv
 // workgroups, and 224 VALU instructions a block and wave would be as many as the softmax's).
 //
 // Bound: the matrix cores' work and the softmax's instructions on the same two waves a SIMD, and the power of the two: 6001
-// queries with a window of 1500 of a q8_0 cache, 149 GFLOP as pairs, 176 µs with 13 of reading back (MFMA busy 51 %, VALU
+// queries with a window of 1500 of a q8_0 cache, 149 GFLOP as pairs, 178 µs with 13 of reading back (MFMA busy 52 %, VALU
 // 44 %; of zeros, at the full clock, 143). 1925 with a window of 512 27.2 µs. 128 rows a workgroup, 8 waves: 198 (their barriers
 // hold twice as many).
 constexpr int WR = 2, WP = 2;  // row tiles, key parts

@@ -9,8 +9,9 @@
 // half of a block whose scale is among f16's last subnormals). Both are exact: the quotient's rounding is checked against
 // the exact remainder x − q·d, which f32 holds. A block with a NaN or an infinity gets a NaN scale.
 //
-// Bound: memory; each value passes once. Times below are of calls one after another on an MI355X, where a large copy reaches
-// 4.9 TB/s.
+// Bound: memory; each value passes once. Times below are of calls one after another on an MI355X, where 480008 rows of 8 heads,
+// past every cache, pass at 5.7 TB/s (f16 rows copied, 3.9 GB), 5.8 (quantised), 6.0 (read back, 3.0 GB each) and 6.3 (q8_0
+// rows copied, 2.1 GB), and a plain copy of 4 GiB at 5.0.
 #include <algorithm>
 
 #include "kv_ops.h"

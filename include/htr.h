@@ -192,36 +192,39 @@ enum { HTR_TREE_MAX = 64 };
 /* host only: the masks and depths of a tree of n nodes (1 … 64) whose node i continues node h_parent[i] < i, or the last
  * committed token (−1): h_mask[i] has the bits of the nodes on the path to i, i among them; a root's depth is 0 */
 int htr_tree_masks(const int32_t *h_parent, int n, uint64_t *h_mask, int32_t *h_depth);
-/* htr_qkv_post for n rows at once, into either type of cache: the raw q [n] rows q_stride floats apart (n_head heads of
+/* htr_qkv_post's work for n rows at once, into either type of cache: the raw q [n] rows q_stride floats apart (n_head heads of
  * 128), k and v rows kv_stride floats apart (n_kv heads), each q and k head RMS-normed with its weights and turned by
  * RoPE at position pos0 + h_depth[t] (row t of a draft: n ≤ 64, depths 0 … 63; h_depth NULL: pos0 + t) from the table
  * d_rope [n_pos][64] × (cos, sin); q to d_q_out [n][n_head·128], k and v to the cache's rows row0 + t. The norm and the
  * turn are computed in f64 and rounded to f32, then to f16 or q8_0 (a block's scale the smallest f16 number d with
  * 127·d ≥ max |x|, its quants x / d to the nearest integer, ties to even; finite values saturate at ±65468.5 = 127·515.5,
- * a block with a NaN or an infinity is NaN). Strides multiples of 4, pointers 16-byte aligned; d_q_out may be d_q where its rows are
- * n_head·128 apart, and overlaps the inputs in no other way; the cache is apart from both, and its planes from each other
- * (else refused). */
+ * a block with a NaN or an infinity is NaN). htr_qkv_post and the decode step work in f32: of the K values that they store
+ * some 3 in 10000 are the neighbouring f16 number, so a kept draft's rows are a step's to that, not bit for bit. Strides
+ * multiples of 4, pointers 16-byte aligned; d_q_out may be d_q where its rows are n_head·128 apart, and overlaps the inputs
+ * in no other way; the cache is apart from both, and its planes from each other; n·(n_head + 2·n_kv) ≤ 2^28 − 16 (else
+ * refused). */
 int htr_qkv_post_rows(htr_device *dev, const float *d_q, size_t q_stride, const float *d_k, const float *d_v,
                       size_t kv_stride, int n, const float *d_q_norm, const float *d_k_norm, const float *d_rope,
                       int n_pos, int pos0, const int32_t *h_depth, int n_head, float eps, const htr_kv *kv, int row0,
                       float *d_q_out);
 /* rows src_row … + n − 1 of one cache to rows dst_row … of another of as many KV heads: f16 to q8_0 quantises as above,
- * q8_0 to f16 reads back f16(q·d), like types copy. The caches' memory is apart, or it is one cache and the rows are
- * (else refused). */
+ * q8_0 to f16 reads back f16(q·d), like types copy. The caches' memory is apart, or it is one cache and the rows are;
+ * n ≤ 2^29 − 32 (else refused). */
 int htr_kv_copy(htr_device *dev, const htr_kv *src, int src_row, const htr_kv *dst, int dst_row, int n);
 /* rows row0 + h_idx[i] to rows row0 + i, i < n ≤ 64, all read before any is written (any order, a row more than once): a
- * draft's accepted path moved together, or beams reordered. The rows from row0 + n on stay as they are. */
+ * draft's accepted path moved together. The rows from row0 + n on stay as they are. */
 int htr_kv_keep(htr_device *dev, const htr_kv *kv, int row0, const int32_t *h_idx, int n);
 /* attention of a drafted tree over a cache: queries d_q [n], rows q_stride floats apart (n ≤ 64 nodes, n_head heads of
  * 128, n_head a multiple of n_kv), query t over rows 0 … n_past − 1 and the rows n_past + j whose bit j h_mask[t] has (the
  * host array of htr_tree_masks, or any other: read before the call returns; NULL: a chain, j ≤ t) →
- * d_out [n][n_head·128] = softmax(scale·q·Kᵀ)·V, zeros for a query that sees no row. n = 1 is a decode step's attention.
+ * d_out [n][n_head·128] = softmax(scale·q·Kᵀ)·V, zeros for a query that sees no row. n = 1 is a decode step's attention
+ * (over f16 rows with two q heads to a KV head htr_decode_attention is faster up to 8000 keys).
  * A row that a query does not see does not touch its output, whatever it holds; of one that it sees a V value that is not
  * finite gives one that is not, a K value that is not a score of NaN or of an infinity (−∞: no weight). All sums in f32,
  * q held to 22 bits of its row's largest value, a weight to 22 bits or 2^-35 of its row's largest weight; over a q8_0 cache
  * the same bits as over its read-back, and the same bits every time.
  * Scratch: 4.4 MB, the same for every size, made at the first call that splits a query's keys; and for a q8_0 cache that
- * many rows read (over 12000 rows of q heads), its rows in f16: at least 32 MB, doubled when it grows (where that finds no
+ * many rows read (n·n_head > 24576 on 256 CUs), its rows in f16: at least 32 MB, doubled when it grows (where that finds no
  * room, what the call needs), what it was before kept until the device is closed, so that graphs recorded over it stay
  * good. A call that makes or grows scratch cannot be one that is being captured. The output is apart from the queries and
  * the cache (else refused); strides multiples of 4, pointers 16-byte aligned. */
