@@ -140,7 +140,10 @@ struct PostRowsArgs {
     HtrKvPlanes kv;
     double eps;
     int n, n_head, pos0, row0;
+    const int32_t *pos, *slot;  // PAGES: each row's position and its row of the cache
+    int n_pos;
 };
+enum Place { IN_ORDER, DRAFT, PAGES };  // rows one after another; a draft's positions by depth; both from arrays
 struct TreeDepth {
     uint8_t at[HTR_TREE_MAX];
 };
@@ -151,11 +154,16 @@ struct TreeDepth {
 // summation a cache of its own. Its 70 operations a lane hide behind the lane's 100 bytes: 1925 rows of 16 + 2·8 heads into
 // q8_0 (51 MB) 10.5 µs, 4.9 TB/s, into f16 (55 MB) 10.1; with the library's 1 / sqrt, and V's heads taken through it all too,
 // 11.9 and 11.2; with 8 dims in a row to a lane, whose loads skip every other 16 bytes, 13.5 and 13.4. One row: 4 µs, a launch.
-template <bool Q8, bool TREE> __global__ __launch_bounds__(256) void k_post_rows(PostRowsArgs a, TreeDepth depth) {
+template <bool Q8, Place PLACE> __global__ __launch_bounds__(256) void k_post_rows(PostRowsArgs a, TreeDepth depth) {
     const int lane = threadIdx.x & 63, j = lane & 15, heads = a.n_head + 2 * a.kv.n_kv;
     const uint32_t id = blockIdx.x * 16u + (threadIdx.x >> 4), count = (uint32_t)a.n * heads, at = min(id, count - 1);
     const int t = (int)(at / (uint32_t)heads), h = (int)at - t * heads, kvh = h - a.n_head;
     const bool is_q = kvh < 0, is_v = kvh >= a.kv.n_kv;
+    int pos = a.pos0 + (PLACE == DRAFT ? depth.at[t] : t), to = a.row0 + t;
+    if constexpr (PLACE == PAGES) {  // (the 16 lanes of a head's row go together)
+        pos = a.pos[t], to = is_q ? 0 : a.slot[t];
+        if ((uint32_t)pos >= (uint32_t)a.n_pos || (uint32_t)to >= (uint32_t)a.kv.n_ctx) return;
+    }
     const float *src = is_q   ? a.q + t * a.q_stride + (size_t)h * D
                        : is_v ? a.v + t * a.kv_stride + (size_t)(kvh - a.kv.n_kv) * D
                               : a.k + t * a.kv_stride + (size_t)kvh * D;
@@ -163,7 +171,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256) void k_post_rows
 #pragma unroll
     for (int u = 0; u < 2; u++) *reinterpret_cast<float4 *>(y[u]) = *reinterpret_cast<const float4 *>(src + 64 * u + 4 * j);
     if (!is_v) {
-        const float *w = is_q ? a.qn : a.kn, *turn = a.rope + (size_t)(a.pos0 + (TREE ? depth.at[t] : t)) * D + 8 * j;
+        const float *w = is_q ? a.qn : a.kn, *turn = a.rope + (size_t)pos * D + 8 * j;
         float wf[2][4], cs[8];
 #pragma unroll
         for (int u = 0; u < 2; u++) *reinterpret_cast<float4 *>(wf[u]) = *reinterpret_cast<const float4 *>(w + 64 * u + 4 * j);
@@ -191,7 +199,7 @@ template <bool Q8, bool TREE> __global__ __launch_bounds__(256) void k_post_rows
         return;
     }
     const int head = is_v ? kvh - a.kv.n_kv : kvh;
-    const size_t row = (size_t)head * a.kv.n_ctx + a.row0 + t;
+    const size_t row = (size_t)head * a.kv.n_ctx + to;
     if constexpr (Q8) {
         uint32_t db[2];
 #pragma unroll
@@ -344,9 +352,7 @@ template <bool Q8> __global__ __launch_bounds__(256) void k_kv_keep(KeepArgs a) 
     if (Q8 && tid < a.n) scales[tid] = d;
 }
 
-bool overlap(const void *a, size_t na, const void *b, size_t nb) {
-    return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
-}
+constexpr auto overlap = htr_overlap;
 
 }  // namespace
 
@@ -429,14 +435,12 @@ extern "C" int htr_tree_masks(const int32_t *h_parent, int n, uint64_t *h_mask, 
     return 0;
 }
 
-extern "C" int htr_qkv_post_rows(htr_device *dev, const float *d_q, size_t q_stride, const float *d_k, const float *d_v,
-                                 size_t kv_stride, int n, const float *d_q_norm, const float *d_k_norm,
-                                 const float *d_rope, int n_pos, int pos0, const int32_t *h_depth, int n_head, float eps,
-                                 const htr_kv *kv, int row0, float *d_q_out) {
-    const char *me = "htr_qkv_post_rows";
-    PostRowsArgs a{};
-    HTR_TRY(htr_kv_check(me, kv, &a.kv));
-    HTR_TRY(check_apart(me, a.kv));
+namespace {
+// the arguments that the two row writers share, checked; `rows` of the cache or of a table are theirs to check
+int post_args(const char *me, const float *d_q, size_t q_stride, const float *d_k, const float *d_v, size_t kv_stride, int n,
+              const float *d_q_norm, const float *d_k_norm, const float *d_rope, int n_pos, int n_head, float eps,
+              const htr_kv *kv, float *d_q_out, PostRowsArgs *out, size_t *groups) {
+    PostRowsArgs &a = *out;
     if (!d_q || !d_k || !d_v || !d_q_norm || !d_k_norm || !d_rope || !d_q_out) return htr_fail("%s: null argument", me);
     if (n_head < 1 || n_head % kv->n_kv) return htr_fail("%s: %d q heads on %d KV heads", me, n_head, kv->n_kv);
     const size_t qd = (size_t)n_head * D, kvd = (size_t)kv->n_kv * D;
@@ -446,6 +450,47 @@ extern "C" int htr_qkv_post_rows(htr_device *dev, const float *d_q, size_t q_str
     if (((uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_q_norm | (uintptr_t)d_k_norm | (uintptr_t)d_rope |
          (uintptr_t)d_q_out) & 15)
         return htr_fail("%s: pointers must be 16-byte aligned", me);
+    a.q = d_q, a.k = d_k, a.v = d_v, a.q_stride = q_stride, a.kv_stride = kv_stride;
+    a.qn = d_q_norm, a.kn = d_k_norm, a.rope = d_rope, a.q_out = d_q_out;
+    a.eps = (double)eps, a.n = n, a.n_head = n_head, a.n_pos = n_pos;
+    *groups = ((size_t)n * ((size_t)n_head + 2 * kv->n_kv) + 15) / 16;
+    return 0;
+}
+int post_apart(const char *me, const PostRowsArgs &a, size_t groups) {
+    // in place (q_out on q's own rows) is the only overlap that the kernel allows
+    const size_t n = (size_t)a.n, qd = (size_t)a.n_head * D, kvd = (size_t)a.kv.n_kv * D;
+    const size_t q_bytes = 4 * (a.q_stride * (n - 1) + qd), out_bytes = 4 * qd * n;
+    const size_t kv_bytes = 4 * (a.kv_stride * (n - 1) + kvd);
+    if ((overlap(a.q, q_bytes, a.q_out, out_bytes) && !(a.q == a.q_out && (n == 1 || a.q_stride == qd))) ||
+        overlap(a.k, kv_bytes, a.q_out, out_bytes) || overlap(a.v, kv_bytes, a.q_out, out_bytes))
+        return htr_fail("%s: the q output overlaps the input rows", me);
+    if (htr_kv_overlaps(a.kv, a.q, q_bytes) || htr_kv_overlaps(a.kv, a.k, kv_bytes) || htr_kv_overlaps(a.kv, a.v, kv_bytes) ||
+        htr_kv_overlaps(a.kv, a.q_out, out_bytes))
+        return htr_fail("%s: the rows or the q output overlap the cache", me);
+    const Plane read[5] = {{a.qn, 4 * D}, {a.kn, 4 * D}, {a.rope, (size_t)a.n_pos * D * 4}, {a.pos, a.pos ? 4 * n : 0},
+                           {a.slot, a.slot ? 4 * n : 0}};
+    for (const auto &w : read)
+        if (w.n && (overlap(w.p, w.n, a.q_out, out_bytes) || htr_kv_overlaps(a.kv, w.p, w.n)))
+            return htr_fail("%s: the q output or the cache overlaps the norms' weights or the rope table%s", me,
+                            a.pos ? ", or the rows' places" : "");
+    if (groups > HTR_MAX_GROUPS)
+        return htr_fail("%s: %d rows of %d + %d heads in one call (at most %zu heads' rows)", me, a.n, a.n_head, 2 * a.kv.n_kv,
+                        16 * HTR_MAX_GROUPS);
+    return 0;
+}
+}  // namespace
+
+extern "C" int htr_qkv_post_rows(htr_device *dev, const float *d_q, size_t q_stride, const float *d_k, const float *d_v,
+                                 size_t kv_stride, int n, const float *d_q_norm, const float *d_k_norm,
+                                 const float *d_rope, int n_pos, int pos0, const int32_t *h_depth, int n_head, float eps,
+                                 const htr_kv *kv, int row0, float *d_q_out) {
+    const char *me = "htr_qkv_post_rows";
+    PostRowsArgs a{};
+    size_t groups;
+    HTR_TRY(htr_kv_check(me, kv, &a.kv));
+    HTR_TRY(check_apart(me, a.kv));
+    HTR_TRY(post_args(me, d_q, q_stride, d_k, d_v, kv_stride, n, d_q_norm, d_k_norm, d_rope, n_pos, n_head, eps, kv, d_q_out, &a,
+                      &groups));
     if (n < 1 || row0 < 0 || row0 > kv->n_ctx - n)
         return htr_fail("%s: %d rows from row %d of a %d-row cache", me, n, row0, kv->n_ctx);
     if (h_depth && n > HTR_TREE_MAX) return htr_fail("%s: %d drafted rows (at most %d)", me, n, HTR_TREE_MAX);
@@ -462,36 +507,42 @@ extern "C" int htr_qkv_post_rows(htr_device *dev, const float *d_q, size_t q_str
     }
     if (pos0 < 0 || n_pos < 1 || deepest >= n_pos || pos0 > n_pos - 1 - deepest)
         return htr_fail("%s: positions %d … %lld of a %d-position rope table", me, pos0, (long long)pos0 + deepest, n_pos);
-    // in place (q_out on q's own rows) is the only overlap that the kernel allows
-    const size_t q_bytes = 4 * (q_stride * (n - 1) + qd), out_bytes = 4 * qd * n;
-    const size_t kv_bytes = 4 * (kv_stride * (n - 1) + kvd);
-    if ((overlap(d_q, q_bytes, d_q_out, out_bytes) && !(d_q == d_q_out && (n == 1 || q_stride == qd))) ||
-        overlap(d_k, kv_bytes, d_q_out, out_bytes) || overlap(d_v, kv_bytes, d_q_out, out_bytes))
-        return htr_fail("%s: the q output overlaps the input rows", me);
-    if (htr_kv_overlaps(a.kv, d_q, q_bytes) || htr_kv_overlaps(a.kv, d_k, kv_bytes) || htr_kv_overlaps(a.kv, d_v, kv_bytes) ||
-        htr_kv_overlaps(a.kv, d_q_out, out_bytes))
-        return htr_fail("%s: the rows or the q output overlap the cache", me);
-    const Plane read[3] = {{d_q_norm, 4 * D}, {d_k_norm, 4 * D}, {d_rope, (size_t)n_pos * D * 4}};
-    for (const auto &w : read)
-        if (overlap(w.p, w.n, d_q_out, out_bytes) || htr_kv_overlaps(a.kv, w.p, w.n))
-            return htr_fail("%s: the q output or the cache overlaps the norms' weights or the rope table", me);
-    const size_t count = (size_t)n * ((size_t)n_head + 2 * kv->n_kv), grid = (count + 15) / 16;
-    if (grid > HTR_MAX_GROUPS)
-        return htr_fail("%s: %d rows of %d + %d heads in one call (at most %zu heads' rows)", me, n, n_head, 2 * kv->n_kv,
-                        16 * HTR_MAX_GROUPS);
+    HTR_TRY(post_apart(me, a, groups));
     HTR_TRY(htr_check_alive(dev));
     const HtrOnDevice on(dev);
-    a.q = d_q, a.k = d_k, a.v = d_v, a.q_stride = q_stride, a.kv_stride = kv_stride;
-    a.qn = d_q_norm, a.kn = d_k_norm, a.rope = d_rope, a.q_out = d_q_out;
-    a.eps = (double)eps, a.n = n, a.n_head = n_head, a.pos0 = pos0, a.row0 = row0;
-    const dim3 g((unsigned)grid), b(256);
-#define HTR_POST(Q8, TREE) hipLaunchKernelGGL((k_post_rows<Q8, TREE>), g, b, 0, dev->stream, a, depth)
-    if (a.kv.q8 && h_depth) HTR_POST(true, true);
-    else if (a.kv.q8) HTR_POST(true, false);
-    else if (h_depth) HTR_POST(false, true);
-    else HTR_POST(false, false);
-#undef HTR_POST
+    a.pos0 = pos0, a.row0 = row0;
+    const dim3 g((unsigned)groups), b(256);
+#define HTR_POST(Q8, PLACE) hipLaunchKernelGGL((k_post_rows<Q8, PLACE>), g, b, 0, dev->stream, a, depth)
+    if (a.kv.q8 && h_depth) HTR_POST(true, DRAFT);
+    else if (a.kv.q8) HTR_POST(true, IN_ORDER);
+    else if (h_depth) HTR_POST(false, DRAFT);
+    else HTR_POST(false, IN_ORDER);
     return htr_launched(dev, a.kv.q8 ? "k_post_rows<q8_0>" : "k_post_rows<f16>");
+}
+
+extern "C" int htr_qkv_post_pages(htr_device *dev, const float *d_q, size_t q_stride, const float *d_k, const float *d_v,
+                                  size_t kv_stride, const htr_pages *pages, const float *d_q_norm, const float *d_k_norm,
+                                  const float *d_rope, int n_pos, int n_head, float eps, const htr_kv *kv, float *d_q_out) {
+    const char *me = "htr_qkv_post_pages";
+    PostRowsArgs a{};
+    HtrPages p;
+    size_t groups;
+    HTR_TRY(htr_kv_check(me, kv, &a.kv));
+    HTR_TRY(check_apart(me, a.kv));
+    HTR_TRY(htr_pages_check(me, pages, HTR_PAGES_ROWS, &p));
+    HTR_TRY(post_args(me, d_q, q_stride, d_k, d_v, kv_stride, p.n_row, d_q_norm, d_k_norm, d_rope, n_pos, n_head, eps, kv,
+                      d_q_out, &a, &groups));
+    if (n_pos < 1) return htr_fail("%s: a rope table of %d positions", me, n_pos);
+    a.pos = p.pos, a.slot = p.slot;
+    HTR_TRY(post_apart(me, a, groups));
+    HTR_TRY(htr_check_alive(dev));
+    const HtrOnDevice on(dev);
+    const TreeDepth depth{};
+    const dim3 g((unsigned)groups), b(256);
+    if (a.kv.q8) HTR_POST(true, PAGES);
+    else HTR_POST(false, PAGES);
+#undef HTR_POST
+    return htr_launched(dev, a.kv.q8 ? "k_post_rows<q8_0, pages>" : "k_post_rows<f16, pages>");
 }
 
 extern "C" int htr_kv_copy(htr_device *dev, const htr_kv *src, int src_row, const htr_kv *dst, int dst_row, int n) {

@@ -51,6 +51,19 @@ bool htr_kv_overlaps(const HtrKvPlanes &kv, const void *p, size_t n);
 // rows of a q8_0 cache as f16 into another's (n ≥ 1, in range: not checked)
 int htr_kv_read_back(htr_device *dev, const HtrKvPlanes &src, int src_row, const HtrKvPlanes &dst, int dst_row, int n);
 
+// a checked batch of reads over a cache in pages, as the kernels take it
+struct HtrPages {
+    int n_seq, n_row, shift, max_pages;  // shift: log2 of a page's rows
+    int32_t *start, *past, *table, *pos, *slot;
+};
+constexpr int HTR_MAX_SEQ = 1024, HTR_MAX_ROW = 1 << 21;  // reads and rows of a step: their sums fit 32 bits
+// 0 with *out filled, or -1 with the message of what is wrong with the sizes, or with the arrays that the call uses
+enum { HTR_PAGES_TABLE = 1, HTR_PAGES_ROWS = 2 };  // start, past and table; pos and slot
+int htr_pages_check(const char *what, const htr_pages *p, int uses, HtrPages *out);
+inline bool htr_overlap(const void *a, size_t na, const void *b, size_t nb) {
+    return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
 // the device made current for a call's launches, and the caller's own again afterwards
 struct HtrOnDevice {
     explicit HtrOnDevice(htr_device *dev);

@@ -1,0 +1,197 @@
+// The tables and row maps of a step of several reads over a cache in pages, made on the device from the reads' lengths.
+//
+// A cache's rows (htr_kv's n_ctx of them, the same for each KV head) are cut into pages of 2^shift; a read's row i is row
+// i % page of page table[read][i / page]. A step takes new rows of many reads, packed in their order. For it
+//
+//   held = ⌈len / page⌉, need = ⌈(len + new) / page⌉ − held        the pages a read has, and those its new rows ask for
+//   upto = Σ need, end = Σ new, both up to and with the read        (a read that ends here, new = −1, asks for none)
+//   served: the read's rows fit the table's width and, with end, the step's buffers, and upto ≤ the free pages, or need = 0
+//
+// Free pages are a ring: page i of those given out in this step is ring[head + i], so where a page goes follows from the sums
+// alone, and pages of ended reads go behind the last free one, which no read of this step looks at. So a call writes nothing
+// that it reads but the lengths and the pool, each of which its thread has read before the sums: both may be written in place.
+#include <algorithm>
+
+#include "kv_ops.h"
+
+namespace {
+
+constexpr int THREADS = HTR_MAX_SEQ;  // a thread a read
+constexpr int ROWS_ONE = 4096;        // rows that the one workgroup of the sums maps itself; more: a second launch
+
+struct MapArgs {
+    HtrPages p;
+    const int32_t *len, *add, *pool;
+    int32_t *ring, *len_out, *pool_out;
+    int n_page;
+};
+
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+// Σ of v over the threads up to and with this one
+__device__ uint32_t block_scan(uint32_t v, uint32_t *s_wave) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    v = wave_scan(v);
+    __syncthreads();  // (the waves' sums of the scan before are read)
+    if (lane == 63) s_wave[wave] = v;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) v += s_wave[w];
+    return v;
+}
+// the first of n ascending sums that is past i, n where none is
+__device__ __forceinline__ int first_past(const uint32_t *sums, int n, uint32_t i) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sums[mid] > i) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+// a row's place in the cache: −1 where the table has no page of the cache there
+__device__ __forceinline__ int slot_of(int page, int n_page, int pos, int shift) {
+    return (uint32_t)page < (uint32_t)n_page ? (page << shift) + (pos & ((1 << shift) - 1)) : -1;
+}
+
+__global__ __launch_bounds__(THREADS) void k_page_map(MapArgs a, int map_rows) {
+    __shared__ uint32_t s_end[THREADS], s_upto[THREADS], s_back[THREADS], s_wave[THREADS / 64], s_taken;
+    __shared__ int s_past[THREADS], s_held[THREADS], s_need[THREADS];
+    const int b = threadIdx.x, shift = a.p.shift;
+    const bool there = b < a.p.n_seq;
+    const int len = there ? a.len[b] : 0, add = there ? a.add[b] : 0;
+    // (a ring's state that is none: as near to it as one is)
+    const uint32_t n_page = (uint32_t)a.n_page, head = (uint32_t)a.pool[0] % n_page;
+    const uint32_t count = (uint32_t)min(max(a.pool[1], 0), a.n_page);
+    const bool ends = add < 0;
+    const uint32_t mask = (1u << shift) - 1, held = len <= 0 ? 0 : ((uint32_t)len + mask) >> shift;
+    if (b == 0) s_taken = 0;
+    const uint32_t end = block_scan(ends ? 0u : (uint32_t)min(add, a.p.n_row + 1), s_wave);
+    const bool fits = there && !ends && len >= 0 && (int64_t)len + add <= (int64_t)a.p.max_pages << shift && end <= (uint32_t)a.p.n_row;
+    const uint32_t need = fits ? (((uint32_t)len + (uint32_t)add + mask) >> shift) - held : 0u;
+    const uint32_t upto = block_scan(need, s_wave);
+    const bool served = fits && (need == 0 || upto <= count);
+    const uint32_t back = block_scan(ends ? min(held, (uint32_t)a.p.max_pages) : 0u, s_wave);
+    s_end[b] = min(end, (uint32_t)a.p.n_row), s_upto[b] = upto, s_back[b] = back;
+    s_past[b] = served ? len : -1, s_held[b] = (int)held, s_need[b] = (int)need;
+    if (served && need) atomicMax(&s_taken, upto);
+    __syncthreads();
+    const uint32_t taken = s_taken, returned = min(s_back[THREADS - 1], n_page - count);
+    if (there) {
+        a.p.start[b + 1] = (int)s_end[b];
+        a.p.past[b] = s_past[b];
+        a.len_out[b] = ends ? 0 : served ? len + add : len;
+    }
+    if (b == 0) {
+        a.p.start[0] = 0;
+        a.pool_out[0] = (int)(head + taken >= n_page ? head + taken - n_page : head + taken);
+        a.pool_out[1] = (int)(count - taken + returned);
+    }
+    auto ring_at = [&](uint32_t i) {  // (i < n_page)
+        const uint32_t at = head + i;
+        return a.ring + (at >= n_page ? at - n_page : at);
+    };
+    for (uint32_t i = b; i < taken; i += THREADS) {
+        const int s = first_past(s_upto, a.p.n_seq, i);
+        a.p.table[(size_t)s * a.p.max_pages + s_held[s] + (i - (s_upto[s] - s_need[s]))] = *ring_at(i);
+    }
+    for (uint32_t i = b; i < returned; i += THREADS) {
+        const int s = first_past(s_back, a.p.n_seq, i);
+        *ring_at(count + i) = a.p.table[(size_t)s * a.p.max_pages + (i - (s ? s_back[s - 1] : 0u))];
+    }
+    if (!map_rows) return;
+    for (int r = b; r < a.p.n_row; r += THREADS) {
+        const int s = first_past(s_end, a.p.n_seq, (uint32_t)r);
+        int pos = -1, slot = -1;
+        if (s < a.p.n_seq && s_past[s] >= 0) {
+            pos = s_past[s] + r - (s ? (int)s_end[s - 1] : 0);
+            const int k = pos >> shift;
+            // a page that this step gives out is in the ring yet
+            const int page = k < s_held[s] ? a.p.table[(size_t)s * a.p.max_pages + k]
+                                           : *ring_at(s_upto[s] - s_need[s] + (k - s_held[s]));
+            slot = slot_of(page, a.n_page, pos, shift);
+        }
+        a.p.pos[r] = pos;
+        a.p.slot[r] = slot;
+    }
+}
+
+// the rows' places of many rows, from the tables
+__global__ __launch_bounds__(256) void k_page_rows(MapArgs a) {
+    __shared__ uint32_t s_end[HTR_MAX_SEQ];
+    for (int b = threadIdx.x; b < a.p.n_seq; b += 256) s_end[b] = (uint32_t)a.p.start[b + 1];
+    __syncthreads();
+    for (int r = blockIdx.x * 256 + threadIdx.x; r < a.p.n_row; r += gridDim.x * 256) {
+        const int s = first_past(s_end, a.p.n_seq, (uint32_t)r);
+        int pos = -1, slot = -1;
+        if (s < a.p.n_seq && a.p.past[s] >= 0) {
+            pos = a.p.past[s] + r - (s ? (int)s_end[s - 1] : 0);
+            slot = slot_of(a.p.table[(size_t)s * a.p.max_pages + (pos >> a.p.shift)], a.n_page, pos, a.p.shift);
+        }
+        a.p.pos[r] = pos;
+        a.p.slot[r] = slot;
+    }
+}
+
+}  // namespace
+
+int htr_pages_check(const char *what, const htr_pages *p, int uses, HtrPages *out) {
+    if (!p) return htr_fail("%s: null pages", what);
+    if (p->n_seq < 1 || p->n_seq > HTR_MAX_SEQ || p->n_row < 1 || p->n_row > HTR_MAX_ROW)
+        return htr_fail("%s: %d reads of %d rows (1 … %d reads, 1 … %d rows)", what, p->n_seq, p->n_row, HTR_MAX_SEQ, HTR_MAX_ROW);
+    if (p->page < 16 || p->page > 1024 || (p->page & (p->page - 1)))
+        return htr_fail("%s: pages of %d rows (a power of two, 16 … 1024)", what, p->page);
+    if (p->max_pages < 1 || (int64_t)p->max_pages * p->page > INT32_MAX || (int64_t)p->max_pages * p->n_seq > INT32_MAX)
+        return htr_fail("%s: a table of %d pages of %d rows for each of %d reads", what, p->max_pages, p->page, p->n_seq);
+    if ((uses & HTR_PAGES_TABLE) && (!p->d_start || !p->d_past || !p->d_table)) return htr_fail("%s: null start, past or table", what);
+    if ((uses & HTR_PAGES_ROWS) && (!p->d_pos || !p->d_slot)) return htr_fail("%s: null positions or slots", what);
+    const uintptr_t t = uses & HTR_PAGES_TABLE ? (uintptr_t)p->d_start | (uintptr_t)p->d_past | (uintptr_t)p->d_table : 0;
+    const uintptr_t r = uses & HTR_PAGES_ROWS ? (uintptr_t)p->d_pos | (uintptr_t)p->d_slot : 0;
+    if ((t | r) & 3) return htr_fail("%s: the pages' arrays must be 4-byte aligned", what);
+    *out = HtrPages{p->n_seq, p->n_row, __builtin_ctz((unsigned)p->page), p->max_pages, p->d_start, p->d_past, p->d_table, p->d_pos,
+                    p->d_slot};
+    return 0;
+}
+
+// ---- ABI -----------------------------------------------------------------------------------------------------------------
+
+extern "C" int htr_page_map(htr_device *dev, const htr_pages *pages, int n_page, const int32_t *d_len, const int32_t *d_new,
+                            int32_t *d_ring, const int32_t *d_pool, int32_t *d_len_out, int32_t *d_pool_out) {
+    const char *me = "htr_page_map";
+    MapArgs a{};
+    HTR_TRY(htr_pages_check(me, pages, HTR_PAGES_TABLE | HTR_PAGES_ROWS, &a.p));
+    if (!d_len || !d_new || !d_ring || !d_pool || !d_len_out || !d_pool_out) return htr_fail("%s: null argument", me);
+    if (n_page < 1 || (int64_t)n_page * pages->page > INT32_MAX)
+        return htr_fail("%s: %d pages of %d rows (at most 2^31 - 1 rows)", me, n_page, pages->page);
+    if (((uintptr_t)d_len | (uintptr_t)d_new | (uintptr_t)d_ring | (uintptr_t)d_pool | (uintptr_t)d_len_out | (uintptr_t)d_pool_out) & 3)
+        return htr_fail("%s: arrays must be 4-byte aligned", me);
+    const size_t n = (size_t)a.p.n_seq, rows = (size_t)a.p.n_row;
+    const struct {
+        const void *p;
+        size_t n;
+        bool written;
+    } of[11] = {{a.p.start, 4 * (n + 1), true}, {a.p.past, 4 * n, true}, {a.p.table, 4 * n * a.p.max_pages, true},
+                {a.p.pos, 4 * rows, true}, {a.p.slot, 4 * rows, true}, {d_ring, 4 * (size_t)n_page, true},
+                {d_len_out, 4 * n, true}, {d_pool_out, 8, true}, {d_len, 4 * n, false}, {d_new, 4 * n, false}, {d_pool, 8, false}};
+    for (int i = 0; i < 8; i++)
+        for (int j = i + 1; j < 11; j++) {
+            if (!htr_overlap(of[i].p, of[i].n, of[j].p, of[j].n)) continue;
+            if (of[i].p == of[j].p && ((i == 6 && j == 8) || (i == 7 && j == 10))) continue;  // in place
+            return htr_fail("%s: arrays overlap (the new lengths and the new pool may be the old ones')", me);
+        }
+    HTR_TRY(htr_check_alive(dev));
+    const HtrOnDevice on(dev);
+    a.len = d_len, a.add = d_new, a.pool = d_pool, a.ring = d_ring, a.len_out = d_len_out, a.pool_out = d_pool_out, a.n_page = n_page;
+    const bool one = a.p.n_row <= ROWS_ONE;
+    hipLaunchKernelGGL(k_page_map, dim3(1), dim3(THREADS), 0, dev->stream, a, one ? 1 : 0);
+    HTR_TRY(htr_launched(dev, "k_page_map"));
+    if (one) return 0;
+    hipLaunchKernelGGL(k_page_rows, dim3((unsigned)std::min((a.p.n_row + 255) / 256, 2048)), dim3(256), 0, dev->stream, a);
+    return htr_launched(dev, "k_page_rows");
+}

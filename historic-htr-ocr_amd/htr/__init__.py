@@ -41,6 +41,7 @@ SYMBOLS = [
     "htr_graph_free", "htr_decode_attention_static", "htr_session_profile_step", "htr_session_set_fused_step",
     "htr_session_fused_step", "htr_session_profile_fused_step", "htr_debug_handover", "htr_session_set_wait_limit",
     "htr_tree_masks", "htr_qkv_post_rows", "htr_kv_copy", "htr_kv_keep", "htr_tree_attention", "htr_window_attention",
+    "htr_page_map", "htr_qkv_post_pages", "htr_page_attention", "htr_token_logprobs",
 ]
 STEP_EMBED, STEP_QKV, STEP_ATTENTION, STEP_O, STEP_FFN, STEP_DOWN, STEP_HEAD, STEP_ALL = 1, 2, 4, 8, 16, 32, 64, 127
 
@@ -81,6 +82,11 @@ class KvViewC(C.Structure):
 class KvC(C.Structure):
     _fields_ = [("type", C.c_int), ("n_kv", C.c_int), ("n_ctx", C.c_int), ("d_k", C.c_void_p), ("d_v", C.c_void_p),
                 ("d_kd", C.c_void_p), ("d_vd", C.c_void_p)]
+
+
+class PagesC(C.Structure):
+    _fields_ = [("n_seq", C.c_int), ("n_row", C.c_int), ("page", C.c_int), ("max_pages", C.c_int), ("d_start", C.c_void_p),
+                ("d_past", C.c_void_p), ("d_table", C.c_void_p), ("d_pos", C.c_void_p), ("d_slot", C.c_void_p)]
 
 
 class PresetC(C.Structure):
@@ -204,6 +210,10 @@ def lib() -> C.CDLL:
             "htr_kv_keep": (i32, [vp, vp, i32, vp, i32]),
             "htr_tree_attention": (i32, [vp, vp, sz, i32, vp, i32, vp, i32, f32, vp]),
             "htr_window_attention": (i32, [vp, vp, sz, i32, i32, i32, i32, vp, i32, f32, vp]),
+            "htr_page_map": (i32, [vp, vp, i32, vp, vp, vp, vp, vp, vp]),
+            "htr_qkv_post_pages": (i32, [vp, vp, sz, vp, vp, sz, vp, vp, vp, vp, i32, i32, f32, vp, vp]),
+            "htr_page_attention": (i32, [vp, vp, sz, vp, vp, i32, f32, vp]),
+            "htr_token_logprobs": (i32, [vp, vp, sz, i32, i32, vp, vp, vp, i32, vp, vp]),
             "htr_synth_q8_0": (i32, [C.c_uint64, sz, sz, vp]),
             "htr_synth_normal": (i32, [C.c_uint64, sz, f32, f32, vp]),
             "htr_choose_host": (i32, [vp, sz, C.POINTER(PresetC), vp, sz, vp, vp, sz, C.POINTER(C.c_uint64),
@@ -577,6 +587,79 @@ def window_attention(dev: Device, q, n_q: int, pos0: int, window: int, n_sink: i
     """attention of the queries at pos0 … over the last `window` rows up to each one's own and the first n_sink"""
     _check(lib().htr_window_attention(dev.h, q.ptr, n_head * 128 if q_stride is None else q_stride, n_q, pos0, window,
                                       n_sink, kv.ref, n_head, scale, out.ptr))
+
+
+class Pages:
+    """The arrays of a step of several reads over a cache in pages (htr_pages): at most n_row new rows of n_seq reads, whose
+    rows lie in up to max_pages pages each. ``Pages(dev, …)`` allocates them (freed by ``free``, and refused by every call from
+    then on; the table starts with no pages); ``Pages.of`` takes buffers that the caller holds for as long as they are used."""
+
+    def __init__(self, dev: Device, n_seq: int, n_row: int, page: int, max_pages: int):
+        self._check(n_seq, n_row, page, max_pages)
+        self.held, self.c = [], PagesC()
+        try:
+            for n in (n_seq + 1, n_seq, n_seq * max_pages, n_row, n_row):
+                self.held.append(Buffer(dev, 4 * n))
+            self.held[2].upload(np.full(n_seq * max_pages, -1, np.int32))
+        except HtrError:
+            self.free()
+            raise
+        self._set(n_seq, n_row, page, max_pages, *self.held)
+
+    @classmethod
+    def of(cls, n_seq: int, n_row: int, page: int, max_pages: int, start, past, table, pos=None, slot=None) -> "Pages":
+        """on buffers (anything with ``ptr``) of int32: start [n_seq + 1], past [n_seq], table [n_seq][max_pages], and the
+        rows' pos and slot [n_row] where they are used"""
+        cls._check(n_seq, n_row, page, max_pages)
+        self = cls.__new__(cls)
+        self.held = []
+        self._set(n_seq, n_row, page, max_pages, start, past, table, pos, slot)
+        return self
+
+    @staticmethod
+    def _check(*sizes: int) -> None:
+        if not all(1 <= s < 2 ** 31 for s in sizes):
+            raise ValueError(f"pages of sizes {sizes} (each 1 … 2^31 - 1)")
+
+    def _set(self, n_seq: int, n_row: int, page: int, max_pages: int, start, past, table, pos, slot) -> None:
+        self.n_seq, self.n_row, self.page, self.max_pages = n_seq, n_row, page, max_pages
+        self.start, self.past, self.table, self.pos, self.slot = start, past, table, pos, slot
+        self.c = PagesC(n_seq, n_row, page, max_pages, start.ptr, past.ptr, table.ptr, _p(pos), _p(slot))
+        self.ref = C.addressof(self.c)
+
+    def free(self) -> None:
+        if self.held:
+            self.c.d_start = self.c.d_past = self.c.d_table = self.c.d_pos = self.c.d_slot = None
+        for b in self.held:
+            b.free()
+        self.held = []
+
+
+def page_map(dev: Device, pages: Pages, n_page: int, length, new, ring, pool, length_out, pool_out) -> None:
+    """the step's arrays from the reads' lengths and new rows (-1: the read ends), pages taken from and given back to the ring
+    [n_page] of free ones, whose first and number are pool [2]; length_out and pool_out may be length and pool"""
+    _check(lib().htr_page_map(dev.h, pages.ref, n_page, length.ptr, new.ptr, ring.ptr, pool.ptr, length_out.ptr, pool_out.ptr))
+
+
+def qkv_post_pages(dev: Device, q, k, v, pages: Pages, q_norm, k_norm, rope, n_pos: int, n_head: int, eps: float, kv: KvCache,
+                   q_out, q_stride: int | None = None, kv_stride: int | None = None) -> None:
+    """qkv_post_rows of a step's rows: row t at position pages.pos[t], k and v to the cache's row pages.slot[t]"""
+    _check(lib().htr_qkv_post_pages(dev.h, q.ptr, n_head * 128 if q_stride is None else q_stride, k.ptr, v.ptr,
+                                    kv.n_kv * 128 if kv_stride is None else kv_stride, pages.ref, q_norm.ptr, k_norm.ptr,
+                                    rope.ptr, n_pos, n_head, eps, kv.ref, q_out.ptr))
+
+
+def page_attention(dev: Device, q, pages: Pages, kv: KvCache, n_head: int, scale: float, out, q_stride: int | None = None) -> None:
+    """attention of a step's rows, each read's over its own rows of the cache up to each one's position"""
+    _check(lib().htr_page_attention(dev.h, q.ptr, n_head * 128 if q_stride is None else q_stride, pages.ref, kv.ref, n_head,
+                                    scale, out.ptr))
+
+
+def token_logprobs(dev: Device, logits, n: int, n_vocab: int, ids, logprob, entropy, top: int = 0, top_ids=None,
+                   top_logprob=None, stride: int | None = None) -> None:
+    """of n rows of logits (stride floats apart; None: without a gap) each one's log p(ids), entropy, and `top` alternatives"""
+    _check(lib().htr_token_logprobs(dev.h, logits.ptr, n_vocab if stride is None else stride, n, n_vocab, ids.ptr, logprob.ptr,
+                                    entropy.ptr, top, _p(top_ids), _p(top_logprob)))
 
 
 def choose(dev: Device, logits: Buffer, n_vocab: int, hist: Buffer, length: int, window: int, rp: float, tok: Buffer,

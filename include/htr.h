@@ -236,6 +236,43 @@ int htr_tree_attention(htr_device *dev, const float *d_q, size_t q_stride, int n
  * read (read back first: also a gap of up to a quarter of the rows). */
 int htr_window_attention(htr_device *dev, const float *d_q, size_t q_stride, int n_q, int pos0, int window, int n_sink,
                          const htr_kv *kv, int n_head, float scale, float *d_out);
+/* ---- a step of several reads over one cache in pages (no reference counterpart: the reference reads one page at a time) ---- */
+/* One layer's htr_kv whose rows are cut into pages of `page` rows, shared by n_seq reads: a read's row i is row i % page of
+ * page d_table[read][i / page] (an entry outside the cache's pages 0 … n_ctx / page − 1 stands for no rows: nothing is stored
+ * there, nobody sees them). A step's rows are packed: read b's new ones are the rows d_start[b] … d_start[b + 1] − 1 of its
+ * buffers of n_row rows, at positions d_past[b] … (d_past[b] < 0: the read is not served, its rows have no place); what lies
+ * behind d_start[n_seq] belongs to no read. The arrays are device memory, written by htr_page_map or by the caller, ascending
+ * starts within 0 … n_row; all layers share them, and no call waits for what they hold, so that a step is recorded into a graph
+ * once and replayed over reads of any length. 1 … 1024 reads, n_row ≤ 2^21, page a power of two 16 … 1024. */
+typedef struct {
+    int n_seq, n_row, page, max_pages;   /* max_pages: the table's width */
+    int32_t *d_start;                    /* [n_seq + 1] */
+    int32_t *d_past;                     /* [n_seq] */
+    int32_t *d_table;                    /* [n_seq][max_pages] */
+    int32_t *d_pos, *d_slot;             /* [n_row]: each row's position and its row of the cache; −1: none */
+} htr_pages;
+/* the step's arrays from the reads' lengths: d_len[b] rows that read b has in the cache, d_new[b] ≥ 0 new ones, or −1: the
+ * read ends. Free pages wait in the ring d_ring [n_page]: those at d_pool[0], d_pool[0] + 1, … (mod n_page), d_pool[1] of them.
+ * Reads are served in their order: read b takes the pages that its new rows need from the ring's front, into its row of the
+ * table behind those it has (its other entries stay), if its rows fit the table's width and the step's n_row, and if the free
+ * pages are enough for it and all before it that fit (or it needs none). One that is not served has d_past −1, keeps its length
+ * and takes no page; d_start counts its rows all the same (up to n_row). A read that ends gives its pages back, behind the
+ * ring's last (not for this step's reads), and has length 0. d_len_out and d_pool_out get the lengths and the pool after the
+ * step, and may be d_len and d_pool; the arrays overlap in no other way. The maps of more than 4096 rows take a second launch. */
+int htr_page_map(htr_device *dev, const htr_pages *pages, int n_page, const int32_t *d_len, const int32_t *d_new,
+                 int32_t *d_ring, const int32_t *d_pool, int32_t *d_len_out, int32_t *d_pool_out);
+/* htr_qkv_post_rows' work for the n_row rows of a step: row t at position d_pos[t], its k and v to the cache's row d_slot[t].
+ * Of a row whose position lies outside the rope table nothing is stored and its q output stays as it was; one whose slot lies
+ * outside the cache has its q stored alone. No slot stands for two rows. Reads pages->d_pos and d_slot. */
+int htr_qkv_post_pages(htr_device *dev, const float *d_q, size_t q_stride, const float *d_k, const float *d_v, size_t kv_stride,
+                       const htr_pages *pages, const float *d_q_norm, const float *d_k_norm, const float *d_rope, int n_pos,
+                       int n_head, float eps, const htr_kv *kv, float *d_q_out);
+/* attention of a step's rows: read b's i-th new row over the read's rows 0 … d_past[b] + i → d_out [n_row][n_head·128], zeros
+ * for the rows of a read that is not served, the rows behind the last read left as they were. Rows past the table's width are
+ * not there. Otherwise as htr_tree_attention (what a row does not see, what it holds its numbers to). Reads pages->d_start,
+ * d_past and d_table. */
+int htr_page_attention(htr_device *dev, const float *d_q, size_t q_stride, const htr_pages *pages, const htr_kv *kv, int n_head,
+                       float scale, float *d_out);
 /* the GPU token choice of a greedy preset on n_vocab logits (choose_pen → choose_max → choose_pick,
  * text.rs:222-231; semantics of ocr-decode sampling.rs:38-62, bit-exact): the repetition penalty rp over the distinct
  * ids of d_hist[len − window … len) applied in place (< 0: × rp, else ÷ rp, IEEE round-to-nearest), the frequency
@@ -247,6 +284,17 @@ int htr_choose(htr_device *dev, float *d_logits, int n_vocab, uint32_t *d_hist, 
  * the 10k-step measurement of the choice kernel (no reference counterpart) */
 int htr_choose_many(htr_device *dev, float *d_logits, int n_vocab, int n, uint32_t *d_hist, int hist_stride, int len,
                     int window, float rp, uint32_t *d_tok);
+
+/* how sure a choice was: of n rows of logits, `stride` floats apart, the log probability of each row's token d_ids[n] (an id
+ * outside the vocabulary: NaN), the entropy of the row's distribution in nats, and its n_top likeliest tokens (≤ 32, ≤ n_vocab;
+ * 0: none) in falling order, of equal ones the lower id first, with their log probabilities [n][n_top]. Natural logarithms of
+ * softmax(logits) as they are: of htr_choose's penalised ones those after the penalty. A logit of −∞ has no weight; a row of
+ * nothing else has log probabilities of −∞ and entropy 0; a NaN or +∞ makes a row's log probabilities and entropy NaN, and its
+ * alternatives keep their order, a NaN behind −∞. f32 throughout; pointers 4-byte aligned, the outputs apart from each other
+ * and the inputs. */
+enum { HTR_TOP_MAX = 32 };
+int htr_token_logprobs(htr_device *dev, const float *d_logits, size_t stride, int n, int n_vocab, const int32_t *d_ids,
+                       float *d_logprob, float *d_entropy, int n_top, int32_t *d_top_ids, float *d_top_logprob);
 
 /* Y[m][N] (+= with acc) X·Wᵀ, X f32 [m][K], W q8_0 [N][K] (gpu.rs:1963-2014 Batch::matmul with a q8_0 weight, the
  * prefill's GEMMs): on the device's compute path — F32: exact dequant, f32 sums over all of f32's range

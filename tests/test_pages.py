@@ -1,0 +1,147 @@
+"""The operators of a step over a cache in pages and the log probabilities without a GPU: the refusals, which the entry points
+give before they look at the device (a null one here, so that nothing can be launched)."""
+import ctypes as C
+import re
+
+import pytest
+
+import htr
+
+M = 16 << 20  # addresses that no call follows, far apart
+Q8 = dict(type=8, kd=3 << 20, vd=4 << 20)
+
+
+def kv(type=1, n_kv=2, n_ctx=640, k=1 << 20, v=2 << 20, kd=0, vd=0):
+    return htr.KvC(type, n_kv, n_ctx, k, v, kd, vd)
+
+
+def pages(n_seq=3, n_row=10, page=16, max_pages=5, start=20 * M, past=21 * M, table=22 * M, pos=23 * M, slot=24 * M):
+    return htr.PagesC(n_seq, n_row, page, max_pages, start, past, table, pos, slot)
+
+
+BAD_PAGES = [(dict(n_seq=0), "0 reads"), (dict(n_seq=1025), "1025 reads"), (dict(n_row=0), "of 0 rows"),
+             (dict(n_row=2 ** 21 + 1), "2097153 rows"), (dict(page=8), "pages of 8 rows"), (dict(page=48), "pages of 48 rows"),
+             (dict(page=2048), "pages of 2048"), (dict(page=0), "pages of 0"), (dict(max_pages=0), "table of 0 pages"),
+             (dict(max_pages=2 ** 27), "table of 134217728 pages"), (dict(n_seq=1000, max_pages=2 ** 22), "table of 4194304 pages")]
+TABLES = [(dict(start=0), "null start"), (dict(past=0), "null start"), (dict(table=0), "null start"),
+          (dict(start=20 * M + 2), "4-byte aligned"), (dict(table=22 * M + 1), "4-byte aligned")]
+ROWS = [(dict(pos=0), "null positions"), (dict(slot=0), "null positions"), (dict(slot=24 * M + 3), "4-byte aligned")]
+
+
+def page_map(p=None, n_page=40, length=M, new=2 * M, ring=3 * M, pool=4 * M, length_out=5 * M, pool_out=6 * M):
+    p = pages() if p is None else p
+    return htr.lib().htr_page_map(None, C.addressof(p) if p else None, n_page, length, new, ring, pool, length_out, pool_out)
+
+
+def post(p=None, c=None, q=M, qs=512, k=2 * M, v=3 * M, ks=256, qn=4 * M, kn=5 * M, rope=6 * M, n_pos=200, n_head=4, out=7 * M):
+    p, c = pages() if p is None else p, kv() if c is None else c
+    return htr.lib().htr_qkv_post_pages(None, q, qs, k, v, ks, C.addressof(p) if p else None, qn, kn, rope, n_pos, n_head, 1e-6,
+                                        C.addressof(c), out)
+
+
+def attend(p=None, c=None, q=M, qs=512, n_head=4, out=2 * M):
+    p, c = pages() if p is None else p, kv() if c is None else c
+    return htr.lib().htr_page_attention(None, q, qs, C.addressof(p) if p else None, C.addressof(c), n_head, 0.1, out)
+
+
+def score(x=M, stride=1000, n=3, vocab=1000, ids=2 * M, lp=3 * M, h=4 * M, top=5, top_ids=5 * M, top_lp=6 * M):
+    return htr.lib().htr_token_logprobs(None, x, stride, n, vocab, ids, lp, h, top, top_ids, top_lp)
+
+
+def refused(rc, match):
+    assert rc < 0 and re.search(match, htr.last_error()), htr.last_error()
+
+
+def test_good_arguments_reach_the_device():
+    for call in (page_map, post, attend, score):
+        refused(call(), "null device")
+    for c in (kv(), kv(**Q8)):
+        refused(attend(c=c), "null device")
+        refused(post(c=c), "null device")
+    refused(page_map(length_out=M, pool_out=4 * M), "null device")  # in place
+    refused(post(q=M, out=M), "null device")
+    refused(attend(p=pages(pos=0, slot=0)), "null device")  # each call wants the arrays that it uses
+    refused(post(p=pages(start=0, past=0, table=0)), "null device")
+    refused(score(top=0, top_ids=0, top_lp=0), "null device")
+    refused(score(x=M + 4, lp=3 * M + 4), "null device")
+    for page in (16, 32, 1024):
+        refused(attend(p=pages(page=page), c=kv(n_ctx=1024)), "null device")
+
+
+@pytest.mark.parametrize("change,match", BAD_PAGES)
+def test_sizes_of_pages(change, match):
+    for call in (page_map, post, attend):
+        refused(call(pages(**change)), match)
+
+
+def test_null_pages():
+    for call in (page_map, post, attend):
+        refused(call(p=False), "null pages")
+
+
+@pytest.mark.parametrize("change,match", TABLES)
+def test_tables(change, match):
+    refused(page_map(pages(**change)), match)
+    refused(attend(pages(**change)), match)
+
+
+@pytest.mark.parametrize("change,match", ROWS)
+def test_rows(change, match):
+    refused(page_map(pages(**change)), match)
+    refused(post(pages(**change)), match)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(length=0), "null argument"), (dict(pool_out=0), "null argument"), (dict(ring=0), "null argument"),
+    (dict(n_page=0), "0 pages"), (dict(n_page=2 ** 27), "at most 2"), (dict(new=2 * M + 2), "4-byte aligned"),
+    (dict(length_out=M + 4), "overlap"), (dict(length_out=2 * M), "overlap"), (dict(ring=22 * M), "overlap"),
+    (dict(pool_out=4 * M + 4), "overlap"), (dict(pool=M, pool_out=M), "overlap"), (dict(length=21 * M), "overlap"),
+    (dict(new=23 * M + 36), "overlap"), (dict(ring=24 * M - 156), "overlap"), (dict(pool=20 * M + 12), "overlap")])
+def test_map(change, match):
+    refused(page_map(**change), match)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(q=0), "null argument"), (dict(rope=0), "null argument"), (dict(n_head=3), "3 q heads on 2"), (dict(n_head=0), "0 q heads"),
+    (dict(qs=511), "511 and 256 floats"), (dict(ks=252), "512 and 252"), (dict(v=3 * M + 4), "16-byte"), (dict(n_pos=0), "0 positions"),
+    (dict(out=M + 16), "overlaps the input rows"), (dict(q=M, qs=516, out=M), "overlaps the input rows"),
+    (dict(out=2 * M), "overlaps the input rows"), (dict(out=1 << 20), "overlap the cache"), (dict(k=2 << 20), "overlap the cache"),
+    (dict(rope=7 * M), "rows' places"), (dict(out=23 * M), "rows' places"), (dict(c=kv(type=0)), "type 0"),
+    (dict(c=kv(v=(1 << 20) + 4096)), "planes overlap"), (dict(p=pages(slot=1 << 20)), "rows' places")])
+def test_post(change, match):
+    refused(post(**change), match)
+
+
+def test_post_of_more_rows_than_a_launch_takes():
+    refused(post(p=pages(n_row=2 ** 21), c=kv(n_kv=64, n_ctx=1, k=1 << 44, v=1 << 45), n_head=64, qs=64 * 128, ks=64 * 128,
+                 q=1 << 46, k=1 << 47, v=1 << 48, out=1 << 49), "heads' rows")
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(q=0), "null argument"), (dict(out=0), "null argument"), (dict(n_head=5), "5 q heads on 2"), (dict(qs=508), "508 floats"),
+    (dict(qs=514), "514 floats"), (dict(out=2 * M + 8), "16-byte"), (dict(out=M + 1024), "overlaps the queries"),
+    (dict(out=2 << 20), "overlaps the cache"), (dict(out=22 * M), "overlaps the pages"), (dict(c=kv(n_ctx=15)), "15 rows in pages of 16"),
+    (dict(c=kv(n_kv=0)), "0 KV heads"), (dict(c=kv(type=8)), "without scales")])
+def test_attention(change, match):
+    refused(attend(**change), match)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(x=0), "null argument"), (dict(ids=0), "null argument"), (dict(lp=0), "null argument"), (dict(h=0), "null argument"),
+    (dict(n=0), "0 rows"), (dict(n=2 ** 21 + 1), "2097153 rows"), (dict(vocab=0), "of 0 logits"), (dict(stride=999), "999 apart"),
+    (dict(vocab=2 ** 28 + 1, stride=2 ** 28 + 1), "268435457 logits"), (dict(top=-1), "-1 alternatives"), (dict(top=33), "33 alternatives"),
+    (dict(top=4, vocab=3), "4 alternatives of 3"), (dict(top_ids=0), "null alternatives"), (dict(top_lp=0), "null alternatives"),
+    (dict(lp=3 * M + 2), "4-byte"), (dict(x=M + 1), "4-byte"), (dict(lp=4 * M + 8), "overlaps another"), (dict(top_lp=5 * M + 56), "overlaps another"),
+    (dict(h=M + 4 * 2999), "overlaps another"), (dict(top_ids=2 * M + 8), "overlaps another")])
+def test_logprobs(change, match):
+    refused(score(**change), match)
+
+
+def test_python_sizes():
+    class Ref:
+        ptr = M
+
+    with pytest.raises(ValueError, match="pages of sizes"):
+        htr.Pages.of(1, 0, 16, 1, Ref, Ref, Ref)
+    with pytest.raises(ValueError, match="pages of sizes"):
+        htr.Pages.of(2 ** 31, 1, 16, 1, Ref, Ref, Ref)
