@@ -18,6 +18,21 @@
 // sets the calling thread's message; returns -1 (the ABI's error code)
 int htr_fail(const char *fmt, ...) __attribute__((format(printf, 1, 2)));
 
+enum {
+    SCR_CHOOSE_PART = 0,
+    SCR_CHOOSE_CNT = 1,
+    SCR_ATTN_PART = 2,
+    SCR_ATTN_CNT = 3,
+    SCR_CAUSAL_KV = 4,  // aligned copies of caches that are not
+    SCR_GEMM_PART = 5,  // split-K products [split][M][N]
+    SCR_HANDOVER = 6,   // htr_debug_handover's words
+    SCR_KV_ATTN = 7,    // the tree and window attention's partial sums (one size)
+    SCR_KV_TICKET = 8,  // their tickets (one size; zero, self-resetting)
+    SCR_KV_ROWS = 9,    // q8_0 rows read back for the window attention (htr_scratch_kept)
+    SCR_PAGE_ATTN = 10, // the parts of the page attention's cut tiles (one size)
+    SCR_SLOTS
+};
+
 struct htr_device {
     int ordinal = 0;
     hipStream_t stream = nullptr;
@@ -33,8 +48,8 @@ struct htr_device {
     void *pinned = nullptr;
     size_t pinned_bytes = 0;
     // scratch of the standalone kernel entry points, grown on demand (zero-filled when (re)allocated)
-    void *scratch[10] = {nullptr};
-    size_t scratch_bytes[10] = {0};
+    void *scratch[SCR_SLOTS] = {nullptr};
+    size_t scratch_bytes[SCR_SLOTS] = {0};
     // the measurement timer's events
     hipEvent_t t0 = nullptr, t1 = nullptr;
     // decode steps replayed as captured HIP graphs (HTR_GRAPHS=0 at open: launched one by one)
@@ -64,18 +79,6 @@ int attn_static_scratch_init(htr_device *dev);
 // part of a graph), else 0
 int htr_check_not_capturing(htr_device *dev, const char *what);
 
-enum {
-    SCR_CHOOSE_PART = 0,
-    SCR_CHOOSE_CNT = 1,
-    SCR_ATTN_PART = 2,
-    SCR_ATTN_CNT = 3,
-    SCR_CAUSAL_KV = 4,  // aligned copies of caches that are not
-    SCR_GEMM_PART = 5,  // split-K products [split][M][N]
-    SCR_HANDOVER = 6,   // htr_debug_handover's words
-    SCR_KV_ATTN = 7,    // the tree and window attention's partial sums (one size)
-    SCR_KV_TICKET = 8,  // their tickets (one size; zero, self-resetting)
-    SCR_KV_ROWS = 9,    // q8_0 rows read back for the window attention (htr_scratch_kept)
-};
 // the device's scratch buffer `slot` with at least `bytes` bytes (a larger one replaces it: the tickets' and best
 // keys' slots zero-filled, the others as htr_dev_alloc fills)
 int htr_scratch(htr_device *dev, int slot, size_t bytes, void **out);
