@@ -3,15 +3,19 @@
 //
 //   out[t][h] = Σ_j p_j·v_j / Σ_j p_j,  p_j = e^(scale·q·k_j − m)  over the rows j ≤ past + i of the read whose i-th row t is
 //
-// The q heads of a KV head share its keys: a read's rows for a KV head are (i, head of the group), packed, in tiles of 32. The
+// The q heads of a KV head share its keys: a read's rows for a KV head are (i, head of the group), packed, in tiles. The
 // operands, the softmax and what is held to how many bits are kv_attention.hip's.
 //
 // The reads' lengths are on the device, and the launch knows their bounds alone: it is as many workgroups as the card holds at
-// once, whatever the reads. Each KV head's tiles in order are a line of work, a tile's length on it its keys and COST more for
-// its start and end, and the head's workgroups take equal pieces of the line, wherever that cuts a tile: one read of many keys
-// goes to all of them, of many short ones each takes a few, and no list of work is made first. Where a piece begins follows
-// from sums over the reads, a lane a read, and within a read from a quadratic equation (a tile's keys grow with its rows'
-// positions). The parts of cut tiles go to memory and are joined by a second launch.
+// once, whatever the reads (twice: once for each height of tile). Each KV head's tiles in order are a line of work, a tile's
+// length on it its keys and COST more for its start and end, and the head's workgroups take equal pieces of the line, wherever
+// that cuts a tile: one read of many keys goes to all of them, of many short ones each takes a few, and no list of work is made
+// first. Where a piece begins follows from sums over the reads, a lane a read. The parts of a cut tile are joined by
+// a second launch.
+//
+// Tiles come in two heights, each with a line of its own. Of up to 32 rows (a step's token, or what is left of a prompt) the waves
+// share out the keys, every fourth block of 32 to each, loaded into LDS of its own, so that nobody waits for anybody until the
+// four sums are merged. More are tiles of 128, 32 to a wave, all of which use each block, staged for them together.
 #include <algorithm>
 #include <type_traits>
 
@@ -19,11 +23,25 @@
 
 namespace {
 
-constexpr int PW = 4;            // waves of a workgroup, two of which a CU holds
-constexpr int COST = 64;         // keys that take as long as a tile's start and end
-constexpr int LEAST = 128;       // keys of a piece of work, at least: a block for each wave
-constexpr int QT = 256 + 256 + 16 + 16;  // 16-byte chunks of a q8_0 buffer: K, V, K scales, V scales
+constexpr int PW = 4;                       // waves of a workgroup, two of which a CU holds
+constexpr int NARROW = KB, WIDE = KB * PW;  // rows of a tile
+constexpr int COST = 128;                    // keys that take as long as a tile's start and end
+constexpr int LEAST = 192;                  // a piece's length, at least: a block for each wave, and a tile's start
+constexpr int SLIVER = 4;                   // blocks of a tile's beginning or end that are not cut off for themselves
+constexpr int SHARES = 4;                   // workgroups of the join to a wide piece
+constexpr int QT = 256 + 256 + 16 + 16;     // 16-byte chunks of a q8_0 buffer: K, V, K scales, V scales
 
+// where the parts of a height's cut tiles wait. A piece has two places: 1 for the tile that it begins and does not end, 0 for
+// the one that it goes on with
+struct Part {
+    int first, n;        // the pieces that have a part of the tile: first … first + n − 1; n = 0: the place is empty
+    int start, r0, rows; // its read's first row of the buffers; its first row of the read, its rows
+};
+struct Parts {
+    float *sums;  // [n_kv·pieces][2][rows of a tile][128]
+    float4 *ml;   // [n_kv·pieces][2][rows of a tile]: a row's (m, l, c)
+    Part *of;     // [n_kv·pieces][2]
+};
 struct Args {
     const float *q;
     size_t q_stride;
@@ -34,102 +52,141 @@ struct Args {
     uint32_t per_group;  // ⌈2^32 / group⌉ (group > 1): the quotient of a row below 2^32 / group by one product
     int n_page, cap;     // the cache's pages; the rows that the table has room for
     float scale;
-    int parts;           // workgroups of a KV head
-    float *part;         // [n_kv·parts][2][32] sums o[128], and each row's (m, l, c)
-    float4 *part_ml;
+    int pieces;          // workgroups of a KV head and height
+    int wide;            // those of the wide tiles: pieces, or none where no read has so many rows
+    double per_piece;    // 1 / pieces
+    Parts part[2];
 };
 
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
     const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
     return (int64_t)((uint64_t)hi << 32 | lo);
 }
+// row r's query
+__device__ __forceinline__ int query_of(const Args &a, int r) { return a.group == 1 ? r : (int)__umulhi((uint32_t)r, a.per_group); }
 
-// the line of work: the reads' tiles in order. Uniform but for the 64 reads at hand, a lane each
-struct Line {
+// 64 reads of the line of work at hand, in LDS
+struct Reads {
+    int64_t end[64];                 // the line's length up to and with each
+    int start[64], n[64], past[64];  // its rows and keys; past −1: not served
+};
+// a height's line: the reads' tiles in order. A narrow read's length is its keys and COST. A wide tile's is group times that, up
+// to its last row (of a read's first k tiles k·step + 64·k·(k + 1) in all, step = group·(past + COST))
+template <bool W> struct Line {
     const Args &a;
-    int first = 0;                // the reads at hand: first …
-    int64_t base = 0;             // the line's length before them
-    int64_t end;                  // and up to and with each
-    int start, n, past;           // its rows and keys; past −1: not served
-    __device__ __forceinline__ explicit Line(const Args &args) : a(args) { load(); }
-
-    __device__ __forceinline__ int64_t tile(int held, int rows_to) const { return (int64_t)a.group * (max(held, 0) + COST) + rows_to; }
-    __device__ __forceinline__ void load() {
+    Reads &r;
+    int first = 0;     // the reads at hand: first …
+    int64_t base = 0;  // the line's length before them
+    int64_t total, piece;
+    __device__ __forceinline__ Line(const Args &args, Reads &reads) : a(args), r(reads) {
+        total = load();
+        if (a.p.n_seq > 64) {
+            for (; first + 64 < a.p.n_seq; total = load()) base = total, first += 64;
+            first = 0, base = 0;
+            load();
+        }
+        piece = max((int64_t)((double)total * a.per_piece) + 1, (int64_t)LEAST * (W ? a.group : 1));
+    }
+    // where piece i begins
+    __device__ __forceinline__ int64_t cut(int i) const { return i >= a.pieces ? total : min(i * piece, total); }
+    __device__ __forceinline__ int piece_of(int64_t x) const {
+        int i = min((int)((double)x / (double)piece), a.pieces - 1);
+        while (i > 0 && cut(i) > x) i--;
+        while (i + 1 < a.pieces && cut(i + 1) <= x) i++;
+        return uniform(i);
+    }
+    __device__ __forceinline__ int64_t step(int past) const { return (int64_t)(W ? a.group : 1) * (max(past, 0) + COST); }
+    // the reads from `first` on; their end on the line
+    __device__ __forceinline__ int64_t load() {
         const int lane = threadIdx.x & 63, b = first + lane;
         const bool there = b < a.p.n_seq;
         const int s0 = there ? a.p.start[b] : 0, s1 = there ? a.p.start[b + 1] : 0, held = there ? a.p.past[b] : -1;
-        start = min(max(s0, 0), a.p.n_row);
-        n = min(max(s1, start), a.p.n_row) - start;
-        past = min(max(held, -1), a.cap);
-        const int rows = n * a.group, full = rows / KB;
-        end = full * tile(past, 0) + (int64_t)(KB / 2) * full * (full + 1) + (rows % KB ? tile(past, rows) : 0);
+        const int start = min(max(s0, 0), a.p.n_row), past = min(max(held, -1), a.cap);
+        int n = min(max(s1, start), a.p.n_row) - start;
+        const int rows = n * a.group, full = rows / WIDE, rest = rows % WIDE;
+        int64_t end;
+        if constexpr (W) {
+            end = full * step(past) + (int64_t)(WIDE / 2) * full * (full + 1) + (rest > NARROW ? step(past) + rows : 0);
+        } else {
+            if (rest > NARROW || rest == 0) n = 0;
+            end = n ? step(past) + n : 0;
+        }
+        if (W && end == 0) n = 0;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const int64_t o = __shfl_up((long long)end, d);
             if (lane >= d) end += o;
         }
         end += base;
-    }
-    __device__ __forceinline__ bool next() {
-        if (first + 64 >= a.p.n_seq) return false;
-        base = lane_of(end, 63), first += 64;
-        load();
-        return true;
-    }
-    __device__ __forceinline__ int64_t total() {
-        while (next()) {}
-        const int64_t t = lane_of(end, 63);
-        if (first) {
-            first = 0, base = 0;
-            load();
-        }
-        return t;
+        r.end[lane] = end, r.start[lane] = start, r.n[lane] = n, r.past[lane] = past;
+        return lane_of(end, 63);
     }
 };
-// how many pieces the line is cut into, and where
-__device__ __forceinline__ int pieces(const Args &a, int64_t total) {
-    return (int)min((int64_t)a.parts, max((int64_t)1, total / ((int64_t)a.group * (LEAST + COST))));
-}
-__device__ __forceinline__ int64_t cut(int64_t total, int i, int n) { return i == n ? total : (int64_t)((double)total * i / n); }
 
 // a tile on the line
-struct Tile {
-    int at;                   // its read: lane `at` of those at hand
-    int start, n, past, rows; // the read's
-    int tau;                  // its place among the read's tiles
-    int64_t begin, len;       // and on the line
+template <bool W> struct Tile {
+    int at;                    // its read: of those at hand
+    int start, n, past;        // the read's
+    int r0, rows;              // narrow: its first row of the read, its rows; wide: the read's rows in wide tiles
+    int tau;                   // its place among the read's tiles
+    int last, nb;              // the last key that one of its rows sees; its blocks of keys
+    int64_t begin, len;        // and on the line
 
-    __device__ __forceinline__ void of_read(Line &w, int lane) {
-        at = lane;
-        start = __builtin_amdgcn_readlane(w.start, at), n = __builtin_amdgcn_readlane(w.n, at), past = __builtin_amdgcn_readlane(w.past, at);
-        rows = n * w.a.group;
+    // the last key that query i sees (past + i < 2^32)
+    __device__ __forceinline__ int last_key(const Args &a, int i) const {
+        return past < 0 ? -1 : (int)min((uint32_t)past + (uint32_t)i, (uint32_t)a.cap - 1u);
     }
-    __device__ __forceinline__ void measure(const Line &w) { len = w.tile(past, min(KB * (tau + 1), rows)); }
+    __device__ __forceinline__ int last_of(const Args &a, int r) const { return last_key(a, query_of(a, min(r, rows - 1))); }
+    __device__ __forceinline__ void of_read(const Line<W> &w, int i) {
+        at = i, start = uniform(w.r.start[i]), n = uniform(w.r.n[i]), past = uniform(w.r.past[i]);
+        rows = n * w.a.group, r0 = rows / WIDE * WIDE;
+        if constexpr (!W) rows -= r0;
+        else if (rows - r0 <= NARROW) rows = r0;
+    }
+    __device__ __forceinline__ void measure(const Line<W> &w) {
+        len = w.step(past) + (W ? min(WIDE * (tau + 1), rows) : n);
+        last = W ? last_of(w.a, WIDE * (tau + 1) - 1) : last_key(w.a, n - 1);
+        nb = (last + KB) / KB;
+    }
+    // the block that place x of the line (begin < x < begin + len) cuts the tile in front of; 0 and nb: it does not
+    __device__ __forceinline__ int block_at(const Line<W> &w, int64_t x) const {
+        const int64_t u = x - begin;
+        const int b = W ? uniform((int)((double)u / (double)(KB * w.a.group))) : (int)(u / KB);
+        return b < SLIVER ? 0 : b > nb - SLIVER ? nb : b;
+    }
     // the one that holds place x of the line, x before its end
-    __device__ __forceinline__ Tile(Line &w, int64_t x) {
-        while (lane_of(w.end, 63) <= x && w.next()) {}
-        of_read(w, min((int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(w.end > x) | 1ull << 63), 63));
-        const int64_t from = at ? lane_of(w.end, at - 1) : w.base;
-        const int64_t y = x - from, step = w.tile(past, 0);
-        // tau tiles are tau·step + 16·tau·(tau + 1) long
-        const double h = 0.5 * ((double)step + KB / 2);
-        const int tiles = (rows + KB - 1) / KB;
-        tau = min((int)((sqrt(h * h + (double)(KB / 2) * (double)y) - h) / (KB / 2)), tiles - 1);
-        auto upto = [&](int t) { return t * step + (int64_t)(KB / 2) * t * (t + 1); };
-        while (tau > 0 && upto(tau) > y) tau--;
-        while (tau + 1 < tiles && upto(tau + 1) <= y) tau++;
-        begin = from + upto(tau);
+    __device__ __forceinline__ Tile(Line<W> &w, int64_t x) {
+        int64_t mine = w.r.end[threadIdx.x & 63];
+        for (int64_t t; (t = lane_of(mine, 63)) <= x && w.first + 64 < w.a.p.n_seq; mine = w.r.end[threadIdx.x & 63]) {
+            w.base = t, w.first += 64;
+            w.load();
+        }
+        of_read(w, (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(mine > x) | 1ull << 63));
+        begin = at ? lane_of(mine, at - 1) : w.base;
+        tau = 0;
+        if constexpr (W) {
+            const int64_t y = x - begin, step = w.step(past);
+            const double half = WIDE / 2, mid = 0.5 * ((double)step + half);
+            const int tiles = (rows + WIDE - 1) / WIDE;
+            tau = uniform(min((int)((sqrt(mid * mid + half * (double)y) - mid) / half), tiles - 1));
+            auto upto = [&](int t) { return t * step + (int64_t)(WIDE / 2) * t * (t + 1); };
+            while (tau > 0 && upto(tau) > y) tau--;
+            while (tau + 1 < tiles && upto(tau + 1) <= y) tau++;
+            begin += upto(tau);
+        }
         measure(w);
     }
     // the next one (there is one)
-    __device__ __forceinline__ void next(Line &w) {
+    __device__ __forceinline__ void next(Line<W> &w) {
         begin += len;
-        if (KB * ++tau >= rows) {
+        if (!W || WIDE * ++tau >= rows) {
             uint64_t more;
-            int from = at + 1;
-            while ((more = from < 64 ? __builtin_amdgcn_ballot_w64(w.n > 0) >> from << from : 0) == 0) {
-                if (!w.next()) break;
-                from = 0;
+            for (int from = at + 1;; from = 0) {
+                more = from < 64 ? __builtin_amdgcn_ballot_w64(w.r.n[threadIdx.x & 63] > 0) >> from << from : 0;
+                if (more || w.first + 64 >= w.a.p.n_seq) break;
+                w.base = begin, w.first += 64;
+                w.load();
             }
             of_read(w, more ? (int)__builtin_ctzll(more) : 63);
             tau = 0;
@@ -138,11 +195,72 @@ struct Tile {
     }
 };
 
-// row r's query
-__device__ __forceinline__ int query_of(const Args &a, int r) { return a.group == 1 ? r : (int)__umulhi((uint32_t)r, a.per_group); }
-__device__ __forceinline__ float *out_row(const Args &a, const Tile &t, int kvh, int r) {
+// the blocks i0 … i1 − 1 of a tile that are a piece's
+struct Share {
+    int i0, i1;
+    bool all;
+};
+template <bool W> __device__ __forceinline__ Share share_of(const Line<W> &w, const Tile<W> &t, int64_t x0, int64_t x1) {
+    Share s{0, t.nb, true};
+    if (x0 > t.begin) s.i0 = t.block_at(w, x0);
+    if (x1 < t.begin + t.len) s.i1 = t.block_at(w, x1);
+    s.all = s.i0 == 0 && s.i1 == t.nb;
+    return s;
+}
+// a piece's place for its part of a cut tile, and which pieces have the others
+template <bool W> __device__ __forceinline__ size_t part_of(const Line<W> &w, const Tile<W> &t, const Share &share, int kvh, int piece) {
+    int first = w.piece_of(t.begin), end = first + 1;
+    if (w.cut(end) < t.begin + t.len && t.block_at(w, w.cut(end)) == 0) first++, end++;  // (it leaves the beginning to the next one)
+    while (end < w.a.pieces && w.cut(end) < t.begin + t.len && t.block_at(w, w.cut(end)) < t.nb) end++;
+    const size_t place = ((size_t)kvh * w.a.pieces + piece) * 2 + (share.i0 == 0);
+    if (threadIdx.x == 0) w.a.part[W].of[place] = W ? Part{first, end - first, t.start, WIDE * t.tau, min(WIDE, t.rows - WIDE * t.tau)}
+                                                    : Part{first, end - first, t.start, t.r0, t.rows};
+    return place * (W ? WIDE : NARROW);
+}
+// the two places of a piece that has no cut tile are empty
+template <bool W> __device__ __forceinline__ void no_parts(const Args &a, int kvh, int piece) {
+    if (threadIdx.x < 2) a.part[W].of[((size_t)kvh * a.pieces + piece) * 2 + threadIdx.x].n = 0;
+}
+__device__ __forceinline__ float *out_row(const Args &a, int start, int kvh, int r) {
     const int i = query_of(a, r);
-    return a.out + ((size_t)(t.start + i) * a.n_head + (size_t)kvh * a.group + (r - i * a.group)) * D;
+    return a.out + ((size_t)(start + i) * a.n_head + (size_t)kvh * a.group + (r - i * a.group)) * D;
+}
+__device__ __forceinline__ const float *q_row(const Args &a, int start, int kvh, int r) {
+    const int i = query_of(a, r);
+    return a.q + (size_t)(start + i) * a.q_stride + ((size_t)kvh * a.group + (r - i * a.group)) * D;
+}
+
+// the first rows of the halves of a run of blocks b0, b0 + step, …: lane 2j + h has the j-th one's half h, of 32 at a time. Half a
+// block lies in one page
+struct Rows {
+    int at[2];
+    uint32_t bad;  // bit h: half h has no page
+};
+struct Run {
+    const int32_t *table;
+    int b0, step, last, shift, n_page;
+    int row;
+    uint64_t gone;  // the halves without a page
+    __device__ __forceinline__ void fetch(int j) {
+        const int lane = threadIdx.x & 63;
+        const uint32_t key = min(KB * (uint32_t)(b0 + step * (j + (lane >> 1))) + 16u * (lane & 1), (uint32_t)last & ~15u);
+        const int page = table[key >> shift];
+        const bool bad = (uint32_t)page >= (uint32_t)n_page;
+        row = bad ? 0 : (page << shift) + (int)(key & ((1u << shift) - 1));
+        gone = __builtin_amdgcn_ballot_w64(bad);
+    }
+    __device__ __forceinline__ Rows of(int j) {
+        if (j && (j & 31) == 0) fetch(j);
+        return Rows{{__builtin_amdgcn_readlane(row, 2 * (j & 31)), __builtin_amdgcn_readlane(row, 2 * (j & 31) + 1)},
+                    (uint32_t)(gone >> (2 * (j & 31))) & 3u};
+    }
+};
+template <bool W> __device__ __forceinline__ Run run_of(const Args &a, const Line<W> &w, const Tile<W> &t, int b0, int step) {
+    return Run{a.p.table + (size_t)(w.first + t.at) * a.p.max_pages, b0, step, t.last, a.p.shift, a.n_page, 0, 0};
+}
+// the keys of block i that a row of `keys` sees, of the lane's 16 (bits 0 … 3, 8 … 11, 16 …, 24 …)
+__device__ __forceinline__ uint32_t sees(int keys, int i, int hf, uint32_t bad) {
+    return low_bits(keys - (KB * i + here(4 * hf))) & (bad & 1 ? 0xFFFF0000u : ~0u) & (bad & 2 ? 0x0000FFFFu : ~0u);
 }
 
 // 4 bytes a lane from p to LDS bytes lds + 4·lane
@@ -150,25 +268,24 @@ __device__ __forceinline__ void lds_load4_at(const void *p, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(p) : "memory", "m0");
 }
 
-// A workgroup's waves take every fourth block of 32 keys of a tile each, into LDS of their own, as k_kv_attn_split's do (the
-// layouts there), and wait for nobody until their sums are merged.
-template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_attn(Args a) {
-    constexpr int WAVE = Q8 ? 2 * QT + 16 : TILE;  // chunks of a wave's LDS
+constexpr int WAVE_F16 = TILE, WAVE_Q8 = 2 * QT + 16;  // 16-byte chunks of a wave's LDS: K and V of a block; two raw ones
+struct Shared {
+    Reads reads[PW];  // (each wave its own: nobody waits)
+    float ml[PW][2][KB];
+};
+
+// ---- reads of few rows -------------------------------------------------------------------------------------------------------
+
+template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh, int piece, uint4_t *s_kv, Shared &sh) {
+    constexpr int WAVE = Q8 ? WAVE_Q8 : WAVE_F16;
     static_assert(WAVE >= 1024, "a wave's sums fit");
-    __shared__ __attribute__((aligned(16))) uint4_t s_kv[PW][WAVE];
-    __shared__ float s_ml[PW][2][KB];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hf = lane >> 5, c = lane & 31;
-    const int kvh = blockIdx.x % a.kv.n_kv, piece = blockIdx.x / a.kv.n_kv;
-    Line line(a);
-    const int64_t total = line.total();
-    const int n_piece = pieces(a, total);
-    if (piece >= n_piece) return;
-    const int64_t x0 = cut(total, piece, n_piece), x1 = cut(total, piece + 1, n_piece);
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), hf = lane >> 5, c = lane & 31;
+    if (a.pieces > 1) no_parts<false>(a, kvh, piece);
+    Line<false> line(a, sh.reads[wave]);
+    const int64_t x0 = line.cut(piece), x1 = line.cut(piece + 1);
     if (x0 >= x1) return;
     const size_t head0 = (size_t)kvh * a.kv.n_ctx;
-
-    uint4_t *tile = s_kv[wave];
+    uint4_t *tile = s_kv + WAVE * wave;
     const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint4_t *)tile;
     // a wave's instruction is 4 (8) whole rows; half a block lies in one page
     const uint32_t kx = 16 * ((lane & 15) ^ (lane >> 4)), vx = 16 * ((lane & 15) ^ (4 * (lane >> 4))), r4 = 2 * D * (lane >> 4);
@@ -202,293 +319,570 @@ template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_attn(Arg
     for (int u = 0; u < 4; u++)
         va[u] = Q8 ? 16 * (256 + 8 * vrow + ((2 * u + ((lane >> 4) & 1)) ^ (vrow & 2) ^ ((vrow & 8) >> 1))) + 8 * (lane & 1)
                    : 16 * (K_CHUNKS + 16 * vrow + ((4 * u + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (4 * (vrow & 3)))) + 8 * (lane & 1);
-
-    for (Tile t(line, x0);; t.next(line)) {
-        const int64_t u0 = max(x0 - t.begin, (int64_t)0), u1 = min(x1 - t.begin, t.len);
-        const int r0 = KB * t.tau, r_end = min(r0 + KB, t.rows);
-        // the last key that a query sees (past + cap < 2^32)
-        auto last_key = [&](int i) { return (int)min((uint32_t)t.past + (uint32_t)i, (uint32_t)a.cap - 1u); };
-        const int all_to = t.past < 0 ? 0 : (last_key(query_of(a, r0)) + 1) / KB, last = t.past < 0 ? -1 : last_key(query_of(a, r_end - 1));
-        const int nb = (last + KB) / KB;
-        const int i0 = u0 == 0 ? 0 : (int)((double)nb * (double)u0 / (double)t.len);
-        const int i1 = u1 == t.len ? nb : (int)((double)nb * (double)u1 / (double)t.len);
-
-        // the first rows of the halves of 32 of the wave's blocks: lane 2j + h has block j's half h
-        const int32_t *table = a.p.table + (size_t)(line.first + t.at) * a.p.max_pages;
-        int rowno = 0, j = 0;  // j: the wave's block
-        uint64_t gone = 0;     // of those the ones without a page
-        auto pages_from = [&](int jb) {
-            const uint32_t key = min(KB * (uint32_t)(i0 + wave + PW * (jb + (lane >> 1))) + 16u * (lane & 1), (uint32_t)last & ~15u);
-            const int page = table[key >> a.p.shift];
-            const bool bad = (uint32_t)page >= (uint32_t)a.n_page;
-            rowno = bad ? 0 : (page << a.p.shift) + (int)(key & ((1u << a.p.shift) - 1));
-            gone = __builtin_amdgcn_ballot_w64(bad);
-        };
-        int i = i0 + wave, b = 0, row0 = 0, row1 = 0;
-        uint32_t bad = 0, bad_next = 0;
-        auto rows_of = [&](int jn) {
-            if (jn && (jn & 31) == 0) pages_from(jn);
-            row0 = __builtin_amdgcn_readlane(rowno, 2 * (jn & 31)), row1 = __builtin_amdgcn_readlane(rowno, 2 * (jn & 31) + 1);
-            bad_next = (uint32_t)(gone >> (2 * (jn & 31))) & 3u;
-        };
-        if (i < i1) pages_from(0);
-        const int r = r0 + c, rc = min(r, t.rows - 1), qi = query_of(a, rc);
-        float qx[8][8];
-        q_load<8, Q8>(a.q + (size_t)(t.start + qi) * a.q_stride + ((size_t)kvh * a.group + (rc - qi * a.group)) * D + (Q8 ? 16 : 8) * hf, qx);
-        __syncthreads();  // (the sums of the tile before are read)
-        if (i < i1) {
-            rows_of(0);
-            bad = bad_next;
-            if constexpr (Q8) {
-                load_q8(row0, row1, 0);
-            } else {
-                load(row0, row1, false);
-                load(row0, row1, true);
-            }
-        }
-        half8 qh[8], ql[8];
-        const float sc = q_split<8, 2>(qx, a.scale, qh, ql);
-        const int keys = t.past < 0 ? 0 : last_key(qi) + 1;  // that the row sees
-        float m = M_NONE, l = 0.0f;
-        f32x16 o[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-#pragma unroll
-            for (int x = 0; x < 16; x++) o[u][x] = 0.0f;
-
-        // block i; MASK: not every row sees all of it, or half of it has no page
-        auto step = [&](auto is_masked) {
-            constexpr bool MASK = decltype(is_masked)::value;
-            const bool more = i + PW < i1;
-            uint4_t *buf = tile + (Q8 ? QT * b : 0);
-            if constexpr (Q8) {
-                if (more) {
-                    rows_of(j + 1);
-                    wait_reads();  // of the other buffer, a block ago
-                    load_q8(row0, row1, b ^ 1);
-                    wait_loads<10>();
+    for (Tile<false> t(line, x0);; t.next(line)) {
+        const Share sh_ = share_of(line, t, x0, x1);
+        if (sh_.i0 < sh_.i1 || sh_.all) {
+            const int i1 = sh_.i1, rc = t.r0 + min(c, t.rows - 1);
+            const int all_to = (t.last_key(a, query_of(a, t.r0)) + 1) / KB;  // blocks that all rows see the whole of
+            const int keys = t.last_key(a, query_of(a, rc)) + 1;             // keys that the lane's row sees
+            int i = sh_.i0 + wave, j = 0, b = 0;
+            Run run = run_of(a, line, t, i, PW);
+            if (i < i1) run.fetch(0);
+            float qx[8][8];
+            q_load<8, Q8>(q_row(a, t.start, kvh, rc) + (Q8 ? 16 : 8) * hf, qx);
+            __syncthreads();  // (the sums of the tile before are read)
+            Rows now{{0, 0}, 0}, then{{0, 0}, 0};
+            if (i < i1) {
+                now = run.of(0);
+                if constexpr (Q8) {
+                    load_q8(now.at[0], now.at[1], 0);
                 } else {
-                    wait_loads<0>();
+                    load(now.at[0], now.at[1], false);
+                    load(now.at[0], now.at[1], true);
                 }
-            } else {
-                wait_loads<8>();  // K; V is still on its way
             }
-            f32x16 s;
-            if constexpr (Q8) {
-                // V's scales into the order of the operands' slots
-                const uint32_t d2 = reinterpret_cast<const uint32_t *>(buf + 528)[lane];
-                uint16_t *vt = reinterpret_cast<uint16_t *>(tile + 2 * QT);
-                const int key = lane >> 1, at = 16 * (key >> 4) + 8 * ((key >> 2) & 1) + 4 * ((key >> 3) & 1) + (key & 3);
-                vt[32 * (2 * (lane & 1)) + at] = (uint16_t)d2;
-                vt[32 * (2 * (lane & 1) + 1) + at] = (uint16_t)(d2 >> 16);
-                const uint2_t dk = reinterpret_cast<const uint2_t *>(buf + 512)[c];
-                half2_t d4[2];
-                __builtin_memcpy(d4, &dk, 8);
-                uint4_t w;
+            const size_t part = sh_.all ? 0 : part_of(line, t, sh_, kvh, piece);
+            half8 qh[8], ql[8];
+            const float sc = q_split<8, 2>(qx, a.scale, qh, ql);
+            float m = M_NONE, l = 0.0f;
+            f32x16 o[4];
 #pragma unroll
-                for (int ks = 0; ks < 8; ks++) {
-                    if (ks % 2 == 0) w = buf[8 * c + ((ks + hf) ^ ((c >> 1) & 7))];
-                    const _Float16 d = d4[ks >> 2][(ks >> 1) & 1];
-                    const half8 f = dequant8(w[2 * (ks & 1)], w[2 * (ks & 1) + 1], half2_t{d, d});
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qh[ks], ks ? s : f32x16{}, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, ql[ks], s, 0, 0, 0);
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) o[u][x] = 0.0f;
+
+            // block i; MASK: not every row sees all of it, or half of it has no page
+            auto step = [&](auto is_masked) {
+                constexpr bool MASK = decltype(is_masked)::value;
+                const bool more = i + PW < i1;
+                uint4_t *buf = tile + (Q8 ? QT * b : 0);
+                if constexpr (Q8) {
+                    if (more) {
+                        then = run.of(j + 1);
+                        wait_reads();  // of the other buffer, a block ago
+                        load_q8(then.at[0], then.at[1], b ^ 1);
+                        wait_loads<10>();
+                    } else {
+                        wait_loads<0>();
+                    }
+                } else {
+                    wait_loads<8>();  // K; V is still on its way
                 }
-            } else {
-                half8 f[4];
+                f32x16 s;
+                if constexpr (Q8) {
+                    // V's scales into the order of the operands' slots
+                    const uint32_t d2 = reinterpret_cast<const uint32_t *>(buf + 528)[lane];
+                    uint16_t *vt = reinterpret_cast<uint16_t *>(tile + 2 * QT);
+                    const int key = lane >> 1, at = 16 * (key >> 4) + 8 * ((key >> 2) & 1) + 4 * ((key >> 3) & 1) + (key & 3);
+                    vt[32 * (2 * (lane & 1)) + at] = (uint16_t)d2;
+                    vt[32 * (2 * (lane & 1) + 1) + at] = (uint16_t)(d2 >> 16);
+                    const uint2_t dk = reinterpret_cast<const uint2_t *>(buf + 512)[c];
+                    half2_t d4[2];
+                    __builtin_memcpy(d4, &dk, 8);
+                    uint4_t w;
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                    for (int ks = 0; ks < 8; ks++) {
+                        if (ks % 2 == 0) w = buf[8 * c + ((ks + hf) ^ ((c >> 1) & 7))];
+                        const _Float16 d = d4[ks >> 2][(ks >> 1) & 1];
+                        const half8 f = dequant8(w[2 * (ks & 1)], w[2 * (ks & 1) + 1], half2_t{d, d});
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qh[ks], ks ? s : f32x16{}, 0, 0, 0);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, ql[ks], s, 0, 0, 0);
+                    }
+                } else {
+                    half8 f[4];
 #pragma unroll
-                    for (int ks = 0; ks < 4; ks++) f[ks] = *reinterpret_cast<const half8 *>(buf + 16 * c + (dims8(4 * h + ks) ^ (c & 15)));
-                    if (h == 1) {
-                        wait_reads();
-                        if (more) {
-                            rows_of(j + 1);
-                            load(row0, row1, false);
+                    for (int h = 0; h < 2; h++) {
+#pragma unroll
+                        for (int ks = 0; ks < 4; ks++) f[ks] = *reinterpret_cast<const half8 *>(buf + 16 * c + (dims8(4 * h + ks) ^ (c & 15)));
+                        if (h == 1) {
+                            wait_reads();
+                            if (more) {
+                                then = run.of(j + 1);
+                                load(then.at[0], then.at[1], false);
+                            }
+                        }
+#pragma unroll
+                        for (int ks = 0; ks < 4; ks++) {
+                            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[ks], qh[4 * h + ks], h || ks ? s : f32x16{}, 0, 0, 0);
+                            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[ks], ql[4 * h + ks], s, 0, 0, 0);
                         }
                     }
+                }
+                uint32_t seen = 0;
+                if constexpr (MASK) {
+                    seen = sees(keys, i, hf, now.bad);
 #pragma unroll
-                    for (int ks = 0; ks < 4; ks++) {
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[ks], qh[4 * h + ks], h || ks ? s : f32x16{}, 0, 0, 0);
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[ks], ql[4 * h + ks], s, 0, 0, 0);
+                    for (int x = 0; x < 16; x++) s[x] = seen >> (8 * (x >> 2) + (x & 3)) & 1 ? s[x] : -INFINITY;
+                }
+                float mx = s[0];
+#pragma unroll
+                for (int x = 1; x < 16; x++) mx = fmaxf(mx, s[x]);
+                mx = pair_max<32>(mx);
+                const bool up = (mx - m) * sc > P_ROOM;
+                if (__builtin_amdgcn_ballot_w64(up)) {
+                    const float to = up ? mx : m, corr = __builtin_amdgcn_exp2f((m - to) * sc);
+                    m = to;
+                    l *= corr;
+#pragma unroll
+                    for (int u = 0; u < 4; u++) o[u] *= corr;
+                }
+                float ls = 0.0f;
+                uint32_t ph[8], pl[8];
+#pragma unroll
+                for (int x = 0; x < 8; x++) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * x] - m, sc, P_SHIFT));  // not seen: 2^(−∞) = 0
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * x + 1] - m, sc, P_SHIFT));
+                    ls += p0;
+                    ls += p1;
+                    split2(p0, p1, ph[x], pl[x]);
+                }
+                l += ls;
+                if constexpr (!Q8) {  // V
+                    if (more) wait_loads<8>();
+                    else wait_loads<0>();
+                }
+                auto vread = [&](int u, int ss) {
+                    half8 v;
+                    if constexpr (Q8) {
+                        const auto *p = (const __attribute__((address_space(3))) char *)buf + va[u] + 16 * 128 * ss;
+                        const int2_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2_t *)p);
+                        const half8 d = *reinterpret_cast<const half8 *>(tile + 2 * QT + 4 * u + 2 * ss + hf);
+                        v = dequant8((uint32_t)w[0], (uint32_t)w[1], d);
+                    } else {
+                        const auto *p = (const __attribute__((address_space(3))) char *)buf + va[u] + 256 * 16 * ss;
+                        const fp16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)p);
+                        const fp16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)(p + 256 * 8));
+                        __builtin_memcpy(&v, &lo, 8);
+                        __builtin_memcpy((char *)&v + 8, &hi, 8);
+                    }
+                    return v;
+                };
+                bool odd = false;
+                if constexpr (MASK && Q8) {
+                    odd = __builtin_amdgcn_ballot_w64(scale_past(reinterpret_cast<const uint32_t *>(buf + 528)[here(lane)])) != 0;
+                } else if constexpr (MASK) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int u = 0; u < 4; u++) largest(vread(u, 0), top), largest(vread(u, 1), top);
+                    odd = any_not_finite(top);
+                }
+#pragma unroll
+                for (int ss = 0; ss < 2; ss++) {
+                    half8 h8, l8;
+                    __builtin_memcpy(&h8, &ph[4 * ss], 16);
+                    __builtin_memcpy(&l8, &pl[4 * ss], 16);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        half8 v = vread(u, ss);
+                        if (odd) v = finite(v);
+                        o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, h8, o[u], 0, 0, 0);
+                        o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, l8, o[u], 0, 0, 0);
+                        if constexpr (MASK) __builtin_amdgcn_sched_barrier(0);  // (few operands in registers at once)
                     }
                 }
-            }
-            uint32_t seen = 0;
-            if constexpr (MASK) {
-                seen = low_bits(keys - (KB * i + here(4 * hf))) & (bad & 1 ? 0xFFFF0000u : ~0u) & (bad & 2 ? 0x0000FFFFu : ~0u);
-#pragma unroll
-                for (int x = 0; x < 16; x++) s[x] = seen >> (8 * (x >> 2) + (x & 3)) & 1 ? s[x] : -INFINITY;
-            }
-            float mx = s[0];
-#pragma unroll
-            for (int x = 1; x < 16; x++) mx = fmaxf(mx, s[x]);
-            mx = pair_max<32>(mx);
-            const bool up = (mx - m) * sc > P_ROOM;
-            if (__builtin_amdgcn_ballot_w64(up)) {
-                const float to = up ? mx : m, corr = __builtin_amdgcn_exp2f((m - to) * sc);
-                m = to;
-                l *= corr;
-#pragma unroll
-                for (int u = 0; u < 4; u++) o[u] *= corr;
-            }
-            float ls = 0.0f;
-            uint32_t ph[8], pl[8];
-#pragma unroll
-            for (int x = 0; x < 8; x++) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * x] - m, sc, P_SHIFT));  // not seen: 2^(−∞) = 0
-                const float p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * x + 1] - m, sc, P_SHIFT));
-                ls += p0;
-                ls += p1;
-                split2(p0, p1, ph[x], pl[x]);
-            }
-            l += ls;
-            if constexpr (!Q8) {  // V
-                if (more) wait_loads<8>();
-                else wait_loads<0>();
-            }
-            auto vread = [&](int u, int ss) {
-                half8 v;
-                if constexpr (Q8) {
-                    const auto *p = (const __attribute__((address_space(3))) char *)buf + va[u] + 16 * 128 * ss;
-                    const int2_t w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2_t *)p);
-                    const half8 d = *reinterpret_cast<const half8 *>(tile + 2 * QT + 4 * u + 2 * ss + hf);
-                    v = dequant8((uint32_t)w[0], (uint32_t)w[1], d);
-                } else {
-                    const auto *p = (const __attribute__((address_space(3))) char *)buf + va[u] + 256 * 16 * ss;
-                    const fp16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)p);
-                    const fp16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)(p + 256 * 8));
-                    __builtin_memcpy(&v, &lo, 8);
-                    __builtin_memcpy((char *)&v + 8, &hi, 8);
+                if constexpr (MASK)
+                    if (odd) put_nan(o, seen, vread);
+                if constexpr (!Q8) {
+                    wait_reads();
+                    if (more) load(then.at[0], then.at[1], true);
                 }
-                return v;
+                i += PW, j++;
+                b ^= Q8;
+                now = then;
             };
-            bool odd = false;
-            if constexpr (MASK && Q8) {
-                odd = __builtin_amdgcn_ballot_w64(scale_past(reinterpret_cast<const uint32_t *>(buf + 528)[here(lane)])) != 0;
-            } else if constexpr (MASK) {
-                uint32_t top = 0;
-#pragma unroll
-                for (int u = 0; u < 4; u++) largest(vread(u, 0), top), largest(vread(u, 1), top);
-                odd = any_not_finite(top);
+            auto whole = [&] { return i < all_to && now.bad == 0; };
+            while (i < i1) {
+                for (bool all = whole(); all; all = i < i1 && whole()) step(std::false_type{});
+                for (bool some = i < i1; some; some = i < i1 && !whole()) step(std::true_type{});
             }
+            l = pair_sum<32>(l);
+
+            // the waves' sums through LDS (each its own tile's place): wave w finishes dims 32w … of every row
+            wait_reads();
+            float4 *so = reinterpret_cast<float4 *>(tile);
 #pragma unroll
-            for (int ss = 0; ss < 2; ss++) {
-                half8 h8, l8;
-                __builtin_memcpy(&h8, &ph[4 * ss], 16);
-                __builtin_memcpy(&l8, &pl[4 * ss], 16);
+            for (int u = 0; u < 4; u++)
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    half8 v = vread(u, ss);
-                    if (odd) v = finite(v);
-                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, h8, o[u], 0, 0, 0);
-                    o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, l8, o[u], 0, 0, 0);
-                    if constexpr (MASK) __builtin_amdgcn_sched_barrier(0);  // (few operands in registers at once)
+                for (int x = 0; x < 4; x++)
+                    so[(4 * u + x) * 64 + lane] = make_float4(o[u][4 * x], o[u][4 * x + 1], o[u][4 * x + 2], o[u][4 * x + 3]);
+            if (hf == 0) sh.ml[wave][0][c] = m, sh.ml[wave][1][c] = l;
+            __syncthreads();
+            m = M_NONE, l = 0.0f;
+#pragma unroll
+            for (int w = 0; w < PW; w++) m = fmaxf(m, sh.ml[w][0][c]);
+            float4 y[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) y[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < PW; w++) {
+                const float f = __builtin_amdgcn_exp2f((sh.ml[w][0][c] - m) * sc);
+                l = fmaf(sh.ml[w][1][c], f, l);
+                const float4 *from = reinterpret_cast<const float4 *>(s_kv + WAVE * w) + 4 * 64 * wave + lane;
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const float4 z = from[64 * x];
+                    y[x].x = fmaf(z.x, f, y[x].x), y[x].y = fmaf(z.y, f, y[x].y), y[x].z = fmaf(z.z, f, y[x].z), y[x].w = fmaf(z.w, f, y[x].w);
                 }
             }
-            if constexpr (MASK)
-                if (odd) put_nan(o, seen, vread);
-            if constexpr (!Q8) {
-                wait_reads();
-                if (more) load(row0, row1, true);
-            }
-            i += PW, j++;
-            b ^= Q8;
-            bad = bad_next;
-        };
-        auto whole = [&] { return i < all_to && bad == 0; };
-        while (i < i1) {
-            for (bool all = whole(); all; all = i < i1 && whole()) step(std::false_type{});
-            for (bool some = i < i1; some; some = i < i1 && !whole()) step(std::true_type{});
-        }
-        l = pair_sum<32>(l);
-
-        // the waves' sums through LDS (each its own tile's place): wave w finishes dims 32w … of every row
-        wait_reads();
-        float4 *so = reinterpret_cast<float4 *>(tile);
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-#pragma unroll
-            for (int x = 0; x < 4; x++)
-                so[(4 * u + x) * 64 + lane] = make_float4(o[u][4 * x], o[u][4 * x + 1], o[u][4 * x + 2], o[u][4 * x + 3]);
-        if (hf == 0) s_ml[wave][0][c] = m, s_ml[wave][1][c] = l;
-        __syncthreads();
-        m = M_NONE, l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < PW; w++) m = fmaxf(m, s_ml[w][0][c]);
-        float4 y[4];
-#pragma unroll
-        for (int x = 0; x < 4; x++) y[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < PW; w++) {
-            const float f = __builtin_amdgcn_exp2f((s_ml[w][0][c] - m) * sc);
-            l = fmaf(s_ml[w][1][c], f, l);
-            const float4 *from = reinterpret_cast<const float4 *>(s_kv[w]) + 4 * 64 * wave + lane;
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const float4 z = from[64 * x];
-                y[x].x = fmaf(z.x, f, y[x].x), y[x].y = fmaf(z.y, f, y[x].y);
-                y[x].z = fmaf(z.z, f, y[x].z), y[x].w = fmaf(z.w, f, y[x].w);
-            }
-        }
-        if (r < t.rows) {
+            const float by = !sh_.all ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
             float *to;
-            float by = 1.0f;
-            if (u0 == 0 && u1 == t.len) {
-                by = l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
-                to = out_row(a, t, kvh, r);
+            if (sh_.all) {
+                to = out_row(a, t.start, kvh, rc);
             } else {
-                const size_t pr = (((size_t)kvh * a.parts + piece) * 2 + (u0 == 0)) * KB + c;
-                to = a.part + pr * D;
-                if (wave == 0 && hf == 0) a.part_ml[pr] = make_float4(m, l, sc, 0.0f);
+                const size_t row = part + c;
+                to = a.part[0].sums + row * D;
+                if (c < t.rows && wave == 0 && hf == 0) a.part[0].ml[row] = make_float4(m, l, sc, 0.0f);
             }
+            to += 32 * wave + 4 * hf;
+            if (c < t.rows)
 #pragma unroll
-            for (int x = 0; x < 4; x++)
-                *reinterpret_cast<float4 *>(to + 32 * wave + 8 * x + 4 * hf) = make_float4(y[x].x * by, y[x].y * by, y[x].z * by, y[x].w * by);
+                for (int x = 0; x < 4; x++)
+                    *reinterpret_cast<float4 *>(to + 8 * x) = make_float4(y[x].x * by, y[x].y * by, y[x].z * by, y[x].w * by);
         }
         if (t.begin + t.len >= x1) break;
     }
 }
 
-// the tile that the cut behind a piece goes through, if it is the first cut through it: its parts joined. A piece's two places
-// are for the tile that it ends with (1) and the one that it goes on with or begins and ends inside (0). 8 lanes a row
-__global__ __launch_bounds__(256) void k_page_attn_join(Args a) {
-    const int tid = threadIdx.x, row = tid >> 3, j = tid & 7;
+// ---- reads of many rows ------------------------------------------------------------------------------------------------------
+
+template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, int piece, uint4_t *s_kv, Shared &sh) {
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), hf = lane >> 5, c = lane & 31;
+    if (a.pieces > 1) no_parts<true>(a, kvh, piece);
+    Line<true> line(a, sh.reads[wave]);
+    const int64_t x0 = line.cut(piece), x1 = line.cut(piece + 1);
+    if (x0 >= x1) return;
+    const size_t head0 = (size_t)kvh * a.kv.n_ctx;
+
+    // K and V of a block as f16 in one of two buffers each, K a block ahead of V: the next block's scores are computed under this
+    // one's softmax (the layouts are k_kv_attn's). f16 rows: a wave loads 4 rows of each half straight into LDS. q8_0 rows: a
+    // thread loads 16 quants of a row into registers and makes them f16 a block later
+    char *stage = reinterpret_cast<char *>(s_kv);
+    const uint32_t slds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)stage + 16u * 64 * wave;
+    const int lrow = Q8 ? 8 * wave + (lane >> 3) : 4 * wave + (lane >> 4), lc = Q8 ? lane & 7 : lane & 15;
+    const uint32_t koff = 2 * D * lrow + 16 * (lc ^ (lrow & 15)), voff = 2 * D * lrow + 16 * (lc ^ (4 * (lrow & 3)));  // the same for row lrow + 16
+    auto issue = [&](const Rows &x, int b, bool is_v) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            lds_load16((const char *)(is_v ? a.kv.v : a.kv.k) + (head0 + x.at[h]) * (2 * D), is_v ? voff : koff,
+                       slds + 16u * (b * TILE + (is_v ? K_CHUNKS : 0) + 256 * h));
+    };
+    struct Raw {
+        uint4_t q;
+        uint16_t d;
+    };
+    auto fetch = [&](const Rows &x, bool is_v) {
+        const size_t row = head0 + x.at[wave >> 1] + (lrow & 15);
+        return Raw{*reinterpret_cast<const uint4_t *>((const char *)(is_v ? a.kv.v : a.kv.k) + row * D + 16 * lc),
+                   (is_v ? a.kv.vd : a.kv.kd)[row * 4 + (lc >> 1)]};
+    };
+    auto commit = [&](const Raw &x, int b, bool is_v) {
+        _Float16 d;
+        __builtin_memcpy(&d, &x.d, 2);
+        const int swz = is_v ? 4 * (lrow & 3) : lrow & 15;
+        uint4_t *to = s_kv + b * TILE + (is_v ? K_CHUNKS : 0) + 16 * lrow;
+        *reinterpret_cast<half8 *>(to + ((2 * lc) ^ swz)) = dequant8(x.q[0], x.q[1], half2_t{d, d});
+        *reinterpret_cast<half8 *>(to + ((2 * lc + 1) ^ swz)) = dequant8(x.q[2], x.q[3], half2_t{d, d});
+    };
+    // the lane's bytes of a block: K's step ks at k_at ^ 32·ks (chunk 2ks + hf of row c), V's tile u at v_at ^ 64·u
+    const int vrow = 4 * hf + ((lane & 15) >> 2);
+    const int k_at = 16 * (16 * c + (hf ^ (c & 15)));
+    const int v_at = 16 * (K_CHUNKS + 16 * vrow + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (4 * (vrow & 3)))) + 8 * (lane & 1);
+
+    for (Tile<true> t(line, x0);; t.next(line)) {
+        const Share sh_ = share_of(line, t, x0, x1);
+        if (sh_.i0 < sh_.i1 || sh_.all) {
+            const int i0 = sh_.i0, n_st = sh_.i1 - i0;
+            const int r0 = WIDE * t.tau + KB * wave, r = r0 + c, rc = min(r, t.rows - 1);
+            const int all_to = (t.last_of(a, r0) + 1) / KB;                                  // blocks that all of the wave's rows see the whole of
+            const int own_to = r0 < t.rows ? (t.last_of(a, r0 + KB - 1) + KB) / KB : 0;    // blocks that one of them sees
+            const int keys = t.last_key(a, query_of(a, rc)) + 1;                            // keys that the lane's row sees
+            Run run = run_of(a, line, t, i0, 1);
+            if (n_st > 0) run.fetch(0);
+            Rows r_last{{0, 0}, 0};  // f16: of the last stage whose K is on its way
+            uint32_t gone = 0;       // and the halves without a page of this stage and those after it, a pair of bits each
+            half8 qh[8], ql[8];
+            float sc;
+            size_t part = 0;
+            Rows r_now{{0, 0}, 0}, r_next{{0, 0}, 0};  // of this stage and the next one
+            Raw k_raw{}, v_raw{};                      // q8_0: the stage after the next one's K, the next one's V
+            {
+                float qx[8][8];
+                q_load<8>(q_row(a, t.start, kvh, rc) + 8 * hf, qx);
+                __syncthreads();  // (the tile before is done with the buffers)
+                if (n_st > 0) r_now = run.of(0);
+                if (n_st > 1) r_next = run.of(1);
+                if constexpr (Q8) {
+                    if (n_st > 0) commit(fetch(r_now, false), 0, false), commit(fetch(r_now, true), 0, true);
+                    if (n_st > 1) commit(fetch(r_next, false), 1, false), v_raw = fetch(r_next, true);
+                } else {
+                    if (n_st > 0) {
+                        const Rows one = run.of(0), two = run.of(min(1, n_st - 1));
+                        r_last = run.of(min(2, n_st - 1));
+                        gone = one.bad | two.bad << 2 | r_last.bad << 4;
+                        issue(one, 0, false), issue(two, 1, false), issue(r_last, 2, false);
+                        issue(one, 0, true), issue(two, 1, true);
+                    }
+                }
+                if (!sh_.all) part = part_of(line, t, sh_, kvh, piece);
+                sc = q_split<8, 2>(qx, a.scale, qh, ql);
+            }
+            Rows r_third{{0, 0}, 0};  // q8_0: of the stage whose K is in k_raw
+            if constexpr (Q8)
+                if (n_st > 2) r_third = run.of(2), k_raw = fetch(r_third, false);
+            float m = M_NONE, l = 0.0f;
+            f32x16 o[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) o[u][x] = 0.0f;
+
+            // stage st in buffer b: its scores are in s; the next stage's are computed into sn under the softmax's VALU work
+            auto step = [&](int st, int b, f32x16 &s, f32x16 &sn, auto is_masked) {
+                constexpr bool MASK = decltype(is_masked)::value;
+                // this wave's loads of K stage st + 1 and V stage st (f16: of the stages after them too) are in, its reads of K stage
+                // st and V stage st − 1 have their values; behind the barrier everyone's, and the buffers are free
+                if (Q8 || (st & 1) == 0) {
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                }
+                const uint32_t bad = Q8 ? r_now.bad : gone & 3u;
+                r_now = r_next;
+                if constexpr (Q8) {
+                    r_next = r_third;
+                    if (st + 2 < n_st) commit(k_raw, b, false);
+                    if (st + 1 < n_st) commit(v_raw, b ^ 1, true);
+                    if (st + 3 < n_st) r_third = run.of(st + 3), k_raw = fetch(r_third, false);
+                    if (st + 2 < n_st) v_raw = fetch(r_next, true);
+                } else {  // (past the last stage: its loads once more)
+                    if ((st & 1) == 0) {
+                        const Rows three = run.of(min(st + 3, n_st - 1)), four = run.of(min(st + 4, n_st - 1));
+                        gone |= three.bad << 6 | four.bad << 8;
+                        issue(three, (st + 3) & 3, false), issue(four, st & 3, false);
+                        issue(r_last, (st + 2) & 3, true), issue(three, (st + 3) & 3, true);
+                        r_last = four;
+                    }
+                    gone >>= 2;
+                }
+                const int i = i0 + st;
+                if constexpr (MASK)
+                    if (i >= own_to) return;
+                uint32_t seen = 0;
+                if constexpr (MASK) {
+                    seen = sees(keys, i, hf, bad);
+#pragma unroll
+                    for (int x = 0; x < 16; x++) s[x] = seen >> (8 * (x >> 2) + (x & 3)) & 1 ? s[x] : -INFINITY;
+                }
+                float mx = s[0];
+#pragma unroll
+                for (int x = 1; x < 16; x++) mx = fmaxf(mx, s[x]);
+                mx = pair_max<32>(mx);
+                const bool up = (mx - m) * sc > P_ROOM;
+                if (__builtin_amdgcn_ballot_w64(up)) {
+                    const float to = up ? mx : m, corr = __builtin_amdgcn_exp2f((m - to) * sc);
+                    m = to;
+                    l *= corr;
+#pragma unroll
+                    for (int u = 0; u < 4; u++) o[u] *= corr;
+                }
+                // the order pinned: behind each score MFMA of the next stage its share of this stage's softmax
+                // (past the last stage: scores of what the buffer holds, not used)
+                const char *kb = stage + (Q8 ? 16 * TILE * (b ^ 1) : 0);
+                // (the sums below are not kept from stage to stage)
+                const int k0 = here(k_at + (Q8 ? 0 : 16 * TILE * ((st + 1) & 3))), v0 = here(v_at + (Q8 ? 0 : 16 * TILE * (st & 3)));
+                const auto *vb = (const __attribute__((address_space(3))) char *)stage + (Q8 ? 16 * TILE * b : 0);
+                auto vread = [&](int u, int ss) {
+                    const auto *p = vb + (v0 ^ 64 * u) + 256 * 16 * ss;
+                    const fp16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)p);
+                    const fp16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)(p + 256 * 8));
+                    half8 v;
+                    __builtin_memcpy(&v, &lo, 8);
+                    __builtin_memcpy((char *)&v + 8, &hi, 8);
+                    return v;
+                };
+                uint32_t ph[8], pl[8];
+                float ls;
+                half8 f[8], v[4];
+#pragma unroll
+                for (int ks = 0; ks < 3; ks++) f[ks] = *reinterpret_cast<const half8 *>(kb + (k0 ^ 32 * ks));
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int ks = 0; ks < 8; ks++) {
+                    sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[ks], qh[ks], ks ? sn : f32x16{}, 0, 0, 0);
+                    if (ks + 3 < 8) f[ks + 3] = *reinterpret_cast<const half8 *>(kb + (k0 ^ 32 * (ks + 3)));
+                    else v[ks - 5] = vread(ks - 5, 0);
+                    const float2_t p = {__builtin_amdgcn_exp2f(fmaf(s[2 * ks] - m, sc, P_SHIFT)),
+                                        __builtin_amdgcn_exp2f(fmaf(s[2 * ks + 1] - m, sc, P_SHIFT))};  // not seen: 2^(−∞) = 0
+                    const half2_t hi = __builtin_convertvector(p, half2_t);
+                    __builtin_memcpy(&ph[ks], &hi, 4);
+                    asm volatile("" : "+v"(ph[ks]));  // holds the conversion here
+                    __builtin_amdgcn_sched_barrier(0);
+                    sn = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[ks], ql[ks], sn, 0, 0, 0);
+                    ls = ks ? ls + p[0] : p[0];
+                    ls += p[1];
+                    const half2_t lo = __builtin_convertvector((float2_t{minus_half<0>(p[0], ph[ks]), minus_half<1>(p[1], ph[ks])}), half2_t);
+                    __builtin_memcpy(&pl[ks], &lo, 4);
+                    asm volatile("" : "+v"(pl[ks]));
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                v[3] = vread(3, 0);
+                l += ls;
+                bool odd = false;
+                if constexpr (MASK) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int u = 0; u < 4; u++) largest(v[u], top), largest(vread(u, 1), top);
+                    odd = any_not_finite(top);
+                }
+#pragma unroll
+                for (int ss = 0; ss < 2; ss++) {
+                    half8 h8, l8;
+                    __builtin_memcpy(&h8, &ph[4 * ss], 16);
+                    __builtin_memcpy(&l8, &pl[4 * ss], 16);
+                    half8 vn[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        if (odd) v[u] = finite(v[u]);
+                        o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[u], h8, o[u], 0, 0, 0);
+                        if (ss == 0) vn[u] = vread(u, 1);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        o[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[u], l8, o[u], 0, 0, 0);
+                        if (ss == 0) v[u] = vn[u];
+                    }
+                }
+                if constexpr (MASK)
+                    if (odd) put_nan(o, seen, vread);
+            };
+            // K and V of stage 0, K of stage 1
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            f32x16 s0, s1;
+#pragma unroll
+            for (int ks = 0; ks < 8; ks++) {  // (without a stage: scores of what the buffer holds, not used)
+                const half8 f = *reinterpret_cast<const half8 *>(stage + (k_at ^ 32 * ks));
+                s0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, qh[ks], ks ? s0 : f32x16{}, 0, 0, 0);
+                s0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, ql[ks], s0, 0, 0, 0);
+            }
+            // two stages at a time, both kinds of step passing one barrier a stage: a wave's blocks may be masked where another's
+            // are not
+            auto whole2 = [&](int st) { return st + 1 < n_st && i0 + st + 1 < all_to && (Q8 ? r_now.bad | r_next.bad : gone & 15u) == 0; };
+            for (int st = 0; st < n_st;) {
+                for (; whole2(st); st += 2) {
+                    step(st, 0, s0, s1, std::false_type{});
+                    step(st + 1, 1, s1, s0, std::false_type{});
+                }
+                for (int e = st + 2; st < min(e, n_st); st++) {
+                    step(st, st & 1, s0, s1, std::true_type{});
+                    s0 = s1;
+                }
+            }
+            l = pair_sum<32>(l);
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (the next tile's loads go over these buffers)
+
+            const float by = !sh_.all ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
+            float *to;
+            if (sh_.all) {
+                to = out_row(a, t.start, kvh, rc);
+            } else {
+                const size_t row = part + KB * wave + c;
+                to = a.part[1].sums + row * D;
+                if (r < t.rows && hf == 0) a.part[1].ml[row] = make_float4(m, l, sc, 0.0f);
+            }
+            if (r < t.rows)
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        *reinterpret_cast<float4 *>(to + 4 * hf + 32 * u + 8 * x) =
+                            make_float4(o[u][4 * x] * by, o[u][4 * x + 1] * by, o[u][4 * x + 2] * by, o[u][4 * x + 3] * by);
+        }
+        if (t.begin + t.len >= x1) break;
+    }
+}
+
+// all workgroups of wide tiles, then all of narrow ones
+template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_attn(Args a) {
+    __shared__ __attribute__((aligned(16))) uint4_t s_kv[PW * (Q8 ? WAVE_Q8 : WAVE_F16)];
+    __shared__ Shared sh;
     const int kvh = blockIdx.x % a.kv.n_kv, piece = blockIdx.x / a.kv.n_kv;
-    Line line(a);
-    const int64_t total = line.total();
-    const int n_piece = pieces(a, total);
-    if (piece + 1 >= n_piece) return;
-    const int64_t x = cut(total, piece + 1, n_piece);
-    if (x >= total) return;
-    const Tile t(line, x);
-    if (t.begin == x || t.begin < cut(total, piece, n_piece)) return;
-    int more = 0;  // pieces past this one that have part of it
-    while (piece + 1 + more < n_piece && cut(total, piece + 1 + more, n_piece) < t.begin + t.len) more++;
-    const int r = KB * t.tau + row;
-    if (r >= t.rows) return;
-    const size_t first = (((size_t)kvh * a.parts + piece) * 2 + 1) * KB + row;
-    auto place = [&](int e) { return e == 0 ? first : first - KB + (size_t)e * (2 * KB); };
-    float m = M_NONE;
-    for (int e = 0; e <= more; e++) m = fmaxf(m, a.part_ml[place(e)].x);
-    float l = 0.0f;
-    float4 y[4];
+    if (piece < a.wide) wide<Q8>(a, kvh, piece, s_kv, sh);
+    else narrow<Q8>(a, kvh, piece - a.wide, s_kv, sh);
+}
+
+// The second launch: the rows of a cut tile shared out among as many workgroups as it has parts (SHARES times as many), those of
+// the pieces. 32 lanes of 4 dims to a row; where the rows are fewer than the groups of 32, several groups to a row's parts
+__global__ __launch_bounds__(256) void k_page_attn_join(Args a) {
+    __shared__ float4 s_y[8][32];
+    __shared__ float2 s_ml[8];
+    const int tid = threadIdx.x, gr = tid >> 5, j = tid & 31;
+    const int kvh = blockIdx.x % a.kv.n_kv, unit = blockIdx.x / a.kv.n_kv, piece = unit % a.pieces, share = unit / a.pieces;
+    const int w = unit < SHARES * a.wide, shares = w ? SHARES : 1;
+    const Parts &p = a.part[w];
+    const int height = w ? WIDE : NARROW;
+    const size_t mine = ((size_t)kvh * a.pieces + piece) * 2;
+    const Part both[2] = {p.of[mine], p.of[mine + 1]};
+    for (int k = 0; k < 2; k++) {
+        const Part &t = both[k];
+        if (t.n == 0) continue;
+        const int mth = (piece - t.first) * shares + (w ? share : 0), of = t.n * shares;
+        const int ra = t.rows * mth / of, rb = t.rows * (mth + 1) / of, nr = rb - ra;
+        const int lg = nr > 4 ? 3 : nr > 2 ? 2 : nr > 1 ? 1 : 0, G = 8 >> lg;  // 2^lg rows at once, G groups to each
+        for (int r = ra; r < rb; r += 1 << lg) {
+            const int row = min(r + (gr & ((1 << lg) - 1)), rb - 1), g = gr >> lg;
+            float top = M_NONE, sum = 0.0f;
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float c = 0.0f;
+            for (int e0 = g; e0 < t.n; e0 += 4 * G) {
+                float4 ml[4], in[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) y[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int e = 0; e <= more; e++) {
-        const float4 ml = a.part_ml[place(e)];
-        const float f = __builtin_amdgcn_exp2f((ml.x - m) * ml.z);
-        l = fmaf(ml.y, f, l);
-        const float *from = a.part + place(e) * D + 4 * j;
+                for (int q = 0; q < 4; q++) {
+                    const int e = e0 + q * G;
+                    ml[q] = make_float4(M_NONE, 0.0f, c, 0.0f), in[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (e < t.n) {
+                        const size_t at = (((size_t)kvh * a.pieces + t.first + e) * 2 + (e == 0)) * height + row;
+                        ml[q] = p.ml[at];
+                        in[q] = *reinterpret_cast<const float4 *>(p.sums + at * D + 4 * j);
+                    }
+                }
+                c = ml[0].z;  // (a row's parts have the same)
+                const float to = fmaxf(fmaxf(top, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+                const float f = __builtin_amdgcn_exp2f((top - to) * c);
+                top = to, sum *= f, y.x *= f, y.y *= f, y.z *= f, y.w *= f;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float4 z = *reinterpret_cast<const float4 *>(from + 32 * k);
-            y[k].x = fmaf(z.x, f, y[k].x), y[k].y = fmaf(z.y, f, y[k].y), y[k].z = fmaf(z.z, f, y[k].z), y[k].w = fmaf(z.w, f, y[k].w);
+                for (int q = 0; q < 4; q++) {
+                    const float h = __builtin_amdgcn_exp2f((ml[q].x - to) * c);
+                    sum = fmaf(ml[q].y, h, sum);
+                    y.x = fmaf(in[q].x, h, y.x), y.y = fmaf(in[q].y, h, y.y), y.z = fmaf(in[q].z, h, y.z), y.w = fmaf(in[q].w, h, y.w);
+                }
+            }
+            if (G > 1) {  // (one pass)
+                __syncthreads();
+                s_y[gr][j] = y;
+                if (j == 0) s_ml[gr] = make_float2(top, sum);
+                __syncthreads();
+                if (g == 0) {
+                    float to = top;
+                    for (int e = 1; e < G; e++) to = fmaxf(to, s_ml[gr + (e << lg)].x);
+                    const float f = __builtin_amdgcn_exp2f((top - to) * c);
+                    sum *= f, y.x *= f, y.y *= f, y.z *= f, y.w *= f;
+                    for (int e = 1; e < G; e++) {
+                        const float4 z = s_y[gr + (e << lg)][j];
+                        const float2 ml = s_ml[gr + (e << lg)];
+                        const float h = __builtin_amdgcn_exp2f((ml.x - to) * c);
+                        sum = fmaf(ml.y, h, sum);
+                        y.x = fmaf(z.x, h, y.x), y.y = fmaf(z.y, h, y.y), y.z = fmaf(z.z, h, y.z), y.w = fmaf(z.w, h, y.w);
+                    }
+                }
+            }
+            if (g == 0 && r + (gr & ((1 << lg) - 1)) < rb) {
+                const float by = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
+                *reinterpret_cast<float4 *>(out_row(a, t.start, kvh, t.r0 + row) + 4 * j) = make_float4(y.x * by, y.y * by, y.z * by, y.w * by);
+            }
         }
     }
-    const float by = l == 0.0f ? 0.0f : 1.0f / l;
-    float *to = out_row(a, t, kvh, r) + 4 * j;
-#pragma unroll
-    for (int k = 0; k < 4; k++) *reinterpret_cast<float4 *>(to + 32 * k) = make_float4(y[k].x * by, y[k].y * by, y[k].z * by, y[k].w * by);
 }
 
 }  // namespace
@@ -522,19 +916,24 @@ extern "C" int htr_page_attention(htr_device *dev, const float *d_q, size_t q_st
     a.q = d_q, a.q_stride = q_stride, a.out = d_out, a.n_head = n_head, a.group = n_head / kv->n_kv;
     a.n_page = kv->n_ctx / pages->page, a.scale = scale;
     a.per_group = (uint32_t)(((1ull << 32) + a.group - 1) / a.group), a.cap = a.p.max_pages << a.p.shift;
-    a.parts = std::max(1, 2 * dev->n_cu / kv->n_kv);
-    const unsigned groups = (unsigned)(a.parts * kv->n_kv);
-    if (a.parts > 1) {
-        const size_t rows = (size_t)4 * dev->n_cu * KB;  // two places for each of 2·n_cu pieces
+    a.pieces = std::max(1, 2 * dev->n_cu / kv->n_kv), a.per_piece = 1.0 / a.pieces;
+    if (a.pieces > 1) {
+        const size_t n = (size_t)2 * dev->n_cu;
         void *p;
-        HTR_TRY(htr_scratch(dev, SCR_PAGE_ATTN, rows * (D + 4) * 4, &p));
-        a.part = (float *)p;
-        a.part_ml = (float4 *)(a.part + rows * D);
+        HTR_TRY(htr_scratch(dev, SCR_PAGE_ATTN, 2 * n * ((NARROW + WIDE) * (D + 4) * 4 + 2 * sizeof(Part)), &p));
+        float *at = (float *)p;
+        for (int w = 0; w < 2; w++) {
+            const size_t rows = 2 * n * (w ? WIDE : NARROW);
+            a.part[w] = Parts{at, (float4 *)(at + rows * D), (Part *)(at + rows * (D + 4))};
+            at += rows * (D + 4) + 2 * n * sizeof(Part) / 4;
+        }
     }
+    a.wide = n * group > NARROW ? a.pieces : 0;
+    const unsigned groups = (unsigned)((a.wide + a.pieces) * kv->n_kv);
     if (a.kv.q8) hipLaunchKernelGGL(k_page_attn<true>, dim3(groups), dim3(64 * PW), 0, dev->stream, a);
     else hipLaunchKernelGGL(k_page_attn<false>, dim3(groups), dim3(64 * PW), 0, dev->stream, a);
     HTR_TRY(htr_launched(dev, a.kv.q8 ? "k_page_attn<q8_0>" : "k_page_attn<f16>"));
-    if (a.parts == 1) return 0;
-    hipLaunchKernelGGL(k_page_attn_join, dim3(groups - (unsigned)kv->n_kv), dim3(256), 0, dev->stream, a);
+    if (a.pieces == 1) return 0;
+    hipLaunchKernelGGL(k_page_attn_join, dim3((unsigned)((SHARES * a.wide + a.pieces) * kv->n_kv)), dim3(256), 0, dev->stream, a);
     return htr_launched(dev, "k_page_attn_join");
 }
