@@ -30,6 +30,8 @@ enum {
     SCR_KV_TICKET = 8,  // their tickets (one size; zero, self-resetting)
     SCR_KV_ROWS = 9,    // q8_0 rows read back for the window attention (htr_scratch_kept)
     SCR_PAGE_ATTN = 10, // the parts of the page attention's cut tiles (one size)
+    SCR_SCORE = 11,     // the log probabilities' parts of rows (one size)
+    SCR_SCORE_TICKET = 12,  // their tickets (one size; zero, self-resetting)
     SCR_SLOTS
 };
 
