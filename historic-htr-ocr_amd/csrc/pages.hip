@@ -16,8 +16,10 @@
 
 namespace {
 
-constexpr int THREADS = HTR_MAX_SEQ;  // a thread a read
-constexpr int ROWS_ONE = 4096;        // rows that the one workgroup of the sums maps itself; more: a second launch
+// A thread a read: one workgroup, of 256 threads for up to 256 reads and 1024 rows (24 reads of a token 3.6 µs, by 1024 threads
+// 4.4), else of 1024. Up to 4096 rows it maps the rows too, more are a second launch's.
+constexpr int SMALL = 256, SMALL_ROWS = 1024, ROWS_ONE = 4096;
+constexpr int AT_ONCE = 4;  // searches of a thread beside each other: each is ten LDS reads behind one another
 
 struct MapArgs {
     HtrPages p;
@@ -45,22 +47,25 @@ __device__ uint32_t block_scan(uint32_t v, uint32_t *s_wave) {
     for (int w = 0; w < wave; w++) v += s_wave[w];
     return v;
 }
-// the first of n ascending sums that is past i, n where none is
-__device__ __forceinline__ int first_past(const uint32_t *sums, int n, uint32_t i) {
-    int lo = 0, hi = n;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (sums[mid] > i) hi = mid;
-        else lo = mid + 1;
+// for each of N numbers the first of n ≤ 1024 ascending sums that is past it, n where none is
+template <int N> __device__ __forceinline__ void first_past(const uint32_t *sums, int n, const uint32_t (&i)[N], int (&at)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; k++) at[k] = 0;
+    for (int step = 1 << (31 - __builtin_clz((unsigned)n)); step; step >>= 1) {
+        uint32_t sum[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) sum[k] = sums[min(at[k] + step, n) - 1];
+#pragma unroll
+        for (int k = 0; k < N; k++) at[k] = at[k] + step <= n && sum[k] <= i[k] ? at[k] + step : at[k];
     }
-    return lo;
 }
+
 // a row's place in the cache: −1 where the table has no page of the cache there
 __device__ __forceinline__ int slot_of(int page, int n_page, int pos, int shift) {
     return (uint32_t)page < (uint32_t)n_page ? (page << shift) + (pos & ((1 << shift) - 1)) : -1;
 }
 
-__global__ __launch_bounds__(THREADS) void k_page_map(MapArgs a, int map_rows) {
+template <int THREADS> __global__ __launch_bounds__(THREADS) void k_page_map(MapArgs a, int map_rows) {
     __shared__ uint32_t s_end[THREADS], s_upto[THREADS], s_back[THREADS], s_wave[THREADS / 64], s_taken;
     __shared__ int s_past[THREADS], s_held[THREADS], s_need[THREADS];
     const int b = threadIdx.x, shift = a.p.shift;
@@ -97,28 +102,53 @@ __global__ __launch_bounds__(THREADS) void k_page_map(MapArgs a, int map_rows) {
         const uint32_t at = head + i;
         return a.ring + (at >= n_page ? at - n_page : at);
     };
-    for (uint32_t i = b; i < taken; i += THREADS) {
-        const int s = first_past(s_upto, a.p.n_seq, i);
-        a.p.table[(size_t)s * a.p.max_pages + s_held[s] + (i - (s_upto[s] - s_need[s]))] = *ring_at(i);
+    for (uint32_t i0 = b; i0 < taken; i0 += AT_ONCE * THREADS) {
+        uint32_t i[AT_ONCE];
+        int at[AT_ONCE], page[AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++) i[k] = min(i0 + THREADS * k, taken - 1), page[k] = *ring_at(i[k]);
+        first_past(s_upto, a.p.n_seq, i, at);
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++)
+            if (i0 + THREADS * k < taken)
+                a.p.table[(size_t)at[k] * a.p.max_pages + s_held[at[k]] + (i[k] - (s_upto[at[k]] - s_need[at[k]]))] = page[k];
     }
-    for (uint32_t i = b; i < returned; i += THREADS) {
-        const int s = first_past(s_back, a.p.n_seq, i);
-        *ring_at(count + i) = a.p.table[(size_t)s * a.p.max_pages + (i - (s ? s_back[s - 1] : 0u))];
+    for (uint32_t i0 = b; i0 < returned; i0 += AT_ONCE * THREADS) {
+        uint32_t i[AT_ONCE];
+        int at[AT_ONCE], page[AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++) i[k] = min(i0 + THREADS * k, returned - 1);
+        first_past(s_back, a.p.n_seq, i, at);
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++) page[k] = a.p.table[(size_t)at[k] * a.p.max_pages + (i[k] - (at[k] ? s_back[at[k] - 1] : 0u))];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++)
+            if (i0 + THREADS * k < returned) *ring_at(count + i[k]) = page[k];
     }
     if (!map_rows) return;
-    for (int r = b; r < a.p.n_row; r += THREADS) {
-        const int s = first_past(s_end, a.p.n_seq, (uint32_t)r);
-        int pos = -1, slot = -1;
-        if (s < a.p.n_seq && s_past[s] >= 0) {
-            pos = s_past[s] + r - (s ? (int)s_end[s - 1] : 0);
-            const int k = pos >> shift;
-            // a page that this step gives out is in the ring yet
-            const int page = k < s_held[s] ? a.p.table[(size_t)s * a.p.max_pages + k]
-                                           : *ring_at(s_upto[s] - s_need[s] + (k - s_held[s]));
-            slot = slot_of(page, a.n_page, pos, shift);
+    for (int r0 = b; r0 < a.p.n_row; r0 += AT_ONCE * THREADS) {
+        uint32_t i[AT_ONCE];
+        int at[AT_ONCE], pos[AT_ONCE], page[AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++) i[k] = (uint32_t)min(r0 + THREADS * k, a.p.n_row - 1);
+        first_past(s_end, a.p.n_seq, i, at);
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++) {
+            const int s = at[k];
+            pos[k] = page[k] = -1;
+            if (s < a.p.n_seq && s_past[s] >= 0) {
+                pos[k] = s_past[s] + (int)i[k] - (s ? (int)s_end[s - 1] : 0);
+                const int n = pos[k] >> shift;
+                // a page that this step gives out is in the ring yet
+                page[k] = n < s_held[s] ? a.p.table[(size_t)s * a.p.max_pages + n] : *ring_at(s_upto[s] - s_need[s] + (n - s_held[s]));
+            }
         }
-        a.p.pos[r] = pos;
-        a.p.slot[r] = slot;
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; k++)
+            if (r0 + THREADS * k < a.p.n_row) {
+                a.p.pos[i[k]] = pos[k];
+                a.p.slot[i[k]] = slot_of(page[k], a.n_page, pos[k], shift);
+            }
     }
 }
 
@@ -128,7 +158,10 @@ __global__ __launch_bounds__(256) void k_page_rows(MapArgs a) {
     for (int b = threadIdx.x; b < a.p.n_seq; b += 256) s_end[b] = (uint32_t)a.p.start[b + 1];
     __syncthreads();
     for (int r = blockIdx.x * 256 + threadIdx.x; r < a.p.n_row; r += gridDim.x * 256) {
-        const int s = first_past(s_end, a.p.n_seq, (uint32_t)r);
+        const uint32_t i[1] = {(uint32_t)r};
+        int at[1];
+        first_past(s_end, a.p.n_seq, i, at);
+        const int s = at[0];
         int pos = -1, slot = -1;
         if (s < a.p.n_seq && a.p.past[s] >= 0) {
             pos = a.p.past[s] + r - (s ? (int)s_end[s - 1] : 0);
@@ -189,7 +222,8 @@ extern "C" int htr_page_map(htr_device *dev, const htr_pages *pages, int n_page,
     const HtrOnDevice on(dev);
     a.len = d_len, a.add = d_new, a.pool = d_pool, a.ring = d_ring, a.len_out = d_len_out, a.pool_out = d_pool_out, a.n_page = n_page;
     const bool one = a.p.n_row <= ROWS_ONE;
-    hipLaunchKernelGGL(k_page_map, dim3(1), dim3(THREADS), 0, dev->stream, a, one ? 1 : 0);
+    if (a.p.n_seq <= SMALL && a.p.n_row <= SMALL_ROWS) hipLaunchKernelGGL(k_page_map<SMALL>, dim3(1), dim3(SMALL), 0, dev->stream, a, 1);
+    else hipLaunchKernelGGL(k_page_map<HTR_MAX_SEQ>, dim3(1), dim3(HTR_MAX_SEQ), 0, dev->stream, a, one ? 1 : 0);
     HTR_TRY(htr_launched(dev, "k_page_map"));
     if (one) return 0;
     hipLaunchKernelGGL(k_page_rows, dim3((unsigned)std::min((a.p.n_row + 255) / 256, 2048)), dim3(256), 0, dev->stream, a);
