@@ -10,12 +10,18 @@
 // once, whatever the reads (twice: once for each height of tile). Each KV head's tiles in order are a line of work, a tile's
 // length on it its keys and COST more for its start and end, and the head's workgroups take equal pieces of the line, wherever
 // that cuts a tile: one read of many keys goes to all of them, of many short ones each takes a few, and no list of work is made
-// first. Where a piece begins follows from sums over the reads, a lane a read. The parts of a cut tile are joined by
-// a second launch.
+// first. Where a piece begins follows from sums over the reads, a lane a read. The parts of a cut tile are joined by a second
+// launch. (Joined by a tile's last workgroup in the same launch one token took 12.5 µs, but 32 parts of a wide tile went through
+// one workgroup, 65 tokens over 8000 keys 182 µs for 47; in pairs 75. More and smaller pieces, or smaller ones for the workgroups
+// that begin later, were slower: 64 reads' tokens 110 … 124 µs for 105.)
 //
 // Tiles come in two heights, each with a line of its own. Of up to 32 rows (a step's token, or what is left of a prompt) the waves
 // share out the keys, every fourth block of 32 to each, loaded into LDS of its own, so that nobody waits for anybody until the
-// four sums are merged. More are tiles of 128, 32 to a wave, all of which use each block, staged for them together.
+// four sums are merged. More are tiles of 128, 32 to a wave, all of which use each block, staged for them together. (Four prompts
+// of 1925 in tiles of 32 rows alone 309 µs, with both 158.) The wide tiles' workgroups come first in the launch: in turn with the
+// narrow ones' a CU got two of one kind and its neighbour none, 263 µs for 178.
+//
+// Times here and below are of calls one after another on an MI355X, 16 q heads on 8 KV heads.
 #include <algorithm>
 #include <type_traits>
 
@@ -25,7 +31,7 @@ namespace {
 
 constexpr int PW = 4;                       // waves of a workgroup, two of which a CU holds
 constexpr int NARROW = KB, WIDE = KB * PW;  // rows of a tile
-constexpr int COST = 128;                    // keys that take as long as a tile's start and end
+constexpr int COST = 128;                   // keys that take as long as a tile's start and end (with 64 four prompts 182 µs for 166)
 constexpr int LEAST = 192;                  // a piece's length, at least: a block for each wave, and a tile's start
 constexpr int SLIVER = 4;                   // blocks of a tile's beginning or end that are not cut off for themselves
 constexpr int SHARES = 4;                   // workgroups of the join to a wide piece
@@ -275,7 +281,13 @@ struct Shared {
 };
 
 // ---- reads of few rows -------------------------------------------------------------------------------------------------------
-
+//
+// A wave's block is K and V in its own LDS (layouts and products are k_kv_attn_split's): f16 one buffer each, filled again as soon
+// as it is read, q8_0 raw in two.
+//
+// Bound: of few keys latency (a token over 1300 keys 13.5 µs, of which lengths, pages, keys, each a load that the next one waits
+// for, 6 µs, and the second launch 4); of many HBM: 64 reads' tokens over 300 … 6000 f16 keys (505 MB) 105 µs, over q8_0 rows
+// (269 MB) 74, at 6.6 TB/s while all workgroups run, which end between 56 and 101 µs.
 template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh, int piece, uint4_t *s_kv, Shared &sh) {
     constexpr int WAVE = Q8 ? WAVE_Q8 : WAVE_F16;
     static_assert(WAVE >= 1024, "a wave's sums fit");
@@ -320,12 +332,12 @@ template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh
         va[u] = Q8 ? 16 * (256 + 8 * vrow + ((2 * u + ((lane >> 4) & 1)) ^ (vrow & 2) ^ ((vrow & 8) >> 1))) + 8 * (lane & 1)
                    : 16 * (K_CHUNKS + 16 * vrow + ((4 * u + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (4 * (vrow & 3)))) + 8 * (lane & 1);
     for (Tile<false> t(line, x0);; t.next(line)) {
-        const Share sh_ = share_of(line, t, x0, x1);
-        if (sh_.i0 < sh_.i1 || sh_.all) {
-            const int i1 = sh_.i1, rc = t.r0 + min(c, t.rows - 1);
+        const Share own = share_of(line, t, x0, x1);
+        if (own.i0 < own.i1 || own.all) {
+            const int i1 = own.i1, rc = t.r0 + min(c, t.rows - 1);
             const int all_to = (t.last_key(a, query_of(a, t.r0)) + 1) / KB;  // blocks that all rows see the whole of
             const int keys = t.last_key(a, query_of(a, rc)) + 1;             // keys that the lane's row sees
-            int i = sh_.i0 + wave, j = 0, b = 0;
+            int i = own.i0 + wave, j = 0, b = 0;
             Run run = run_of(a, line, t, i, PW);
             if (i < i1) run.fetch(0);
             float qx[8][8];
@@ -341,7 +353,7 @@ template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh
                     load(now.at[0], now.at[1], true);
                 }
             }
-            const size_t part = sh_.all ? 0 : part_of(line, t, sh_, kvh, piece);
+            const size_t part = own.all ? 0 : part_of(line, t, own, kvh, piece);
             half8 qh[8], ql[8];
             const float sc = q_split<8, 2>(qx, a.scale, qh, ql);
             float m = M_NONE, l = 0.0f;
@@ -524,9 +536,9 @@ template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh
                     y[x].x = fmaf(z.x, f, y[x].x), y[x].y = fmaf(z.y, f, y[x].y), y[x].z = fmaf(z.z, f, y[x].z), y[x].w = fmaf(z.w, f, y[x].w);
                 }
             }
-            const float by = !sh_.all ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
+            const float by = !own.all ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
             float *to;
-            if (sh_.all) {
+            if (own.all) {
                 to = out_row(a, t.start, kvh, rc);
             } else {
                 const size_t row = part + c;
@@ -544,7 +556,11 @@ template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh
 }
 
 // ---- reads of many rows ------------------------------------------------------------------------------------------------------
-
+//
+// Bound: the matrix cores and their power: four chunks of 2000 over 8000 keys (590 GFLOP, as pairs twice that) 1.05 ms, 1.12
+// PFLOP/s, where a library f16 product of 8192³ reaches 1.14; four prompts of 1925 (121 GFLOP as pairs) 158 µs, of which 9 % of
+// the products are of keys past a row's own, 13 µs the second launch, 20 that workgroups wait for the last. Loads four stages
+// ahead or one, and a barrier a stage or every second one, take the same time.
 template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, int piece, uint4_t *s_kv, Shared &sh) {
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), hf = lane >> 5, c = lane & 31;
     if (a.pieces > 1) no_parts<true>(a, kvh, piece);
@@ -553,9 +569,9 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
     if (x0 >= x1) return;
     const size_t head0 = (size_t)kvh * a.kv.n_ctx;
 
-    // K and V of a block as f16 in one of two buffers each, K a block ahead of V: the next block's scores are computed under this
-    // one's softmax (the layouts are k_kv_attn's). f16 rows: a wave loads 4 rows of each half straight into LDS. q8_0 rows: a
-    // thread loads 16 quants of a row into registers and makes them f16 a block later
+    // K and V of a block as f16, K a block ahead of V: the next block's scores are computed under this one's softmax (the layouts
+    // are k_kv_attn's). f16 rows: four buffers, filled two at a time, behind every second barrier; a wave loads 4 rows of each half
+    // straight into LDS. q8_0 rows: two buffers; a thread loads 16 quants of a row into registers and makes them f16 a block later
     char *stage = reinterpret_cast<char *>(s_kv);
     const uint32_t slds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)stage + 16u * 64 * wave;
     const int lrow = Q8 ? 8 * wave + (lane >> 3) : 4 * wave + (lane >> 4), lc = Q8 ? lane & 7 : lane & 15;
@@ -589,13 +605,13 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
     const int v_at = 16 * (K_CHUNKS + 16 * vrow + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (4 * (vrow & 3)))) + 8 * (lane & 1);
 
     for (Tile<true> t(line, x0);; t.next(line)) {
-        const Share sh_ = share_of(line, t, x0, x1);
-        if (sh_.i0 < sh_.i1 || sh_.all) {
-            const int i0 = sh_.i0, n_st = sh_.i1 - i0;
+        const Share own = share_of(line, t, x0, x1);
+        if (own.i0 < own.i1 || own.all) {
+            const int i0 = own.i0, n_st = own.i1 - i0;
             const int r0 = WIDE * t.tau + KB * wave, r = r0 + c, rc = min(r, t.rows - 1);
-            const int all_to = (t.last_of(a, r0) + 1) / KB;                                  // blocks that all of the wave's rows see the whole of
-            const int own_to = r0 < t.rows ? (t.last_of(a, r0 + KB - 1) + KB) / KB : 0;    // blocks that one of them sees
-            const int keys = t.last_key(a, query_of(a, rc)) + 1;                            // keys that the lane's row sees
+            const int all_to = (t.last_of(a, r0) + 1) / KB;                              // blocks that all of the wave's rows see the whole of
+            const int any_to = r0 < t.rows ? (t.last_of(a, r0 + KB - 1) + KB) / KB : 0;  // blocks that one of them sees
+            const int keys = t.last_key(a, query_of(a, rc)) + 1;                         // keys that the lane's row sees
             Run run = run_of(a, line, t, i0, 1);
             if (n_st > 0) run.fetch(0);
             Rows r_last{{0, 0}, 0};  // f16: of the last stage whose K is on its way
@@ -603,15 +619,15 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
             half8 qh[8], ql[8];
             float sc;
             size_t part = 0;
-            Rows r_now{{0, 0}, 0}, r_next{{0, 0}, 0};  // of this stage and the next one
-            Raw k_raw{}, v_raw{};                      // q8_0: the stage after the next one's K, the next one's V
+            Rows r_now{{0, 0}, 0}, r_next{{0, 0}, 0};  // q8_0: of this stage and the next one
+            Raw k_raw{}, v_raw{};                      // and the stage after the next one's K, the next one's V
             {
                 float qx[8][8];
                 q_load<8>(q_row(a, t.start, kvh, rc) + 8 * hf, qx);
                 __syncthreads();  // (the tile before is done with the buffers)
-                if (n_st > 0) r_now = run.of(0);
-                if (n_st > 1) r_next = run.of(1);
                 if constexpr (Q8) {
+                    if (n_st > 0) r_now = run.of(0);
+                    if (n_st > 1) r_next = run.of(1);
                     if (n_st > 0) commit(fetch(r_now, false), 0, false), commit(fetch(r_now, true), 0, true);
                     if (n_st > 1) commit(fetch(r_next, false), 1, false), v_raw = fetch(r_next, true);
                 } else {
@@ -623,10 +639,10 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                         issue(one, 0, true), issue(two, 1, true);
                     }
                 }
-                if (!sh_.all) part = part_of(line, t, sh_, kvh, piece);
+                if (!own.all) part = part_of(line, t, own, kvh, piece);
                 sc = q_split<8, 2>(qx, a.scale, qh, ql);
             }
-            Rows r_third{{0, 0}, 0};  // q8_0: of the stage whose K is in k_raw
+            Rows r_third{{0, 0}, 0};                   // of the stage whose K is in k_raw
             if constexpr (Q8)
                 if (n_st > 2) r_third = run.of(2), k_raw = fetch(r_third, false);
             float m = M_NONE, l = 0.0f;
@@ -647,9 +663,8 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                     asm volatile("" ::: "memory");
                 }
                 const uint32_t bad = Q8 ? r_now.bad : gone & 3u;
-                r_now = r_next;
                 if constexpr (Q8) {
-                    r_next = r_third;
+                    r_now = r_next, r_next = r_third;
                     if (st + 2 < n_st) commit(k_raw, b, false);
                     if (st + 1 < n_st) commit(v_raw, b ^ 1, true);
                     if (st + 3 < n_st) r_third = run.of(st + 3), k_raw = fetch(r_third, false);
@@ -666,7 +681,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                 }
                 const int i = i0 + st;
                 if constexpr (MASK)
-                    if (i >= own_to) return;
+                    if (i >= any_to) return;
                 uint32_t seen = 0;
                 if constexpr (MASK) {
                     seen = sees(keys, i, hf, bad);
@@ -782,9 +797,9 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
             l = pair_sum<32>(l);
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (the next tile's loads go over these buffers)
 
-            const float by = !sh_.all ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
+            const float by = !own.all ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
             float *to;
-            if (sh_.all) {
+            if (own.all) {
                 to = out_row(a, t.start, kvh, rc);
             } else {
                 const size_t row = part + KB * wave + c;
@@ -803,7 +818,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
     }
 }
 
-// all workgroups of wide tiles, then all of narrow ones
+// the workgroups of wide tiles, then those of narrow ones
 template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_attn(Args a) {
     __shared__ __attribute__((aligned(16))) uint4_t s_kv[PW * (Q8 ? WAVE_Q8 : WAVE_F16)];
     __shared__ Shared sh;

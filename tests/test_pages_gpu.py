@@ -300,6 +300,90 @@ def test_attention_of_many_reads(dev):
     r.free()
 
 
+@pytest.mark.parametrize("q8_0", [False, True], ids=["f16", "q8_0"])
+@pytest.mark.parametrize("reads,n_head,n_kv", [
+    ([(20000, 300)], 2, 1),                 # wide tiles cut into many parts each, and the rows behind them
+    ([(9000, 16)], 2, 1),                   # a narrow one of 32 rows
+    ([(7000, 64), (3, 1), (0, 66)], 2, 1),  # whole tiles of 128 rows and one of 4 more
+    ([(5000, 1), (30, 130), (6000, 1)], 2, 1)])
+def test_attention_of_tiles_in_many_parts(dev, reads, n_head, n_kv, q8_0):
+    r = Reads(dev, reads, 64, n_kv, q8_0, seed=21, pad=1)
+    q = normal(22, r.n, n_head, 128)
+    got = r.run(q, n_head)
+    assert rel_rows(got, r.want(q, SCALE)) < BAR
+    assert np.array_equal(bits(got), bits(r.run(q, n_head)))
+    r.free()
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_attention_of_any_batch(dev, seed):
+    rng = np.random.default_rng(seed)
+    n_kv = int(rng.choice([1, 2, 3, 8]))
+    n_head = n_kv * int(rng.choice([1, 2, 3, 5, 17]))
+    reads = []
+    for _ in range(int(rng.integers(1, 30))):
+        kind = rng.random()
+        past = int(2 ** rng.uniform(0, 11)) - 1
+        reads.append((past, 1) if kind < 0.5 else (past, int(2 ** rng.uniform(0, 7))) if kind < 0.85 else (past, 0) if kind < 0.92 else
+                     (-1, int(rng.integers(0, 5))))
+    r = Reads(dev, reads, int(rng.choice([16, 32, 64, 256])), n_kv, bool(rng.integers(2)), seed=seed, pad=int(rng.integers(3)))
+    q = normal(40 + seed, r.n, n_head, 128)
+    if r.n:
+        assert rel_rows(r.run(q, n_head, gap=4 * int(rng.integers(2))), r.want(q, SCALE)) < BAR
+    r.free()
+
+
+def test_attention_of_arrays_that_are_none(dev):
+    """starts below 0 and past the buffers, a past beyond the table: each read has the rows that are there, over the rows that
+    the table has room for"""
+    page, n_kv, n_head, n_row = 16, 2, 4, 10
+    table = np.array([[2, 0], [1, 1], [4, 3]], np.int32)
+    start, past = np.array([-4, 2, 2, 100], np.int32), np.array([2 ** 31 - 1, 5, 3], np.int32)
+    c = cache(dev, 3, n_kv, 5 * page)
+    bufs = [dev.upload(a) for a in (start, past, table)]
+    q = normal(1, n_row, n_head, 128)
+    qb, out = dev.upload(q), dev.alloc(q.nbytes)
+    htr.page_attention(dev, qb, htr.Pages.of(3, n_row, page, 2, *bufs), c.kv, n_head, SCALE, out)
+    got = out.download(np.float32, q.size).reshape(n_row, -1)
+    j = np.arange(2 * page)
+    rows = table[:, j // page] * page + j % page
+    want = np.zeros((n_row, n_head * 128))
+    want[:2] = attention(q[:2], c.k[:, rows[0]], c.v[:, rows[0]], np.ones((2, 32), bool), SCALE)
+    want[2:] = attention(q[2:], c.k[:, rows[2]], c.v[:, rows[2]], j[None, :] <= 3 + np.arange(8)[:, None], SCALE)
+    assert rel_rows(got, want) < BAR
+    for b in (*bufs, qb, out):
+        b.free()
+    c.free()
+
+
+def test_recorded_calls_share_the_scratch(dev):
+    """two recorded attentions of different batches replayed in turn, with eager work between: each gives its eager bits"""
+    batches = [Reads(dev, reads, page, 2, q8_0, seed=seed) for reads, page, q8_0, seed in
+               (([(900, 1), (20, 1)], 16, False, 1), ([(1500, 150), (40, 1)], 64, True, 2))]
+    runs = []
+    for r in batches:
+        q = normal(r.n, r.n, 4, 128)
+        qb, out = dev.upload(q), dev.alloc(q.nbytes)
+        want = r.run(q, 4)
+        dev.capture_begin()
+        htr.page_attention(dev, qb, r.pages, r.cache.kv, 4, SCALE, out)
+        runs.append((r, q, qb, out, want, dev.capture_end()))
+    for i in range(4):
+        for r, q, qb, out, want, g in runs[::1 if i % 2 else -1]:
+            out.upload(np.full(q.size, 3.5, np.float32))
+            g.launch()
+            if i == 2:
+                dev.sync()
+        for r, q, qb, out, want, g in runs:
+            np.testing.assert_array_equal(bits(out.download(np.float32, q.size)), bits(want.ravel()))
+            np.testing.assert_array_equal(bits(r.run(q, 4)), bits(want))
+    for r, q, qb, out, want, g in runs:
+        g.free()
+        qb.free()
+        out.free()
+        r.free()
+
+
 def test_attention_of_scores_of_every_size(dev):
     """keys and scales that put most of a row's weight on few keys, or on one: the weights' reference moves"""
     for std, scale in ((8.0, SCALE), (1.0, 1.0), (30.0, 0.3), (1.0, -0.2), (1e-3, 1e-3), (1.0, 0.0)):
