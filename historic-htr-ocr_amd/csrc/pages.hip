@@ -16,7 +16,7 @@
 
 namespace {
 
-// A thread a read: one workgroup, of 256 threads for up to 256 reads and 1024 rows (24 reads of a token 3.6 µs, by 1024 threads
+// A thread a read: one workgroup, of 256 threads for up to 256 reads and 1024 rows (24 reads of a token 4.0 µs, by 1024 threads
 // 4.4), else of 1024. Up to 4096 rows it maps the rows too, more are a second launch's.
 constexpr int SMALL = 256, SMALL_ROWS = 1024, ROWS_ONE = 4096;
 constexpr int AT_ONCE = 4;  // searches of a thread beside each other: each is ten LDS reads behind one another

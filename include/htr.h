@@ -269,8 +269,10 @@ int htr_qkv_post_pages(htr_device *dev, const float *d_q, size_t q_stride, const
                        int n_head, float eps, const htr_kv *kv, float *d_q_out);
 /* attention of a step's rows: read b's i-th new row over the read's rows 0 … d_past[b] + i → d_out [n_row][n_head·128], zeros
  * for the rows of a read that is not served, the rows behind the last read left as they were. Rows past the table's width are
- * not there. Otherwise as htr_tree_attention (what a row does not see, what it holds its numbers to). Reads pages->d_start,
- * d_past and d_table. */
+ * not there. Otherwise as htr_tree_attention in what a row does not see and in what numbers are held to; the same call gives
+ * the same bits every time, while a read's last bits depend on the reads beside it (their lengths say where its keys are shared
+ * out). Scratch: two workgroups a CU for each of two heights of tile, 86 MB on 256 CUs, the same for every call, made at the
+ * first one, which cannot be one that is being captured. Reads pages->d_start, d_past and d_table. */
 int htr_page_attention(htr_device *dev, const float *d_q, size_t q_stride, const htr_pages *pages, const htr_kv *kv, int n_head,
                        float scale, float *d_out);
 /* the GPU token choice of a greedy preset on n_vocab logits (choose_pen → choose_max → choose_pick,
@@ -291,7 +293,8 @@ int htr_choose_many(htr_device *dev, float *d_logits, int n_vocab, int n, uint32
  * softmax(logits) as they are: of htr_choose's penalised ones those after the penalty. A logit of −∞ has no weight; a row of
  * nothing else has log probabilities of −∞ and entropy 0; a NaN or +∞ makes a row's log probabilities and entropy NaN, and its
  * alternatives keep their order, a NaN behind −∞. f32 throughout; pointers 4-byte aligned, the outputs apart from each other
- * and the inputs. */
+ * and the inputs. Scratch: under 1 MB, the same for every call, made at the first one of so few rows that a row is shared out,
+ * which cannot be one that is being captured. */
 enum { HTR_TOP_MAX = 32 };
 int htr_token_logprobs(htr_device *dev, const float *d_logits, size_t stride, int n, int n_vocab, const int32_t *d_ids,
                        float *d_logprob, float *d_entropy, int n_top, int32_t *d_top_ids, float *d_top_logprob);
