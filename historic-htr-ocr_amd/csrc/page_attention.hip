@@ -72,6 +72,9 @@ __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
 // row r's query
 __device__ __forceinline__ int query_of(const Args &a, int r) { return a.group == 1 ? r : (int)__umulhi((uint32_t)r, a.per_group); }
 
+// the blocks of the keys 0 … last (−1: none; last + 32 passes 31 bits)
+__device__ __forceinline__ int blocks_to(int last) { return (int)(((uint32_t)last + KB) / KB); }
+
 // 64 reads of the line of work at hand, in LDS
 struct Reads {
     int64_t end[64];                 // the line's length up to and with each
@@ -102,7 +105,7 @@ template <bool W> struct Line {
         while (i + 1 < a.pieces && cut(i + 1) <= x) i++;
         return uniform(i);
     }
-    __device__ __forceinline__ int64_t step(int past) const { return (int64_t)(W ? a.group : 1) * (max(past, 0) + COST); }
+    __device__ __forceinline__ int64_t step(int past) const { return (int64_t)(W ? a.group : 1) * (max(past, 0) + (int64_t)COST); }
     // the reads from `first` on; their end on the line
     __device__ __forceinline__ int64_t load() {
         const int lane = threadIdx.x & 63, b = first + lane;
@@ -153,7 +156,7 @@ template <bool W> struct Tile {
     __device__ __forceinline__ void measure(const Line<W> &w) {
         len = w.step(past) + (W ? min(WIDE * (tau + 1), rows) : n);
         last = W ? last_of(w.a, WIDE * (tau + 1) - 1) : last_key(w.a, n - 1);
-        nb = (last + KB) / KB;
+        nb = blocks_to(last);
     }
     // the block that place x of the line (begin < x < begin + len) cuts the tile in front of; 0 and nb: it does not
     __device__ __forceinline__ int block_at(const Line<W> &w, int64_t x) const {
@@ -610,7 +613,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
             const int i0 = own.i0, n_st = own.i1 - i0;
             const int r0 = WIDE * t.tau + KB * wave, r = r0 + c, rc = min(r, t.rows - 1);
             const int all_to = (t.last_of(a, r0) + 1) / KB;                              // blocks that all of the wave's rows see the whole of
-            const int any_to = r0 < t.rows ? (t.last_of(a, r0 + KB - 1) + KB) / KB : 0;  // blocks that one of them sees
+            const int any_to = r0 < t.rows ? blocks_to(t.last_of(a, r0 + KB - 1)) : 0;  // blocks that one of them sees
             const int keys = t.last_key(a, query_of(a, rc)) + 1;                         // keys that the lane's row sees
             Run run = run_of(a, line, t, i0, 1);
             if (n_st > 0) run.fetch(0);
@@ -926,6 +929,9 @@ extern "C" int htr_page_attention(htr_device *dev, const float *d_q, size_t q_st
         if (htr_overlap(r.p, r.n, d_out, 4 * qd * n)) return htr_fail("%s: the output overlaps the pages' arrays", me);
     const uint64_t group = (uint64_t)(n_head / kv->n_kv);  // (rows · group < 2^32: the kernel's quotients)
     if (n * group * group >= 1ull << 32 || n * group > 1u << 30) return htr_fail("%s: %zu rows of %d heads", me, n, n_head);
+    const double rows = (double)(n * group), held = (double)a.p.max_pages * pages->page;  // (a line's length, whatever the arrays hold)
+    if (a.p.n_seq * (rows / WIDE + 2) * group * (held + rows + COST) >= 0x1p62)
+        return htr_fail("%s: %d reads of %zu rows of %d heads over up to %.0f rows", me, a.p.n_seq, n, n_head, held);
     HTR_TRY(htr_check_alive(dev));
     const HtrOnDevice on(dev);
     a.q = d_q, a.q_stride = q_stride, a.out = d_out, a.n_head = n_head, a.group = n_head / kv->n_kv;

@@ -137,6 +137,14 @@ def test_logprobs(change, match):
     refused(score(**change), match)
 
 
+@pytest.mark.parametrize("n_row,n_head,n_seq,page,max_pages,match", [
+    (2 ** 21, 46, 1, 16, 5, "2097152 rows of 46 heads"), (2 ** 16, 256, 1, 16, 5, "65536 rows of 256 heads"),
+    (2 ** 21, 16, 1024, 1024, 2 ** 21 - 1, "1024 reads of 2097152 rows of 16 heads over up to 2147482624 rows")])
+def test_attention_of_more_than_is_counted(n_row, n_head, n_seq, page, max_pages, match):
+    p = pages(n_seq, n_row, page, max_pages, start=1 << 50, past=1 << 51, table=1 << 52)
+    refused(attend(p=p, c=kv(n_kv=1, n_ctx=2048), q=1 << 46, qs=n_head * 128, n_head=n_head, out=1 << 48), match)
+
+
 def test_python_sizes():
     class Ref:
         ptr = M

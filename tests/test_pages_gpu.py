@@ -485,6 +485,30 @@ def test_attention_over_a_long_cache(dev):
         b.free()
 
 
+@pytest.mark.parametrize("q8_0", [False, True], ids=["f16", "q8_0"])
+@pytest.mark.parametrize("n_row", [1, 40])
+def test_attention_up_to_the_last_row_that_is_counted(dev, q8_0, n_row):
+    """a table of 2^27 − 1 pages of 16 rows of which the first and the last two are there, and rows whose keys end at 2^31 − 17, the
+    last that it has room for"""
+    page, max_pages = 16, 2 ** 27 - 1
+    table = np.full(max_pages, -1, np.int32)
+    table[0], table[-2], table[-1] = 1, 2, 0
+    past = max_pages * page - n_row
+    c = Cache(dev, normal(9, 1, 48, 128).astype(np.float16), normal(10, 1, 48, 128, std=4.0).astype(np.float16), q8_0)
+    arrays = [dev.upload(np.array(a, np.int32)) for a in ([0, n_row], [past], table)]
+    q = normal(3, n_row, 1, 128)
+    qb, out = dev.upload(q), dev.alloc(q.nbytes)
+    htr.page_attention(dev, qb, htr.Pages.of(1, n_row, page, max_pages, *arrays), c.kv, 1, SCALE, out)
+    got = out.download(np.float32, q.size).reshape(n_row, 128)
+    rows = np.concatenate([np.arange(16, 48), np.arange(16)])
+    at = np.concatenate([np.arange(16), np.arange(max_pages * page - 32, max_pages * page)])
+    seen = at[None, :] <= past + np.arange(n_row)[:, None]
+    assert rel_rows(got, attention(q, c.k[:, rows], c.v[:, rows], seen, SCALE)) < BAR
+    for b in (*arrays, qb, out):
+        b.free()
+    c.free()
+
+
 # ---- the operators together -----------------------------------------------------------------------------------------------
 
 def _loop(dev, q8_0, replay):
