@@ -593,3 +593,58 @@ def test_freed_pages_are_refused(dev):
     with pytest.raises(htr.HtrError, match="null start"):
         htr.page_map(dev, p, 1, b, b, b, b, b, b)
     b.free()
+
+
+@pytest.fixture(scope="module")
+def poisoned():
+    """another device handle on the same GPU, with a stream and scratch of its own, whose memory starts as NaN"""
+    with pytest.MonkeyPatch.context() as env:
+        env.setenv("HTR_POISON", "1")
+        d = htr.Device(0)
+    yield d
+    d.close()
+
+
+def test_two_devices_at_once(dev, poisoned):
+    """calls of two handles that overlap, eager and replayed, each with tiles and rows in parts: the bits of either alone, where
+    scratch was NaN before its first use too"""
+    reads, n_head, vocab, top = [(2500, 1), (300, 140), (4000, 1), (-1, 2)], 4, 151936, 7
+    logits = normal(4, 3, vocab, std=2.5)
+    sides = []
+    for d in (dev, poisoned):
+        r = Reads(d, reads, 32, 2, seed=6)
+        q = normal(8, r.n, n_head, 128)
+        b = [d.upload(a) for a in (q, logits, np.array([5, 70000, vocab - 1], np.int32))]
+        out = [d.alloc(4 * n) for n in (q.size, 3, 3, 3 * top, 3 * top)]
+
+        def call(d=d, r=r, b=b, out=out):
+            htr.page_attention(d, b[0], r.pages, r.cache.kv, n_head, SCALE, out[0])
+            htr.token_logprobs(d, b[1], 3, vocab, b[2], out[1], out[2], top, out[3], out[4])
+
+        sides.append((d, r, q, b, out, call))
+    want = []
+    for d, r, q, b, out, call in sides:
+        call()
+        want.append([o.download(np.uint32, o.nbytes // 4) for o in out])
+    for x, y in zip(*want):
+        np.testing.assert_array_equal(x, y)
+    d, r, q, *_ = sides[0]
+    assert rel_rows(want[0][0].view(np.float32).reshape(r.n, -1), r.want(q, SCALE)) < BAR
+    graphs = []
+    for d, r, q, b, out, call in sides:
+        d.capture_begin()
+        call()
+        graphs.append(d.capture_end())
+    for i in range(6):
+        for (d, r, q, b, out, call), g in zip(sides, graphs):
+            for _ in range(4):
+                g.launch() if i % 2 else call()
+        for d, r, q, b, out, call in sides:
+            for o, w in zip(out, want[0]):
+                np.testing.assert_array_equal(o.download(np.uint32, w.size), w)
+    for g in graphs:
+        g.free()
+    for d, r, q, b, out, call in sides:
+        for o in (*b, *out):
+            o.free()
+        r.free()
