@@ -278,6 +278,7 @@ __device__ __forceinline__ void lds_load4_at(const void *p, uint32_t lds) {
 }
 
 constexpr int WAVE_F16 = TILE, WAVE_Q8 = 2 * QT + 16;  // 16-byte chunks of a wave's LDS: K and V of a block; two raw ones
+constexpr int RAW = 1024 + 1024 + 256;                 // bytes of 8 raw rows: K, V, their scales (64 + 64, twice)
 struct Shared {
     Reads reads[PW];  // (each wave its own: nobody waits)
     float ml[PW][2][KB];
@@ -561,7 +562,8 @@ template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh
 // ---- reads of many rows ------------------------------------------------------------------------------------------------------
 //
 // Bound: the matrix cores and their power: four chunks of 2000 over 8000 keys (590 GFLOP, as pairs twice that) 1.05 ms, 1.12
-// PFLOP/s, where a library f16 product of 8192³ reaches 1.14; four prompts of 1925 (121 GFLOP as pairs) 158 µs, of which 9 % of
+// PFLOP/s, where a library f16 product of 8192³ reaches 1.14, over q8_0 rows 1.15 ms (with a block's quants in registers until they
+// are made f16, 56 of them spilled, 2.06); four prompts of 1925 (121 GFLOP as pairs) 158 µs, of which 9 % of
 // the products are of keys past a row's own, 13 µs the second launch, 20 that workgroups wait for the last. Loads four stages
 // ahead or one, and a barrier a stage or every second one, take the same time.
 template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, int piece, uint4_t *s_kv, Shared &sh) {
@@ -574,9 +576,10 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
 
     // K and V of a block as f16, K a block ahead of V: the next block's scores are computed under this one's softmax (the layouts
     // are k_kv_attn's). f16 rows: four buffers, filled two at a time, behind every second barrier; a wave loads 4 rows of each half
-    // straight into LDS. q8_0 rows: two buffers; a thread loads 16 quants of a row into registers and makes them f16 a block later
+    // straight into LDS. q8_0 rows: two buffers, and four raw ones of each wave's own, which has 8 rows of a block: loaded straight
+    // into LDS four blocks ahead, and made f16 by the wave that loaded them, K two blocks and V one before they are used
     char *stage = reinterpret_cast<char *>(s_kv);
-    const uint32_t slds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)stage + 16u * 64 * wave;
+    const uint32_t slds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)stage, slds = slds0 + 16u * 64 * wave;
     const int lrow = Q8 ? 8 * wave + (lane >> 3) : 4 * wave + (lane >> 4), lc = Q8 ? lane & 7 : lane & 15;
     const uint32_t koff = 2 * D * lrow + 16 * (lc ^ (lrow & 15)), voff = 2 * D * lrow + 16 * (lc ^ (4 * (lrow & 3)));  // the same for row lrow + 16
     auto issue = [&](const Rows &x, int b, bool is_v) {
@@ -585,22 +588,22 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
             lds_load16((const char *)(is_v ? a.kv.v : a.kv.k) + (head0 + x.at[h]) * (2 * D), is_v ? voff : koff,
                        slds + 16u * (b * TILE + (is_v ? K_CHUNKS : 0) + 256 * h));
     };
-    struct Raw {
-        uint4_t q;
-        uint16_t d;
+    const int raw0 = 16 * 2 * TILE + RAW * 4 * wave;
+    auto issue_q8 = [&](const Rows &x, int slot) {
+        const size_t row = head0 + uniform(wave & 2 ? x.at[1] : x.at[0]) + 8 * (wave & 1);
+        const uint32_t to = slds0 + raw0 + RAW * slot;
+        lds_load16((const char *)a.kv.k + row * D, 16 * lane, to);
+        lds_load16((const char *)a.kv.v + row * D, 16 * lane, to + 1024);
+        lds_load4_at((const char *)(lane & 16 ? a.kv.vd : a.kv.kd) + row * 8 + 4 * (lane & 15), to + 2048);  // a row's scales are 8 bytes
     };
-    auto fetch = [&](const Rows &x, bool is_v) {
-        const size_t row = head0 + x.at[wave >> 1] + (lrow & 15);
-        return Raw{*reinterpret_cast<const uint4_t *>((const char *)(is_v ? a.kv.v : a.kv.k) + row * D + 16 * lc),
-                   (is_v ? a.kv.vd : a.kv.kd)[row * 4 + (lc >> 1)]};
-    };
-    auto commit = [&](const Raw &x, int b, bool is_v) {
-        _Float16 d;
-        __builtin_memcpy(&d, &x.d, 2);
+    auto commit = [&](int slot, int b, bool is_v) {
+        const char *from = stage + raw0 + RAW * slot;
+        const uint4_t q = *reinterpret_cast<const uint4_t *>(from + (is_v ? 1024 : 0) + 16 * lane);
+        const _Float16 d = *reinterpret_cast<const _Float16 *>(from + 2048 + (is_v ? 64 : 0) + 8 * (lane >> 3) + 2 * (lc >> 1));
         const int swz = is_v ? 4 * (lrow & 3) : lrow & 15;
         uint4_t *to = s_kv + b * TILE + (is_v ? K_CHUNKS : 0) + 16 * lrow;
-        *reinterpret_cast<half8 *>(to + ((2 * lc) ^ swz)) = dequant8(x.q[0], x.q[1], half2_t{d, d});
-        *reinterpret_cast<half8 *>(to + ((2 * lc + 1) ^ swz)) = dequant8(x.q[2], x.q[3], half2_t{d, d});
+        *reinterpret_cast<half8 *>(to + ((2 * lc) ^ swz)) = dequant8(q[0], q[1], half2_t{d, d});
+        *reinterpret_cast<half8 *>(to + ((2 * lc + 1) ^ swz)) = dequant8(q[2], q[3], half2_t{d, d});
     };
     // the lane's bytes of a block: K's step ks at k_at ^ 32·ks (chunk 2ks + hf of row c), V's tile u at v_at ^ 64·u
     const int vrow = 4 * hf + ((lane & 15) >> 2);
@@ -622,17 +625,18 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
             half8 qh[8], ql[8];
             float sc;
             size_t part = 0;
-            Rows r_now{{0, 0}, 0}, r_next{{0, 0}, 0};  // q8_0: of this stage and the next one
-            Raw k_raw{}, v_raw{};                      // and the stage after the next one's K, the next one's V
             {
                 float qx[8][8];
                 q_load<8>(q_row(a, t.start, kvh, rc) + 8 * hf, qx);
                 __syncthreads();  // (the tile before is done with the buffers)
                 if constexpr (Q8) {
-                    if (n_st > 0) r_now = run.of(0);
-                    if (n_st > 1) r_next = run.of(1);
-                    if (n_st > 0) commit(fetch(r_now, false), 0, false), commit(fetch(r_now, true), 0, true);
-                    if (n_st > 1) commit(fetch(r_next, false), 1, false), v_raw = fetch(r_next, true);
+                    if (n_st > 0)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const Rows x = run.of(min(e, n_st - 1));
+                            gone |= x.bad << (2 * e);
+                            issue_q8(x, e);
+                        }
                 } else {
                     if (n_st > 0) {
                         const Rows one = run.of(0), two = run.of(min(1, n_st - 1));
@@ -645,9 +649,10 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                 if (!own.all) part = part_of(line, t, own, kvh, piece);
                 sc = q_split<8, 2>(qx, a.scale, qh, ql);
             }
-            Rows r_third{{0, 0}, 0};                   // of the stage whose K is in k_raw
-            if constexpr (Q8)
-                if (n_st > 2) r_third = run.of(2), k_raw = fetch(r_third, false);
+            if constexpr (Q8) {
+                wait_loads<0>();
+                commit(0, 0, false), commit(0, 0, true), commit(1, 1, false);
+            }
             float m = M_NONE, l = 0.0f;
             f32x16 o[4];
 #pragma unroll
@@ -661,19 +666,18 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                 // this wave's loads of K stage st + 1 and V stage st (f16: of the stages after them too) are in, its reads of K stage
                 // st and V stage st − 1 have their values; behind the barrier everyone's, and the buffers are free
                 if (Q8 || (st & 1) == 0) {
-                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    if constexpr (Q8) asm volatile("s_waitcnt vmcnt(3) lgkmcnt(0)" ::: "memory");
+                    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                     __builtin_amdgcn_s_barrier();
                     asm volatile("" ::: "memory");
                 }
-                const uint32_t bad = Q8 ? r_now.bad : gone & 3u;
-                if constexpr (Q8) {
-                    r_now = r_next, r_next = r_third;
-                    if (st + 2 < n_st) commit(k_raw, b, false);
-                    if (st + 1 < n_st) commit(v_raw, b ^ 1, true);
-                    if (st + 3 < n_st) r_third = run.of(st + 3), k_raw = fetch(r_third, false);
-                    if (st + 2 < n_st) v_raw = fetch(r_next, true);
-                } else {  // (past the last stage: its loads once more)
-                    if ((st & 1) == 0) {
+                const uint32_t bad = gone & 3u;
+                {  // (past the last stage: its loads once more)
+                    if constexpr (Q8) {
+                        const Rows four = run.of(min(st + 4, n_st - 1));
+                        gone |= four.bad << 8;
+                        issue_q8(four, st & 3);
+                    } else if ((st & 1) == 0) {
                         const Rows three = run.of(min(st + 3, n_st - 1)), four = run.of(min(st + 4, n_st - 1));
                         gone |= three.bad << 6 | four.bad << 8;
                         issue(three, (st + 3) & 3, false), issue(four, st & 3, false);
@@ -682,9 +686,15 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                     }
                     gone >>= 2;
                 }
+                auto convert = [&] {
+                    if constexpr (Q8) commit((st + 2) & 3, b, false), commit((st + 1) & 3, b ^ 1, true);
+                };
                 const int i = i0 + st;
                 if constexpr (MASK)
-                    if (i >= any_to) return;
+                    if (i >= any_to) {
+                        convert();
+                        return;
+                    }
                 uint32_t seen = 0;
                 if constexpr (MASK) {
                     seen = sees(keys, i, hf, bad);
@@ -745,6 +755,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                 }
                 v[3] = vread(3, 0);
                 l += ls;
+                convert();
                 bool odd = false;
                 if constexpr (MASK) {
                     uint32_t top = 0;
@@ -786,7 +797,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
             }
             // two stages at a time, both kinds of step passing one barrier a stage: a wave's blocks may be masked where another's
             // are not
-            auto whole2 = [&](int st) { return st + 1 < n_st && i0 + st + 1 < all_to && (Q8 ? r_now.bad | r_next.bad : gone & 15u) == 0; };
+            auto whole2 = [&](int st) { return st + 1 < n_st && i0 + st + 1 < all_to && (gone & 15u) == 0; };
             for (int st = 0; st < n_st;) {
                 for (; whole2(st); st += 2) {
                     step(st, 0, s0, s1, std::false_type{});
@@ -824,6 +835,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
 // the workgroups of wide tiles, then those of narrow ones
 template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_attn(Args a) {
     __shared__ __attribute__((aligned(16))) uint4_t s_kv[PW * (Q8 ? WAVE_Q8 : WAVE_F16)];
+    static_assert(!Q8 || 16 * PW * WAVE_Q8 >= 16 * 2 * TILE + 4 * RAW * PW, "the wide tiles' buffers fit");
     __shared__ Shared sh;
     const int kvh = blockIdx.x % a.kv.n_kv, piece = blockIdx.x / a.kv.n_kv;
     if (piece < a.wide) wide<Q8>(a, kvh, piece, s_kv, sh);
