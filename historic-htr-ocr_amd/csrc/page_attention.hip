@@ -561,11 +561,12 @@ template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh
 
 // ---- reads of many rows ------------------------------------------------------------------------------------------------------
 //
-// Bound: the matrix cores and their power: four chunks of 2000 over 8000 keys (590 GFLOP, as pairs twice that) 1.05 ms, 1.12
-// PFLOP/s, where a library f16 product of 8192³ reaches 1.14, over q8_0 rows 1.15 ms (with a block's quants in registers until they
-// are made f16, 56 of them spilled, 2.06); four prompts of 1925 (121 GFLOP as pairs) 158 µs, of which 9 % of
-// the products are of keys past a row's own, 13 µs the second launch, 20 that workgroups wait for the last. Loads four stages
-// ahead or one, and a barrier a stage or every second one, take the same time.
+// Bound: the matrix cores and their power: four chunks of 2000 over 8000 keys (590 GFLOP, as pairs twice that) 1.025 ms, 1.15
+// PFLOP/s, where a library f16 product of 8192³ reaches 1.14, over q8_0 rows 1.15 ms (with a block's quants in registers until
+// they are made f16, 56 registers spilled, 2.06); four prompts of 1925 (121 GFLOP as pairs) 158 µs, of which 9 % of the products
+// are of keys past a row's own, 13 µs the second launch, 20 that workgroups wait for the last. Of two waves on a SIMD the one at
+// its scores goes first (without 1.046 ms; the one at its values first 1.043). Loads four stages ahead or one, and a barrier a
+// stage or every second one, take the same time.
 template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, int piece, uint4_t *s_kv, Shared &sh) {
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), hf = lane >> 5, c = lane & 31;
     if (a.pieces > 1) no_parts<true>(a, kvh, piece);
@@ -756,6 +757,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                 v[3] = vread(3, 0);
                 l += ls;
                 convert();
+                __builtin_amdgcn_s_setprio(0);
                 bool odd = false;
                 if constexpr (MASK) {
                     uint32_t top = 0;
@@ -781,6 +783,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                         if (ss == 0) v[u] = vn[u];
                     }
                 }
+                __builtin_amdgcn_s_setprio(1);  // (scores before a neighbour's values)
                 if constexpr (MASK)
                     if (odd) put_nan(o, seen, vread);
             };
