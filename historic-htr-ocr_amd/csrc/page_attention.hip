@@ -220,7 +220,7 @@ template <bool W> __device__ __forceinline__ Share share_of(const Line<W> &w, co
 template <bool W> __device__ __forceinline__ size_t part_of(const Line<W> &w, const Tile<W> &t, const Share &share, int kvh, int piece) {
     int first = w.piece_of(t.begin), end = first + 1;
     if (w.cut(end) < t.begin + t.len && t.block_at(w, w.cut(end)) == 0) first++, end++;  // (it leaves the beginning to the next one)
-    while (end < w.a.pieces && w.cut(end) < t.begin + t.len && t.block_at(w, w.cut(end)) < t.nb) end++;
+    for (end = max(w.piece_of(t.begin + t.len - 1) + 1, end); end - 1 > first && t.block_at(w, w.cut(end - 1)) == t.nb;) end--;
     const size_t place = ((size_t)kvh * w.a.pieces + piece) * 2 + (share.i0 == 0);
     if (threadIdx.x == 0) w.a.part[W].of[place] = W ? Part{first, end - first, t.start, WIDE * t.tau, min(WIDE, t.rows - WIDE * t.tau)}
                                                     : Part{first, end - first, t.start, t.r0, t.rows};
@@ -568,52 +568,54 @@ template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh
 // its scores goes first (without 1.046 ms; the one at its values first 1.043). Loads four stages ahead or one, and a barrier a
 // stage or every second one, take the same time.
 template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, int piece, uint4_t *s_kv, Shared &sh) {
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), hf = lane >> 5, c = lane & 31;
+    const int wave = uniform(threadIdx.x >> 6);
     if (a.pieces > 1) no_parts<true>(a, kvh, piece);
     Line<true> line(a, sh.reads[wave]);
     const int64_t x0 = line.cut(piece), x1 = line.cut(piece + 1);
     if (x0 >= x1) return;
     const size_t head0 = (size_t)kvh * a.kv.n_ctx;
 
-    // K and V of a block as f16, K a block ahead of V: the next block's scores are computed under this one's softmax (the layouts
-    // are k_kv_attn's). f16 rows: four buffers, filled two at a time, behind every second barrier; a wave loads 4 rows of each half
-    // straight into LDS. q8_0 rows: two buffers, and four raw ones of each wave's own, which has 8 rows of a block: loaded straight
-    // into LDS four blocks ahead, and made f16 by the wave that loaded them, K two blocks and V one before they are used
-    char *stage = reinterpret_cast<char *>(s_kv);
-    const uint32_t slds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)stage, slds = slds0 + 16u * 64 * wave;
-    const int lrow = Q8 ? 8 * wave + (lane >> 3) : 4 * wave + (lane >> 4), lc = Q8 ? lane & 7 : lane & 15;
-    const uint32_t koff = 2 * D * lrow + 16 * (lc ^ (lrow & 15)), voff = 2 * D * lrow + 16 * (lc ^ (4 * (lrow & 3)));  // the same for row lrow + 16
-    auto issue = [&](const Rows &x, int b, bool is_v) {
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-            lds_load16((const char *)(is_v ? a.kv.v : a.kv.k) + (head0 + x.at[h]) * (2 * D), is_v ? voff : koff,
-                       slds + 16u * (b * TILE + (is_v ? K_CHUNKS : 0) + 256 * h));
-    };
-    const int raw0 = 16 * 2 * TILE + RAW * 4 * wave;
-    auto issue_q8 = [&](const Rows &x, int slot) {
-        const size_t row = head0 + uniform(wave & 2 ? x.at[1] : x.at[0]) + 8 * (wave & 1);
-        const uint32_t to = slds0 + raw0 + RAW * slot;
-        lds_load16((const char *)a.kv.k + row * D, 16 * lane, to);
-        lds_load16((const char *)a.kv.v + row * D, 16 * lane, to + 1024);
-        lds_load4_at((const char *)(lane & 16 ? a.kv.vd : a.kv.kd) + row * 8 + 4 * (lane & 15), to + 2048);  // a row's scales are 8 bytes
-    };
-    auto commit = [&](int slot, int b, bool is_v) {
-        const char *from = stage + raw0 + RAW * slot;
-        const uint4_t q = *reinterpret_cast<const uint4_t *>(from + (is_v ? 1024 : 0) + 16 * lane);
-        const _Float16 d = *reinterpret_cast<const _Float16 *>(from + 2048 + (is_v ? 64 : 0) + 8 * (lane >> 3) + 2 * (lc >> 1));
-        const int swz = is_v ? 4 * (lrow & 3) : lrow & 15;
-        uint4_t *to = s_kv + b * TILE + (is_v ? K_CHUNKS : 0) + 16 * lrow;
-        *reinterpret_cast<half8 *>(to + ((2 * lc) ^ swz)) = dequant8(q[0], q[1], half2_t{d, d});
-        *reinterpret_cast<half8 *>(to + ((2 * lc + 1) ^ swz)) = dequant8(q[2], q[3], half2_t{d, d});
-    };
-    // the lane's bytes of a block: K's step ks at k_at ^ 32·ks (chunk 2ks + hf of row c), V's tile u at v_at ^ 64·u
-    const int vrow = 4 * hf + ((lane & 15) >> 2);
-    const int k_at = 16 * (16 * c + (hf ^ (c & 15)));
-    const int v_at = 16 * (K_CHUNKS + 16 * vrow + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (4 * (vrow & 3)))) + 8 * (lane & 1);
-
     for (Tile<true> t(line, x0);; t.next(line)) {
         const Share own = share_of(line, t, x0, x1);
         if (own.i0 < own.i1 || own.all) {
+            // (worked out anew for each tile: kept beside the loop they take registers from it)
+            const int lane = here(threadIdx.x & 63), hf = lane >> 5, c = lane & 31;
+            // K and V of a block as f16, K a block ahead of V: the next block's scores are computed under this one's softmax (the layouts
+            // are k_kv_attn's). f16 rows: four buffers, filled two at a time, behind every second barrier; a wave loads 4 rows of each half
+            // straight into LDS. q8_0 rows: two buffers, and four raw ones of each wave's own, which has 8 rows of a block: loaded straight
+            // into LDS four blocks ahead, and made f16 by the wave that loaded them, K two blocks and V one before they are used
+            char *stage = reinterpret_cast<char *>(s_kv);
+            const uint32_t slds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)stage, slds = slds0 + 16u * 64 * wave;
+            const int lrow = Q8 ? 8 * wave + (lane >> 3) : 4 * wave + (lane >> 4), lc = Q8 ? lane & 7 : lane & 15;
+            const uint32_t koff = 2 * D * lrow + 16 * (lc ^ (lrow & 15)), voff = 2 * D * lrow + 16 * (lc ^ (4 * (lrow & 3)));  // the same for row lrow + 16
+            auto issue = [&](const Rows &x, int b, bool is_v) {
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    lds_load16((const char *)(is_v ? a.kv.v : a.kv.k) + (head0 + x.at[h]) * (2 * D), is_v ? voff : koff,
+                               slds + 16u * (b * TILE + (is_v ? K_CHUNKS : 0) + 256 * h));
+            };
+            const int raw0 = 16 * 2 * TILE + RAW * 4 * wave;
+            auto issue_q8 = [&](const Rows &x, int slot) {
+                const size_t row = head0 + uniform(wave & 2 ? x.at[1] : x.at[0]) + 8 * (wave & 1);
+                const uint32_t to = slds0 + raw0 + RAW * slot;
+                lds_load16((const char *)a.kv.k + row * D, 16 * lane, to);
+                lds_load16((const char *)a.kv.v + row * D, 16 * lane, to + 1024);
+                lds_load4_at((const char *)(lane & 16 ? a.kv.vd : a.kv.kd) + row * 8 + 4 * (lane & 15), to + 2048);  // a row's scales are 8 bytes
+            };
+            // the lane's bytes: 16 raw quants, their scale, and two f16 chunks of K and of V (the other one at ^ 16)
+            const int c_raw = raw0 + 16 * lane, c_d = raw0 + 2048 + 8 * (lane >> 3) + 2 * (lc >> 1);
+            const int c_k = 16 * (16 * lrow + ((2 * lc) ^ (lrow & 15))), c_v = 16 * (K_CHUNKS + 16 * lrow + ((2 * lc) ^ (4 * (lrow & 3))));
+            auto commit = [&](int slot, int b, bool is_v) {
+                const uint4_t q = *reinterpret_cast<const uint4_t *>(stage + here(c_raw) + RAW * slot + (is_v ? 1024 : 0));
+                const _Float16 d = *reinterpret_cast<const _Float16 *>(stage + here(c_d) + RAW * slot + (is_v ? 64 : 0));
+                const int to = here(is_v ? c_v : c_k);
+                *reinterpret_cast<half8 *>(stage + to + 16 * TILE * b) = dequant8(q[0], q[1], half2_t{d, d});
+                *reinterpret_cast<half8 *>(stage + (to ^ 16) + 16 * TILE * b) = dequant8(q[2], q[3], half2_t{d, d});
+            };
+            // the lane's bytes of a block: K's step ks at k_at ^ 32·ks (chunk 2ks + hf of row c), V's tile u at v_at ^ 64·u
+            const int vrow = 4 * hf + ((lane & 15) >> 2);
+            const int k_at = 16 * (16 * c + (hf ^ (c & 15)));
+            const int v_at = 16 * (K_CHUNKS + 16 * vrow + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (4 * (vrow & 3)))) + 8 * (lane & 1);
             const int i0 = own.i0, n_st = own.i1 - i0;
             const int r0 = WIDE * t.tau + KB * wave, r = r0 + c, rc = min(r, t.rows - 1);
             const int all_to = (t.last_of(a, r0) + 1) / KB;                              // blocks that all of the wave's rows see the whole of
