@@ -55,7 +55,7 @@ struct Args {
     HtrKvPlanes kv;
     HtrPages p;
     int n_head, group;
-    uint32_t per_group;  // ⌈2^32 / group⌉ (group > 1): the quotient of a row below 2^32 / group by one product
+    uint32_t per_group;  // ⌈2^31 / group⌉: the quotient of a row below 2^31 / group by one product
     int n_page, cap;     // the cache's pages; the rows that the table has room for
     float scale;
     int pieces;          // workgroups of a KV head and height
@@ -69,8 +69,10 @@ __device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
     const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
     return (int64_t)((uint64_t)hi << 32 | lo);
 }
+__device__ __forceinline__ int64_t uniform(int64_t v) { return lane_of(v, 0); }
+__device__ __forceinline__ int lane_id() { return here(threadIdx.x & 63); }  // (here: what is made of it is not kept in registers for later)
 // row r's query
-__device__ __forceinline__ int query_of(const Args &a, int r) { return a.group == 1 ? r : (int)__umulhi((uint32_t)r, a.per_group); }
+__device__ __forceinline__ int query_of(const Args &a, int r) { return (int)__umulhi(2u * (uint32_t)r, a.per_group); }
 
 // the blocks of the keys 0 … last (−1: none; last + 32 passes 31 bits)
 __device__ __forceinline__ int blocks_to(int last) { return (int)(((uint32_t)last + KB) / KB); }
@@ -95,12 +97,13 @@ template <bool W> struct Line {
             first = 0, base = 0;
             load();
         }
-        piece = max((int64_t)((double)total * a.per_piece) + 1, (int64_t)LEAST * (W ? a.group : 1));
+        piece = uniform(max((int64_t)((double)total * a.per_piece) + 1, (int64_t)LEAST * (W ? a.group : 1)));
     }
     // where piece i begins
     __device__ __forceinline__ int64_t cut(int i) const { return i >= a.pieces ? total : min(i * piece, total); }
     __device__ __forceinline__ int piece_of(int64_t x) const {
-        int i = min((int)((double)x / (double)piece), a.pieces - 1);
+        const float each = (float)(int64_t)((uint64_t)(uint32_t)here((int)(piece >> 32)) << 32 | (uint32_t)here((int)piece));
+        int i = min((int)((float)x * __builtin_amdgcn_rcpf(each)), a.pieces - 1);  // (or one beside it)
         while (i > 0 && cut(i) > x) i--;
         while (i + 1 < a.pieces && cut(i + 1) <= x) i++;
         return uniform(i);
@@ -108,7 +111,7 @@ template <bool W> struct Line {
     __device__ __forceinline__ int64_t step(int past) const { return (int64_t)(W ? a.group : 1) * (max(past, 0) + (int64_t)COST); }
     // the reads from `first` on; their end on the line
     __device__ __forceinline__ int64_t load() {
-        const int lane = threadIdx.x & 63, b = first + lane;
+        const int lane = lane_id(), b = first + lane;
         const bool there = b < a.p.n_seq;
         const int s0 = there ? a.p.start[b] : 0, s1 = there ? a.p.start[b + 1] : 0, held = there ? a.p.past[b] : -1;
         const int start = min(max(s0, 0), a.p.n_row), past = min(max(held, -1), a.cap);
@@ -124,8 +127,8 @@ template <bool W> struct Line {
         if (W && end == 0) n = 0;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            const int64_t o = __shfl_up((long long)end, d);
-            if (lane >= d) end += o;
+            const uint32_t lo = __builtin_amdgcn_ds_bpermute(4 * (lane - d), (int)(uint32_t)end), hi = __builtin_amdgcn_ds_bpermute(4 * (lane - d), (int)(end >> 32));
+            if (lane >= d) end += (int64_t)((uint64_t)hi << 32 | lo);
         }
         end += base;
         r.end[lane] = end, r.start[lane] = start, r.n[lane] = n, r.past[lane] = past;
@@ -161,13 +164,13 @@ template <bool W> struct Tile {
     // the block that place x of the line (begin < x < begin + len) cuts the tile in front of; 0 and nb: it does not
     __device__ __forceinline__ int block_at(const Line<W> &w, int64_t x) const {
         const int64_t u = x - begin;
-        const int b = W ? uniform((int)((double)u / (double)(KB * w.a.group))) : (int)(u / KB);
+        const int b = W ? uniform((int)((double)u / (double)here(KB * w.a.group))) : (int)(u / KB);
         return b < SLIVER ? 0 : b > nb - SLIVER ? nb : b;
     }
     // the one that holds place x of the line, x before its end
     __device__ __forceinline__ Tile(Line<W> &w, int64_t x) {
-        int64_t mine = w.r.end[threadIdx.x & 63];
-        for (int64_t t; (t = lane_of(mine, 63)) <= x && w.first + 64 < w.a.p.n_seq; mine = w.r.end[threadIdx.x & 63]) {
+        int64_t mine = w.r.end[lane_id()];
+        for (int64_t t; (t = lane_of(mine, 63)) <= x && w.first + 64 < w.a.p.n_seq; mine = w.r.end[lane_id()]) {
             w.base = t, w.first += 64;
             w.load();
         }
@@ -192,7 +195,7 @@ template <bool W> struct Tile {
         if (!W || WIDE * ++tau >= rows) {
             uint64_t more;
             for (int from = at + 1;; from = 0) {
-                more = from < 64 ? __builtin_amdgcn_ballot_w64(w.r.n[threadIdx.x & 63] > 0) >> from << from : 0;
+                more = from < 64 ? __builtin_amdgcn_ballot_w64(w.r.n[lane_id()] > 0) >> from << from : 0;
                 if (more || w.first + 64 >= w.a.p.n_seq) break;
                 w.base = begin, w.first += 64;
                 w.load();
@@ -216,19 +219,23 @@ template <bool W> __device__ __forceinline__ Share share_of(const Line<W> &w, co
     s.all = s.i0 == 0 && s.i1 == t.nb;
     return s;
 }
-// a piece's place for its part of a cut tile, and which pieces have the others
+// a piece's place for its part of a cut tile, and which pieces have the others (the last wave's work: of few keys it has the least)
 template <bool W> __device__ __forceinline__ size_t part_of(const Line<W> &w, const Tile<W> &t, const Share &share, int kvh, int piece) {
-    int first = w.piece_of(t.begin), end = first + 1;
-    if (w.cut(end) < t.begin + t.len && t.block_at(w, w.cut(end)) == 0) first++, end++;  // (it leaves the beginning to the next one)
-    for (end = max(w.piece_of(t.begin + t.len - 1) + 1, end); end - 1 > first && t.block_at(w, w.cut(end - 1)) == t.nb;) end--;
     const size_t place = ((size_t)kvh * w.a.pieces + piece) * 2 + (share.i0 == 0);
-    if (threadIdx.x == 0) w.a.part[W].of[place] = W ? Part{first, end - first, t.start, WIDE * t.tau, min(WIDE, t.rows - WIDE * t.tau)}
-                                                    : Part{first, end - first, t.start, t.r0, t.rows};
+    if (threadIdx.x >= 64 * (PW - 1)) {
+        int first = w.piece_of(t.begin), end = first + 1;
+        if (w.cut(end) < t.begin + t.len && t.block_at(w, w.cut(end)) == 0) first++, end++;  // (it leaves the beginning to the next one)
+        for (end = max(w.piece_of(t.begin + t.len - 1) + 1, end); end - 1 > first && t.block_at(w, w.cut(end - 1)) == t.nb;) end--;
+        if (threadIdx.x == 64 * (PW - 1))
+            w.a.part[W].of[place] = W ? Part{first, end - first, t.start, WIDE * t.tau, min(WIDE, t.rows - WIDE * t.tau)}
+                                      : Part{first, end - first, t.start, t.r0, t.rows};
+    }
     return place * (W ? WIDE : NARROW);
 }
-// the two places of a piece that has no cut tile are empty
+// the two places of a piece that has no cut tile are empty (the same wave's stores, in order)
 template <bool W> __device__ __forceinline__ void no_parts(const Args &a, int kvh, int piece) {
-    if (threadIdx.x < 2) a.part[W].of[((size_t)kvh * a.pieces + piece) * 2 + threadIdx.x].n = 0;
+    const int k = (int)threadIdx.x - 64 * (PW - 1);
+    if (k >= 0 && k < 2) a.part[W].of[((size_t)kvh * a.pieces + piece) * 2 + k].n = 0;
 }
 __device__ __forceinline__ float *out_row(const Args &a, int start, int kvh, int r) {
     const int i = query_of(a, r);
@@ -251,7 +258,7 @@ struct Run {
     int row;
     uint64_t gone;  // the halves without a page
     __device__ __forceinline__ void fetch(int j) {
-        const int lane = threadIdx.x & 63;
+        const int lane = lane_id();
         const uint32_t key = min(KB * (uint32_t)(b0 + step * (j + (lane >> 1))) + 16u * (lane & 1), (uint32_t)last & ~15u);
         const int page = table[key >> shift];
         const bool bad = (uint32_t)page >= (uint32_t)n_page;
@@ -289,13 +296,13 @@ struct Shared {
 // A wave's block is K and V in its own LDS (layouts and products are k_kv_attn_split's): f16 one buffer each, filled again as soon
 // as it is read, q8_0 raw in two.
 //
-// Bound: of few keys latency (a token over 1300 keys 13.5 µs, of which lengths, pages, keys, each a load that the next one waits
+// Bound: of few keys latency (a token over 1300 keys 12.5 µs, of which lengths, pages, keys, each a load that the next one waits
 // for, 6 µs, and the second launch 4); of many HBM: 64 reads' tokens over 300 … 6000 f16 keys (505 MB) 105 µs, over q8_0 rows
 // (269 MB) 74, at 6.6 TB/s while all workgroups run, which end between 56 and 101 µs.
 template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh, int piece, uint4_t *s_kv, Shared &sh) {
     constexpr int WAVE = Q8 ? WAVE_Q8 : WAVE_F16;
     static_assert(WAVE >= 1024, "a wave's sums fit");
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), hf = lane >> 5, c = lane & 31;
+    const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), hf = lane >> 5, c = lane & 31;
     if (a.pieces > 1) no_parts<false>(a, kvh, piece);
     Line<false> line(a, sh.reads[wave]);
     const int64_t x0 = line.cut(piece), x1 = line.cut(piece + 1);
@@ -562,13 +569,13 @@ template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh
 // ---- reads of many rows ------------------------------------------------------------------------------------------------------
 //
 // Bound: the matrix cores and their power: four chunks of 2000 over 8000 keys (590 GFLOP, as pairs twice that) 1.025 ms, 1.15
-// PFLOP/s, where a library f16 product of 8192³ reaches 1.14, over q8_0 rows 1.15 ms (with a block's quants in registers until
+// PFLOP/s, where a library f16 product of 8192³ reaches 1.14, over q8_0 rows 1.14 ms (with a block's quants in registers until
 // they are made f16, 56 registers spilled, 2.06); four prompts of 1925 (121 GFLOP as pairs) 158 µs, of which 9 % of the products
 // are of keys past a row's own, 13 µs the second launch, 20 that workgroups wait for the last. Of two waves on a SIMD the one at
 // its scores goes first (without 1.046 ms; the one at its values first 1.043). Loads four stages ahead or one, and a barrier a
 // stage or every second one, take the same time.
 template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, int piece, uint4_t *s_kv, Shared &sh) {
-    const int wave = uniform(threadIdx.x >> 6);
+    const int wave = uniform((int)threadIdx.x >> 6);
     if (a.pieces > 1) no_parts<true>(a, kvh, piece);
     Line<true> line(a, sh.reads[wave]);
     const int64_t x0 = line.cut(piece), x1 = line.cut(piece + 1);
@@ -578,8 +585,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
     for (Tile<true> t(line, x0);; t.next(line)) {
         const Share own = share_of(line, t, x0, x1);
         if (own.i0 < own.i1 || own.all) {
-            // (worked out anew for each tile: kept beside the loop they take registers from it)
-            const int lane = here(threadIdx.x & 63), hf = lane >> 5, c = lane & 31;
+            const int lane = lane_id(), hf = lane >> 5, c = lane & 31;
             // K and V of a block as f16, K a block ahead of V: the next block's scores are computed under this one's softmax (the layouts
             // are k_kv_attn's). f16 rows: four buffers, filled two at a time, behind every second barrier; a wave loads 4 rows of each half
             // straight into LDS. q8_0 rows: two buffers, and four raw ones of each wave's own, which has 8 rows of a block: loaded straight
@@ -596,7 +602,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
             };
             const int raw0 = 16 * 2 * TILE + RAW * 4 * wave;
             auto issue_q8 = [&](const Rows &x, int slot) {
-                const size_t row = head0 + uniform(wave & 2 ? x.at[1] : x.at[0]) + 8 * (wave & 1);
+                const size_t row = head0 + x.at[0] + (x.at[1] - x.at[0]) * (wave >> 1) + 8 * (wave & 1);
                 const uint32_t to = slds0 + raw0 + RAW * slot;
                 lds_load16((const char *)a.kv.k + row * D, 16 * lane, to);
                 lds_load16((const char *)a.kv.v + row * D, 16 * lane, to + 1024);
@@ -617,7 +623,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
             const int k_at = 16 * (16 * c + (hf ^ (c & 15)));
             const int v_at = 16 * (K_CHUNKS + 16 * vrow + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (4 * (vrow & 3)))) + 8 * (lane & 1);
             const int i0 = own.i0, n_st = own.i1 - i0;
-            const int r0 = WIDE * t.tau + KB * wave, r = r0 + c, rc = min(r, t.rows - 1);
+            const int r0 = WIDE * t.tau + KB * wave, rc = min(r0 + c, t.rows - 1);
             const int all_to = (t.last_of(a, r0) + 1) / KB;                              // blocks that all of the wave's rows see the whole of
             const int any_to = r0 < t.rows ? blocks_to(t.last_of(a, r0 + KB - 1)) : 0;  // blocks that one of them sees
             const int keys = t.last_key(a, query_of(a, rc)) + 1;                         // keys that the lane's row sees
@@ -816,21 +822,22 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
             l = pair_sum<32>(l);
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (the next tile's loads go over these buffers)
 
+            const int ln = lane_id(), row_of = KB * wave + (ln & 31), r = WIDE * t.tau + row_of, half = ln >> 5;
             const float by = !own.all ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
             float *to;
             if (own.all) {
-                to = out_row(a, t.start, kvh, rc);
+                to = out_row(a, t.start, kvh, min(r, t.rows - 1));
             } else {
-                const size_t row = part + KB * wave + c;
+                const size_t row = part + row_of;
                 to = a.part[1].sums + row * D;
-                if (r < t.rows && hf == 0) a.part[1].ml[row] = make_float4(m, l, sc, 0.0f);
+                if (r < t.rows && half == 0) a.part[1].ml[row] = make_float4(m, l, sc, 0.0f);
             }
             if (r < t.rows)
 #pragma unroll
                 for (int u = 0; u < 4; u++)
 #pragma unroll
                     for (int x = 0; x < 4; x++)
-                        *reinterpret_cast<float4 *>(to + 4 * hf + 32 * u + 8 * x) =
+                        *reinterpret_cast<float4 *>(to + 4 * half + 32 * u + 8 * x) =
                             make_float4(o[u][4 * x] * by, o[u][4 * x + 1] * by, o[u][4 * x + 2] * by, o[u][4 * x + 3] * by);
         }
         if (t.begin + t.len >= x1) break;
@@ -944,8 +951,8 @@ extern "C" int htr_page_attention(htr_device *dev, const float *d_q, size_t q_st
     } read[3] = {{a.p.start, 4 * ((size_t)a.p.n_seq + 1)}, {a.p.past, 4 * (size_t)a.p.n_seq}, {a.p.table, 4 * (size_t)a.p.n_seq * a.p.max_pages}};
     for (const auto &r : read)
         if (htr_overlap(r.p, r.n, d_out, 4 * qd * n)) return htr_fail("%s: the output overlaps the pages' arrays", me);
-    const uint64_t group = (uint64_t)(n_head / kv->n_kv);  // (rows · group < 2^32: the kernel's quotients)
-    if (n * group * group >= 1ull << 32 || n * group > 1u << 30) return htr_fail("%s: %zu rows of %d heads", me, n, n_head);
+    const uint64_t group = (uint64_t)(n_head / kv->n_kv);  // (rows · group < 2^31: the kernel's quotients)
+    if (n * group * group >= 1ull << 31 || n * group > 1u << 30) return htr_fail("%s: %zu rows of %d heads", me, n, n_head);
     const double rows = (double)(n * group), held = (double)a.p.max_pages * pages->page;  // (a line's length, whatever the arrays hold)
     if (a.p.n_seq * (rows / WIDE + 2) * group * (held + rows + COST) >= 0x1p62)
         return htr_fail("%s: %d reads of %zu rows of %d heads over up to %.0f rows", me, a.p.n_seq, n, n_head, held);
@@ -953,7 +960,7 @@ extern "C" int htr_page_attention(htr_device *dev, const float *d_q, size_t q_st
     const HtrOnDevice on(dev);
     a.q = d_q, a.q_stride = q_stride, a.out = d_out, a.n_head = n_head, a.group = n_head / kv->n_kv;
     a.n_page = kv->n_ctx / pages->page, a.scale = scale;
-    a.per_group = (uint32_t)(((1ull << 32) + a.group - 1) / a.group), a.cap = a.p.max_pages << a.p.shift;
+    a.per_group = (uint32_t)(((1ull << 31) + a.group - 1) / a.group), a.cap = a.p.max_pages << a.p.shift;
     a.pieces = std::max(1, 2 * dev->n_cu / kv->n_kv), a.per_piece = 1.0 / a.pieces;
     if (a.pieces > 1) {
         const size_t n = (size_t)2 * dev->n_cu;
