@@ -164,7 +164,8 @@ template <bool W> struct Tile {
     // the block that place x of the line (begin < x < begin + len) cuts the tile in front of; 0 and nb: it does not
     __device__ __forceinline__ int block_at(const Line<W> &w, int64_t x) const {
         const int64_t u = x - begin;
-        const int b = W ? uniform((int)((double)u / (double)here(KB * w.a.group))) : (int)(u / KB);
+        // (wide: to 22 bits, the same for all that ask)
+        const int b = W ? uniform((int)((float)u * __builtin_amdgcn_rcpf((float)here(KB * w.a.group)))) : (int)(u / KB);
         return b < SLIVER ? 0 : b > nb - SLIVER ? nb : b;
     }
     // the one that holds place x of the line, x before its end
@@ -179,9 +180,9 @@ template <bool W> struct Tile {
         tau = 0;
         if constexpr (W) {
             const int64_t y = x - begin, step = w.step(past);
-            const double half = WIDE / 2, mid = 0.5 * ((double)step + half);
+            const float half = WIDE / 2, mid = 0.5f * ((float)step + half);
             const int tiles = (rows + WIDE - 1) / WIDE;
-            tau = uniform(min((int)((sqrt(mid * mid + half * (double)y) - mid) / half), tiles - 1));
+            tau = uniform(min((int)((float)y / (__builtin_sqrtf(mid * mid + half * (float)y) + mid)), tiles - 1));  // (or one beside it)
             auto upto = [&](int t) { return t * step + (int64_t)(WIDE / 2) * t * (t + 1); };
             while (tau > 0 && upto(tau) > y) tau--;
             while (tau + 1 < tiles && upto(tau + 1) <= y) tau++;
@@ -633,7 +634,6 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
             uint32_t gone = 0;       // and the halves without a page of this stage and those after it, a pair of bits each
             half8 qh[8], ql[8];
             float sc;
-            size_t part = 0;
             {
                 float qx[8][8];
                 q_load<8>(q_row(a, t.start, kvh, rc) + 8 * hf, qx);
@@ -655,7 +655,6 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                         issue(one, 0, true), issue(two, 1, true);
                     }
                 }
-                if (!own.all) part = part_of(line, t, own, kvh, piece);
                 sc = q_split<8, 2>(qx, a.scale, qh, ql);
             }
             if constexpr (Q8) {
@@ -819,6 +818,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                     s0 = s1;
                 }
             }
+            const size_t part = own.all ? 0 : part_of(line, t, own, kvh, piece);
             l = pair_sum<32>(l);
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (the next tile's loads go over these buffers)
 
