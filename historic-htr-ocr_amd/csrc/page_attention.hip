@@ -18,8 +18,7 @@
 // Tiles come in two heights, each with a line of its own. Of up to 32 rows (a step's token, or what is left of a prompt) the waves
 // share out the keys, every fourth block of 32 to each, loaded into LDS of its own, so that nobody waits for anybody until the
 // four sums are merged. More are tiles of 128, 32 to a wave, all of which use each block, staged for them together. (Four prompts
-// of 1925 in tiles of 32 rows alone 309 µs, with both 158.) The wide tiles' workgroups come first in the launch: in turn with the
-// narrow ones' a CU got two of one kind and its neighbour none, 263 µs for 178.
+// of 1925 in tiles of 32 rows alone 309 µs, with both 158.)
 //
 // Times here and below are of calls one after another on an MI355X, 16 q heads on 8 KV heads.
 #include <algorithm>
@@ -82,6 +81,26 @@ struct Reads {
     int64_t end[64];                 // the line's length up to and with each
     int start[64], n[64], past[64];  // its rows and keys; past −1: not served
 };
+// read b: its rows of the buffers, the keys before them
+struct Read {
+    int start, n, past;
+    __device__ __forceinline__ Read(const Args &a, int b) {
+        const bool there = b < a.p.n_seq;
+        const int s0 = there ? a.p.start[b] : 0, s1 = there ? a.p.start[b + 1] : 0, held = there ? a.p.past[b] : -1;
+        start = min(max(s0, 0), a.p.n_row), n = min(max(s1, start), a.p.n_row) - start, past = min(max(held, -1), a.cap);
+    }
+};
+template <bool W> __device__ __forceinline__ int64_t line_step(const Args &a, int past) {
+    return (int64_t)(W ? a.group : 1) * (max(past, 0) + (int64_t)COST);
+}
+// its length on the line of a height; n: 0 where it has no tile on it
+template <bool W> __device__ __forceinline__ int64_t line_length(const Args &a, Read &x) {
+    const int rows = x.n * a.group, full = rows / WIDE, rest = rows % WIDE;
+    const int64_t step = line_step<W>(a, x.past);
+    x.n = (W ? full == 0 && rest <= NARROW : rest > NARROW || rest == 0) ? 0 : x.n;
+    const int64_t len = W ? full * step + (int64_t)(WIDE / 2) * full * (full + 1) + (rest > NARROW ? step + rows : 0) : step + x.n;
+    return x.n ? len : 0;
+}
 // a height's line: the reads' tiles in order. A narrow read's length is its keys and COST. A wide tile's is group times that, up
 // to its last row (of a read's first k tiles k·step + 64·k·(k + 1) in all, step = group·(past + COST))
 template <bool W> struct Line {
@@ -90,12 +109,12 @@ template <bool W> struct Line {
     int first = 0;     // the reads at hand: first …
     int64_t base = 0;  // the line's length before them
     int64_t total, piece;
-    __device__ __forceinline__ Line(const Args &args, Reads &reads) : a(args), r(reads) {
-        total = load();
+    __device__ __forceinline__ Line(const Args &args, Reads &reads, const Read &x) : a(args), r(reads) {  // x: read `lane`
+        total = load(x);
         if (a.p.n_seq > 64) {
             for (; first + 64 < a.p.n_seq; total = load()) base = total, first += 64;
             first = 0, base = 0;
-            load();
+            load(x);
         }
         piece = uniform(max((int64_t)((double)total * a.per_piece) + 1, (int64_t)LEAST * (W ? a.group : 1)));
     }
@@ -108,30 +127,19 @@ template <bool W> struct Line {
         while (i + 1 < a.pieces && cut(i + 1) <= x) i++;
         return uniform(i);
     }
-    __device__ __forceinline__ int64_t step(int past) const { return (int64_t)(W ? a.group : 1) * (max(past, 0) + (int64_t)COST); }
+    __device__ __forceinline__ int64_t step(int past) const { return line_step<W>(a, past); }
     // the reads from `first` on; their end on the line
-    __device__ __forceinline__ int64_t load() {
-        const int lane = lane_id(), b = first + lane;
-        const bool there = b < a.p.n_seq;
-        const int s0 = there ? a.p.start[b] : 0, s1 = there ? a.p.start[b + 1] : 0, held = there ? a.p.past[b] : -1;
-        const int start = min(max(s0, 0), a.p.n_row), past = min(max(held, -1), a.cap);
-        int n = min(max(s1, start), a.p.n_row) - start;
-        const int rows = n * a.group, full = rows / WIDE, rest = rows % WIDE;
-        int64_t end;
-        if constexpr (W) {
-            end = full * step(past) + (int64_t)(WIDE / 2) * full * (full + 1) + (rest > NARROW ? step(past) + rows : 0);
-        } else {
-            if (rest > NARROW || rest == 0) n = 0;
-            end = n ? step(past) + n : 0;
-        }
-        if (W && end == 0) n = 0;
+    __device__ __forceinline__ int64_t load() { return load(Read(a, first + lane_id())); }
+    __device__ __forceinline__ int64_t load(Read x) {
+        const int lane = lane_id();
+        int64_t end = line_length<W>(a, x);
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t lo = __builtin_amdgcn_ds_bpermute(4 * (lane - d), (int)(uint32_t)end), hi = __builtin_amdgcn_ds_bpermute(4 * (lane - d), (int)(end >> 32));
             if (lane >= d) end += (int64_t)((uint64_t)hi << 32 | lo);
         }
         end += base;
-        r.end[lane] = end, r.start[lane] = start, r.n[lane] = n, r.past[lane] = past;
+        r.end[lane] = end, r.start[lane] = x.start, r.n[lane] = x.n, r.past[lane] = x.past;
         return lane_of(end, 63);
     }
 };
@@ -300,12 +308,12 @@ struct Shared {
 // Bound: of few keys latency (a token over 1300 keys 12.5 µs, of which lengths, pages, keys, each a load that the next one waits
 // for, 6 µs, and the second launch 4); of many HBM: 64 reads' tokens over 300 … 6000 f16 keys (505 MB) 105 µs, over q8_0 rows
 // (269 MB) 74, at 6.6 TB/s while all workgroups run, which end between 56 and 101 µs.
-template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh, int piece, uint4_t *s_kv, Shared &sh) {
+template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh, int piece, const Read &x, uint4_t *s_kv, Shared &sh) {
     constexpr int WAVE = Q8 ? WAVE_Q8 : WAVE_F16;
     static_assert(WAVE >= 1024, "a wave's sums fit");
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), hf = lane >> 5, c = lane & 31;
     if (a.pieces > 1) no_parts<false>(a, kvh, piece);
-    Line<false> line(a, sh.reads[wave]);
+    Line<false> line(a, sh.reads[wave], x);
     const int64_t x0 = line.cut(piece), x1 = line.cut(piece + 1);
     if (x0 >= x1) return;
     const size_t head0 = (size_t)kvh * a.kv.n_ctx;
@@ -575,10 +583,10 @@ template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh
 // are of keys past a row's own, 13 µs the second launch, 20 that workgroups wait for the last. Of two waves on a SIMD the one at
 // its scores goes first (without 1.046 ms; the one at its values first 1.043). Loads four stages ahead or one, and a barrier a
 // stage or every second one, take the same time.
-template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, int piece, uint4_t *s_kv, Shared &sh) {
+template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, int piece, const Read &x, uint4_t *s_kv, Shared &sh) {
     const int wave = uniform((int)threadIdx.x >> 6);
     if (a.pieces > 1) no_parts<true>(a, kvh, piece);
-    Line<true> line(a, sh.reads[wave]);
+    Line<true> line(a, sh.reads[wave], x);
     const int64_t x0 = line.cut(piece), x1 = line.cut(piece + 1);
     if (x0 >= x1) return;
     const size_t head0 = (size_t)kvh * a.kv.n_ctx;
@@ -844,14 +852,39 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
     }
 }
 
-// the workgroups of wide tiles, then those of narrow ones
+// The workgroups of wide tiles and those of narrow ones, of the kind first that has more to do: 64 tokens beside 512 rows 134 µs,
+// narrow first, for 145; four prompts with their last narrow tiles 159, wide first, for 166. Where neither has much more (f16; over
+// q8_0 rows it is no faster), half of each kind in turn, so that a CU has one of each: two chunks of 509 rows beside 61 tokens 148
+// µs for 160 (wide first) and 161. To tell costs 1 µs. In turn one by one, a CU got two of one kind and its neighbour none.
 template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_attn(Args a) {
     __shared__ __attribute__((aligned(16))) uint4_t s_kv[PW * (Q8 ? WAVE_Q8 : WAVE_F16)];
     static_assert(!Q8 || 16 * PW * WAVE_Q8 >= 16 * 2 * TILE + 4 * RAW * PW, "the wide tiles' buffers fit");
     __shared__ Shared sh;
-    const int kvh = blockIdx.x % a.kv.n_kv, piece = blockIdx.x / a.kv.n_kv;
-    if (piece < a.wide) wide<Q8>(a, kvh, piece, s_kv, sh);
-    else narrow<Q8>(a, kvh, piece - a.wide, s_kv, sh);
+    const int kvh = blockIdx.x % a.kv.n_kv, unit = blockIdx.x / a.kv.n_kv;
+    const Read mine(a, lane_id());
+    bool is_narrow = true;
+    int piece = unit;
+    if (a.wide) {
+        float lw = 0.0f, ln = 0.0f;  // the lines' lengths, about
+        Read x = mine;
+        for (int first = 64;; x = Read(a, first + lane_id()), first += 64) {
+            const int rows = x.n * a.group, rest = rows % WIDE;
+            const float tiles = (float)(rows / WIDE + (rest > NARROW)), held = (float)max(x.past, 0) + COST;
+            lw = fmaf(tiles, fmaf(held, (float)a.group, WIDE / 2 * tiles), lw);
+            ln += rest > 0 && rest <= NARROW ? held + (float)x.n : 0.0f;
+            if (first >= a.p.n_seq) break;
+        }
+        lw = wave_sum(lw, lane_id()), ln = wave_sum(ln, lane_id());
+        const bool narrow_first = __builtin_amdgcn_ballot_w64(ln >= 2.0f * lw) != 0;  // (alike in all lanes)
+        const bool halves = !Q8 && __builtin_amdgcn_ballot_w64(ln < 2.0f * lw && ln > 0.25f * lw && lw > 2.0f * LEAST * a.group * a.pieces) != 0;
+        // n of the one kind, n of the other, and what is left of each
+        const int n = halves ? (a.pieces + 1) / 2 : a.pieces, left = a.pieces - n;
+        const bool other = unit >= n && (unit < 2 * n || unit >= 2 * n + left);
+        piece = unit < n ? unit : unit < 2 * n + left ? unit - n : unit - n - left;
+        is_narrow = other != narrow_first;
+    }
+    if (is_narrow) narrow<Q8>(a, kvh, piece, mine, s_kv, sh);
+    else wide<Q8>(a, kvh, piece, mine, s_kv, sh);
 }
 
 // The second launch: the rows of a cut tile shared out among as many workgroups as it has parts (SHARES times as many), those of
@@ -860,8 +893,8 @@ __global__ __launch_bounds__(256) void k_page_attn_join(Args a) {
     __shared__ float4 s_y[8][32];
     __shared__ float2 s_ml[8];
     const int tid = threadIdx.x, gr = tid >> 5, j = tid & 31;
-    const int kvh = blockIdx.x % a.kv.n_kv, unit = blockIdx.x / a.kv.n_kv, piece = unit % a.pieces, share = unit / a.pieces;
-    const int w = unit < SHARES * a.wide, shares = w ? SHARES : 1;
+    const int kvh = blockIdx.x % a.kv.n_kv, unit = blockIdx.x / a.kv.n_kv, share = unit / a.pieces, piece = unit - share * a.pieces;
+    const int w = share > 0, shares = w ? SHARES : 1;  // (share 0: the narrow tiles')
     const Parts &p = a.part[w];
     const int height = w ? WIDE : NARROW;
     const size_t mine = ((size_t)kvh * a.pieces + piece) * 2;
@@ -869,7 +902,7 @@ __global__ __launch_bounds__(256) void k_page_attn_join(Args a) {
     for (int k = 0; k < 2; k++) {
         const Part &t = both[k];
         if (t.n == 0) continue;
-        const int mth = (piece - t.first) * shares + (w ? share : 0), of = t.n * shares;
+        const int mth = (piece - t.first) * shares + (w ? share - 1 : 0), of = t.n * shares;
         const int ra = t.rows * mth / of, rb = t.rows * (mth + 1) / of, nr = rb - ra;
         const int lg = nr > 4 ? 3 : nr > 2 ? 2 : nr > 1 ? 1 : 0, G = 8 >> lg;  // 2^lg rows at once, G groups to each
         for (int r = ra; r < rb; r += 1 << lg) {
@@ -877,6 +910,8 @@ __global__ __launch_bounds__(256) void k_page_attn_join(Args a) {
             float top = M_NONE, sum = 0.0f;
             float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             float c = 0.0f;
+            // (in floats: below 2^25)
+            const uint32_t at0 = ((uint32_t)(kvh * a.pieces + t.first) * 2) * height + row;
             for (int e0 = g; e0 < t.n; e0 += 4 * G) {
                 float4 ml[4], in[4];
 #pragma unroll
@@ -884,9 +919,9 @@ __global__ __launch_bounds__(256) void k_page_attn_join(Args a) {
                     const int e = e0 + q * G;
                     ml[q] = make_float4(M_NONE, 0.0f, c, 0.0f), in[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     if (e < t.n) {
-                        const size_t at = (((size_t)kvh * a.pieces + t.first + e) * 2 + (e == 0)) * height + row;
+                        const uint32_t at = at0 + (uint32_t)(2 * e + (e == 0)) * height;
                         ml[q] = p.ml[at];
-                        in[q] = *reinterpret_cast<const float4 *>(p.sums + at * D + 4 * j);
+                        in[q] = *reinterpret_cast<const float4 *>(p.sums + (at * D + 4 * j));
                     }
                 }
                 c = ml[0].z;  // (a row's parts have the same)
