@@ -123,8 +123,8 @@ template <bool W> struct Line {
     __device__ __forceinline__ int piece_of(int64_t x) const {
         const float each = (float)(int64_t)((uint64_t)(uint32_t)here((int)(piece >> 32)) << 32 | (uint32_t)here((int)piece));
         int i = min((int)((float)x * __builtin_amdgcn_rcpf(each)), a.pieces - 1);  // (or one beside it)
-        while (i > 0 && cut(i) > x) i--;
-        while (i + 1 < a.pieces && cut(i + 1) <= x) i++;
+        i -= i > 0 && cut(i) > x;
+        i += i + 1 < a.pieces && cut(i + 1) <= x;
         return uniform(i);
     }
     __device__ __forceinline__ int64_t step(int past) const { return line_step<W>(a, past); }
@@ -192,8 +192,8 @@ template <bool W> struct Tile {
             const int tiles = (rows + WIDE - 1) / WIDE;
             tau = uniform(min((int)((float)y / (__builtin_sqrtf(mid * mid + half * (float)y) + mid)), tiles - 1));  // (or one beside it)
             auto upto = [&](int t) { return t * step + (int64_t)(WIDE / 2) * t * (t + 1); };
-            while (tau > 0 && upto(tau) > y) tau--;
-            while (tau + 1 < tiles && upto(tau + 1) <= y) tau++;
+            tau -= tau > 0 && upto(tau) > y;
+            tau += tau + 1 < tiles && upto(tau + 1) <= y;
             begin += upto(tau);
         }
         measure(w);
