@@ -635,7 +635,6 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
             const int r0 = WIDE * t.tau + KB * wave, rc = min(r0 + c, t.rows - 1);
             const int all_to = (t.last_of(a, r0) + 1) / KB;                              // blocks that all of the wave's rows see the whole of
             const int any_to = r0 < t.rows ? blocks_to(t.last_of(a, r0 + KB - 1)) : 0;  // blocks that one of them sees
-            const int keys = t.last_key(a, query_of(a, rc)) + 1;                         // keys that the lane's row sees
             Run run = run_of(a, line, t, i0, 1);
             if (n_st > 0) run.fetch(0);
             Rows r_last{{0, 0}, 0};  // f16: of the last stage whose K is on its way
@@ -713,6 +712,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                     }
                 uint32_t seen = 0;
                 if constexpr (MASK) {
+                    const int keys = t.last_of(a, r0 + (lane_id() & 31)) + 1;  // that the lane's row sees
                     seen = sees(keys, i, hf, bad);
 #pragma unroll
                     for (int x = 0; x < 16; x++) s[x] = seen >> (8 * (x >> 2) + (x & 3)) & 1 ? s[x] : -INFINITY;
@@ -883,7 +883,7 @@ template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_attn(Arg
         piece = unit < n ? unit : unit < 2 * n + left ? unit - n : unit - n - left;
         is_narrow = other != narrow_first;
     }
-    if (is_narrow) narrow<Q8>(a, kvh, piece, mine, s_kv, sh);
+    if (uniform((int)is_narrow)) narrow<Q8>(a, kvh, piece, mine, s_kv, sh);
     else wide<Q8>(a, kvh, piece, mine, s_kv, sh);
 }
 
