@@ -32,6 +32,7 @@ enum {
     SCR_PAGE_ATTN = 10, // the parts of the page attention's cut tiles (one size)
     SCR_SCORE = 11,     // the log probabilities' parts of rows (one size)
     SCR_SCORE_TICKET = 12,  // their tickets (one size; zero, self-resetting)
+    SCR_PAGE_TICKET = 13,   // the tickets of the page attention's tiles (one size; zero, self-resetting)
     SCR_SLOTS
 };
 

@@ -33,6 +33,7 @@ constexpr int NARROW = KB, WIDE = KB * PW;  // rows of a tile
 constexpr int COST = 128;                   // keys that take as long as a tile's start and end (with 64 four prompts 182 µs for 166)
 constexpr int LEAST = 192;                  // a piece's length, at least: a block for each wave, and a tile's start
 constexpr int SLIVER = 4;                   // blocks of a tile's beginning or end that are not cut off for themselves
+constexpr int TICKET = 32;                  // words between tickets (128 bytes)
 constexpr int SHARES = 4;                   // workgroups of the join to a wide piece
 constexpr int QT = 256 + 256 + 16 + 16;     // 16-byte chunks of a q8_0 buffer: K, V, K scales, V scales
 
@@ -60,6 +61,7 @@ struct Args {
     int pieces;          // workgroups of a KV head and height
     int wide;            // those of the wide tiles: pieces, or none where no read has so many rows
     double per_piece;    // 1 / pieces
+    uint32_t *tickets;   // [n_kv·pieces], TICKET words apart
     Parts part[2];
 };
 
@@ -228,18 +230,19 @@ template <bool W> __device__ __forceinline__ Share share_of(const Line<W> &w, co
     s.all = s.i0 == 0 && s.i1 == t.nb;
     return s;
 }
-// a piece's place for its part of a cut tile, and which pieces have the others (the last wave's work: of few keys it has the least)
-template <bool W> __device__ __forceinline__ size_t part_of(const Line<W> &w, const Tile<W> &t, const Share &share, int kvh, int piece) {
-    const size_t place = ((size_t)kvh * w.a.pieces + piece) * 2 + (share.i0 == 0);
-    if (threadIdx.x >= 64 * (PW - 1)) {
-        int first = w.piece_of(t.begin), end = first + 1;
-        if (w.cut(end) < t.begin + t.len && t.block_at(w, w.cut(end)) == 0) first++, end++;  // (it leaves the beginning to the next one)
-        for (end = max(w.piece_of(t.begin + t.len - 1) + 1, end); end - 1 > first && t.block_at(w, w.cut(end - 1)) == t.nb;) end--;
-        if (threadIdx.x == 64 * (PW - 1))
-            w.a.part[W].of[place] = W ? Part{first, end - first, t.start, WIDE * t.tau, min(WIDE, t.rows - WIDE * t.tau)}
-                                      : Part{first, end - first, t.start, t.r0, t.rows};
-    }
-    return place * (W ? WIDE : NARROW);
+// a piece's place for its part of a cut tile, and in `to` (of that place, or of LDS) which pieces have the others (the last wave's
+// work: of few keys it has the least)
+__device__ __forceinline__ size_t place_of(const Args &a, const Share &share, int kvh, int piece) {
+    return ((size_t)kvh * a.pieces + piece) * 2 + (share.i0 == 0);
+}
+template <bool W> __device__ __forceinline__ void part_of(const Line<W> &w, const Tile<W> &t, Part &to) {
+    if (threadIdx.x < 64 * (PW - 1)) return;
+    int first = w.piece_of(t.begin), end = first + 1;
+    if (w.cut(end) < t.begin + t.len && t.block_at(w, w.cut(end)) == 0) first++, end++;  // (it leaves the beginning to the next one)
+    for (end = max(w.piece_of(t.begin + t.len - 1) + 1, end); end - 1 > first && t.block_at(w, w.cut(end - 1)) == t.nb;) end--;
+    if (threadIdx.x == 64 * (PW - 1))
+        to = W ? Part{first, end - first, t.start, WIDE * t.tau, min(WIDE, t.rows - WIDE * t.tau)}
+               : Part{first, end - first, t.start, t.r0, t.rows};
 }
 // the two places of a piece that has no cut tile are empty (the same wave's stores, in order)
 template <bool W> __device__ __forceinline__ void no_parts(const Args &a, int kvh, int piece) {
@@ -298,7 +301,81 @@ constexpr int RAW = 1024 + 1024 + 256;                 // bytes of 8 raw rows: K
 struct Shared {
     Reads reads[PW];  // (each wave its own: nobody waits)
     float ml[PW][2][KB];
+    Part part;  // of the tile at hand
+    int last;   // its last part is this one
 };
+
+// The rows ra … rb − 1 of a cut tile: 32 lanes of 4 dims to a row; where the rows are fewer than the groups of 32, several groups to
+// a row's parts. XL: parts that workgroups of this launch stored, in the L2 of the XCD that they share
+struct Join {
+    float4 y[8][32];
+    float2 ml[8];
+};
+template <bool XL> __device__ __forceinline__ void join_rows(const Args &a, int w, int kvh, const Part &t, int ra, int rb, Join &sh) {
+    const int tid = threadIdx.x, gr = tid >> 5, j = tid & 31, nr = rb - ra;
+    const Parts &p = a.part[w];
+    const int height = w ? WIDE : NARROW;
+    auto get = [](const float4 *from) {
+        if constexpr (!XL) return *from;
+        const float2 lo = get64(from), hi = get64(&from->z);
+        return make_float4(lo.x, lo.y, hi.x, hi.y);
+    };
+            const int lg = nr > 4 ? 3 : nr > 2 ? 2 : nr > 1 ? 1 : 0, G = 8 >> lg;  // 2^lg rows at once, G groups to each
+            for (int r = ra; r < rb; r += 1 << lg) {
+                const int row = min(r + (gr & ((1 << lg) - 1)), rb - 1), g = gr >> lg;
+                float top = M_NONE, sum = 0.0f;
+                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                float c = 0.0f;
+                // (in floats: below 2^25)
+                const uint32_t at0 = ((uint32_t)(kvh * a.pieces + t.first) * 2) * height + row;
+                for (int e0 = g; e0 < t.n; e0 += 4 * G) {
+                    float4 ml[4], in[4];
+    #pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const int e = e0 + q * G;
+                        ml[q] = make_float4(M_NONE, 0.0f, c, 0.0f), in[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (e < t.n) {
+                            const uint32_t at = at0 + (uint32_t)(2 * e + (e == 0)) * height;
+                            ml[q] = get(p.ml + at);
+                            in[q] = get(reinterpret_cast<const float4 *>(p.sums + (at * D + 4 * j)));
+                        }
+                    }
+                    c = ml[0].z;  // (a row's parts have the same)
+                    const float to = fmaxf(fmaxf(top, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+                    const float f = __builtin_amdgcn_exp2f((top - to) * c);
+                    top = to, sum *= f, y.x *= f, y.y *= f, y.z *= f, y.w *= f;
+    #pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const float h = __builtin_amdgcn_exp2f((ml[q].x - to) * c);
+                        sum = fmaf(ml[q].y, h, sum);
+                        y.x = fmaf(in[q].x, h, y.x), y.y = fmaf(in[q].y, h, y.y), y.z = fmaf(in[q].z, h, y.z), y.w = fmaf(in[q].w, h, y.w);
+                    }
+                }
+                if (G > 1) {  // (one pass)
+                    __syncthreads();
+                    sh.y[gr][j] = y;
+                    if (j == 0) sh.ml[gr] = make_float2(top, sum);
+                    __syncthreads();
+                    if (g == 0) {
+                        float to = top;
+                        for (int e = 1; e < G; e++) to = fmaxf(to, sh.ml[gr + (e << lg)].x);
+                        const float f = __builtin_amdgcn_exp2f((top - to) * c);
+                        sum *= f, y.x *= f, y.y *= f, y.z *= f, y.w *= f;
+                        for (int e = 1; e < G; e++) {
+                            const float4 z = sh.y[gr + (e << lg)][j];
+                            const float2 ml = sh.ml[gr + (e << lg)];
+                            const float h = __builtin_amdgcn_exp2f((ml.x - to) * c);
+                            sum = fmaf(ml.y, h, sum);
+                            y.x = fmaf(z.x, h, y.x), y.y = fmaf(z.y, h, y.y), y.z = fmaf(z.z, h, y.z), y.w = fmaf(z.w, h, y.w);
+                        }
+                    }
+                }
+                if (g == 0 && r + (gr & ((1 << lg) - 1)) < rb) {
+                    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
+                    *reinterpret_cast<float4 *>(out_row(a, t.start, kvh, t.r0 + row) + 4 * j) = make_float4(y.x * by, y.y * by, y.z * by, y.w * by);
+                }
+            }
+}
 
 // ---- reads of few rows -------------------------------------------------------------------------------------------------------
 //
@@ -308,11 +385,11 @@ struct Shared {
 // Bound: of few keys latency (a token over 1300 keys 12.5 µs, of which lengths, pages, keys, each a load that the next one waits
 // for, 6 µs, and the second launch 4); of many HBM: 64 reads' tokens over 300 … 6000 f16 keys (505 MB) 105 µs, over q8_0 rows
 // (269 MB) 74, at 6.6 TB/s while all workgroups run, which end between 56 and 101 µs.
-template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh, int piece, const Read &x, uint4_t *s_kv, Shared &sh) {
+template <bool Q8, bool ONE> __device__ __forceinline__ void narrow(const Args &a, int kvh, int piece, const Read &x, uint4_t *s_kv, Shared &sh) {
     constexpr int WAVE = Q8 ? WAVE_Q8 : WAVE_F16;
     static_assert(WAVE >= 1024, "a wave's sums fit");
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), hf = lane >> 5, c = lane & 31;
-    if (a.pieces > 1) no_parts<false>(a, kvh, piece);
+    if (!ONE && a.pieces > 1) no_parts<false>(a, kvh, piece);
     Line<false> line(a, sh.reads[wave], x);
     const int64_t x0 = line.cut(piece), x1 = line.cut(piece + 1);
     if (x0 >= x1) return;
@@ -373,7 +450,8 @@ template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh
                     load(now.at[0], now.at[1], true);
                 }
             }
-            const size_t part = own.all ? 0 : part_of(line, t, own, kvh, piece);
+            const size_t place = place_of(a, own, kvh, piece), part = place * NARROW;
+            if (!own.all) part_of(line, t, ONE ? sh.part : a.part[0].of[place]);
             half8 qh[8], ql[8];
             const float sc = q_split<8, 2>(qx, a.scale, qh, ql);
             float m = M_NONE, l = 0.0f;
@@ -557,15 +635,32 @@ template <bool Q8> __device__ __forceinline__ void narrow(const Args &a, int kvh
                 }
             }
             const float by = !own.all ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;  // no key seen: zeros
-            float *to;
-            if (own.all) {
-                to = out_row(a, t.start, kvh, rc);
-            } else {
-                const size_t row = part + c;
-                to = a.part[0].sums + row * D;
-                if (c < t.rows && wave == 0 && hf == 0) a.part[0].ml[row] = make_float4(m, l, sc, 0.0f);
-            }
+            float *to = own.all ? out_row(a, t.start, kvh, rc) : a.part[0].sums + (part + c) * D;
             to += 32 * wave + 4 * hf;
+            float4 *ml = a.part[0].ml + part + c;
+            if (ONE && !own.all) {
+                if (c < t.rows) {
+#pragma unroll
+                    for (int x = 0; x < 4; x++) put64(to + 8 * x, y[x].x, y[x].y, true), put64(to + 8 * x + 2, y[x].z, y[x].w, true);
+                    if (wave == 0 && hf == 0) put64(ml, m, l, true), put64(&ml->z, sc, 0.0f, true);
+                }
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's stores are performed
+                __syncthreads();
+                const Part whole = sh.part;
+                if (threadIdx.x == 0) {
+                    uint32_t *ticket = a.tickets + (size_t)TICKET * (kvh * a.pieces + whole.first);
+                    sh.last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) == (uint32_t)(whole.n - 1);
+                    if (sh.last) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);  // for the next call
+                }
+                __syncthreads();
+                if (sh.last) {
+                    join_rows<true>(a, 0, kvh, whole, 0, whole.rows, *reinterpret_cast<Join *>(s_kv));
+                    __syncthreads();  // (the next tile's loads go there)
+                }
+                if (t.begin + t.len >= x1) break;
+                continue;
+            }
+            if (!own.all && c < t.rows && wave == 0 && hf == 0) *ml = make_float4(m, l, sc, 0.0f);
             if (c < t.rows)
 #pragma unroll
                 for (int x = 0; x < 4; x++)
@@ -826,7 +921,8 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                     s0 = s1;
                 }
             }
-            const size_t part = own.all ? 0 : part_of(line, t, own, kvh, piece);
+            const size_t place = place_of(a, own, kvh, piece), part = place * WIDE;
+            if (!own.all) part_of(line, t, a.part[1].of[place]);
             l = pair_sum<32>(l);
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // (the next tile's loads go over these buffers)
 
@@ -883,82 +979,31 @@ template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_attn(Arg
         piece = unit < n ? unit : unit < 2 * n + left ? unit - n : unit - n - left;
         is_narrow = other != narrow_first;
     }
-    if (uniform((int)is_narrow)) narrow<Q8>(a, kvh, piece, mine, s_kv, sh);
+    if (uniform((int)is_narrow)) narrow<Q8, false>(a, kvh, piece, mine, s_kv, sh);
     else wide<Q8>(a, kvh, piece, mine, s_kv, sh);
 }
 
+// Few rows, where a head's workgroups share an XCD: narrow tiles alone, the parts of a cut one joined by the last of them (a token over
+// 1300 keys 11.3 µs, by a second launch 12.5)
+template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_few(Args a) {
+    __shared__ __attribute__((aligned(16))) uint4_t s_kv[PW * (Q8 ? WAVE_Q8 : WAVE_F16)];
+    __shared__ Shared sh;
+    narrow<Q8, true>(a, blockIdx.x % a.kv.n_kv, blockIdx.x / a.kv.n_kv, Read(a, lane_id()), s_kv, sh);
+}
+
 // The second launch: the rows of a cut tile shared out among as many workgroups as it has parts (SHARES times as many), those of
-// the pieces. 32 lanes of 4 dims to a row; where the rows are fewer than the groups of 32, several groups to a row's parts
+// the pieces
 __global__ __launch_bounds__(256) void k_page_attn_join(Args a) {
-    __shared__ float4 s_y[8][32];
-    __shared__ float2 s_ml[8];
-    const int tid = threadIdx.x, gr = tid >> 5, j = tid & 31;
+    __shared__ Join sh;
     const int kvh = blockIdx.x % a.kv.n_kv, unit = blockIdx.x / a.kv.n_kv, share = unit / a.pieces, piece = unit - share * a.pieces;
     const int w = share > 0, shares = w ? SHARES : 1;  // (share 0: the narrow tiles')
-    const Parts &p = a.part[w];
-    const int height = w ? WIDE : NARROW;
     const size_t mine = ((size_t)kvh * a.pieces + piece) * 2;
-    const Part both[2] = {p.of[mine], p.of[mine + 1]};
+    const Part both[2] = {a.part[w].of[mine], a.part[w].of[mine + 1]};
     for (int k = 0; k < 2; k++) {
         const Part &t = both[k];
         if (t.n == 0) continue;
         const int mth = (piece - t.first) * shares + (w ? share - 1 : 0), of = t.n * shares;
-        const int ra = t.rows * mth / of, rb = t.rows * (mth + 1) / of, nr = rb - ra;
-        const int lg = nr > 4 ? 3 : nr > 2 ? 2 : nr > 1 ? 1 : 0, G = 8 >> lg;  // 2^lg rows at once, G groups to each
-        for (int r = ra; r < rb; r += 1 << lg) {
-            const int row = min(r + (gr & ((1 << lg) - 1)), rb - 1), g = gr >> lg;
-            float top = M_NONE, sum = 0.0f;
-            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float c = 0.0f;
-            // (in floats: below 2^25)
-            const uint32_t at0 = ((uint32_t)(kvh * a.pieces + t.first) * 2) * height + row;
-            for (int e0 = g; e0 < t.n; e0 += 4 * G) {
-                float4 ml[4], in[4];
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const int e = e0 + q * G;
-                    ml[q] = make_float4(M_NONE, 0.0f, c, 0.0f), in[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (e < t.n) {
-                        const uint32_t at = at0 + (uint32_t)(2 * e + (e == 0)) * height;
-                        ml[q] = p.ml[at];
-                        in[q] = *reinterpret_cast<const float4 *>(p.sums + (at * D + 4 * j));
-                    }
-                }
-                c = ml[0].z;  // (a row's parts have the same)
-                const float to = fmaxf(fmaxf(top, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
-                const float f = __builtin_amdgcn_exp2f((top - to) * c);
-                top = to, sum *= f, y.x *= f, y.y *= f, y.z *= f, y.w *= f;
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const float h = __builtin_amdgcn_exp2f((ml[q].x - to) * c);
-                    sum = fmaf(ml[q].y, h, sum);
-                    y.x = fmaf(in[q].x, h, y.x), y.y = fmaf(in[q].y, h, y.y), y.z = fmaf(in[q].z, h, y.z), y.w = fmaf(in[q].w, h, y.w);
-                }
-            }
-            if (G > 1) {  // (one pass)
-                __syncthreads();
-                s_y[gr][j] = y;
-                if (j == 0) s_ml[gr] = make_float2(top, sum);
-                __syncthreads();
-                if (g == 0) {
-                    float to = top;
-                    for (int e = 1; e < G; e++) to = fmaxf(to, s_ml[gr + (e << lg)].x);
-                    const float f = __builtin_amdgcn_exp2f((top - to) * c);
-                    sum *= f, y.x *= f, y.y *= f, y.z *= f, y.w *= f;
-                    for (int e = 1; e < G; e++) {
-                        const float4 z = s_y[gr + (e << lg)][j];
-                        const float2 ml = s_ml[gr + (e << lg)];
-                        const float h = __builtin_amdgcn_exp2f((ml.x - to) * c);
-                        sum = fmaf(ml.y, h, sum);
-                        y.x = fmaf(z.x, h, y.x), y.y = fmaf(z.y, h, y.y), y.z = fmaf(z.z, h, y.z), y.w = fmaf(z.w, h, y.w);
-                    }
-                }
-            }
-            if (g == 0 && r + (gr & ((1 << lg) - 1)) < rb) {
-                const float by = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
-                *reinterpret_cast<float4 *>(out_row(a, t.start, kvh, t.r0 + row) + 4 * j) = make_float4(y.x * by, y.y * by, y.z * by, y.w * by);
-            }
-        }
+        join_rows<false>(a, w, kvh, t, t.rows * mth / of, t.rows * (mth + 1) / of, sh);
     }
 }
 
@@ -997,9 +1042,13 @@ extern "C" int htr_page_attention(htr_device *dev, const float *d_q, size_t q_st
     a.n_page = kv->n_ctx / pages->page, a.scale = scale;
     a.per_group = (uint32_t)(((1ull << 31) + a.group - 1) / a.group), a.cap = a.p.max_pages << a.p.shift;
     a.pieces = std::max(1, 2 * dev->n_cu / kv->n_kv), a.per_piece = 1.0 / a.pieces;
+    a.wide = n * group > NARROW ? a.pieces : 0;
     if (a.pieces > 1) {
         const size_t n = (size_t)2 * dev->n_cu;
         void *p;
+        HTR_TRY(htr_scratch(dev, SCR_PAGE_TICKET, n * TICKET * 4, &p));
+        // few rows, and a head's workgroups on one XCD (a launch's go to the 8 XCDs in turn)
+        if (!a.wide && kv->n_kv % 8 == 0 && dev->xcd_round_robin == 1) a.tickets = (uint32_t *)p;
         HTR_TRY(htr_scratch(dev, SCR_PAGE_ATTN, 2 * n * ((NARROW + WIDE) * (D + 4) * 4 + 2 * sizeof(Part)), &p));
         float *at = (float *)p;
         for (int w = 0; w < 2; w++) {
@@ -1008,10 +1057,15 @@ extern "C" int htr_page_attention(htr_device *dev, const float *d_q, size_t q_st
             at += rows * (D + 4) + 2 * n * sizeof(Part) / 4;
         }
     }
-    a.wide = n * group > NARROW ? a.pieces : 0;
     const unsigned groups = (unsigned)((a.wide + a.pieces) * kv->n_kv);
-    if (a.kv.q8) hipLaunchKernelGGL(k_page_attn<true>, dim3(groups), dim3(64 * PW), 0, dev->stream, a);
-    else hipLaunchKernelGGL(k_page_attn<false>, dim3(groups), dim3(64 * PW), 0, dev->stream, a);
+    const dim3 g(groups), b(64 * PW);
+    if (a.tickets) {
+        if (a.kv.q8) hipLaunchKernelGGL(k_page_few<true>, g, b, 0, dev->stream, a);
+        else hipLaunchKernelGGL(k_page_few<false>, g, b, 0, dev->stream, a);
+        return htr_launched(dev, a.kv.q8 ? "k_page_few<q8_0>" : "k_page_few<f16>");
+    }
+    if (a.kv.q8) hipLaunchKernelGGL(k_page_attn<true>, g, b, 0, dev->stream, a);
+    else hipLaunchKernelGGL(k_page_attn<false>, g, b, 0, dev->stream, a);
     HTR_TRY(htr_launched(dev, a.kv.q8 ? "k_page_attn<q8_0>" : "k_page_attn<f16>"));
     if (a.pieces == 1) return 0;
     hipLaunchKernelGGL(k_page_attn_join, dim3((unsigned)((SHARES * a.wide + a.pieces) * kv->n_kv)), dim3(256), 0, dev->stream, a);

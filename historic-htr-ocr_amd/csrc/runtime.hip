@@ -358,7 +358,7 @@ int htr_scratch(htr_device *dev, int slot, size_t bytes, void **out) {
         // the self-resetting words (best keys, tickets) start at zero; the rest is written before it is read
         const bool zero =
             slot == SCR_CHOOSE_PART || slot == SCR_CHOOSE_CNT || slot == SCR_ATTN_CNT || slot == SCR_KV_TICKET ||
-            slot == SCR_SCORE_TICKET;
+            slot == SCR_SCORE_TICKET || slot == SCR_PAGE_TICKET;
         HTR_TRY(alloc_filled(dev, bytes, HTR_MEM_WORK, zero, &dev->scratch[slot]));
         dev->scratch_bytes[slot] = bytes;
     }

@@ -13,3 +13,15 @@ def test_no_lds_access_crosses_a_barrier(tmp_path):
         assert len(barriers) >= 4, name
         assert all(n == 0 for n in barriers.values()), (name, barriers)
     assert seen == 2
+
+
+def test_none_crosses_a_barrier_of_few_rows(tmp_path):
+    seen = 0
+    for name, body in _functions(_assembly("page_attention", tmp_path)):
+        if "k_page_few" not in name:
+            continue
+        seen += 1
+        barriers = _pending_at_barriers(body)
+        assert len(barriers) >= 3, name
+        assert all(n == 0 for n in barriers.values()), (name, barriers)
+    assert seen == 2

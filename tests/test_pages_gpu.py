@@ -291,6 +291,31 @@ def test_attention(dev, reads, page, n_head, n_kv, q8_0):
     r.free()
 
 
+@pytest.mark.parametrize("q8_0", [False, True], ids=["f16", "q8_0"])
+@pytest.mark.parametrize("n_head,n_kv,reads", [
+    (16, 8, [(9000, 1)]), (16, 8, [(5000, 1), (-1, 1), (3000, 2), (0, 1), (17, 3), (700, 1)]), (8, 8, [(4000, 32)]),
+    (48, 16, [(2100, 1), (2100, 1), (33, 2), (6000, 3)]), (64, 8, [(2500, 1), (1300, 3)]), (24, 24, [(1700, 1)] * 30)])
+def test_attention_of_few_rows(dev, n_head, n_kv, reads, q8_0):
+    """rows that one launch takes: the parts of a cut tile joined by the last of its workgroups, call after call, eager and replayed"""
+    r = Reads(dev, reads, 32, n_kv, q8_0, seed=n_head)
+    q = normal(31, r.n, n_head, 128)
+    got = r.run(q, n_head)
+    assert rel_rows(got, r.want(q, SCALE)) < BAR
+    qb, out = dev.upload(q), dev.alloc(q.nbytes)
+    dev.capture_begin()
+    htr.page_attention(dev, qb, r.pages, r.cache.kv, n_head, SCALE, out)
+    g = dev.capture_end()
+    for i in range(5):
+        out.upload(np.full(q.size, 2.5, np.float32))
+        for _ in range(8):
+            g.launch()
+        np.testing.assert_array_equal(bits(out.download(np.float32, q.size)), bits(got.ravel()))
+        np.testing.assert_array_equal(bits(r.run(q, n_head)), bits(got))
+    for b in (g, qb, out):
+        b.free()
+    r.free()
+
+
 def test_attention_of_many_reads(dev):
     """1024 reads, of which the last 24 hold more rows"""
     reads = [(i % 40, 1) for i in range(1000)] + [(400 + 13 * i, 1 + i % 3) for i in range(24)]
