@@ -11,9 +11,9 @@
 // length on it its keys and COST more for its start and end, and the head's workgroups take equal pieces of the line, wherever
 // that cuts a tile: one read of many keys goes to all of them, of many short ones each takes a few, and no list of work is made
 // first. Where a piece begins follows from sums over the reads, a lane a read. The parts of a cut tile are joined by a second
-// launch. (Joined by a tile's last workgroup in the same launch one token took 12.5 µs, but 32 parts of a wide tile went through
-// one workgroup, 65 tokens over 8000 keys 182 µs for 47; in pairs 75. More and smaller pieces, or smaller ones for the workgroups
-// that begin later, were slower: 64 reads' tokens 110 … 124 µs for 105.)
+// launch, of tokens by the last of the tile's workgroups. (So joined, 32 parts of a wide tile went through one workgroup, 65 rows
+// over 8000 keys 182 µs for 47; in pairs 75. More and smaller pieces, or smaller ones for the workgroups that begin later, were
+// slower: 64 reads' tokens 110 … 124 µs for 105.)
 //
 // Tiles come in two heights, each with a line of its own. Of up to 32 rows (a step's token, or what is left of a prompt) the waves
 // share out the keys, every fourth block of 32 to each, loaded into LDS of its own, so that nobody waits for anybody until the
@@ -33,6 +33,8 @@ constexpr int NARROW = KB, WIDE = KB * PW;  // rows of a tile
 constexpr int COST = 128;                   // keys that take as long as a tile's start and end (with 64 four prompts 182 µs for 166)
 constexpr int LEAST = 192;                  // a piece's length, at least: a block for each wave, and a tile's start
 constexpr int SLIVER = 4;                   // blocks of a tile's beginning or end that are not cut off for themselves
+constexpr int FEW = 128;                    // rows of a step (for a KV head) that go by narrow tiles alone where its reads have few
+constexpr float CUT = 2.0f;                 // keys that take as long as joining a row of a part in the launch
 constexpr int TICKET = 32;                  // words between tickets (128 bytes)
 constexpr int SHARES = 4;                   // workgroups of the join to a wide piece
 constexpr int QT = 256 + 256 + 16 + 16;     // 16-byte chunks of a q8_0 buffer: K, V, K scales, V scales
@@ -92,33 +94,44 @@ struct Read {
         start = min(max(s0, 0), a.p.n_row), n = min(max(s1, start), a.p.n_row) - start, past = min(max(held, -1), a.cap);
     }
 };
-template <bool W> __device__ __forceinline__ int64_t line_step(const Args &a, int past) {
-    return (int64_t)(W ? a.group : 1) * (max(past, 0) + (int64_t)COST);
+// the lines: of wide tiles, of the narrow ones behind them, of narrow ones alone
+enum Kind { REST, TALL, ALL };
+template <Kind K> __device__ __forceinline__ int64_t line_step(const Args &a, int past) {
+    return (int64_t)(K == TALL ? a.group : 1) * (max(past, 0) + (int64_t)COST);
 }
-// its length on the line of a height; n: 0 where it has no tile on it
-template <bool W> __device__ __forceinline__ int64_t line_length(const Args &a, Read &x) {
+// a read's length on a line; n: 0 where it has no tile on it
+template <Kind K> __device__ __forceinline__ int64_t line_length(const Args &a, Read &x) {
     const int rows = x.n * a.group, full = rows / WIDE, rest = rows % WIDE;
-    const int64_t step = line_step<W>(a, x.past);
-    x.n = (W ? full == 0 && rest <= NARROW : rest > NARROW || rest == 0) ? 0 : x.n;
-    const int64_t len = W ? full * step + (int64_t)(WIDE / 2) * full * (full + 1) + (rest > NARROW ? step + rows : 0) : step + x.n;
+    const int64_t step = line_step<K>(a, x.past);
+    if constexpr (K == ALL) return (rows + NARROW - 1) / NARROW * (step + x.n);
+    x.n = (K == TALL ? full == 0 && rest <= NARROW : rest > NARROW || rest == 0) ? 0 : x.n;
+    const int64_t len = K == TALL ? full * step + (int64_t)(WIDE / 2) * full * (full + 1) + (rest > NARROW ? step + rows : 0) : step + x.n;
     return x.n ? len : 0;
 }
-// a height's line: the reads' tiles in order. A narrow read's length is its keys and COST. A wide tile's is group times that, up
-// to its last row (of a read's first k tiles k·step + 64·k·(k + 1) in all, step = group·(past + COST))
-template <bool W> struct Line {
+// a line: the reads' tiles in order. A narrow tile's length is its read's keys and COST. A wide one's is group times that, up to
+// its last row (of a read's first k tiles k·step + 64·k·(k + 1) in all, step = group·(past + COST))
+template <Kind K> struct Line {
+    static constexpr bool W = K == TALL;
     const Args &a;
     Reads &r;
     int first = 0;     // the reads at hand: first …
     int64_t base = 0;  // the line's length before them
     int64_t total, piece;
     __device__ __forceinline__ Line(const Args &args, Reads &reads, const Read &x) : a(args), r(reads) {  // x: read `lane`
-        total = load(x);
+        float most = 0.0f;  // ALL: a tile's length by its rows
+        auto look = [&](const Read &y) {
+            if constexpr (K == ALL) most = fmaxf(most, (float)(step(y.past) + y.n) * (float)min(y.n * a.group, NARROW));
+            return load(y);
+        };
+        total = look(x);
         if (a.p.n_seq > 64) {
-            for (; first + 64 < a.p.n_seq; total = load()) base = total, first += 64;
+            while (first + 64 < a.p.n_seq) base = total, first += 64, total = look(Read(a, first + lane_id()));
             first = 0, base = 0;
             load(x);
         }
         piece = uniform(max((int64_t)((double)total * a.per_piece) + 1, (int64_t)LEAST * (W ? a.group : 1)));
+        // (a tile of k keys and r rows in p parts takes k / p keys' time and p·r rows' join, the least at pieces of √(CUT·k·r))
+        if constexpr (K == ALL) piece = max(piece, (int64_t)uniform((int)__builtin_sqrtf(wave_max(most, lane_id()) * CUT)));
     }
     // where piece i begins
     __device__ __forceinline__ int64_t cut(int i) const { return i >= a.pieces ? total : min(i * piece, total); }
@@ -129,12 +142,12 @@ template <bool W> struct Line {
         i += i + 1 < a.pieces && cut(i + 1) <= x;
         return uniform(i);
     }
-    __device__ __forceinline__ int64_t step(int past) const { return line_step<W>(a, past); }
+    __device__ __forceinline__ int64_t step(int past) const { return line_step<K>(a, past); }
     // the reads from `first` on; their end on the line
     __device__ __forceinline__ int64_t load() { return load(Read(a, first + lane_id())); }
     __device__ __forceinline__ int64_t load(Read x) {
         const int lane = lane_id();
-        int64_t end = line_length<W>(a, x);
+        int64_t end = line_length<K>(a, x);
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t lo = __builtin_amdgcn_ds_bpermute(4 * (lane - d), (int)(uint32_t)end), hi = __builtin_amdgcn_ds_bpermute(4 * (lane - d), (int)(end >> 32));
@@ -147,7 +160,8 @@ template <bool W> struct Line {
 };
 
 // a tile on the line
-template <bool W> struct Tile {
+template <Kind K> struct Tile {
+    static constexpr bool W = K == TALL;
     int at;                    // its read: of those at hand
     int start, n, past;        // the read's
     int r0, rows;              // narrow: its first row of the read, its rows; wide: the read's rows in wide tiles
@@ -160,26 +174,28 @@ template <bool W> struct Tile {
         return past < 0 ? -1 : (int)min((uint32_t)past + (uint32_t)i, (uint32_t)a.cap - 1u);
     }
     __device__ __forceinline__ int last_of(const Args &a, int r) const { return last_key(a, query_of(a, min(r, rows - 1))); }
-    __device__ __forceinline__ void of_read(const Line<W> &w, int i) {
+    __device__ __forceinline__ void of_read(const Line<K> &w, int i) {
         at = i, start = uniform(w.r.start[i]), n = uniform(w.r.n[i]), past = uniform(w.r.past[i]);
         rows = n * w.a.group, r0 = rows / WIDE * WIDE;
         if constexpr (!W) rows -= r0;
         else if (rows - r0 <= NARROW) rows = r0;
+        tau = 0;
     }
-    __device__ __forceinline__ void measure(const Line<W> &w) {
+    __device__ __forceinline__ void measure(const Line<K> &w) {
+        if constexpr (K == ALL) r0 = NARROW * tau, rows = min(NARROW, n * w.a.group - r0);
         len = w.step(past) + (W ? min(WIDE * (tau + 1), rows) : n);
-        last = W ? last_of(w.a, WIDE * (tau + 1) - 1) : last_key(w.a, n - 1);
+        last = W ? last_of(w.a, WIDE * (tau + 1) - 1) : last_key(w.a, K == ALL ? query_of(w.a, r0 + rows - 1) : n - 1);
         nb = blocks_to(last);
     }
     // the block that place x of the line (begin < x < begin + len) cuts the tile in front of; 0 and nb: it does not
-    __device__ __forceinline__ int block_at(const Line<W> &w, int64_t x) const {
+    __device__ __forceinline__ int block_at(const Line<K> &w, int64_t x) const {
         const int64_t u = x - begin;
         // (wide: to 22 bits, the same for all that ask)
         const int b = W ? uniform((int)((float)u * __builtin_amdgcn_rcpf((float)here(KB * w.a.group)))) : (int)(u / KB);
         return b < SLIVER ? 0 : b > nb - SLIVER ? nb : b;
     }
     // the one that holds place x of the line, x before its end
-    __device__ __forceinline__ Tile(Line<W> &w, int64_t x) {
+    __device__ __forceinline__ Tile(Line<K> &w, int64_t x) {
         int64_t mine = w.r.end[lane_id()];
         for (int64_t t; (t = lane_of(mine, 63)) <= x && w.first + 64 < w.a.p.n_seq; mine = w.r.end[lane_id()]) {
             w.base = t, w.first += 64;
@@ -187,9 +203,15 @@ template <bool W> struct Tile {
         }
         of_read(w, (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(mine > x) | 1ull << 63));
         begin = at ? lane_of(mine, at - 1) : w.base;
-        tau = 0;
+        const int64_t y = x - begin, step = w.step(past);
+        if constexpr (K == ALL) {
+            const int tiles = (n * w.a.group + NARROW - 1) / NARROW;
+            tau = uniform(min((int)((float)y * __builtin_amdgcn_rcpf((float)(step + n))), tiles - 1));  // (or one beside it)
+            tau -= tau > 0 && tau * (step + n) > y;
+            tau += tau + 1 < tiles && (tau + 1) * (step + n) <= y;
+            begin += tau * (step + n);
+        }
         if constexpr (W) {
-            const int64_t y = x - begin, step = w.step(past);
             const float half = WIDE / 2, mid = 0.5f * ((float)step + half);
             const int tiles = (rows + WIDE - 1) / WIDE;
             tau = uniform(min((int)((float)y / (__builtin_sqrtf(mid * mid + half * (float)y) + mid)), tiles - 1));  // (or one beside it)
@@ -201,9 +223,9 @@ template <bool W> struct Tile {
         measure(w);
     }
     // the next one (there is one)
-    __device__ __forceinline__ void next(Line<W> &w) {
+    __device__ __forceinline__ void next(Line<K> &w) {
         begin += len;
-        if (!W || WIDE * ++tau >= rows) {
+        if (K == REST || (K == ALL ? NARROW * ++tau >= n * w.a.group : WIDE * ++tau >= rows)) {
             uint64_t more;
             for (int from = at + 1;; from = 0) {
                 more = from < 64 ? __builtin_amdgcn_ballot_w64(w.r.n[lane_id()] > 0) >> from << from : 0;
@@ -212,7 +234,6 @@ template <bool W> struct Tile {
                 w.load();
             }
             of_read(w, more ? (int)__builtin_ctzll(more) : 63);
-            tau = 0;
         }
         measure(w);
     }
@@ -223,7 +244,7 @@ struct Share {
     int i0, i1;
     bool all;
 };
-template <bool W> __device__ __forceinline__ Share share_of(const Line<W> &w, const Tile<W> &t, int64_t x0, int64_t x1) {
+template <Kind K> __device__ __forceinline__ Share share_of(const Line<K> &w, const Tile<K> &t, int64_t x0, int64_t x1) {
     Share s{0, t.nb, true};
     if (x0 > t.begin) s.i0 = t.block_at(w, x0);
     if (x1 < t.begin + t.len) s.i1 = t.block_at(w, x1);
@@ -235,14 +256,14 @@ template <bool W> __device__ __forceinline__ Share share_of(const Line<W> &w, co
 __device__ __forceinline__ size_t place_of(const Args &a, const Share &share, int kvh, int piece) {
     return ((size_t)kvh * a.pieces + piece) * 2 + (share.i0 == 0);
 }
-template <bool W> __device__ __forceinline__ void part_of(const Line<W> &w, const Tile<W> &t, Part &to) {
+template <Kind K> __device__ __forceinline__ void part_of(const Line<K> &w, const Tile<K> &t, Part &to) {
     if (threadIdx.x < 64 * (PW - 1)) return;
     int first = w.piece_of(t.begin), end = first + 1;
     if (w.cut(end) < t.begin + t.len && t.block_at(w, w.cut(end)) == 0) first++, end++;  // (it leaves the beginning to the next one)
     for (end = max(w.piece_of(t.begin + t.len - 1) + 1, end); end - 1 > first && t.block_at(w, w.cut(end - 1)) == t.nb;) end--;
     if (threadIdx.x == 64 * (PW - 1))
-        to = W ? Part{first, end - first, t.start, WIDE * t.tau, min(WIDE, t.rows - WIDE * t.tau)}
-               : Part{first, end - first, t.start, t.r0, t.rows};
+        to = K == TALL ? Part{first, end - first, t.start, WIDE * t.tau, min(WIDE, t.rows - WIDE * t.tau)}
+                       : Part{first, end - first, t.start, t.r0, t.rows};
 }
 // the two places of a piece that has no cut tile are empty (the same wave's stores, in order)
 template <bool W> __device__ __forceinline__ void no_parts(const Args &a, int kvh, int piece) {
@@ -283,7 +304,7 @@ struct Run {
                     (uint32_t)(gone >> (2 * (j & 31))) & 3u};
     }
 };
-template <bool W> __device__ __forceinline__ Run run_of(const Args &a, const Line<W> &w, const Tile<W> &t, int b0, int step) {
+template <Kind K> __device__ __forceinline__ Run run_of(const Args &a, const Line<K> &w, const Tile<K> &t, int b0, int step) {
     return Run{a.p.table + (size_t)(w.first + t.at) * a.p.max_pages, b0, step, t.last, a.p.shift, a.n_page, 0, 0};
 }
 // the keys of block i that a row of `keys` sees, of the lane's 16 (bits 0 … 3, 8 … 11, 16 …, 24 …)
@@ -312,6 +333,7 @@ struct Join {
     float2 ml[8];
 };
 template <bool XL> __device__ __forceinline__ void join_rows(const Args &a, int w, int kvh, const Part &t, int ra, int rb, Join &sh) {
+    constexpr int U = XL ? 8 : 4;  // parts of a row at once: here the row's one workgroup waits for each load, there many do
     const int tid = threadIdx.x, gr = tid >> 5, j = tid & 31, nr = rb - ra;
     const Parts &p = a.part[w];
     const int height = w ? WIDE : NARROW;
@@ -320,61 +342,62 @@ template <bool XL> __device__ __forceinline__ void join_rows(const Args &a, int 
         const float2 lo = get64(from), hi = get64(&from->z);
         return make_float4(lo.x, lo.y, hi.x, hi.y);
     };
-            const int lg = nr > 4 ? 3 : nr > 2 ? 2 : nr > 1 ? 1 : 0, G = 8 >> lg;  // 2^lg rows at once, G groups to each
-            for (int r = ra; r < rb; r += 1 << lg) {
-                const int row = min(r + (gr & ((1 << lg) - 1)), rb - 1), g = gr >> lg;
-                float top = M_NONE, sum = 0.0f;
-                float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                float c = 0.0f;
-                // (in floats: below 2^25)
-                const uint32_t at0 = ((uint32_t)(kvh * a.pieces + t.first) * 2) * height + row;
-                for (int e0 = g; e0 < t.n; e0 += 4 * G) {
-                    float4 ml[4], in[4];
-    #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const int e = e0 + q * G;
-                        ml[q] = make_float4(M_NONE, 0.0f, c, 0.0f), in[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (e < t.n) {
-                            const uint32_t at = at0 + (uint32_t)(2 * e + (e == 0)) * height;
-                            ml[q] = get(p.ml + at);
-                            in[q] = get(reinterpret_cast<const float4 *>(p.sums + (at * D + 4 * j)));
-                        }
-                    }
-                    c = ml[0].z;  // (a row's parts have the same)
-                    const float to = fmaxf(fmaxf(top, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
-                    const float f = __builtin_amdgcn_exp2f((top - to) * c);
-                    top = to, sum *= f, y.x *= f, y.y *= f, y.z *= f, y.w *= f;
-    #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const float h = __builtin_amdgcn_exp2f((ml[q].x - to) * c);
-                        sum = fmaf(ml[q].y, h, sum);
-                        y.x = fmaf(in[q].x, h, y.x), y.y = fmaf(in[q].y, h, y.y), y.z = fmaf(in[q].z, h, y.z), y.w = fmaf(in[q].w, h, y.w);
-                    }
-                }
-                if (G > 1) {  // (one pass)
-                    __syncthreads();
-                    sh.y[gr][j] = y;
-                    if (j == 0) sh.ml[gr] = make_float2(top, sum);
-                    __syncthreads();
-                    if (g == 0) {
-                        float to = top;
-                        for (int e = 1; e < G; e++) to = fmaxf(to, sh.ml[gr + (e << lg)].x);
-                        const float f = __builtin_amdgcn_exp2f((top - to) * c);
-                        sum *= f, y.x *= f, y.y *= f, y.z *= f, y.w *= f;
-                        for (int e = 1; e < G; e++) {
-                            const float4 z = sh.y[gr + (e << lg)][j];
-                            const float2 ml = sh.ml[gr + (e << lg)];
-                            const float h = __builtin_amdgcn_exp2f((ml.x - to) * c);
-                            sum = fmaf(ml.y, h, sum);
-                            y.x = fmaf(z.x, h, y.x), y.y = fmaf(z.y, h, y.y), y.z = fmaf(z.z, h, y.z), y.w = fmaf(z.w, h, y.w);
-                        }
-                    }
-                }
-                if (g == 0 && r + (gr & ((1 << lg) - 1)) < rb) {
-                    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
-                    *reinterpret_cast<float4 *>(out_row(a, t.start, kvh, t.r0 + row) + 4 * j) = make_float4(y.x * by, y.y * by, y.z * by, y.w * by);
+    const int lg = nr > 4 ? 3 : nr > 2 ? 2 : nr > 1 ? 1 : 0, G = 8 >> lg;  // 2^lg rows at once, G groups to each
+    for (int r = ra; r < rb; r += 1 << lg) {
+        const int row = min(r + (gr & ((1 << lg) - 1)), rb - 1), g = gr >> lg;
+        float top = M_NONE, sum = 0.0f;
+        float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float c = 0.0f;
+        const uint32_t at0 = ((uint32_t)(kvh * a.pieces + t.first) * 2) * height + row;  // (times 128: below 2^25)
+        for (int e0 = g; e0 < t.n; e0 += U * G) {
+            float4 ml[U], in[U];
+#pragma unroll
+            for (int q = 0; q < U; q++) {
+                const int e = e0 + q * G;
+                ml[q] = make_float4(M_NONE, 0.0f, c, 0.0f), in[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (e < t.n) {
+                    const uint32_t at = at0 + (uint32_t)(2 * e + (e == 0)) * height;
+                    ml[q] = get(p.ml + at);
+                    in[q] = get(reinterpret_cast<const float4 *>(p.sums + (at * D + 4 * j)));
                 }
             }
+            c = ml[0].z;  // (a row's parts have the same)
+            float to = top;
+#pragma unroll
+            for (int q = 0; q < U; q++) to = fmaxf(to, ml[q].x);
+            const float f = __builtin_amdgcn_exp2f((top - to) * c);
+            top = to, sum *= f, y.x *= f, y.y *= f, y.z *= f, y.w *= f;
+#pragma unroll
+            for (int q = 0; q < U; q++) {
+                const float h = __builtin_amdgcn_exp2f((ml[q].x - to) * c);
+                sum = fmaf(ml[q].y, h, sum);
+                y.x = fmaf(in[q].x, h, y.x), y.y = fmaf(in[q].y, h, y.y), y.z = fmaf(in[q].z, h, y.z), y.w = fmaf(in[q].w, h, y.w);
+            }
+        }
+        if (G > 1) {  // (one pass)
+            __syncthreads();
+            sh.y[gr][j] = y;
+            if (j == 0) sh.ml[gr] = make_float2(top, sum);
+            __syncthreads();
+            if (g == 0) {
+                float to = top;
+                for (int e = 1; e < G; e++) to = fmaxf(to, sh.ml[gr + (e << lg)].x);
+                const float f = __builtin_amdgcn_exp2f((top - to) * c);
+                sum *= f, y.x *= f, y.y *= f, y.z *= f, y.w *= f;
+                for (int e = 1; e < G; e++) {
+                    const float4 z = sh.y[gr + (e << lg)][j];
+                    const float2 ml = sh.ml[gr + (e << lg)];
+                    const float h = __builtin_amdgcn_exp2f((ml.x - to) * c);
+                    sum = fmaf(ml.y, h, sum);
+                    y.x = fmaf(z.x, h, y.x), y.y = fmaf(z.y, h, y.y), y.z = fmaf(z.z, h, y.z), y.w = fmaf(z.w, h, y.w);
+                }
+            }
+        }
+        if (g == 0 && r + (gr & ((1 << lg) - 1)) < rb) {
+            const float by = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key seen: zeros
+            *reinterpret_cast<float4 *>(out_row(a, t.start, kvh, t.r0 + row) + 4 * j) = make_float4(y.x * by, y.y * by, y.z * by, y.w * by);
+        }
+    }
 }
 
 // ---- reads of few rows -------------------------------------------------------------------------------------------------------
@@ -382,15 +405,16 @@ template <bool XL> __device__ __forceinline__ void join_rows(const Args &a, int 
 // A wave's block is K and V in its own LDS (layouts and products are k_kv_attn_split's): f16 one buffer each, filled again as soon
 // as it is read, q8_0 raw in two.
 //
-// Bound: of few keys latency (a token over 1300 keys 12.5 µs, of which lengths, pages, keys, each a load that the next one waits
-// for, 6 µs, and the second launch 4); of many HBM: 64 reads' tokens over 300 … 6000 f16 keys (505 MB) 105 µs, over q8_0 rows
-// (269 MB) 74, at 6.6 TB/s while all workgroups run, which end between 56 and 101 µs.
+// Bound: of few keys latency (a token over 1300 keys 10.9 µs, of which lengths, pages, keys, each a load that the next one waits
+// for, 5 µs, and the join 2); of many HBM: 64 reads' tokens over 300 … 6000 f16 keys (505 MB) 100 µs, over 8000 (2.1 GB) 350, 6.2 TB/s
+// of them from one to the other; over q8_0 rows (269 MB) 67, where conversions and softmax take as long as the loads.
 template <bool Q8, bool ONE> __device__ __forceinline__ void narrow(const Args &a, int kvh, int piece, const Read &x, uint4_t *s_kv, Shared &sh) {
     constexpr int WAVE = Q8 ? WAVE_Q8 : WAVE_F16;
     static_assert(WAVE >= 1024, "a wave's sums fit");
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), hf = lane >> 5, c = lane & 31;
     if (!ONE && a.pieces > 1) no_parts<false>(a, kvh, piece);
-    Line<false> line(a, sh.reads[wave], x);
+    constexpr Kind K = ONE ? ALL : REST;
+    Line<K> line(a, sh.reads[wave], x);
     const int64_t x0 = line.cut(piece), x1 = line.cut(piece + 1);
     if (x0 >= x1) return;
     const size_t head0 = (size_t)kvh * a.kv.n_ctx;
@@ -428,7 +452,7 @@ template <bool Q8, bool ONE> __device__ __forceinline__ void narrow(const Args &
     for (int u = 0; u < 4; u++)
         va[u] = Q8 ? 16 * (256 + 8 * vrow + ((2 * u + ((lane >> 4) & 1)) ^ (vrow & 2) ^ ((vrow & 8) >> 1))) + 8 * (lane & 1)
                    : 16 * (K_CHUNKS + 16 * vrow + ((4 * u + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (4 * (vrow & 3)))) + 8 * (lane & 1);
-    for (Tile<false> t(line, x0);; t.next(line)) {
+    for (Tile<K> t(line, x0);; t.next(line)) {
         const Share own = share_of(line, t, x0, x1);
         if (own.i0 < own.i1 || own.all) {
             const int i1 = own.i1, rc = t.r0 + min(c, t.rows - 1);
@@ -681,12 +705,12 @@ template <bool Q8, bool ONE> __device__ __forceinline__ void narrow(const Args &
 template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, int piece, const Read &x, uint4_t *s_kv, Shared &sh) {
     const int wave = uniform((int)threadIdx.x >> 6);
     if (a.pieces > 1) no_parts<true>(a, kvh, piece);
-    Line<true> line(a, sh.reads[wave], x);
+    Line<TALL> line(a, sh.reads[wave], x);
     const int64_t x0 = line.cut(piece), x1 = line.cut(piece + 1);
     if (x0 >= x1) return;
     const size_t head0 = (size_t)kvh * a.kv.n_ctx;
 
-    for (Tile<true> t(line, x0);; t.next(line)) {
+    for (Tile<TALL> t(line, x0);; t.next(line)) {
         const Share own = share_of(line, t, x0, x1);
         if (own.i0 < own.i1 || own.all) {
             const int lane = lane_id(), hf = lane >> 5, c = lane & 31;
@@ -983,8 +1007,9 @@ template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_attn(Arg
     else wide<Q8>(a, kvh, piece, mine, s_kv, sh);
 }
 
-// Few rows, where a head's workgroups share an XCD: narrow tiles alone, the parts of a cut one joined by the last of them (a token over
-// 1300 keys 11.3 µs, by a second launch 12.5)
+// Tokens, where a head's workgroups share an XCD: narrow tiles alone, the parts of a cut one joined by the last of its workgroups. A
+// token over 1300 keys 10.9 µs, by the other kernel and its second launch 12.9; 64 reads' 100 for 104, 16 and 48 rows of another read
+// 33 for 38, 200 tokens 212 for 218. But a read of 16 rows over 32000 keys 41 for 34, of 64 rows 62 for 59, of 130 rows 102 for 72.
 template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_few(Args a) {
     __shared__ __attribute__((aligned(16))) uint4_t s_kv[PW * (Q8 ? WAVE_Q8 : WAVE_F16)];
     __shared__ Shared sh;
@@ -1044,17 +1069,20 @@ extern "C" int htr_page_attention(htr_device *dev, const float *d_q, size_t q_st
     a.pieces = std::max(1, 2 * dev->n_cu / kv->n_kv), a.per_piece = 1.0 / a.pieces;
     a.wide = n * group > NARROW ? a.pieces : 0;
     if (a.pieces > 1) {
-        const size_t n = (size_t)2 * dev->n_cu;
+        const size_t at_once = (size_t)2 * dev->n_cu;
         void *p;
-        HTR_TRY(htr_scratch(dev, SCR_PAGE_TICKET, n * TICKET * 4, &p));
-        // few rows, and a head's workgroups on one XCD (a launch's go to the 8 XCDs in turn)
-        if (!a.wide && kv->n_kv % 8 == 0 && dev->xcd_round_robin == 1) a.tickets = (uint32_t *)p;
-        HTR_TRY(htr_scratch(dev, SCR_PAGE_ATTN, 2 * n * ((NARROW + WIDE) * (D + 4) * 4 + 2 * sizeof(Part)), &p));
+        HTR_TRY(htr_scratch(dev, SCR_PAGE_TICKET, at_once * TICKET * 4, &p));
+        // tokens, by what the sizes say: up to 4 rows a read of few, 1¼ of many; and a head's workgroups on one XCD (a launch's go
+        // to the 8 XCDs in turn)
+        const size_t reads = (size_t)a.p.n_seq;
+        if (n <= (n * group <= FEW ? 4 * reads : reads + reads / 4) && kv->n_kv % 8 == 0 && dev->xcd_round_robin == 1)
+            a.tickets = (uint32_t *)p, a.wide = 0;
+        HTR_TRY(htr_scratch(dev, SCR_PAGE_ATTN, 2 * at_once * ((NARROW + WIDE) * (D + 4) * 4 + 2 * sizeof(Part)), &p));
         float *at = (float *)p;
         for (int w = 0; w < 2; w++) {
-            const size_t rows = 2 * n * (w ? WIDE : NARROW);
+            const size_t rows = 2 * at_once * (w ? WIDE : NARROW);
             a.part[w] = Parts{at, (float4 *)(at + rows * D), (Part *)(at + rows * (D + 4))};
-            at += rows * (D + 4) + 2 * n * sizeof(Part) / 4;
+            at += rows * (D + 4) + 2 * at_once * sizeof(Part) / 4;
         }
     }
     const unsigned groups = (unsigned)((a.wide + a.pieces) * kv->n_kv);

@@ -271,7 +271,7 @@ int htr_qkv_post_pages(htr_device *dev, const float *d_q, size_t q_stride, const
  * for the rows of a read that is not served, the rows behind the last read left as they were. Rows past the table's width are
  * not there. Otherwise as htr_tree_attention in what a row does not see and in what numbers are held to; the same call gives
  * the same bits every time, while a read's last bits depend on the reads beside it (their lengths say where its keys are shared
- * out). Scratch: two workgroups a CU for each of two heights of tile, 86 MB on 256 CUs, the same for every call, made at the
+ * out). Scratch: two workgroups a CU for each of two heights of tile, 87 MB on 256 CUs, the same for every call, made at the
  * first one, which cannot be one that is being captured. With g q heads to a KV head n_row·g² < 2^31, n_row·g ≤ 2^30 and
  * n_seq·g·(n_row·g / 128 + 2)·(max_pages·page + n_row·g + 128) < 2^62 (else refused). Reads pages->d_start, d_past and d_table. */
 int htr_page_attention(htr_device *dev, const float *d_q, size_t q_stride, const htr_pages *pages, const htr_kv *kv, int n_head,
