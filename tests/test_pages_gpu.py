@@ -633,14 +633,16 @@ def poisoned():
     d.close()
 
 
-def test_two_devices_at_once(dev, poisoned):
+@pytest.mark.parametrize("n_head,n_kv,reads", [(4, 2, [(2500, 1), (300, 140), (4000, 1), (-1, 2)]),
+                                               (16, 8, [(2500, 1), (300, 6), (4000, 1), (-1, 2)])], ids=["chunks", "tokens"])
+def test_two_devices_at_once(dev, poisoned, n_head, n_kv, reads):
     """calls of two handles that overlap, eager and replayed, each with tiles and rows in parts: the bits of either alone, where
     scratch was NaN before its first use too"""
-    reads, n_head, vocab, top = [(2500, 1), (300, 140), (4000, 1), (-1, 2)], 4, 151936, 7
+    vocab, top = 151936, 7
     logits = normal(4, 3, vocab, std=2.5)
     sides = []
     for d in (dev, poisoned):
-        r = Reads(d, reads, 32, 2, seed=6)
+        r = Reads(d, reads, 32, n_kv, seed=6)
         q = normal(8, r.n, n_head, 128)
         b = [d.upload(a) for a in (q, logits, np.array([5, 70000, vocab - 1], np.int32))]
         out = [d.alloc(4 * n) for n in (q.size, 3, 3, 3 * top, 3 * top)]
