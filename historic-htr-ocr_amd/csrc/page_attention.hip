@@ -33,7 +33,7 @@ constexpr int NARROW = KB, WIDE = KB * PW;  // rows of a tile
 constexpr int COST = 128;                   // keys that take as long as a tile's start and end (with 64 four prompts 182 µs for 166)
 constexpr int LEAST = 192;                  // a piece's length, at least: a block for each wave, and a tile's start
 constexpr int SLIVER = 4;                   // blocks of a tile's beginning or end that are not cut off for themselves
-constexpr int FEW = 128;                    // rows of a step (for a KV head) that go by narrow tiles alone where its reads have few
+constexpr int FEW = 128;                    // rows of a step (for a KV head) that go by narrow tiles alone, up to 4 of a read's on average
 constexpr float CUT = 2.0f;                 // keys that take as long as joining a row of a part in the launch
 constexpr int TICKET = 32;                  // words between tickets (128 bytes)
 constexpr int SHARES = 4;                   // workgroups of the join to a wide piece
@@ -1009,7 +1009,8 @@ template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_attn(Arg
 
 // Tokens, where a head's workgroups share an XCD: narrow tiles alone, the parts of a cut one joined by the last of its workgroups. A
 // token over 1300 keys 10.9 µs, by the other kernel and its second launch 12.9; 64 reads' 100 for 104, 16 and 48 rows of another read
-// 33 for 38, 200 tokens 212 for 218. But a read of 16 rows over 32000 keys 41 for 34, of 64 rows 62 for 59, of 130 rows 102 for 72.
+// 33 for 38. But a read of 16 rows over 32000 keys 41 for 34, of 64 rows 62 for 59; and of more rows, where a step of 200 tokens
+// would take 212 for 218, one read of 130 102 for 72.
 template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_few(Args a) {
     __shared__ __attribute__((aligned(16))) uint4_t s_kv[PW * (Q8 ? WAVE_Q8 : WAVE_F16)];
     __shared__ Shared sh;
@@ -1072,10 +1073,8 @@ extern "C" int htr_page_attention(htr_device *dev, const float *d_q, size_t q_st
         const size_t at_once = (size_t)2 * dev->n_cu;
         void *p;
         HTR_TRY(htr_scratch(dev, SCR_PAGE_TICKET, at_once * TICKET * 4, &p));
-        // tokens, by what the sizes say: up to 4 rows a read of few, 1¼ of many; and a head's workgroups on one XCD (a launch's go
-        // to the 8 XCDs in turn)
-        const size_t reads = (size_t)a.p.n_seq;
-        if (n <= (n * group <= FEW ? 4 * reads : reads + reads / 4) && kv->n_kv % 8 == 0 && dev->xcd_round_robin == 1)
+        // tokens, by what the sizes say, and a head's workgroups on one XCD (a launch's go to the 8 XCDs in turn)
+        if (n * group <= FEW && n <= 4 * (size_t)a.p.n_seq && kv->n_kv % 8 == 0 && dev->xcd_round_robin == 1)
             a.tickets = (uint32_t *)p, a.wide = 0;
         HTR_TRY(htr_scratch(dev, SCR_PAGE_ATTN, 2 * at_once * ((NARROW + WIDE) * (D + 4) * 4 + 2 * sizeof(Part)), &p));
         float *at = (float *)p;
