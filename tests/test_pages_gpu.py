@@ -297,7 +297,8 @@ def test_attention(dev, reads, page, n_head, n_kv, q8_0):
     (48, 16, [(2100, 1), (2100, 1), (33, 2), (6000, 3)]), (64, 8, [(2500, 1), (1300, 3)]), (24, 24, [(1700, 1)] * 30),
     # reads of many rows among those of few: several tiles to a read
     (16, 8, [(300, 50)] + [(5, 0)] * 14 + [(900, 1)]), (8, 8, [(2, 0)] * 30 + [(-1, 1), (0, 100), (1900, 20)]),
-    (16, 8, [(37 * i % 900, 1) for i in range(190)] + [(700, 30), (0, 12)]), (16, 8, [(9, 0)] * 70 + [(2500, 33), (64, 40), (-1, 9)])])
+    (16, 8, [(37 * i % 900, 1) for i in range(190)] + [(700, 30), (0, 12)]), (16, 8, [(9, 0)] * 70 + [(2500, 33), (64, 40), (-1, 9)]),
+    (8, 8, [(9, 0)] * 70 + [(2500, 33), (64, 40), (-1, 9)] + [(3, 1)] * 30)])
 def test_attention_of_few_rows(dev, n_head, n_kv, reads, q8_0):
     """rows that one launch takes: the parts of a cut tile joined by the last of its workgroups, call after call, eager and replayed"""
     r = Reads(dev, reads, 32, n_kv, q8_0, seed=n_head)
