@@ -327,18 +327,18 @@ struct Shared {
 };
 
 // The rows ra … rb − 1 of a cut tile: 32 lanes of 4 dims to a row; where the rows are fewer than the groups of 32, several groups to
-// a row's parts. XL: parts that workgroups of this launch stored, in the L2 of the XCD that they share
+// a row's parts. HERE: parts that workgroups of this launch stored
 struct Join {
     float4 y[8][32];
     float2 ml[8];
 };
-template <bool XL> __device__ __forceinline__ void join_rows(const Args &a, int w, int kvh, const Part &t, int ra, int rb, Join &sh) {
-    constexpr int U = XL ? 8 : 4;  // parts of a row at once: here the row's one workgroup waits for each load, there many do
+template <bool HERE> __device__ __forceinline__ void join_rows(const Args &a, int w, int kvh, const Part &t, int ra, int rb, Join &sh) {
+    constexpr int U = HERE ? 8 : 4;  // parts of a row at once: here the row's one workgroup waits for each load, there many do
     const int tid = threadIdx.x, gr = tid >> 5, j = tid & 31, nr = rb - ra;
     const Parts &p = a.part[w];
     const int height = w ? WIDE : NARROW;
     auto get = [](const float4 *from) {
-        if constexpr (!XL) return *from;
+        if constexpr (!HERE) return *from;
         const float2 lo = get64(from), hi = get64(&from->z);
         return make_float4(lo.x, lo.y, hi.x, hi.y);
     };
@@ -408,7 +408,10 @@ template <bool XL> __device__ __forceinline__ void join_rows(const Args &a, int 
 // Bound: of few keys latency (a token over 1300 keys 10.9 µs, of which lengths, pages, keys, each a load that the next one waits
 // for, 5 µs, and the join 2); of many HBM: 64 reads' tokens over 300 … 6000 f16 keys (505 MB) 100 µs, over 8000 (2.1 GB) 350, 6.2 TB/s
 // of them from one to the other; over q8_0 rows (269 MB) 67, where conversions and softmax take as long as the loads.
-template <bool Q8, bool ONE> __device__ __forceinline__ void narrow(const Args &a, int kvh, int piece, const Read &x, uint4_t *s_kv, Shared &sh) {
+// JOIN: who joins the parts of a cut tile: a second launch, or the last of its workgroups, which share an XCD or do not
+enum Joins { SECOND, NEAR, FAR };
+template <bool Q8, Joins JOIN> __device__ __forceinline__ void narrow(const Args &a, int kvh, int piece, const Read &x, uint4_t *s_kv, Shared &sh) {
+    constexpr bool ONE = JOIN != SECOND, XL = JOIN == NEAR;
     constexpr int WAVE = Q8 ? WAVE_Q8 : WAVE_F16;
     static_assert(WAVE >= 1024, "a wave's sums fit");
     const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6), hf = lane >> 5, c = lane & 31;
@@ -665,16 +668,17 @@ template <bool Q8, bool ONE> __device__ __forceinline__ void narrow(const Args &
             if (ONE && !own.all) {
                 if (c < t.rows) {
 #pragma unroll
-                    for (int x = 0; x < 4; x++) put64(to + 8 * x, y[x].x, y[x].y, true), put64(to + 8 * x + 2, y[x].z, y[x].w, true);
-                    if (wave == 0 && hf == 0) put64(ml, m, l, true), put64(&ml->z, sc, 0.0f, true);
+                    for (int x = 0; x < 4; x++) put64(to + 8 * x, y[x].x, y[x].y, XL), put64(to + 8 * x + 2, y[x].z, y[x].w, XL);
+                    if (wave == 0 && hf == 0) put64(ml, m, l, XL), put64(&ml->z, sc, 0.0f, XL);
                 }
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's stores are performed
                 __syncthreads();
                 const Part whole = sh.part;
                 if (threadIdx.x == 0) {
                     uint32_t *ticket = a.tickets + (size_t)TICKET * (kvh * a.pieces + whole.first);
-                    sh.last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) == (uint32_t)(whole.n - 1);
-                    if (sh.last) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);  // for the next call
+                    constexpr int SCOPE = XL ? __HIP_MEMORY_SCOPE_WORKGROUP : __HIP_MEMORY_SCOPE_AGENT;
+                    sh.last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, SCOPE) == (uint32_t)(whole.n - 1);
+                    if (sh.last) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, SCOPE);  // for the next call
                 }
                 __syncthreads();
                 if (sh.last) {
@@ -1003,18 +1007,18 @@ template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_attn(Arg
         piece = unit < n ? unit : unit < 2 * n + left ? unit - n : unit - n - left;
         is_narrow = other != narrow_first;
     }
-    if (uniform((int)is_narrow)) narrow<Q8, false>(a, kvh, piece, mine, s_kv, sh);
+    if (uniform((int)is_narrow)) narrow<Q8, SECOND>(a, kvh, piece, mine, s_kv, sh);
     else wide<Q8>(a, kvh, piece, mine, s_kv, sh);
 }
 
-// Tokens, where a head's workgroups share an XCD: narrow tiles alone, the parts of a cut one joined by the last of its workgroups. A
-// token over 1300 keys 10.9 µs, by the other kernel and its second launch 12.9; 64 reads' 100 for 104, 16 and 48 rows of another read
-// 33 for 38. But a read of 16 rows over 32000 keys 41 for 34, of 64 rows 62 for 59; and of more rows, where a step of 200 tokens
-// would take 212 for 218, one read of 130 102 for 72.
-template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_few(Args a) {
+// Tokens: narrow tiles alone, the parts of a cut one joined by the last of its workgroups. A token over 1300 keys 10.9 µs, by the
+// other kernel and its second launch 12.9; 64 reads' 100 for 104, 16 and 48 rows of another read 33 for 38; on one KV head, whose
+// workgroups are on all XCDs, 7 tokens 13.9 for 16.4. But a read of 16 rows over 32000 keys 41 for 34, of 64 rows 62 for 59; and of
+// more rows, where a step of 200 tokens would take 212 for 218, one read of 130 102 for 72.
+template <bool Q8, Joins JOIN> __global__ __launch_bounds__(64 * PW, 2) void k_page_few(Args a) {
     __shared__ __attribute__((aligned(16))) uint4_t s_kv[PW * (Q8 ? WAVE_Q8 : WAVE_F16)];
     __shared__ Shared sh;
-    narrow<Q8, true>(a, blockIdx.x % a.kv.n_kv, blockIdx.x / a.kv.n_kv, Read(a, lane_id()), s_kv, sh);
+    narrow<Q8, JOIN>(a, blockIdx.x % a.kv.n_kv, blockIdx.x / a.kv.n_kv, Read(a, lane_id()), s_kv, sh);
 }
 
 // The second launch: the rows of a cut tile shared out among as many workgroups as it has parts (SHARES times as many), those of
@@ -1073,9 +1077,7 @@ extern "C" int htr_page_attention(htr_device *dev, const float *d_q, size_t q_st
         const size_t at_once = (size_t)2 * dev->n_cu;
         void *p;
         HTR_TRY(htr_scratch(dev, SCR_PAGE_TICKET, at_once * TICKET * 4, &p));
-        // tokens, by what the sizes say, and a head's workgroups on one XCD (a launch's go to the 8 XCDs in turn)
-        if (n * group <= FEW && n <= 4 * (size_t)a.p.n_seq && kv->n_kv % 8 == 0 && dev->xcd_round_robin == 1)
-            a.tickets = (uint32_t *)p, a.wide = 0;
+        if (n * group <= FEW && n <= 4 * (size_t)a.p.n_seq) a.tickets = (uint32_t *)p, a.wide = 0;  // tokens, by what the sizes say
         HTR_TRY(htr_scratch(dev, SCR_PAGE_ATTN, 2 * at_once * ((NARROW + WIDE) * (D + 4) * 4 + 2 * sizeof(Part)), &p));
         float *at = (float *)p;
         for (int w = 0; w < 2; w++) {
@@ -1087,8 +1089,11 @@ extern "C" int htr_page_attention(htr_device *dev, const float *d_q, size_t q_st
     const unsigned groups = (unsigned)((a.wide + a.pieces) * kv->n_kv);
     const dim3 g(groups), b(64 * PW);
     if (a.tickets) {
-        if (a.kv.q8) hipLaunchKernelGGL(k_page_few<true>, g, b, 0, dev->stream, a);
-        else hipLaunchKernelGGL(k_page_few<false>, g, b, 0, dev->stream, a);
+        const bool near = kv->n_kv % 8 == 0 && dev->xcd_round_robin == 1;  // (a launch's workgroups go to the 8 XCDs in turn)
+        if (a.kv.q8 && near) hipLaunchKernelGGL((k_page_few<true, NEAR>), g, b, 0, dev->stream, a);
+        else if (a.kv.q8) hipLaunchKernelGGL((k_page_few<true, FAR>), g, b, 0, dev->stream, a);
+        else if (near) hipLaunchKernelGGL((k_page_few<false, NEAR>), g, b, 0, dev->stream, a);
+        else hipLaunchKernelGGL((k_page_few<false, FAR>), g, b, 0, dev->stream, a);
         return htr_launched(dev, a.kv.q8 ? "k_page_few<q8_0>" : "k_page_few<f16>");
     }
     if (a.kv.q8) hipLaunchKernelGGL(k_page_attn<true>, g, b, 0, dev->stream, a);

@@ -24,4 +24,4 @@ def test_none_crosses_a_barrier_of_few_rows(tmp_path):
         barriers = _pending_at_barriers(body)
         assert len(barriers) >= 3, name
         assert all(n == 0 for n in barriers.values()), (name, barriers)
-    assert seen == 2
+    assert seen == 4
