@@ -11,6 +11,7 @@
 // alone, and pages of ended reads go behind the last free one, which no read of this step looks at. So a call writes nothing
 // that it reads but the lengths and the pool, each of which its thread has read before the sums: both may be written in place.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_ops.h"
 
@@ -19,7 +20,9 @@ namespace {
 // A thread a read: one workgroup, of 256 threads for up to 256 reads and 1024 rows (24 reads of a token 4.0 µs, by 1024 threads
 // 4.4), else of 1024. Up to 4096 rows it maps the rows too, more are a second launch's.
 constexpr int SMALL = 256, SMALL_ROWS = 1024, ROWS_ONE = 4096;
-constexpr int AT_ONCE = 4;  // searches of a thread beside each other: each is ten LDS reads behind one another
+// searches of a thread beside each other, each ten LDS reads behind one another, where there are more than four to a thread (8000
+// pages 17.2 µs for 18.0); fewer go one by one (582 reads of a token, 36 of which end, 7.3 µs for 9.9)
+constexpr int AT_ONCE = 4;
 
 struct MapArgs {
     HtrPages p;
@@ -28,17 +31,17 @@ struct MapArgs {
     int n_page;
 };
 
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+template <typename T> __device__ __forceinline__ T wave_scan(T v) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(v, d);
+        const T o = __shfl_up(v, d);
         if (lane >= d) v += o;
     }
     return v;
 }
 // Σ of v over the threads up to and with this one
-__device__ uint32_t block_scan(uint32_t v, uint32_t *s_wave) {
+template <typename T> __device__ __forceinline__ T block_scan(T v, T *s_wave) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     v = wave_scan(v);
     __syncthreads();  // (the waves' sums of the scan before are read)
@@ -67,6 +70,7 @@ __device__ __forceinline__ int slot_of(int page, int n_page, int pos, int shift)
 
 template <int THREADS> __global__ __launch_bounds__(THREADS) void k_page_map(MapArgs a, int map_rows) {
     __shared__ uint32_t s_end[THREADS], s_upto[THREADS], s_back[THREADS], s_wave[THREADS / 64], s_taken;
+    __shared__ unsigned long long s_two[THREADS / 64];
     __shared__ int s_past[THREADS], s_held[THREADS], s_need[THREADS];
     const int b = threadIdx.x, shift = a.p.shift;
     const bool there = b < a.p.n_seq;
@@ -77,12 +81,13 @@ template <int THREADS> __global__ __launch_bounds__(THREADS) void k_page_map(Map
     const bool ends = add < 0;
     const uint32_t mask = (1u << shift) - 1, held = len <= 0 ? 0 : ((uint32_t)len + mask) >> shift;
     if (b == 0) s_taken = 0;
-    const uint32_t end = block_scan(ends ? 0u : (uint32_t)min(add, a.p.n_row + 1), s_wave);
+    // (both sums fit 32 bits)
+    const unsigned long long two = block_scan(ends ? (unsigned long long)min(held, (uint32_t)a.p.max_pages) << 32 : (unsigned long long)min(add, a.p.n_row + 1), s_two);
+    const uint32_t end = (uint32_t)two, back = (uint32_t)(two >> 32);
     const bool fits = there && !ends && len >= 0 && (int64_t)len + add <= (int64_t)a.p.max_pages << shift && end <= (uint32_t)a.p.n_row;
     const uint32_t need = fits ? (((uint32_t)len + (uint32_t)add + mask) >> shift) - held : 0u;
     const uint32_t upto = block_scan(need, s_wave);
     const bool served = fits && (need == 0 || upto <= count);
-    const uint32_t back = block_scan(ends ? min(held, (uint32_t)a.p.max_pages) : 0u, s_wave);
     s_end[b] = min(end, (uint32_t)a.p.n_row), s_upto[b] = upto, s_back[b] = back;
     s_past[b] = served ? len : -1, s_held[b] = (int)held, s_need[b] = (int)need;
     if (served && need) atomicMax(&s_taken, upto);
@@ -102,53 +107,55 @@ template <int THREADS> __global__ __launch_bounds__(THREADS) void k_page_map(Map
         const uint32_t at = head + i;
         return a.ring + (at >= n_page ? at - n_page : at);
     };
-    for (uint32_t i0 = b; i0 < taken; i0 += AT_ONCE * THREADS) {
-        uint32_t i[AT_ONCE];
-        int at[AT_ONCE], page[AT_ONCE];
+    auto give = [&](auto at_once) {
+        constexpr int N = decltype(at_once)::value;
+        for (uint32_t i0 = b; i0 < taken; i0 += N * THREADS) {
+            uint32_t i[N];
+            int at[N], page[N];
 #pragma unroll
-        for (int k = 0; k < AT_ONCE; k++) i[k] = min(i0 + THREADS * k, taken - 1), page[k] = *ring_at(i[k]);
-        first_past(s_upto, a.p.n_seq, i, at);
+            for (int k = 0; k < N; k++) i[k] = min(i0 + THREADS * k, taken - 1), page[k] = *ring_at(i[k]);
+            first_past(s_upto, a.p.n_seq, i, at);
 #pragma unroll
-        for (int k = 0; k < AT_ONCE; k++)
-            if (i0 + THREADS * k < taken)
-                a.p.table[(size_t)at[k] * a.p.max_pages + s_held[at[k]] + (i[k] - (s_upto[at[k]] - s_need[at[k]]))] = page[k];
-    }
-    for (uint32_t i0 = b; i0 < returned; i0 += AT_ONCE * THREADS) {
-        uint32_t i[AT_ONCE];
-        int at[AT_ONCE], page[AT_ONCE];
-#pragma unroll
-        for (int k = 0; k < AT_ONCE; k++) i[k] = min(i0 + THREADS * k, returned - 1);
-        first_past(s_back, a.p.n_seq, i, at);
-#pragma unroll
-        for (int k = 0; k < AT_ONCE; k++) page[k] = a.p.table[(size_t)at[k] * a.p.max_pages + (i[k] - (at[k] ? s_back[at[k] - 1] : 0u))];
-#pragma unroll
-        for (int k = 0; k < AT_ONCE; k++)
-            if (i0 + THREADS * k < returned) *ring_at(count + i[k]) = page[k];
-    }
-    if (!map_rows) return;
-    for (int r0 = b; r0 < a.p.n_row; r0 += AT_ONCE * THREADS) {
-        uint32_t i[AT_ONCE];
-        int at[AT_ONCE], pos[AT_ONCE], page[AT_ONCE];
-#pragma unroll
-        for (int k = 0; k < AT_ONCE; k++) i[k] = (uint32_t)min(r0 + THREADS * k, a.p.n_row - 1);
-        first_past(s_end, a.p.n_seq, i, at);
-#pragma unroll
-        for (int k = 0; k < AT_ONCE; k++) {
-            const int s = at[k];
-            pos[k] = page[k] = -1;
-            if (s < a.p.n_seq && s_past[s] >= 0) {
-                pos[k] = s_past[s] + (int)i[k] - (s ? (int)s_end[s - 1] : 0);
-                const int n = pos[k] >> shift;
-                // a page that this step gives out is in the ring yet
-                page[k] = n < s_held[s] ? a.p.table[(size_t)s * a.p.max_pages + n] : *ring_at(s_upto[s] - s_need[s] + (n - s_held[s]));
-            }
+            for (int k = 0; k < N; k++)
+                if (i0 + THREADS * k < taken)
+                    a.p.table[(size_t)at[k] * a.p.max_pages + s_held[at[k]] + (i[k] - (s_upto[at[k]] - s_need[at[k]]))] = page[k];
         }
+    };
+    auto take_back = [&](auto at_once) {
+        constexpr int N = decltype(at_once)::value;
+        for (uint32_t i0 = b; i0 < returned; i0 += N * THREADS) {
+            uint32_t i[N];
+            int at[N], page[N];
 #pragma unroll
-        for (int k = 0; k < AT_ONCE; k++)
-            if (r0 + THREADS * k < a.p.n_row) {
-                a.p.pos[i[k]] = pos[k];
-                a.p.slot[i[k]] = slot_of(page[k], a.n_page, pos[k], shift);
-            }
+            for (int k = 0; k < N; k++) i[k] = min(i0 + THREADS * k, returned - 1);
+            first_past(s_back, a.p.n_seq, i, at);
+#pragma unroll
+            for (int k = 0; k < N; k++) page[k] = a.p.table[(size_t)at[k] * a.p.max_pages + (i[k] - (at[k] ? s_back[at[k] - 1] : 0u))];
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (i0 + THREADS * k < returned) *ring_at(count + i[k]) = page[k];
+        }
+    };
+    auto run = [](uint32_t n, auto what) {
+        if (n <= AT_ONCE * THREADS) what(std::integral_constant<int, 1>{});
+        else what(std::integral_constant<int, AT_ONCE>{});
+    };
+    run(taken, give);
+    run(returned, take_back);
+    if (!map_rows) return;
+    for (int row = b; row < a.p.n_row; row += THREADS) {
+        const uint32_t i[1] = {(uint32_t)row};
+        int at[1], pos = -1, page = -1;
+        first_past(s_end, a.p.n_seq, i, at);
+        const int s = at[0];
+        if (s < a.p.n_seq && s_past[s] >= 0) {
+            pos = s_past[s] + row - (s ? (int)s_end[s - 1] : 0);
+            const int n = pos >> shift;
+            // a page that this step gives out is in the ring yet
+            page = n < s_held[s] ? a.p.table[(size_t)s * a.p.max_pages + n] : *ring_at(s_upto[s] - s_need[s] + (n - s_held[s]));
+        }
+        a.p.pos[row] = pos;
+        a.p.slot[row] = slot_of(page, a.n_page, pos, shift);
     }
 }
 
