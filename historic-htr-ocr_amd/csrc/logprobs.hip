@@ -8,14 +8,15 @@
 // The largest logit's own 1 stays out of the sum r, so the log probability and the entropy of a sure choice, both near 0,
 // keep their leading digits (log1p); both are sums of terms of one sign, and nothing cancels.
 //
-// A row is read once, in chunks of 8192 logits (short ones: 2048) that a workgroup holds in registers, 32 (8) a thread; a wave keeps m, and r and W in
-// parts by lane. When a chunk raises m, the old one's own 1 joins r, r and W are scaled, and the new one's is left out. A row's
-// chunks are shared out among workgroups where the rows are few; the last of them to be done joins the parts, in order.
+// A row is read once, in chunks of 8192 logits (short ones: 2048) that a workgroup holds in registers, 32 (8) a thread; a wave keeps
+// m, and r and W in parts by lane. When a chunk raises m, the old one's own 1 joins r, r and W are scaled, and the new one's is left
+// out. A row's chunks are shared out among workgroups where the rows are few; the last of them to be done joins the parts, in order.
 //
 // Alternatives: a wave keeps in LDS every logit past a bound that at least n_top logits reach: the n_top-th largest of its lanes'
-// largest so far, found bit by bit from ballots, and anew after 1, 2, 4, … chunks. Of the few that are kept (1.3·n_top in a first
-// chunk of random logits, as many again over all others) each finds its rank by counting those before it. Where more pass the
-// bound than there is room (equal logits), the wave takes the best one by one.
+// largest so far, found bit by bit from ballots, and anew after 1, 2, 4, … chunks; or the smallest of the waves' (n_top / 4)-th, which
+// n_top of theirs together reach. Of the few that are kept (by a wave's own bound 1.3·n_top in a first chunk of random logits, as many
+// again over all others) each finds its rank by counting those before it. Where more pass the bound than there is room (equal
+// logits), the wave takes the best one by one.
 #include <algorithm>
 
 #include "choose_key.h"
@@ -28,6 +29,7 @@ constexpr int T = 256;                         // threads
 constexpr int ROOM = 256;                      // alternatives that a wave has room for
 constexpr int MAX_PARTS = 64;                  // workgroups of a row
 constexpr int TICKET = 32;                     // words between tickets (128 bytes)
+constexpr int SHARED = 9;                      // alternatives from which the waves look for a bound together (with 5 200 rows 30.7 µs for 30.2)
 constexpr int FEW = 16;                        // logits a thread of a row that goes by chunks of 8 a thread
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float SCALE = 24.0f, ONE = 16777216.0f;  // a wave's sums are held times 2^24: v_exp_f32 gives no subnormal numbers
@@ -107,17 +109,18 @@ __device__ __forceinline__ void rank(uint64_t *s_keys, int n, uint64_t *s_top, i
     }
 }
 
-// Bound: of many rows HBM: 1925 rows of 151936 with one alternative (1.17 GB) 185 µs, 6.3 TB/s, without 179, with 20 213; 200 rows
-// with 5 30 µs. Of few latency: one row 10 µs, 5 for a chunk's loads, sums and alternatives, 4 for handing the part over and joining
-// 19; 61 rows with 20 alternatives 25, without 12: of the 13, a chunk's alternatives (90 for 4 waves) take 2 µs to keep and 2 to
-// rank, 400 of 19 parts 3 more, and 135 of the 1159 workgroups wait for the others. A row's parts on one XCD, in whose L2 they are
-// handed over: 61 rows 16.8 … 12.2 µs, for 19.9 and 15.8 through the coherence point.
+// Bound: of many rows HBM: 1925 rows of 151936 with one alternative (1.17 GB) 185 µs, 6.3 TB/s, without 181, with 20 191 (each wave
+// by its own bound 215); 200 rows with 5 30 µs. Of few latency: one row 10 µs, 5 for a chunk's loads, sums and alternatives, 4 for
+// handing the part over and joining 19; 61 rows with 20 alternatives 23 (each wave by its own bound 25), without 12: what a chunk has
+// past its bound is kept and ranked, 400 of 19 parts are ranked again, and 135 of the 1159 workgroups wait for the others. A row's
+// parts on one XCD, in whose L2 they are handed over: 61 rows 16.8 … 12.2 µs, for 19.9 and 15.8 through the coherence point.
 template <int V, bool TOP, bool XL> __global__ __launch_bounds__(T, 4) void k_logprobs(ScoreArgs a) {
     constexpr int CHUNK = T * V;
     __shared__ __attribute__((aligned(16))) uint64_t s_keys[MAX_PARTS * HTR_TOP_MAX + 8];  // the waves' alternatives, ROOM each; then the parts'
     __shared__ uint64_t s_top[HTR_TOP_MAX];
     __shared__ Sums s_sums[T / 64];
     __shared__ int s_n[T / 64], s_last;
+    __shared__ uint32_t s_bound[2][T / 64];
     static_assert(MAX_PARTS * HTR_TOP_MAX >= T / 64 * ROOM, "room");
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // XL: the workgroups of a row share an XCD (a launch's go to the 8 XCDs in turn), and its L2 shows them each other's stores
@@ -132,7 +135,7 @@ template <int V, bool TOP, bool XL> __global__ __launch_bounds__(T, 4) void k_lo
 
     Sums s{-INFINITY, 0.0f, 0.0f, false};
     float lane_top = -INFINITY, bound = -INFINITY;  // the lane's largest so far; alternatives are larger than the bound
-    int n_kept = 0;
+    int n_kept = 0, looked = 0;
     for (int c = c0; c < c1; c++) {
         const int first = c * CHUNK - shift + 4 * tid;  // the thread's first logit; its quads are 4·T apart
         float v[V];
@@ -197,9 +200,20 @@ template <int V, bool TOP, bool XL> __global__ __launch_bounds__(T, 4) void k_lo
             if (((c - c0) & (c - c0 - 1)) == 0) {
                 // the largest number of 20 leading bits that a.top lanes reach
                 const uint32_t u = ordered(lane_top + 0.0f);  // (−0 as +0)
-                uint32_t t = 0;
-                for (uint32_t bit = 1u << 31; bit >= 1u << 12; bit >>= 1)
-                    if (count(__builtin_amdgcn_ballot_w64(u >= (t | bit))) >= a.top) t |= bit;
+                auto reached = [&](int lanes) {
+                    uint32_t t = 0;
+                    for (uint32_t bit = 1u << 31; bit >= 1u << 12; bit >>= 1)
+                        if (count(__builtin_amdgcn_ballot_w64(u >= (t | bit))) >= lanes) t |= bit;
+                    return t;
+                };
+                uint32_t t = reached(a.top);
+                if (a.top >= SHARED) {  // or that each wave's share of them reaches
+                    const uint32_t share = reached((a.top + T / 64 - 1) / (T / 64));
+                    uint32_t *all = s_bound[looked++ & 1];
+                    if (lane == 0) all[wave] = share;
+                    __syncthreads();
+                    t = max(t, min(min(all[0], all[1]), min(all[2], all[3])));
+                }
                 if (t > ordered(-INFINITY)) bound = fmaxf(bound, from_ordered(t == ordered(0.0f) ? t - 2 : t - 1));  // (past −0 too)
             }
             if (__builtin_amdgcn_ballot_w64(top > bound)) {
