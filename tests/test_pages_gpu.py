@@ -491,6 +491,35 @@ def test_attention_of_values_that_are_not_finite(dev, q8_0):
     r.free()
 
 
+@pytest.mark.parametrize("reads", [[(60, 50), (500, 1)], [(60, 8), (500, 1)]], ids=["wide", "narrow"])
+@pytest.mark.parametrize("scale", [511.75, 512.0, 65504.0])
+def test_attention_of_quants_of_minus_128(dev, reads, scale):
+    """a q8_0 cache made elsewhere may hold the quant -128, which with a scale of 512 and more is an infinity: rows that do not see
+    it are as they were"""
+    r = Reads(dev, reads, 32, 2, True, seed=21)
+    n_ctx, j = r.cache.k.shape[1], 60 + reads[0][1] // 2  # seen from the middle row of the first read on
+    qv = r.cache.bufs[1].download(np.int8, 2 * n_ctx * 128).reshape(2, n_ctx, 128)
+    dv = r.cache.bufs[3].download(np.float16, 2 * n_ctx * 4).reshape(2, n_ctx, 4)
+    qv[1, r.rows[0][j], 32:64], dv[1, r.rows[0][j], 1] = 1, scale
+    qv[1, r.rows[0][j], 37] = -128
+    r.cache.bufs[1].upload(qv)
+    r.cache.bufs[3].upload(dv)
+    with np.errstate(over="ignore"):
+        r.cache.v = values(qv, dv)
+    assert np.isfinite(r.cache.v[1, r.rows[0][j], 37]) == (scale < 512)
+    q = normal(22, r.n, 4, 128)
+    got = r.run(q, 4).reshape(r.n, 4, 128)
+    r.cache.v = np.where(np.isfinite(r.cache.v), r.cache.v, 0)
+    want = r.want(q, SCALE).reshape(r.n, 4, 128)
+    sees = np.zeros((r.n, 4, 128), bool)
+    sees[reads[0][1] // 2:reads[0][1], 2:, 37] = scale >= 512
+    assert not np.isfinite(got[sees]).any() and np.isfinite(got[~sees]).all()
+    clean = ~sees.any(axis=2)
+    assert rel_rows(got[clean], want[clean]) < BAR
+    assert np.allclose(got[~sees], want[~sees], rtol=1e-4, atol=1e-3)
+    r.free()
+
+
 def test_attention_over_a_long_cache(dev):
     """pages whose bytes lie past 4 GiB of a plane: row numbers times a row's bytes pass 32 bits"""
     page, n_ctx = 1024, (1 << 24) + 4096
@@ -679,3 +708,40 @@ def test_two_devices_at_once(dev, poisoned, n_head, n_kv, reads):
         for o in (*b, *out):
             o.free()
         r.free()
+
+
+def test_a_recording_cannot_make_the_scratch(dev):
+    """on a new handle the first call of a graph fails with the reason; after an eager one, of tokens or of chunks, both are
+    recorded"""
+    reads = [[(900, 1), (40, 1)], [(500, 70)]]
+    d = htr.Device(0)
+    runs = []
+    for seed, r in enumerate(reads):
+        r = Reads(d, r, 16, 8, seed=seed)
+        q = normal(seed, r.n, 16, 128)
+        runs.append((r, q, d.upload(q), d.alloc(q.nbytes)))
+
+    def call(i):
+        r, q, qb, out = runs[i]
+        htr.page_attention(d, qb, r.pages, r.cache.kv, 16, SCALE, out)
+
+    for i in range(2):
+        d.capture_begin()
+        with pytest.raises(htr.HtrError, match="captured"):
+            call(i)
+        d.capture_end().free()
+    call(0)
+    for i, (r, q, qb, out) in enumerate(runs):
+        d.capture_begin()
+        call(i)
+        g = d.capture_end()
+        for _ in range(3):
+            out.upload(np.full(q.size, 9.0, np.float32))
+            g.launch()
+            assert rel_rows(out.download(np.float32, q.size).reshape(r.n, -1), r.want(q, SCALE)) < BAR
+        g.free()
+    for r, q, qb, out in runs:
+        qb.free()
+        out.free()
+        r.free()
+    d.close()
