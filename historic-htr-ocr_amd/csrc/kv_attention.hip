@@ -1159,6 +1159,7 @@ int check_rows(const char *me, const float *d_q, size_t q_stride, const htr_kv *
     if (n * group > 1 << 30 || n * group * group >= 1ll << 32 ||
         (n * group + KB * WR - 1) / (KB * WR) * kv->n_kv > (int64_t)HTR_MAX_GROUPS)  // (those of the kernel of many rows)
         return htr_fail("%s: %lld queries of %d heads", me, (long long)n, n_head);
+    if (!htr_rows_fit(q_stride, (size_t)n, qd)) return htr_fail("%s: %lld rows %zu floats apart", me, (long long)n, q_stride);
     const uintptr_t q0 = (uintptr_t)d_q, q1 = q0 + 4 * (q_stride * (n - 1) + qd), o0 = (uintptr_t)d_out, o1 = o0 + 4 * qd * n;
     if (q0 < o1 && o0 < q1) return htr_fail("%s: the output overlaps the queries", me);
     if (htr_kv_overlaps(planes, d_out, 4 * qd * n)) return htr_fail("%s: the output overlaps the cache", me);

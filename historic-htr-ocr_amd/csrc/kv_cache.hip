@@ -459,6 +459,8 @@ int post_args(const char *me, const float *d_q, size_t q_stride, const float *d_
 int post_apart(const char *me, const PostRowsArgs &a, size_t groups) {
     // in place (q_out on q's own rows) is the only overlap that the kernel allows
     const size_t n = (size_t)a.n, qd = (size_t)a.n_head * D, kvd = (size_t)a.kv.n_kv * D;
+    if (!htr_rows_fit(a.q_stride, n, qd) || !htr_rows_fit(a.kv_stride, n, kvd))
+        return htr_fail("%s: %zu rows %zu and %zu floats apart", me, n, a.q_stride, a.kv_stride);
     const size_t q_bytes = 4 * (a.q_stride * (n - 1) + qd), out_bytes = 4 * qd * n;
     const size_t kv_bytes = 4 * (a.kv_stride * (n - 1) + kvd);
     if ((overlap(a.q, q_bytes, a.q_out, out_bytes) && !(a.q == a.q_out && (n == 1 || a.q_stride == qd))) ||

@@ -64,6 +64,10 @@ inline bool htr_overlap(const void *a, size_t na, const void *b, size_t nb) {
     return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
 }
 
+// whether n ≥ 1 rows of `row` floats (below 2^40), `stride` apart, end within 2^62 bytes: what htr_overlap is told of such rows has
+// not wrapped, and no row lies in front of the first
+inline bool htr_rows_fit(size_t stride, size_t n, size_t row) { return n == 1 || stride <= ((1ull << 60) - row) / (n - 1); }
+
 // the device made current for a call's launches, and the caller's own again afterwards
 struct HtrOnDevice {
     explicit HtrOnDevice(htr_device *dev);

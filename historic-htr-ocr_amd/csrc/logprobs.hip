@@ -366,6 +366,7 @@ extern "C" int htr_token_logprobs(htr_device *dev, const float *d_logits, size_t
         return htr_fail("%s: %d alternatives of %d logits (at most %d)", me, n_top, n_vocab, HTR_TOP_MAX);
     if (n_top && (!d_top_ids || !d_top_logprob)) return htr_fail("%s: null alternatives", me);
     const size_t rows = (size_t)n;
+    if (!htr_rows_fit(stride, rows, n_vocab)) return htr_fail("%s: %d rows %zu floats apart", me, n, stride);
     const struct {
         const void *p;
         size_t n;

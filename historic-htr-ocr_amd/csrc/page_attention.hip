@@ -1052,6 +1052,7 @@ extern "C" int htr_page_attention(htr_device *dev, const float *d_q, size_t q_st
     if (kv->n_ctx < pages->page) return htr_fail("%s: a cache of %d rows in pages of %d", me, kv->n_ctx, pages->page);
     const size_t qd = (size_t)n_head * D, n = (size_t)a.p.n_row;
     if (q_stride < qd || (q_stride & 3)) return htr_fail("%s: rows %zu floats apart (a multiple of 4, at least %zu)", me, q_stride, qd);
+    if (!htr_rows_fit(q_stride, n, qd)) return htr_fail("%s: %zu rows %zu floats apart", me, n, q_stride);
     if (((uintptr_t)d_q | (uintptr_t)d_out) & 15) return htr_fail("%s: pointers must be 16-byte aligned", me);
     if (htr_overlap(d_q, 4 * (q_stride * (n - 1) + qd), d_out, 4 * qd * n)) return htr_fail("%s: the output overlaps the queries", me);
     if (htr_kv_overlaps(a.kv, d_out, 4 * qd * n)) return htr_fail("%s: the output overlaps the cache", me);

@@ -262,3 +262,16 @@ def test_more_rows_than_a_launch_takes_are_refused():
     wide = _kv(n_kv=2, n_ctx=2 ** 28, k=T, v=2 * T)
     _refused(_calls(wide)["window"](q=3 * T, out=4 * T, n=2 ** 28, pos0=0), "268435456 queries of 4 heads")
     _refused(_calls(wide)["window"](q=3 * T, out=4 * T, n=2 ** 28 - 32, pos0=0), "null device")
+
+
+@pytest.mark.parametrize("stride", [2 ** 64 - 4, 2 ** 62, 2 ** 61 + 512, 2 ** 60])
+def test_rows_that_end_past_any_memory_are_refused(stride):
+    """of a stride below 0, taken as 64 bits without a sign, or of any other whose rows lie past 2^62 bytes, the check of overlaps
+    would count a few bytes, and the kernels would read in front of the rows"""
+    for kv in (_kv(), _kv(**Q8)):
+        calls = _calls(kv)
+        for name, change in (("post", dict(qs=stride)), ("post", dict(ks=stride)), ("tree", dict(qs=stride)), ("window", dict(qs=stride))):
+            _refused(calls[name](**change), "floats apart")
+            _refused(calls[name](**change, n=1), "null device")  # (one row: no stride)
+        for name in ("post", "tree", "window"):
+            _refused(calls[name](q=1 << 58, qs=2 ** 40), "null device")

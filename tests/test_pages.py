@@ -153,3 +153,22 @@ def test_python_sizes():
         htr.Pages.of(1, 0, 16, 1, Ref, Ref, Ref)
     with pytest.raises(ValueError, match="pages of sizes"):
         htr.Pages.of(2 ** 31, 1, 16, 1, Ref, Ref, Ref)
+
+
+@pytest.mark.parametrize("stride", [2 ** 64 - 4, 2 ** 62, 2 ** 61 + 512, 2 ** 60])
+def test_rows_that_end_past_any_memory(stride):
+    """of a stride below 0, taken as 64 bits without a sign, or of any other whose rows lie past 2^62 bytes, the check of overlaps
+    would count a few bytes, and the kernels would read in front of the rows"""
+    refused(post(qs=stride), "floats apart")
+    refused(post(ks=stride), "floats apart")
+    refused(attend(qs=stride), "floats apart")
+    refused(score(stride=stride), "apart")
+    refused(score(stride=stride, n=2), "apart")
+    refused(score(stride=stride, n=1), "null device")  # (one row: no stride)
+
+
+def test_strides_of_rows_that_memory_could_hold():
+    refused(post(q=1 << 58, qs=2 ** 40), "null device")
+    refused(post(k=1 << 58, v=1 << 59, ks=2 ** 40), "null device")
+    refused(attend(q=1 << 58, qs=2 ** 40), "null device")
+    refused(score(x=1 << 58, stride=2 ** 40 + 1), "null device")
