@@ -617,9 +617,11 @@ class Pages:
         return self
 
     @staticmethod
-    def _check(*sizes: int) -> None:
-        if not all(1 <= s < 2 ** 31 for s in sizes):
-            raise ValueError(f"pages of sizes {sizes} (each 1 … 2^31 - 1)")
+    def _check(n_seq: int, n_row: int, page: int, max_pages: int) -> None:
+        if not (1 <= n_seq <= 1024 and 1 <= n_row <= 2 ** 21 and 16 <= page <= 1024 and not page & (page - 1) and
+                1 <= max_pages and max_pages * max(n_seq, page) < 2 ** 31):
+            raise ValueError(f"pages of sizes {n_seq, n_row, page, max_pages} (1 … 1024 reads, 1 … 2^21 rows, a power of two "
+                             "16 … 1024, at most 2^31 - 1 entries in all and rows to a read)")
 
     def _set(self, n_seq: int, n_row: int, page: int, max_pages: int, start, past, table, pos, slot) -> None:
         self.n_seq, self.n_row, self.page, self.max_pages = n_seq, n_row, page, max_pages

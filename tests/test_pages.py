@@ -172,3 +172,48 @@ def test_strides_of_rows_that_memory_could_hold():
     refused(post(k=1 << 58, v=1 << 59, ks=2 ** 40), "null device")
     refused(attend(q=1 << 58, qs=2 ** 40), "null device")
     refused(score(x=1 << 58, stride=2 ** 40 + 1), "null device")
+
+
+class Memory:
+    """stands in for a device's buffers"""
+    made = []
+
+    def __init__(self, dev, nbytes):
+        self.ptr = (len(self.made) + 1) << 40
+        self.made.append(nbytes)
+
+    def upload(self, a):
+        return self
+
+    def free(self):
+        self.ptr = None
+
+
+class NoDevice:
+    h = None
+
+
+@pytest.mark.parametrize("n_seq,n_row,page,max_pages", [
+    (1025, 1, 16, 1), (0, 1, 16, 1), (-1, 1, 16, 1), (1, 2 ** 21 + 1, 16, 1), (1, -5, 16, 1), (1, 1, 8, 1), (1, 1, 48, 1), (1, 1, 2048, 1),
+    (1, 1, 0, 1), (1, 1, -16, 1), (1, 1, 16, 0), (1, 1, 16, 2 ** 27), (1, 1, 16, -2), (1024, 1, 16, 2 ** 21), (2 ** 32 + 1, 1, 16, 1)])
+def test_pages_of_sizes_that_no_call_takes_ask_for_no_memory(monkeypatch, n_seq, n_row, page, max_pages):
+    """a table of 2^40 entries would be asked for before the first call refused it"""
+    monkeypatch.setattr(htr, "Buffer", Memory)
+    monkeypatch.setattr(Memory, "made", [])
+    with pytest.raises(ValueError, match="pages of sizes"):
+        htr.Pages(NoDevice, n_seq, n_row, page, max_pages)
+    assert not Memory.made
+    ref = type("Ref", (), {"ptr": M})
+    with pytest.raises(ValueError, match="pages of sizes"):
+        htr.Pages.of(n_seq, n_row, page, max_pages, ref, ref, ref)
+
+
+@pytest.mark.parametrize("n_seq,n_row,page,max_pages", [(1, 1, 16, 1), (1024, 2 ** 21, 1024, 7), (15, 2 ** 21, 16, 2 ** 27 - 1),
+                                                        (1, 1, 1024, 2 ** 21 - 1), (1024, 1, 16, 2 ** 21 - 1)])
+def test_pages_of_the_largest_sizes(monkeypatch, n_seq, n_row, page, max_pages):
+    """(what Pages takes the calls take: a null device is the next thing that is wrong)"""
+    ref = type("Ref", (), {"ptr": M})
+    at = [type("Ref", (), {"ptr": i << 50}) for i in range(1, 6)]
+    p = htr.Pages.of(n_seq, n_row, page, max_pages, *at)
+    with pytest.raises(htr.HtrError, match="null device"):
+        htr.page_map(NoDevice, p, 1, ref, *[type("Ref", (), {"ptr": i << 56}) for i in range(1, 6)])
