@@ -550,6 +550,18 @@ class Tree:
         return self
 
 
+def _past_32_bits(**sizes: int) -> ValueError:
+    """ctypes would take a size's low 32 bits. (Asked of the sizes or-ed: one below 0 beside it hides it, and is refused by the
+    library)"""
+    return ValueError(f"sizes past 32 bits: {sizes}")
+
+
+def _stride(floats: int) -> int:
+    if not 0 <= floats < 2 ** 63:
+        raise ValueError(f"rows {floats} floats apart")
+    return floats
+
+
 def qkv_post_rows(dev: Device, q, k, v, n: int, q_norm, k_norm, rope, n_pos: int, pos0: int, n_head: int, eps: float,
                   kv: KvCache, row0: int, q_out, q_stride: int | None = None, kv_stride: int | None = None,
                   tree: Tree | None = None) -> None:
@@ -557,20 +569,26 @@ def qkv_post_rows(dev: Device, q, k, v, n: int, q_norm, k_norm, rope, n_pos: int
     cache's rows row0 + t. Strides in floats (None: rows without a gap)"""
     if tree is not None and tree.n != n:
         raise ValueError(f"{n} rows of a tree of {tree.n} nodes")
-    _check(lib().htr_qkv_post_rows(dev.h, q.ptr, n_head * 128 if q_stride is None else q_stride, k.ptr, v.ptr,
-                                   kv.n_kv * 128 if kv_stride is None else kv_stride, n, q_norm.ptr, k_norm.ptr, rope.ptr,
+    if (n | n_pos | pos0 | n_head | row0) >> 31 not in (0, -1):
+        raise _past_32_bits(n=n, n_pos=n_pos, pos0=pos0, n_head=n_head, row0=row0)
+    _check(lib().htr_qkv_post_rows(dev.h, q.ptr, n_head * 128 if q_stride is None else _stride(q_stride), k.ptr, v.ptr,
+                                   kv.n_kv * 128 if kv_stride is None else _stride(kv_stride), n, q_norm.ptr, k_norm.ptr, rope.ptr,
                                    n_pos, pos0, None if tree is None else tree.depths_ptr, n_head, eps, kv.ref, row0,
                                    q_out.ptr))
 
 
 def kv_copy(dev: Device, src: KvCache, src_row: int, dst: KvCache, dst_row: int, n: int) -> None:
     """n rows between caches: f16 to q8_0 quantises, q8_0 to f16 reads back, like types copy"""
+    if (src_row | dst_row | n) >> 31 not in (0, -1):
+        raise _past_32_bits(src_row=src_row, dst_row=dst_row, n=n)
     _check(lib().htr_kv_copy(dev.h, src.ref, src_row, dst.ref, dst_row, n))
 
 
 def kv_keep(dev: Device, kv: KvCache, row0: int, rows) -> None:
     """rows row0 + rows[i] to row0 + i, all read before any is written"""
     idx = array("i", rows)
+    if row0 >> 31 not in (0, -1):
+        raise _past_32_bits(row0=row0)
     _check(lib().htr_kv_keep(dev.h, kv.ref, row0, idx.buffer_info()[0] if idx else None, len(idx)))
 
 
@@ -578,14 +596,18 @@ def tree_attention(dev: Device, q, tree: Tree | int, n_past: int, kv: KvCache, n
                    q_stride: int | None = None) -> None:
     """attention of a drafted tree's queries (or of a chain of that many) over n_past committed rows and the draft's"""
     n, masks = (tree, None) if isinstance(tree, int) else (tree.n, tree.masks_ptr)
-    _check(lib().htr_tree_attention(dev.h, q.ptr, n_head * 128 if q_stride is None else q_stride, n, masks, n_past, kv.ref,
+    if (n | n_past | n_head) >> 31 not in (0, -1):
+        raise _past_32_bits(n=n, n_past=n_past, n_head=n_head)
+    _check(lib().htr_tree_attention(dev.h, q.ptr, n_head * 128 if q_stride is None else _stride(q_stride), n, masks, n_past, kv.ref,
                                     n_head, scale, out.ptr))
 
 
 def window_attention(dev: Device, q, n_q: int, pos0: int, window: int, n_sink: int, kv: KvCache, n_head: int, scale: float,
                      out, q_stride: int | None = None) -> None:
     """attention of the queries at pos0 … over the last `window` rows up to each one's own and the first n_sink"""
-    _check(lib().htr_window_attention(dev.h, q.ptr, n_head * 128 if q_stride is None else q_stride, n_q, pos0, window,
+    if (n_q | pos0 | window | n_sink | n_head) >> 31 not in (0, -1):
+        raise _past_32_bits(n_q=n_q, pos0=pos0, window=window, n_sink=n_sink, n_head=n_head)
+    _check(lib().htr_window_attention(dev.h, q.ptr, n_head * 128 if q_stride is None else _stride(q_stride), n_q, pos0, window,
                                       n_sink, kv.ref, n_head, scale, out.ptr))
 
 
@@ -640,27 +662,35 @@ class Pages:
 def page_map(dev: Device, pages: Pages, n_page: int, length, new, ring, pool, length_out, pool_out) -> None:
     """the step's arrays from the reads' lengths and new rows (-1: the read ends), pages taken from and given back to the ring
     [n_page] of free ones, whose first and number are pool [2]; length_out and pool_out may be length and pool"""
+    if n_page >> 31 not in (0, -1):
+        raise _past_32_bits(n_page=n_page)
     _check(lib().htr_page_map(dev.h, pages.ref, n_page, length.ptr, new.ptr, ring.ptr, pool.ptr, length_out.ptr, pool_out.ptr))
 
 
 def qkv_post_pages(dev: Device, q, k, v, pages: Pages, q_norm, k_norm, rope, n_pos: int, n_head: int, eps: float, kv: KvCache,
                    q_out, q_stride: int | None = None, kv_stride: int | None = None) -> None:
     """qkv_post_rows of a step's rows: row t at position pages.pos[t], k and v to the cache's row pages.slot[t]"""
-    _check(lib().htr_qkv_post_pages(dev.h, q.ptr, n_head * 128 if q_stride is None else q_stride, k.ptr, v.ptr,
-                                    kv.n_kv * 128 if kv_stride is None else kv_stride, pages.ref, q_norm.ptr, k_norm.ptr,
+    if (n_pos | n_head) >> 31 not in (0, -1):
+        raise _past_32_bits(n_pos=n_pos, n_head=n_head)
+    _check(lib().htr_qkv_post_pages(dev.h, q.ptr, n_head * 128 if q_stride is None else _stride(q_stride), k.ptr, v.ptr,
+                                    kv.n_kv * 128 if kv_stride is None else _stride(kv_stride), pages.ref, q_norm.ptr, k_norm.ptr,
                                     rope.ptr, n_pos, n_head, eps, kv.ref, q_out.ptr))
 
 
 def page_attention(dev: Device, q, pages: Pages, kv: KvCache, n_head: int, scale: float, out, q_stride: int | None = None) -> None:
     """attention of a step's rows, each read's over its own rows of the cache up to each one's position"""
-    _check(lib().htr_page_attention(dev.h, q.ptr, n_head * 128 if q_stride is None else q_stride, pages.ref, kv.ref, n_head,
+    if n_head >> 31 not in (0, -1):
+        raise _past_32_bits(n_head=n_head)
+    _check(lib().htr_page_attention(dev.h, q.ptr, n_head * 128 if q_stride is None else _stride(q_stride), pages.ref, kv.ref, n_head,
                                     scale, out.ptr))
 
 
 def token_logprobs(dev: Device, logits, n: int, n_vocab: int, ids, logprob, entropy, top: int = 0, top_ids=None,
                    top_logprob=None, stride: int | None = None) -> None:
     """of n rows of logits (stride floats apart; None: without a gap) each one's log p(ids), entropy, and `top` alternatives"""
-    _check(lib().htr_token_logprobs(dev.h, logits.ptr, n_vocab if stride is None else stride, n, n_vocab, ids.ptr, logprob.ptr,
+    if (n | n_vocab | top) >> 31 not in (0, -1):
+        raise _past_32_bits(n=n, n_vocab=n_vocab, top=top)
+    _check(lib().htr_token_logprobs(dev.h, logits.ptr, n_vocab if stride is None else _stride(stride), n, n_vocab, ids.ptr, logprob.ptr,
                                     entropy.ptr, top, _p(top_ids), _p(top_logprob)))
 
 

@@ -217,3 +217,53 @@ def test_pages_of_the_largest_sizes(monkeypatch, n_seq, n_row, page, max_pages):
     p = htr.Pages.of(n_seq, n_row, page, max_pages, *at)
     with pytest.raises(htr.HtrError, match="null device"):
         htr.page_map(NoDevice, p, 1, ref, *[type("Ref", (), {"ptr": i << 56}) for i in range(1, 6)])
+
+
+@pytest.mark.parametrize("more", [2 ** 32, -2 ** 32, 2 ** 63])
+def test_sizes_past_32_bits_do_not_reach_the_library_as_others(more):
+    """ctypes takes a size's low 32 bits (a stride's low 64): 2^32 + 3 rows would be answered as 3"""
+    at = [type("Ref", (), {"ptr": M << i}) for i in range(12)]
+    p, c = htr.Pages.of(3, 10, 16, 5, *at[7:12]), htr.KvCache.of(2, 640, at[5], at[6])
+    d = NoDevice
+
+    def page_map(n_page=40):
+        htr.page_map(d, p, n_page, *at[:6])
+
+    def post(n_pos=200, n_head=4, **strides):
+        htr.qkv_post_pages(d, at[0], at[1], at[2], p, at[3], at[3], at[3], n_pos, n_head, 1e-6, c, at[4], **strides)
+
+    def attend(n_head=4, **strides):
+        htr.page_attention(d, at[0], p, c, n_head, 0.1, at[1], **strides)
+
+    def score(n=3, n_vocab=1000, top=5, **strides):
+        htr.token_logprobs(d, at[0], n, n_vocab, *at[1:4], top, *at[4:6], **strides)
+
+    def rows(n=3, n_pos=200, pos0=7, n_head=4, row0=97, **strides):
+        htr.qkv_post_rows(d, at[0], at[1], at[2], n, at[3], at[3], at[3], n_pos, pos0, n_head, 1e-6, c, row0, at[4], **strides)
+
+    def copy(src_row=0, dst_row=90, n=5):
+        htr.kv_copy(d, c, src_row, c, dst_row, n)
+
+    def keep(row0=90):
+        htr.kv_keep(d, c, row0, [0, 3])
+
+    def tree(tree=3, n_past=97, n_head=4, **strides):
+        htr.tree_attention(d, at[0], tree, n_past, c, n_head, 0.1, at[1], **strides)
+
+    def window(n_q=3, pos0=97, window=16, n_sink=4, n_head=4, **strides):
+        htr.window_attention(d, at[0], n_q, pos0, window, n_sink, c, n_head, 0.1, at[1], **strides)
+
+    for call in (page_map, post, attend, score, rows, copy, keep, tree, window):
+        with pytest.raises(htr.HtrError, match="null device"):
+            call()
+        for name, size in zip(call.__code__.co_varnames, call.__defaults__):
+            with pytest.raises(ValueError, match="past 32 bits"):
+                call(**{name: size + more})
+    for call, strides in ((post, dict(q_stride=512, kv_stride=256)), (attend, dict(q_stride=512)), (score, dict(stride=1000)),
+                          (rows, dict(q_stride=512, kv_stride=256)), (tree, dict(q_stride=512)), (window, dict(q_stride=512))):
+        with pytest.raises(htr.HtrError, match="null device"):
+            call(**strides)
+        for name, stride in strides.items():
+            for other in (stride + 2 ** 64, stride - 2 ** 64, -4):
+                with pytest.raises(ValueError, match="floats apart"):
+                    call(**{name: other})
