@@ -53,6 +53,18 @@ __device__ __forceinline__ float2 get64(const void *p) {
 // the lowest n bits (none for n ≤ 0, all from 32 on)
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? ~0u : (1u << max(n, 0)) - 1; }
 
+// the blocks of the keys 0 … last (−1: none; last + 32 passes 31 bits)
+__host__ __device__ __forceinline__ int blocks_to(int last) { return (int)(((uint32_t)last + KB) / KB); }
+// a wave's blocks of a tile: the first `whole` all of its rows see the whole of, the first `any` one of them sees. last0, last1: the
+// last keys that its first and its last row see; a wave without rows has no blocks (with those that a row would have, it made all
+// products of a tile for nobody: 48 chunks of 21 rows of two heads over 4000 keys 216 µs for 182, over q8_0 rows 213 for 175)
+struct WaveBlocks {
+    int whole, any;
+};
+__host__ __device__ __forceinline__ WaveBlocks wave_blocks(bool has_rows, int last0, int last1) {
+    return has_rows ? WaveBlocks{(last0 + 1) / KB, blocks_to(last1)} : WaveBlocks{0, 0};
+}
+
 // p − (float)h for the low (0) or high (1) half of h: one mixed-precision fma
 template <int HI> __device__ __forceinline__ float minus_half(float p, uint32_t h) {
     float r;

@@ -77,9 +77,6 @@ __device__ __forceinline__ int lane_id() { return here(threadIdx.x & 63); }  // 
 // row r's query
 __device__ __forceinline__ int query_of(const Args &a, int r) { return (int)__umulhi(2u * (uint32_t)r, a.per_group); }
 
-// the blocks of the keys 0 … last (−1: none; last + 32 passes 31 bits)
-__device__ __forceinline__ int blocks_to(int last) { return (int)(((uint32_t)last + KB) / KB); }
-
 // 64 reads of the line of work at hand, in LDS
 struct Reads {
     int64_t end[64];                 // the line's length up to and with each
@@ -756,8 +753,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
             const int v_at = 16 * (K_CHUNKS + 16 * vrow + ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ (4 * (vrow & 3)))) + 8 * (lane & 1);
             const int i0 = own.i0, n_st = own.i1 - i0;
             const int r0 = WIDE * t.tau + KB * wave, rc = min(r0 + c, t.rows - 1);
-            const int all_to = (t.last_of(a, r0) + 1) / KB;                              // blocks that all of the wave's rows see the whole of
-            const int any_to = r0 < t.rows ? blocks_to(t.last_of(a, r0 + KB - 1)) : 0;  // blocks that one of them sees
+            const WaveBlocks mine = wave_blocks(r0 < t.rows, t.last_of(a, r0), t.last_of(a, r0 + KB - 1));
             Run run = run_of(a, line, t, i0, 1);
             if (n_st > 0) run.fetch(0);
             Rows r_last{{0, 0}, 0};  // f16: of the last stage whose K is on its way
@@ -829,7 +825,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
                 };
                 const int i = i0 + st;
                 if constexpr (MASK)
-                    if (i >= any_to) {
+                    if (i >= mine.any) {
                         convert();
                         return;
                     }
@@ -938,7 +934,7 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
             }
             // two stages at a time, both kinds of step passing one barrier a stage: a wave's blocks may be masked where another's
             // are not
-            auto whole2 = [&](int st) { return st + 1 < n_st && i0 + st + 1 < all_to && (gone & 15u) == 0; };
+            auto whole2 = [&](int st) { return st + 1 < n_st && i0 + st + 1 < mine.whole && (gone & 15u) == 0; };
             for (int st = 0; st < n_st;) {
                 for (; whole2(st); st += 2) {
                     step(st, 0, s0, s1, std::false_type{});
