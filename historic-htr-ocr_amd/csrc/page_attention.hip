@@ -973,9 +973,15 @@ template <bool Q8> __device__ __forceinline__ void wide(const Args &a, int kvh, 
 }
 
 // The workgroups of wide tiles and those of narrow ones, of the kind first that has more to do: 64 tokens beside 512 rows 134 µs,
-// narrow first, for 145; four prompts with their last narrow tiles 159, wide first, for 166. Where neither has much more (f16; over
-// q8_0 rows it is no faster), half of each kind in turn, so that a CU has one of each: two chunks of 509 rows beside 61 tokens 148
-// µs for 160 (wide first) and 161. To tell costs 1 µs. In turn one by one, a CU got two of one kind and its neighbour none.
+// narrow first, for 145; four prompts with their last narrow tiles 155, wide first, for 161. Where neither has much more (f16; over
+// q8_0 rows it is no faster), half of each kind in turn, so that a CU has one of each: two chunks of 509 rows beside 61 tokens 146
+// µs for 157 (wide first) and 159. To tell costs 1 µs. In turn one by one, a CU got two of one kind and its neighbour none.
+// By r, the narrow line's length over the wide one's (chunks of 512 rows beside 20 or 61 tokens; µs in turn, wide first, narrow first):
+//   over 5000 keys, the wide line 172000: r 0.03 113 108 112, 0.1 115 116 117, 0.2 124 129 131, 0.5 153 169 169, 1.2 229 260 244
+//   over 2000, 76000: r 4.5 295 313 299, 6 375 389 370;   over 900, 41000: r 1.2 75 82 79, 4.5 173 190 177, 6 217 232 218
+//   over 400, 25000: r 0.6 48 42 46, 1.2 53 53 56, 2 69 73 76;   over 1500 q8_0 keys: r 1.7 106 104 102, 2.3 117 121 118
+// so in turn from r 0.15 to 5, where the wide line is 1.5 of the least pieces to each of its workgroups (36864 here), and else by r 2.
+constexpr float TURNS_FROM = 0.15f, TURNS_TO = 5.0f, TURNS_PIECES = 1.5f, NARROW_FIRST = 2.0f;
 template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_attn(Args a) {
     __shared__ __attribute__((aligned(16))) uint4_t s_kv[PW * (Q8 ? WAVE_Q8 : WAVE_F16)];
     static_assert(!Q8 || 16 * PW * WAVE_Q8 >= 16 * 2 * TILE + 4 * RAW * PW, "the wide tiles' buffers fit");
@@ -995,8 +1001,9 @@ template <bool Q8> __global__ __launch_bounds__(64 * PW, 2) void k_page_attn(Arg
             if (first >= a.p.n_seq) break;
         }
         lw = wave_sum(lw, lane_id()), ln = wave_sum(ln, lane_id());
-        const bool narrow_first = __builtin_amdgcn_ballot_w64(ln >= 2.0f * lw) != 0;  // (alike in all lanes)
-        const bool halves = !Q8 && __builtin_amdgcn_ballot_w64(ln < 2.0f * lw && ln > 0.25f * lw && lw > 2.0f * LEAST * a.group * a.pieces) != 0;
+        const bool narrow_first = __builtin_amdgcn_ballot_w64(ln >= NARROW_FIRST * lw) != 0;  // (alike in all lanes)
+        const bool halves = !Q8 && __builtin_amdgcn_ballot_w64(ln > TURNS_FROM * lw && ln < TURNS_TO * lw &&
+                                                               lw > TURNS_PIECES * LEAST * a.group * a.pieces) != 0;
         // n of the one kind, n of the other, and what is left of each
         const int n = halves ? (a.pieces + 1) / 2 : a.pieces, left = a.pieces - n;
         const bool other = unit >= n && (unit < 2 * n || unit >= 2 * n + left);
