@@ -1,10 +1,14 @@
 """The operators of a step of several reads over a cache in pages on the GPU against plain numpy in 64 bits: the tables and row
 maps, rows stored at mapped slots, each read's attention over its pages, and a serving loop of them together, eager and replayed
 as one recorded step."""
+import os
+import re
+
 import numpy as np
 import pytest
 
 import htr
+from test_kernel_waits import PKG
 from test_kv_ops_gpu import BAR, EPS, SCALE, Cache, attention, bits, blocks, cache, heads, normal, rel_rows, strided, values
 
 pytestmark = pytest.mark.gpu
@@ -745,3 +749,49 @@ def test_a_recording_cannot_make_the_scratch(dev):
         out.free()
         r.free()
     d.close()
+
+
+# ---- the order of the two kinds of tiles ----------------------------------------------------------------------------------
+
+def source_constants(*names):
+    with open(os.path.join(PKG, "csrc", "page_attention.hip")) as f:
+        text = f.read()
+    return [float(re.search(rf"\b{n} = ([0-9.]+)f?\b", text)[1]) for n in names]
+
+
+def lines(reads, group):
+    """the lengths of the lines of wide and of narrow tiles (keys and 128 more to a tile; a wide one's by the heads of a group)"""
+    wide, narrow = 0, 0
+    for past, n in reads:
+        rows = n * group
+        rest, tiles, held = rows % 128, rows // 128 + (rows % 128 > 32), max(past, 0) + 128
+        wide += tiles * (held * group + 64 * tiles)
+        narrow += held + n if 0 < rest <= 32 else 0
+    return wide, narrow
+
+
+def beside_tokens(past, n, tokens):
+    """chunks of n and n - 1 rows over past keys, beside tokens over some 500, in an order of their own"""
+    reads = [(430 + 7 * i % 150, 1) for i in range(tokens)]
+    return reads[:tokens // 3] + [(past, n)] + reads[tokens // 3:-2] + [(past - 11, n - 1)] + reads[-2:]
+
+
+@pytest.mark.parametrize("n_head,n_kv,reads,turns", [
+    (16, 8, beside_tokens(2500, 300, 60), True), (14, 7, beside_tokens(2700, 300, 60), True),  # (7 KV heads: an odd number of pieces)
+    (14, 7, beside_tokens(2600, 330, 200), True), (12, 4, beside_tokens(6000, 260, 90), True),
+    # the bounds' other sides: little to do for the narrow tiles, for the wide ones, for either
+    (16, 8, beside_tokens(4000, 300, 6), False), (16, 8, [(2500, 150)] + [(3000, 1)] * 70, False), (14, 7, beside_tokens(300, 130, 20), False)])
+def test_attention_of_kinds_in_turn(dev, n_head, n_kv, reads, turns):
+    """f16 rows: half of the workgroups of wide tiles, half of those of narrow ones, and what is left of each; and one kind behind the
+    other. The outputs start as infinities: a piece that nobody took would be seen"""
+    low, high, pieces_of, least = source_constants("TURNS_FROM", "TURNS_TO", "TURNS_PIECES", "LEAST")
+    wide, narrow = lines(reads, n_head // n_kv)
+    pieces = 2 * dev.info()[1] // n_kv
+    assert turns == (low * wide < narrow < high * wide and wide > pieces_of * least * (n_head // n_kv) * pieces)
+    r = Reads(dev, reads, 32, n_kv, seed=n_kv, pad=2)
+    q = normal(n_head, r.n, n_head, 128)
+    got = r.run(q, n_head, fill=np.inf)
+    assert dev.last_kernel() == "k_page_attn_join"
+    assert rel_rows(got, r.want(q, SCALE)) < BAR
+    assert np.array_equal(bits(got), bits(r.run(q, n_head)))
+    r.free()
