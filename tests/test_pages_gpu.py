@@ -795,3 +795,39 @@ def test_attention_of_kinds_in_turn(dev, n_head, n_kv, reads, turns):
     assert rel_rows(got, r.want(q, SCALE)) < BAR
     assert np.array_equal(bits(got), bits(r.run(q, n_head)))
     r.free()
+
+
+@pytest.mark.parametrize("q8_0", [False, True], ids=["f16", "q8_0"])
+@pytest.mark.parametrize("n_head,n_kv,reads", [
+    # a full tile of 32 rows in many parts, on 8 KV heads, whose workgroups share an XCD, and on 4 and 1, whose do not
+    (8, 8, [(4000, 32)] + [(0, 0)] * 7), (4, 4, [(4000, 32)] + [(0, 0)] * 7), (1, 1, [(9000, 32)] + [(0, 0)] * 7),
+    # 120 rows of many reads; several tiles to a read
+    (8, 8, [(37 * i % 900, 1) for i in range(90)] + [(700, 30), (0, 7)]), (3, 3, [(37 * i % 900, 1) for i in range(90)] + [(700, 30), (0, 7)]),
+    (16, 8, [(9, 0)] * 40 + [(2500, 33), (64, 20), (-1, 9)]), (2, 1, [(9, 0)] * 40 + [(2500, 33), (64, 20), (-1, 9)])])
+def test_attention_in_one_launch(dev, n_head, n_kv, reads, q8_0):
+    """steps that one launch takes (by the rule on sizes, and by the kernel that ran): a cut tile's parts joined by the last of its
+    workgroups, call after call, replayed among others that leave other parts and tickets"""
+    few, = source_constants("FEW")
+    n = sum(new for _, new in reads)
+    assert n * n_head // n_kv <= few and n <= 4 * len(reads)
+    r = Reads(dev, reads, 32, n_kv, q8_0, seed=n_head)
+    q = normal(33, r.n, n_head, 128)
+    got = r.run(q, n_head, fill=np.inf)
+    assert dev.last_kernel().startswith("k_page_few<")
+    assert rel_rows(got, r.want(q, SCALE)) < BAR
+    other = Reads(dev, [(1500, 1), (40, 1), (3000, 1)], 16, n_kv, not q8_0, seed=5)
+    oq = normal(34, other.n, n_head, 128)
+    other_got = other.run(oq, n_head)
+    assert dev.last_kernel().startswith("k_page_few<")
+    qb, out = dev.upload(q), dev.alloc(q.nbytes)
+    dev.capture_begin()
+    htr.page_attention(dev, qb, r.pages, r.cache.kv, n_head, SCALE, out)
+    g = dev.capture_end()
+    for i in range(4):
+        out.upload(np.full(q.size, 2.5, np.float32))
+        g.launch()
+        np.testing.assert_array_equal(bits(other.run(oq, n_head)), bits(other_got))
+        g.launch()
+        np.testing.assert_array_equal(bits(out.download(np.float32, q.size)), bits(got.ravel()))
+    for b in (g, qb, out, r, other):
+        b.free()
