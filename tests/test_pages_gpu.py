@@ -831,3 +831,80 @@ def test_attention_in_one_launch(dev, n_head, n_kv, reads, q8_0):
         np.testing.assert_array_equal(bits(out.download(np.float32, q.size)), bits(got.ravel()))
     for b in (g, qb, out, r, other):
         b.free()
+
+
+# ---- nothing written past an array ----------------------------------------------------------------------------------------
+
+class Guarded:
+    """an int32 array on the device between words of a pattern"""
+    GUARD, WORD = 300, 0x5EED5EED
+
+    def __init__(self, dev, a):
+        self.dev, self.n = dev, np.size(a)
+        words = np.full(self.n + 2 * self.GUARD, self.WORD, np.int32)
+        words[self.GUARD:self.GUARD + self.n] = np.ravel(a)
+        self.buf = dev.upload(words)
+        self.ptr = self.buf.ptr + 4 * self.GUARD
+
+    def upload(self, a):
+        a = np.ascontiguousarray(a, np.int32)
+        assert a.size == self.n
+        htr._check(htr.lib().htr_upload(self.dev.h, self.ptr, a.ctypes.data, a.nbytes))
+
+    def download(self, dtype, count):
+        words = self.buf.download(np.int32)
+        for guard in (words[:self.GUARD], words[self.GUARD + self.n:]):
+            np.testing.assert_array_equal(guard, self.WORD)
+        assert count == self.n
+        return words[self.GUARD:self.GUARD + self.n].view(dtype)
+
+    def free(self):
+        self.buf.free()
+
+
+class GuardedDevice(OnDevice):
+    """OnDevice on guarded arrays, whose guards each check looks at (those that a call only reads too)"""
+
+    def __init__(self, dev, s, in_place):
+        g = lambda a: Guarded(dev, np.asarray(a, np.int64).astype(np.int32))  # noqa: E731
+        self.dev, self.s = dev, s
+        rows = [np.full(n, 77) for n in (s.n_seq + 1, s.n_seq)]
+        self.arrays = [g(rows[0]), g(rows[1]), g(s.table), g(np.full(s.n_row, 77)), g(np.full(s.n_row, 77))]
+        self.pages = htr.Pages.of(s.n_seq, s.n_row, s.page, s.max_pages, *self.arrays)
+        self.len, self.new, self.ring, self.pool = g(s.len), g(np.zeros(s.n_seq)), g(s.ring), g([s.head, s.count])
+        self.len_out, self.pool_out = (self.len, self.pool) if in_place else (g(np.zeros(s.n_seq)), g([0, 0]))
+
+    def check(self, want):
+        super().check(want)
+        for a in (self.len, self.new, self.pool):
+            a.download(np.int32, a.n)
+
+    def free(self):
+        super().free()
+        for a in self.arrays:
+            a.free()
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("n_seq,n_row,page,max_pages", [(1, 1, 16, 1), (5, 50, 16, 4), (256, 512, 16, 3), (257, 512, 32, 2), (1024, 4096, 16, 5),
+                                                        (1000, 5000, 64, 7), (3, 9000, 1024, 9)])
+def test_nothing_is_written_past_a_map_s_arrays(dev, n_seq, n_row, page, max_pages, in_place):
+    """lengths below 0, past the table, at the end of 32 bits; new rows whose sums pass 32 bits, ends of any number below 0; tables
+    without pages: as the definition has it, and nothing in front of or behind an array"""
+    rng = np.random.default_rng(n_seq + n_row)
+    cap = page * max_pages
+    lengths = np.array([-5, -2 ** 31, 0, 1, page, cap - 1, cap, cap + 1, 2 ** 31 - 1, 2 ** 31 - page])
+    news = np.array([0, 1, 1, 7, page, cap, n_row, 2 ** 31 - 1, -1, -7, -2 ** 31])
+    for usual, usual_new in ((0.5, 1.0), (0.9, 0.995), (0.0, 0.0)):
+        s = Serving(n_seq, n_row, page, max_pages, n_seq * max_pages + 3, seed=n_seq)
+        s.len[:] = np.where(rng.random(n_seq) < usual, rng.integers(0, cap + 1, n_seq), rng.choice(lengths, n_seq))
+        s.table[:] = np.where(rng.random(s.table.shape) < 0.8, rng.integers(0, s.n_page, s.table.shape), -1)
+        new = np.where(rng.random(n_seq) < usual_new, rng.integers(0, max(2, n_row // n_seq), n_seq), rng.choice(news, n_seq))
+        held = np.minimum(-(-np.maximum(s.len, 0) // page), max_pages)
+        s.count = min(s.n_page - int(held[new < 0].sum()), max(2, n_seq // 2))  # (room in the ring for what comes back)
+        d = GuardedDevice(dev, s, in_place)
+        d.new.upload(new.astype(np.int32))
+        want = s.step(new)
+        d.map()
+        d.check(want)
+        d.free()
