@@ -111,7 +111,7 @@ __device__ __forceinline__ void rank(uint64_t *s_keys, int n, uint64_t *s_top, i
 
 // Bound: of many rows HBM: 1925 rows of 151936 with one alternative (1.17 GB) 185 µs, 6.3 TB/s, without 181, with 20 191 (each wave
 // by its own bound 215); 200 rows with 5 30 µs. Of few latency: one row 10 µs, 5 for a chunk's loads, sums and alternatives, 4 for
-// handing the part over and joining 19; 61 rows with 20 alternatives 23 (each wave by its own bound 25), without 12: what a chunk has
+// handing the part over and joining 19; 61 rows with 20 alternatives 21 … 23 (each wave by its own bound 2 more), without 12: what a chunk has
 // past its bound is kept and ranked, 400 of 19 parts are ranked again, and 135 of the 1159 workgroups wait for the others. A row's
 // parts on one XCD, in whose L2 they are handed over: 61 rows 16.8 … 12.2 µs, for 19.9 and 15.8 through the coherence point.
 template <int V, bool TOP, bool XL> __global__ __launch_bounds__(T, 4) void k_logprobs(ScoreArgs a) {

@@ -11,9 +11,9 @@
 // length on it its keys and COST more for its start and end, and the head's workgroups take equal pieces of the line, wherever
 // that cuts a tile: one read of many keys goes to all of them, of many short ones each takes a few, and no list of work is made
 // first. Where a piece begins follows from sums over the reads, a lane a read. The parts of a cut tile are joined by a second
-// launch, of tokens by the last of the tile's workgroups. (So joined, 32 parts of a wide tile went through one workgroup, 65 rows
-// over 8000 keys 182 µs for 47; in pairs 75. More and smaller pieces, or smaller ones for the workgroups that begin later, were
-// slower: 64 reads' tokens 110 … 124 µs for 105.)
+// launch, of tokens by the last of the tile's workgroups. (So joined, 32 parts of a wide tile went through one workgroup: 65 rows
+// over 8000 keys, when they took 47 µs by a second launch, 182, in pairs 75. More and smaller pieces, or smaller ones for the
+// workgroups that begin later, were slower: 64 reads' tokens, when they took 105, 110 … 124.)
 //
 // Tiles come in two heights, each with a line of its own. Of up to 32 rows (a step's token, or what is left of a prompt) the waves
 // share out the keys, every fourth block of 32 to each, loaded into LDS of its own, so that nobody waits for anybody until the

@@ -21,7 +21,7 @@ namespace {
 // but 964 rows of 64 reads 6.1 and 5.2), else of 1024. Up to 4096 rows it maps the rows too, more are a second launch's.
 constexpr int SMALL = 256, SMALL_ROWS = 512, ROWS_ONE = 4096;
 // searches of a thread beside each other, each ten LDS reads behind one another, where there are more than four to a thread (8000
-// pages 17.2 µs for 18.0); fewer go one by one (582 reads of a token, 36 of which end, 7.3 µs for 9.9)
+// pages 17.2 µs for 18.7); fewer go one by one (582 reads of a token, 36 of which end, 7.6 µs for 8.9; calls one after another)
 constexpr int AT_ONCE = 4;
 
 struct MapArgs {

@@ -273,7 +273,10 @@ int htr_qkv_post_pages(htr_device *dev, const float *d_q, size_t q_stride, const
  * the same bits every time, while a read's last bits depend on the reads beside it (their lengths say where its keys are shared
  * out). Scratch: two workgroups a CU for each of two heights of tile, 87 MB on 256 CUs, the same for every call, made at the
  * first one, which cannot be one that is being captured. With g q heads to a KV head n_row·g² < 2^31, n_row·g ≤ 2^30 and
- * n_seq·g·(n_row·g / 128 + 2)·(max_pages·page + n_row·g + 128) < 2^62 (else refused). Reads pages->d_start, d_past and d_table. */
+ * n_seq·g·(n_row·g / 128 + 2)·(max_pages·page + n_row·g + 128) < 2^62 (else refused). Reads pages->d_start, d_past and d_table.
+ * Up to 128 / g rows, 4 to a read, are one launch, and more two: by n_row, not by the rows that are there, so that a step sized
+ * for more takes 3 … 4 µs longer when it has tokens alone (a token over 1300 keys 14 µs for 11). One that is recorded is best
+ * recorded twice, with an n_row for tokens and one for prompts beside them. */
 int htr_page_attention(htr_device *dev, const float *d_q, size_t q_stride, const htr_pages *pages, const htr_kv *kv, int n_head,
                        float scale, float *d_out);
 /* the GPU token choice of a greedy preset on n_vocab logits (choose_pen → choose_max → choose_pick,
