@@ -186,3 +186,81 @@ def test_replayed_with_other_rows(dev):
     for s in bufs:
         for x in s:
             x.free()
+
+
+@pytest.mark.parametrize("n,vocab,top", [(1200, 20001, 32), (700, 20001, 32), (500, 30011, 20), (330, 45011, 5), (330, 45011, 32),
+                                         (1200, 4096, 32), (600, 4090, 32)])
+def test_several_chunks_to_a_workgroup(dev, n, vocab, top):
+    """so many rows that a workgroup takes several chunks of one (on 256 CUs three, two of a row in two parts, …): rising and falling
+    logits, equal ones, few values, ±0, random ones with a NaN or an infinity in a later chunk. Rows of a kind are alike"""
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((11, vocab)).astype(np.float32)
+    x[0] = -3.25
+    x[1] = rng.integers(4, size=vocab)
+    x[2] = np.linspace(-9, 9, vocab)
+    x[3] = np.linspace(9, -9, vocab)
+    x[4] = np.where(rng.random(vocab) < 0.5, 0.0, -0.0)
+    x[5, -40:] += 9
+    x[6, ::3] = -np.inf
+    x[7, vocab - 5] = np.nan
+    x[8] = -np.inf
+    x[8, vocab - 2] = 1.0
+    x[9, vocab - 9] = np.inf
+    ids = np.array([0, 5, vocab - 1, 0, 7, vocab - 3, 1, 4, vocab - 2, 3, 70], np.int32)
+    kind = np.arange(n) % 11
+    got = run(dev, x[kind], ids[kind], top)
+    logprob, entropy, order, tops = reference(x, ids, top)
+    np.testing.assert_array_equal(got[2], order[kind])
+    for g, (want, off) in [(got[0], logprob), (got[1], entropy)] + [(got[3][:, k], t) for k, t in enumerate(tops)]:
+        special = ~np.isfinite(want)[kind]
+        np.testing.assert_array_equal(g[special], want[kind][special].astype(np.float32))
+        assert np.all(np.abs(g[~special] - want[kind][~special]) <= off[kind][~special])
+
+
+def upload_at(dev, ptr, a):
+    a = np.ascontiguousarray(a)
+    htr._check(htr.lib().htr_upload(dev.h, ptr, a.ctypes.data, a.nbytes))
+
+
+def test_rows_past_32_bits(dev):
+    """rows 2^31 + 5 logits apart: the third lies 17 GB behind the first"""
+    vocab, stride, top = 9001, 2 ** 31 + 5, 6
+    x, ids = logits(3, 3, vocab)
+    xb = dev.alloc(4 * (2 * stride + vocab))
+    for i in range(3):
+        upload_at(dev, xb.ptr + 4 * stride * i, x[i])
+    ib, lp, h = dev.upload(ids), dev.alloc(12), dev.alloc(12)
+    ti, tl = dev.alloc(12 * top), dev.alloc(12 * top)
+    htr.token_logprobs(dev, xb, 3, vocab, ib, lp, h, top, ti, tl, stride=stride)
+    want = run(dev, x, ids, top)
+    # (another alignment of the rows: the sums' order and so their last bits differ)
+    logprob, entropy, order, tops = reference(x, ids, top)
+    np.testing.assert_array_equal(ti.download(np.int32, 3 * top).reshape(3, top), order)
+    for g, (w, off) in ((lp.download(np.float32, 3), logprob), (h.download(np.float32, 3), entropy)):
+        assert np.all(np.abs(g - w) <= off)
+    np.testing.assert_array_equal(want[2], order)
+    for b in (xb, ib, lp, h, ti, tl):
+        b.free()
+
+
+def test_the_largest_vocabulary(dev):
+    """2^28 logits of a row, all -10 but four. Of 64 parts' 256 threads each sums 2^14 equal terms one after another, each sum off by
+    2^-24 of it at most: 2^-10 of r and W, beside DELTA"""
+    vocab, top = 2 ** 28, 5
+    x = np.full(vocab, -10.0, np.float32)
+    at = {5: 1.0, vocab - 1: 2.0, 2 ** 27 + 3: 1.0, vocab - 8192: 1.5}
+    for i, v in at.items():
+        x[i] = v
+    xb, ib = dev.upload(x), dev.upload(np.array([vocab - 8192], np.int32))
+    lp, h, ti, tl = dev.alloc(4), dev.alloc(4), dev.alloc(4 * top), dev.alloc(4 * top)
+    htr.token_logprobs(dev, xb, 1, vocab, ib, lp, h, top, ti, tl)
+    e = [np.exp(v - 2.0) for v in (1.0, 1.0, 1.5)]
+    r = (vocab - 4) * np.exp(-12.0) + sum(e)
+    w = (vocab - 4) * np.exp(-12.0) * 12 + e[0] + e[1] + 0.5 * e[2]
+    off = 2.0 ** -10 + DELTA
+    assert ti.download(np.int32, top).tolist() == [vocab - 1, vocab - 8192, 5, 2 ** 27 + 3, 0]
+    assert abs(lp.download(np.float32, 1)[0] - (-0.5 - np.log1p(r))) <= off
+    assert np.all(np.abs(tl.download(np.float32, top) - (np.array([0, -0.5, -1, -1, -12]) - np.log1p(r))) <= off)
+    assert abs(h.download(np.float32, 1)[0] - (np.log1p(r) + w / (1 + r))) <= off * (1 + 2 * w / (1 + r))
+    for b in (xb, ib, lp, h, ti, tl):
+        b.free()
