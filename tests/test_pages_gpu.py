@@ -908,3 +908,79 @@ def test_nothing_is_written_past_a_map_s_arrays(dev, n_seq, n_row, page, max_pag
         d.map()
         d.check(want)
         d.free()
+
+
+# ---- what shares a device's scratch; rows far apart -----------------------------------------------------------------------
+
+def test_all_ways_of_joining_in_one_recording(dev):
+    """tokens on 8 KV heads, whose workgroups share an XCD, on 3 and on 1, whose do not, and chunks by two launches, one after another
+    over the same tickets and scratch, recorded as one graph and replayed: the bits of each alone"""
+    runs = []
+    for seed, (reads, n_head, n_kv, q8_0, kernel) in enumerate([
+            ([(5000, 1), (300, 2)], 16, 8, False, "k_page_few<f16>"), ([(4000, 2), (70, 1)], 6, 3, True, "k_page_few<q8_0>"),
+            ([(2000, 150), (900, 1)], 16, 8, False, "k_page_attn_join"), ([(9000, 3)], 2, 1, False, "k_page_few<f16>"),
+            ([(3000, 40), (20, 200)], 4, 1, True, "k_page_attn_join"), ([(5000, 1), (300, 2)], 16, 8, True, "k_page_few<q8_0>")]):
+        r = Reads(dev, reads, 32, n_kv, q8_0, seed=seed)
+        q = normal(50 + seed, r.n, n_head, 128)
+        want = r.run(q, n_head)
+        assert dev.last_kernel() == kernel
+        assert rel_rows(want, r.want(q, SCALE)) < BAR
+        runs.append((r, q, n_head, want, dev.upload(q), dev.alloc(q.nbytes)))
+    dev.capture_begin()
+    for _ in range(2):
+        for r, q, n_head, want, qb, out in runs:
+            htr.page_attention(dev, qb, r.pages, r.cache.kv, n_head, SCALE, out)
+    g = dev.capture_end()
+    for i in range(6):
+        for r, q, n_head, want, qb, out in runs:
+            out.upload(np.full(q.size, -3.5, np.float32))
+        g.launch()
+        for r, q, n_head, want, qb, out in runs[::-1 if i % 2 else 1]:
+            np.testing.assert_array_equal(bits(out.download(np.float32, q.size)), bits(want.ravel()))
+            if i % 3 == 0:
+                np.testing.assert_array_equal(bits(r.run(q, n_head)), bits(want))
+    g.free()
+    for r, q, n_head, want, qb, out in runs:
+        for b in (qb, out, r):
+            b.free()
+
+
+def test_rows_past_32_bits(dev):
+    """q, k and v rows 2^30 + 4 floats apart (the fifth 17 GB behind the first), attended by the kernels of one launch and of two, and
+    stored: as rows without a gap"""
+    n, n_head, n_kv, page, gap = 5, 4, 2, 16, 2 ** 30 + 4
+    x = normal(11, n, n_head + 2 * n_kv, 128)
+    q = x[:, :n_head]
+    big = dev.alloc(4 * ((n - 1) * gap + x[0].size))
+    for i in range(n):
+        row = np.ascontiguousarray(x[i])
+        htr._check(htr.lib().htr_upload(dev.h, big.ptr + 4 * gap * i, row.ctypes.data, row.nbytes))
+    out = dev.alloc(q.nbytes)
+    for reads, kernel in (([(40, 2), (100, 1), (3, 2)], "k_page_few<f16>"), ([(90, 5)], "k_page_attn_join")):
+        r = Reads(dev, reads, page, n_kv, seed=9)
+        want = r.run(q, n_head)
+        assert rel_rows(want, r.want(q, SCALE)) < BAR
+        htr.page_attention(dev, big, r.pages, r.cache.kv, n_head, SCALE, out, q_stride=gap)
+        assert dev.last_kernel() == kernel
+        np.testing.assert_array_equal(bits(out.download(np.float32, q.size)), bits(want.ravel()))
+        r.free()
+    n_pos = 50
+    ang = np.arange(n_pos)[:, None] * 1e6 ** (-np.arange(64) / 64.0)
+    others = [dev.upload(a) for a in (np.full(128, 1.25, np.float32), np.stack([np.cos(ang), np.sin(ang)], axis=2).astype(np.float32),
+                                      np.array([7, 0, 49, 3, 20], np.int32), np.array([31, 4, 0, 17, 16], np.int32))]
+    w, rope, pos, slot = others
+    p = htr.Pages.of(1, n, page, 2, pos, pos, pos, pos, slot)
+    got = []
+    near = dev.upload(x)
+    for base, stride in ((near, x[0].size), (big, gap)):
+        c = cache(dev, 6, n_kv, 2 * page, True)
+        at = [type("Ref", (), {"ptr": base.ptr + 512 * o}) for o in (0, n_head, n_head + n_kv)]
+        out.upload(np.zeros(q.size, np.float32))
+        htr.qkv_post_pages(dev, *at, p, w, w, rope, n_pos, n_head, EPS, c.kv, out, q_stride=stride, kv_stride=stride)
+        got.append([out.download(np.uint32, q.size), *c.rows("k"), *c.rows("v")])
+        c.free()
+    assert got[0][0].any()
+    for a, b in zip(*got):
+        np.testing.assert_array_equal(a, b)
+    for b in (big, near, out, *others):
+        b.free()
